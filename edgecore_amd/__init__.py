@@ -27,7 +27,8 @@ HEADER = REPO_DIR / "include" / "edgecore.h"
 
 __all__ = [
     "EdgeCoreError", "lib", "GPT2", "Model", "gemm_int8", "gemm_fp16_fp32",
-    "gemm_bf16_fp32", "quantize_int8_symmetric", "synth", "sample_full", "sample_candidates", "topk_dev", "PKG_DIR", "LIB_PATH",
+    "gemm_bf16_fp32", "quantize_int8_symmetric", "synth", "sample_full", "sample_candidates", "topk_dev",
+    "qk_norm_rope_dev", "rope_inv_freq", "attention_tree_dev", "sample_dev", "tree_accept_dev", "PKG_DIR", "LIB_PATH",
     "RUNTIME", "SYNTH", "HEADER",
 ]
 
@@ -98,6 +99,12 @@ _SIG = {
     "ec_topk_dev": (_I, [_P, _I, _I, _I, _I, _P, _P, _P]),
     "ec_topk_dev_noalloc": (_I, [_P, _I, _I, _I, _I, _P, _P, _P]),
     "ec_attention_dev": (_I, [_P, _I, _P, _P, _I, _I, _I, _I, _I, _P, _P, _I, _I, _P, _I, _I]),
+    "ec_sample_dev": (_I, [_P, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P]),
+    "ec_qk_norm_rope_dev": (_I, [_P, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _P, _P, C.c_double, _P, _I, _I, C.c_double,
+                                 _P, _P, _P, _P, _I, _I]),
+    "ec_rope_inv_freq": (_I, [_I, _I, C.c_double, C.c_double, C.c_double, _P]),
+    "ec_attention_tree_dev": (_I, [_P, _I, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _I, _I, _I, _I, _P, _I]),
+    "ec_tree_accept_dev": (_I, [_P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _I, _I, _P, _P, _P, _P]),
     "ec_rng_next": (C.c_uint, [C.POINTER(C.c_ulonglong)]),
     "ec_sample_full": (_I, [_P, _I, C.c_float, _I, C.POINTER(C.c_ulonglong)]),
     "ec_sample_candidates": (_I, [_P, _P, _I, _I, C.c_float, _I, C.POINTER(C.c_ulonglong)]),
@@ -480,6 +487,120 @@ def attention_dev(q: np.ndarray, kc: np.ndarray, vc: np.ndarray, pos, slot, H: i
     finally:
         for b in bufs:
             b.close()
+
+
+# ---------------------------------------------------------------------------
+# drafted tokens over the slot cache, on host arrays copied to the device
+# ---------------------------------------------------------------------------
+
+class _Call:
+    """Device copies of a call's arrays, freed at its end; None stays None."""
+
+    def __init__(self):
+        self.bufs = {}
+
+    def put(self, name: str, a, dtype):
+        if a is not None:
+            self.bufs[name] = DeviceBuffer.from_array(np.ascontiguousarray(a, dtype))
+        return self.ptr(name)
+
+    def ptr(self, name: str):
+        return self.bufs[name].ptr if name in self.bufs else None
+
+    def get(self, name: str, dtype, shape) -> np.ndarray:
+        return self.bufs[name].to_array(dtype, shape)
+
+    def tree(self, slot, past, nodes, parent):
+        return [self.put(n, a, np.int32) for n, a in
+                (("slot", slot), ("past", past), ("nodes", nodes), ("parent", parent))]
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        for b in self.bufs.values():
+            b.close()
+
+
+def rope_inv_freq(dim: int, theta: float, rope_type: int = 0, factor: float = 1.0, orig_max: float = 0.0) -> np.ndarray:
+    """ec_rope_inv_freq: rotary frequencies (type 0 plain, 1 YaRN, 2 linear, 3 NTK)."""
+    out = np.empty(max(dim // 2, 1), np.float64)
+    _check(lib().ec_rope_inv_freq(int(rope_type), int(dim), theta, factor, orig_max, _ptr(out)), "ec_rope_inv_freq")
+    return out
+
+
+def qk_norm_rope_dev(qkv: np.ndarray, kc: np.ndarray, vc: np.ndarray, H: int, KVH: int, past, N: int,
+                     q_gamma=None, k_gamma=None, eps: float = 1e-6, inv_freq=None, layout: int = 0,
+                     factor: float = 1.0, slot=None, nodes=None, parent=None, q: Optional[np.ndarray] = None):
+    """ec_qk_norm_rope_dev on host arrays: qkv [B*N][(H+2*KVH)*hd] fp32, kc / vc
+    [nslots][C][KVH*hd] fp16 bits (uint16); returns (q [B*N][H*hd], kc, vc)
+    after the call (q: what the padding rows hold)."""
+    M, width = qkv.shape
+    nslots, Cr, kv = kc.shape
+    hd = kv // KVH
+    assert width == (H + 2 * KVH) * hd and M % N == 0
+    with _Call() as c:
+        x = c.put("x", qkv, np.float32)
+        qp = c.put("q", np.zeros((M, H * hd), np.float32) if q is None else q, np.float32)
+        k, v = c.put("kc", kc, np.uint16), c.put("vc", vc, np.uint16)
+        g = [c.put("qg", q_gamma, np.float32), c.put("kg", k_gamma, np.float32)]
+        f = c.put("f", inv_freq, np.float64)
+        rot = 0 if inv_freq is None else 2 * len(inv_freq)
+        _check(lib().ec_qk_norm_rope_dev(x, width, qp, H * hd, k, v, nslots, Cr, H, KVH, hd, *g, eps, f, rot, layout,
+                                         factor, *c.tree(slot, past, nodes, parent), M // N, N), "ec_qk_norm_rope_dev")
+        _check(lib().ec_sync(), "ec_sync")
+        return (c.get("q", np.float32, (M, H * hd)), c.get("kc", np.uint16, kc.shape), c.get("vc", np.uint16, vc.shape))
+
+
+def attention_tree_dev(q: np.ndarray, kc: np.ndarray, vc: np.ndarray, H: int, KVH: int, past, N: int, slot=None,
+                       nodes=None, parent=None, window: int = 0, max_past: Optional[int] = None,
+                       out: Optional[np.ndarray] = None) -> np.ndarray:
+    """ec_attention_tree_dev on host arrays: q [B*N][H*hd] fp32, kc / vc
+    [nslots][C][KVH*hd] fp16 bits; returns out [B*N][H*hd] (out: what the
+    padding rows hold; max_past: the cache's length by default)."""
+    M, E = q.shape
+    nslots, Cr, _ = kc.shape
+    with _Call() as c:
+        p = [c.put("q", q, np.float32), c.put("kc", kc, np.uint16), c.put("vc", vc, np.uint16)]
+        o = c.put("out", np.zeros_like(q) if out is None else out, np.float32)
+        _check(lib().ec_attention_tree_dev(p[0], E, p[1], p[2], nslots, Cr, H, KVH, E // H,
+                                           *c.tree(slot, past, nodes, parent), M // N, N,
+                                           Cr if max_past is None else int(max_past), int(window), o, E),
+               "ec_attention_tree_dev")
+        _check(lib().ec_sync(), "ec_sync")
+        return c.get("out", np.float32, (M, E))
+
+
+def sample_dev(logits: np.ndarray, u, temp=None, top_k=None, top_p=None, min_p=None, vocab: Optional[int] = None):
+    """ec_sample_dev on host rows [rows][ld] (vocab: the columns that count);
+    returns (token, prob) [rows]."""
+    rows, ld = logits.shape
+    with _Call() as c:
+        x = c.put("x", logits, np.float32)
+        p = [c.put("t", temp, np.float32), c.put("k", top_k, np.int32), c.put("p", top_p, np.float32),
+             c.put("m", min_p, np.float32), c.put("u", u, np.float64)]
+        tok, prob = c.put("token", np.zeros(rows), np.int32), c.put("prob", np.zeros(rows), np.float32)
+        _check(lib().ec_sample_dev(x, rows, ld if vocab is None else int(vocab), ld, *p, tok, prob), "ec_sample_dev")
+        _check(lib().ec_sync(), "ec_sync")
+        return c.get("token", np.int32, rows), c.get("prob", np.float32, rows)
+
+
+def tree_accept_dev(kc: np.ndarray, vc: np.ndarray, past, token, sampled, slot=None, nodes=None, parent=None):
+    """ec_tree_accept_dev on host arrays: kc / vc [layers][nslots][C][kv] fp16
+    bits, token / sampled [B][N]; returns (path [B][N], npath, next, new_past
+    [B], kc, vc) after the call."""
+    layers, nslots, Cr, kv = kc.shape
+    B, N = np.shape(token)
+    with _Call() as c:
+        k, v = c.put("kc", kc, np.uint16), c.put("vc", vc, np.uint16)
+        t = [c.put("token", token, np.int32), c.put("sampled", sampled, np.int32)]
+        o = [c.put(n, np.zeros(s), np.int32) for n, s in
+             (("path", B * N), ("npath", B), ("next", B), ("new_past", B))]
+        _check(lib().ec_tree_accept_dev(k, v, layers, nslots, Cr, kv, *c.tree(slot, past, nodes, parent), *t, B, N, *o),
+               "ec_tree_accept_dev")
+        _check(lib().ec_sync(), "ec_sync")
+        return (c.get("path", np.int32, (B, N)), *(c.get(n, np.int32, B) for n in ("npath", "next", "new_past")),
+                c.get("kc", np.uint16, kc.shape), c.get("vc", np.uint16, vc.shape))
 
 
 # ---------------------------------------------------------------------------

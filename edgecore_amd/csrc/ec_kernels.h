@@ -8,6 +8,8 @@
 
 #include <type_traits>
 
+#include "ec_tree.h"
+
 namespace ec {
 
 // Per-launch timing: when a profiler sets g_launch_ev, the next kernel launch
@@ -466,6 +468,62 @@ hipError_t topk_select(const float *L, int rows, int V, int ld, int top_k, unsig
                        unsigned char *nan_flag, hipStream_t st);
 hipError_t topk_merge(const unsigned long long *cand, const unsigned char *nan_flag, int rows, int V, int top_k,
                       float *vals, int *idx, int *status, hipStream_t st);
+
+// sampling from given numbers (sample_rows.hip): one token per row of logits,
+// parameters per row (null: off); prob may be null
+struct SampleArgs {
+  const float *logits;
+  int rows, V, ld;
+  const float *temp;
+  const int *top_k;
+  const float *top_p, *min_p;
+  const double *u;
+  int *token;
+  float *prob;
+};
+hipError_t sample_rows(const SampleArgs &a, hipStream_t st);
+
+// rows of drafted tokens (tree_rows.hip, attn_tree.hip): ec_tree.h's batch
+struct NormRopeArgs {
+  EcTreeBatch t;
+  const float *x;  // [M][ldx]: q | k | v
+  int ldx;
+  float *q;
+  int ldq;
+  uint16_t *kc, *vc;
+  int H, KVH, hd;
+  const float *q_gamma, *k_gamma;
+  float eps;
+  const double *inv_freq;
+  int rot, layout;
+  float factor;
+};
+int qk_norm_rope_max_hd();
+hipError_t qk_norm_rope(const NormRopeArgs &a, hipStream_t st);
+
+struct TreeAttnArgs {
+  EcTreeBatch t;
+  const float *q;
+  int ldq;
+  const uint16_t *kc, *vc;
+  int H, KVH, hd, window;
+  float scale;
+  float *out;
+  int ldo;
+  void *ws;
+};
+int attention_tree_max_hd();
+size_t attention_tree_workspace(const TreeAttnArgs &a);  // bytes of ws
+hipError_t attention_tree(const TreeAttnArgs &a, hipStream_t st);
+
+struct AcceptArgs {
+  EcTreeBatch t;
+  uint16_t *kc, *vc;
+  int layers, kv;
+  const int *token, *sampled;
+  int *path, *npath, *next, *new_past;
+};
+hipError_t tree_accept(const AcceptArgs &a, hipStream_t st);
 
 // elementwise device math (ec_device_math)
 enum { MATH_EXPF = 0, MATH_SILU = 1, MATH_GELU = 2, MATH_F32_TO_F16 = 3, MATH_F16_TO_F32 = 4, MATH_QUANT1 = 5, MATH_COPY = 6 };

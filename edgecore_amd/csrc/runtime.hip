@@ -453,17 +453,17 @@ struct W16Buf {
   void *retired[64] = {};
   int nretired = 0;
 };
-static W16Buf g_w16_parts, g_w16_rs;
+static W16Buf g_w16_parts, g_w16_rs, g_tree_ws;
 
-static int w16_grow(W16Buf &b, size_t bytes) {
+static int w16_grow(W16Buf &b, size_t bytes, const char *fn = "gemm") {
   if (bytes <= b.n) return 0;
   hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
   EC_HIP(hipStreamIsCapturing(g_stream, &cap));
   if (cap != hipStreamCaptureStatusNone)
-    return set_err(-3, "gemm: the workspace would grow inside a stream capture (run such a call before it)");
+    return set_err(-3, "%s: the workspace would grow inside a stream capture (run such a call before it)", fn);
   size_t want = bytes;
   if (b.p) {
-    if (b.nretired == 64) return set_err(-3, "gemm: 64 workspaces are held for captured graphs");
+    if (b.nretired == 64) return set_err(-3, "%s: 64 workspaces are held for captured graphs", fn);
     b.retired[b.nretired++] = b.p;
     if (want < 2 * b.n) want = 2 * b.n;
   }
@@ -953,6 +953,43 @@ static bool tail_shape_ok(const GPT2 *g, const DevModel *d) {
          batch_tail_shape_ok(g->n_embd, d->F, g->n_embd + 2 * g->n_kv_embd);
 }
 
+// rotary frequencies of dim / 2 pairs: the reference's qwen_inv_freq
+// (src/gpt2.c:608-654) for ROPE_DEFAULT and ROPE_YARN, two more scalings beside it
+static void rope_inv_freq(int type, int dim, double theta, double factor, double orig_max, double *invf) {
+  const int half = dim / 2;
+  if (type == ROPE_NTK && dim > 2) theta *= pow(factor, (double)dim / (double)(dim - 2));
+  const double inv_base = 1.0 / theta;
+  for (int i = 0; i < half; i++) invf[i] = pow(inv_base, (double)(2 * i) / (double)dim);
+  if (type == ROPE_LINEAR)
+    for (int i = 0; i < half; i++) invf[i] /= factor;
+  if (type == ROPE_YARN) {
+    const double pi2 = 6.28318530717958647692, logbase = log(theta);
+    double lo_ = floor((double)dim * log(orig_max / (32.0 * pi2)) / (2.0 * logbase));
+    double hi_ = ceil((double)dim * log(orig_max / (1.0 * pi2)) / (2.0 * logbase));
+    if (lo_ < 0.0) lo_ = 0.0;
+    if (hi_ > (double)(dim - 1)) hi_ = (double)(dim - 1);
+    double span = hi_ - lo_;
+    if (span < 1.0) span = 1.0;
+    for (int i = 0; i < half; i++) {
+      double ramp = ((double)i - lo_) / span;
+      if (ramp < 0.0) ramp = 0.0;
+      if (ramp > 1.0) ramp = 1.0;
+      const double extrap = invf[i], interp = invf[i] / factor;
+      invf[i] = interp * ramp + extrap * (1.0 - ramp);
+    }
+  }
+}
+
+extern "C" int ec_rope_inv_freq(int rope_type, int dim, double theta, double factor, double orig_max, double *inv_freq) {
+  if (rope_type < ROPE_DEFAULT || rope_type > ROPE_NTK || dim < 2 || dim % 2 || !(theta > 0.0) || !inv_freq)
+    return set_err(-1, "ec_rope_inv_freq: type %d, dim %d (even), theta %g and an array of dim / 2", rope_type, dim, theta);
+  if (rope_type != ROPE_DEFAULT && !(factor > 0.0)) return set_err(-1, "ec_rope_inv_freq: factor %g", factor);
+  if (rope_type == ROPE_YARN && (!(orig_max > 0.0) || theta == 1.0))
+    return set_err(-1, "ec_rope_inv_freq: YaRN over an original %g positions, theta %g", orig_max, theta);
+  rope_inv_freq(rope_type, dim, theta, factor, orig_max, inv_freq);
+  return 0;
+}
+
 static int load_impl(GPT2 *g, const char *path, int batch_cap, int max_ctx) {
   memset(g, 0, sizeof *g);
   g->batch_cap = batch_cap < 1 ? 1 : batch_cap;
@@ -1144,25 +1181,8 @@ static int load_impl(GPT2 *g, const char *path, int batch_cap, int max_ctx) {
     if (half > 512) half = 512;
     d->half = half;
     std::vector<double> invf(half);
-    const int dim = 2 * half;
-    const double inv_base = 1.0 / g->rope_theta;
-    for (int i = 0; i < half; i++) invf[i] = pow(inv_base, (double)(2 * i) / (double)dim);
-    if (g->rope_type == ROPE_YARN) {
-      const double pi2 = 6.28318530717958647692, logbase = log(g->rope_theta);
-      double lo_ = floor((double)dim * log(g->yarn_orig_max / (32.0 * pi2)) / (2.0 * logbase));
-      double hi_ = ceil((double)dim * log(g->yarn_orig_max / (1.0 * pi2)) / (2.0 * logbase));
-      if (lo_ < 0.0) lo_ = 0.0;
-      if (hi_ > (double)(dim - 1)) hi_ = (double)(dim - 1);
-      double span = hi_ - lo_;
-      if (span < 1.0) span = 1.0;
-      for (int i = 0; i < half; i++) {
-        double ramp = ((double)i - lo_) / span;
-        if (ramp < 0.0) ramp = 0.0;
-        if (ramp > 1.0) ramp = 1.0;
-        const double extrap = invf[i], interp = invf[i] / g->yarn_factor;
-        invf[i] = interp * ramp + extrap * (1.0 - ramp);
-      }
-    }
+    rope_inv_freq(g->rope_type == ROPE_YARN ? ROPE_YARN : ROPE_DEFAULT, 2 * half, g->rope_theta, g->yarn_factor,
+                  g->yarn_orig_max, invf.data());
     std::vector<double2> tab((size_t)eff * half);
     const double scale = g->yarn_attention_factor;
     for (int p = 0; p < eff; p++)
@@ -2338,6 +2358,101 @@ extern "C" int ec_attention_dev(const float *q, int ldq, const uint16_t *kc, con
   return 0;
 }
 
+// ---------------------------------------------------------------------------
+// drafted tokens: rows into the cache, their attention, sampling, what stays
+// ---------------------------------------------------------------------------
+
+// What these entry points share.  Arguments are checked before the device is
+// opened; what device arrays hold is checked in the kernels (ec_tree.h).
+constexpr long kMaxRows = 1L << 22;  // rows of a call (grids and row offsets stay in 32 bits)
+
+static int tree_check(const char *fn, const EcTreeBatch &t, bool wide) {
+  if (t.B < 1 || t.N < 1 || t.B > 65535 || (long)t.B * t.N > kMaxRows)
+    return set_err(-1, "%s: B=%d sequences of N=%d rows (up to 65535, and %ld rows together)", fn, t.B, t.N, kMaxRows);
+  if (t.N > EC_TREE_MAX && (t.parent || !wide))
+    return set_err(-1, "%s: N=%d, more than the %d nodes of a tree", fn, t.N, EC_TREE_MAX);
+  if (t.nslots < 1 || t.C < 1) return set_err(-1, "%s: a cache of %d slots of %d rows", fn, t.nslots, t.C);
+  if (!t.past) return set_err(-1, "%s: null pointer", fn);
+  return 0;
+}
+
+static int heads_check(const char *fn, int H, int KVH, int hd, int max_hd) {
+  if (H < 1 || KVH < 1 || H % KVH || H > 65535 || hd < 1 || hd > max_hd)
+    return set_err(-1, "%s: H=%d KVH=%d hd=%d (H a multiple of KVH, hd up to %d)", fn, H, KVH, hd, max_hd);
+  return 0;
+}
+
+extern "C" int ec_sample_dev(const float *logits, int rows, int vocab, int ld, const float *temp, const int *top_k,
+                             const float *top_p, const float *min_p, const double *u, int *token, float *prob) {
+  if (rows < 0 || rows > kMaxRows || vocab < 1 || vocab > 1 << 18 || ld < vocab)
+    return set_err(-1, "ec_sample_dev: rows=%d vocab=%d (up to %d) ld=%d", rows, vocab, 1 << 18, ld);
+  if (rows == 0) return 0;
+  if (!logits || !u || !token) return set_err(-1, "ec_sample_dev: null pointer");
+  EC_INIT();
+  const SampleArgs a{logits, rows, vocab, ld, temp, top_k, top_p, min_p, u, token, prob};
+  EC_LAUNCH("sample", 4.0 * rows * vocab, sample_rows(a, g_stream));
+  return 0;
+}
+
+extern "C" int ec_qk_norm_rope_dev(const float *qkv, int ldx, float *q, int ldq, uint16_t *kc, uint16_t *vc, int nslots,
+                                   int C, int H, int KVH, int hd, const float *q_gamma, const float *k_gamma, double eps,
+                                   const double *inv_freq, int rot, int layout, double factor, const int *slot,
+                                   const int *past, const int *nodes, const int *parent, int B, int N) {
+  const char *fn = "ec_qk_norm_rope_dev";
+  const EcTreeBatch t{B, N, slot, past, nodes, parent, nslots, C, C};
+  int r;
+  if ((r = tree_check(fn, t, true)) || (r = heads_check(fn, H, KVH, hd, qk_norm_rope_max_hd()))) return r;
+  if ((long)ldx < (long)(H + 2 * (long)KVH) * hd || (long)ldq < (long)H * hd)
+    return set_err(-1, "%s: row strides ldx=%d ldq=%d", fn, ldx, ldq);
+  if (rot < 0 || rot > hd || rot % 2 || layout < 0 || layout > 1 || !(eps >= 0.0))
+    return set_err(-1, "%s: rot=%d (even, up to hd) layout=%d (0 half, 1 interleaved) eps=%g", fn, rot, layout, eps);
+  if (!qkv || !q || !kc || !vc || (rot > 0 && !inv_freq)) return set_err(-1, "%s: null pointer", fn);
+  EC_INIT();
+  const NormRopeArgs a{t, qkv, ldx, q, ldq, kc, vc, H, KVH, hd, q_gamma, k_gamma, (float)eps, inv_freq, rot, layout,
+                       (float)factor};
+  EC_LAUNCH("qk_norm_rope", (double)B * N * hd * (8.0 * H + 12.0 * KVH), qk_norm_rope(a, g_stream));
+  return 0;
+}
+
+extern "C" int ec_attention_tree_dev(const float *q, int ldq, const uint16_t *kc, const uint16_t *vc, int nslots, int C,
+                                     int H, int KVH, int hd, const int *slot, const int *past, const int *nodes,
+                                     const int *parent, int B, int N, int max_past, int window, float *out, int ldo) {
+  const char *fn = "ec_attention_tree_dev";
+  const EcTreeBatch t{B, N, slot, past, nodes, parent, nslots, C, max_past};
+  int r;
+  if ((r = tree_check(fn, t, false)) || (r = heads_check(fn, H, KVH, hd, attention_tree_max_hd()))) return r;
+  if ((long)ldq < (long)H * hd || (long)ldo < (long)H * hd || window < 0 || max_past < 0 || max_past > C)
+    return set_err(-1, "%s: ldq=%d ldo=%d window=%d max_past=%d (C=%d)", fn, ldq, ldo, window, max_past, C);
+  if (!q || !kc || !vc || !out) return set_err(-1, "%s: null pointer", fn);
+  EC_INIT();
+  TreeAttnArgs a{t, q, ldq, kc, vc, H, KVH, hd, window, (float)(1.0 / sqrt((double)hd)), out, ldo, nullptr};
+  const size_t need = attention_tree_workspace(a);
+  if (need && (r = w16_grow(g_tree_ws, need, fn))) return r;
+  a.ws = g_tree_ws.p;
+  EC_LAUNCH("attention_tree", 4.0 * B * (max_past + N) * KVH * hd, attention_tree(a, g_stream));
+  return 0;
+}
+
+extern "C" int ec_tree_accept_dev(uint16_t *kc, uint16_t *vc, int layers, int nslots, int C, int kv, const int *slot,
+                                  const int *past, const int *nodes, const int *parent, const int *token,
+                                  const int *sampled, int B, int N, int *path, int *npath, int *next, int *new_past) {
+  const char *fn = "ec_tree_accept_dev";
+  const EcTreeBatch t{B, N, slot, past, nodes, parent, nslots, C, C};
+  int r;
+  if ((r = tree_check(fn, t, false))) return r;
+  if (layers < 1 || kv < 1) return set_err(-1, "%s: %d layers of rows of %d", fn, layers, kv);
+  if (!kc || !vc || !token || !sampled || !path || !npath || !next || !new_past)
+    return set_err(-1, "%s: null pointer", fn);
+  const int *in[] = {slot, past, nodes};
+  for (const int *p : in)
+    for (int *o : {npath, next, new_past})
+      if (p && p < o + B && o < p + B) return set_err(-1, "%s: an output overlaps slot, past or nodes", fn);
+  EC_INIT();
+  const AcceptArgs a{t, kc, vc, layers, kv, token, sampled, path, npath, next, new_past};
+  EC_LAUNCH("tree_accept", 8.0 * layers * B * kv, tree_accept(a, g_stream));
+  return 0;
+}
+
 extern "C" void gpt2_forward(GPT2 *g, const int *tokens, const int *positions, const int *seqs, int M,
                              float *logits) {
   if (forward_impl(g, tokens, positions, seqs, M, 0, logits, nullptr)) {
@@ -2383,7 +2498,7 @@ extern "C" int ec_release(void) {
     if (g_kept_host.p) EC_HIP(hipHostFree(g_kept_host.p));
     g_kept_dev = g_kept_host = Staging{};
   }
-  for (W16Buf *b : {&g_w16_parts, &g_w16_rs}) {
+  for (W16Buf *b : {&g_w16_parts, &g_w16_rs, &g_tree_ws}) {
     if (b->p) EC_HIP(hipFree(b->p));
     for (int i = 0; i < b->nretired; i++) EC_HIP(hipFree(b->retired[i]));
     *b = W16Buf{};

@@ -40,6 +40,9 @@ extern "C" {
 /* rope scaling variants, meta `rope_type` (src/edgecore.h:27-28) */
 #define ROPE_DEFAULT 0
 #define ROPE_YARN 1
+/* further scalings of ec_rope_inv_freq (an .ecm file has the two above) */
+#define ROPE_LINEAR 2
+#define ROPE_NTK 3
 
 /* ------------------------------------------------------------------ */
 /* host conversions (src/edgecore.h:34-109)                             */
@@ -411,6 +414,95 @@ unsigned ec_rng_next(unsigned long long *state);
 int ec_sample_full(const float *logits, int vocab, float temp, int top_k, unsigned long long *state);
 int ec_sample_candidates(const float *vals, const int *idx, int ncand, int vocab, float temp, int top_k,
                          unsigned long long *state);
+
+/* ---- drafted tokens over the fp16 slot cache ----
+ *
+ * No reference counterpart.  A serving step that checks drafted tokens: the
+ * rows of a tree of drafted tokens per sequence (or of a chain: one row is an
+ * ordinary decode step) go into the cache (ec_qk_norm_rope_dev), attend over
+ * it (ec_attention_tree_dev), their logits give a token each (ec_sample_dev),
+ * and the rows that these tokens confirm stay (ec_tree_accept_dev).
+ *
+ * All arrays are device pointers; the calls enqueue on ec_stream(), return 0
+ * or a negative error code (ec_last_error()) and may be captured there.
+ * Arguments are checked before anything is launched.
+ *
+ * The batch: B sequences of N rows each (B <= 65535, B * N <= 2^22), row b * N
+ * + i being node i of sequence b.
+ *   slot [B]       the sequence's cache slot; NULL: b
+ *   past [B]       rows of the slot that are cached already
+ *   nodes [B]      how many of the N rows are nodes; NULL: N.  The rows behind
+ *                  them are padding: what they would write stays as it was
+ *   parent [B * N] the node's parent, before it in the order, or -1; NULL: the
+ *                  node before it.  With parents N <= 64
+ * Node i's key and value are at row past + i of the slot, its place in the
+ * text is past + the number of its ancestors.
+ *
+ * What these arrays hold is checked on the device: a sequence whose slot, past
+ * or nodes name no rows of the cache, or with a parent that does not come
+ * before its node, takes no part.  Its rows of q / out are NaN (with nodes
+ * outside [0, N]: all N), no cache row is written, its path is empty.  Where
+ * rows are written, so it is for a sequence whose rows overlap those of an
+ * earlier one of the call. */
+
+/* Rows of q | k | v (fp32, H + 2 KVH heads of hd <= 512, row stride ldx) into
+ * q (fp32, row stride ldq; it may be qkv itself) and the fp16 caches kc, vc
+ * [nslots][C][KVH*hd] of one layer: per head of q and k
+ *   y = x / sqrt(mean(x^2) + eps) * gamma    (a NULL gamma: y = x)
+ * then the first rot elements (even; 0: none) rotated by the angles position *
+ * inv_freq[rot / 2] (device, fp64), cosine and sine times factor: pairs (i, i
+ * + rot / 2) for layout 0, (2 i, 2 i + 1) for layout 1.  v is copied.  Without
+ * parents N is any number: prompts. */
+int ec_qk_norm_rope_dev(const float *qkv, int ldx, float *q, int ldq, uint16_t *kc, uint16_t *vc, int nslots, int C,
+                        int H, int KVH, int hd, const float *q_gamma, const float *k_gamma, double eps,
+                        const double *inv_freq, int rot, int layout, double factor, const int *slot, const int *past,
+                        const int *nodes, const int *parent, int B, int N);
+
+/* The rotary frequencies of dim / 2 pairs (host array): theta^(-2i/dim), for
+ * ROPE_LINEAR divided by factor, for ROPE_NTK of theta * factor^(dim/(dim-2)),
+ * for ROPE_YARN between the plain and the divided ones by the reference's ramp
+ * over orig_max positions (src/gpt2.c:608-654).  0 or <0. */
+int ec_rope_inv_freq(int rope_type, int dim, double theta, double factor, double orig_max, double *inv_freq);
+
+/* Attention of the nodes (N <= 64, hd <= 512) over their slots, scores times 1
+ * / sqrt(hd), fp32: node i sees rows [0, past) and its ancestors and itself,
+ * with window > 0 only those fewer than window places before it.  q [B * N]
+ * [H*hd] (row stride ldq), out likewise (ldo); q head h reads KV head h * KVH /
+ * H.  max_past: the largest past of the call (it sizes the launch; a sequence
+ * with a larger one takes no part).  Rows that a node does not see do not
+ * reach it, whatever they hold.  Uses the library's workspace: a captured call
+ * needs one of its size before the capture, as the matrix-core GEMMs do. */
+int ec_attention_tree_dev(const float *q, int ldq, const uint16_t *kc, const uint16_t *vc, int nslots, int C, int H,
+                          int KVH, int hd, const int *slot, const int *past, const int *nodes, const int *parent, int B,
+                          int N, int max_past, int window, float *out, int ldo);
+
+/* A token for every row of logits ([rows][vocab <= 2^18] fp32, row stride ld)
+ * from the given numbers u [rows] in [0, 1): the tokens in the order of
+ * ec_sample_full (largest logit first, equal ones by index), w = e^((l - max) /
+ * temp); the first top_k of them stay (<= 0: all), of these those with a sum of
+ * w before them below top_p times their sum (>= 1: all), of these those with w
+ * >= min_p (<= 0: all; above 1 counts as 1); the first token always stays.  The
+ * drawn token is the first whose running sum of w passes u times the sum of
+ * those that stay.  temp, top_k, top_p, min_p: one per row, or NULL (1 and
+ * off); temp not above 0 takes the largest logit.  NaN counts as -inf, -inf is
+ * not drawn, a row of nothing else gives -1.  prob [rows] (nullable): the
+ * drawn token's share of the sum, 1 for the largest logit, 0 for -1.  Weights
+ * and sums are 64-bit in an order-independent form: equal calls give equal
+ * tokens. */
+int ec_sample_dev(const float *logits, int rows, int vocab, int ld, const float *temp, const int *top_k,
+                  const float *top_p, const float *min_p, const double *u, int *token, float *prob);
+
+/* What the sampled tokens confirm: from node 0 to the child whose token [B *
+ * N] equals its parent's sampled [B * N] (the lowest index of several; a
+ * negative token confirms nothing), while there is one.  path [B][N] receives
+ * these nodes, then -1, npath [B] their number, next [B] the last one's sampled
+ * token, new_past [B] past + npath, and in every layer of kc, vc
+ * [layers][nslots][C][kv] the rows past + path[j] move to past + j.  No nodes,
+ * or a sequence that takes no part: npath 0, next -1, new_past = past.  N <=
+ * 64.  The outputs may not overlap slot, past or nodes. */
+int ec_tree_accept_dev(uint16_t *kc, uint16_t *vc, int layers, int nslots, int C, int kv, const int *slot,
+                       const int *past, const int *nodes, const int *parent, const int *token, const int *sampled,
+                       int B, int N, int *path, int *npath, int *next, int *new_past);
 
 /* sizeof(GPT2) as compiled into the library (lets foreign-function hosts
  * check their mirror of the struct). */
