@@ -16,6 +16,11 @@ namespace ec {
 
 namespace {
 
+// the first cached position that a node of this depth sees
+__device__ __forceinline__ int window_lo(int window, int past, int depth) {
+  return window && past + depth >= window ? min(past + depth - window + 1, past) : 0;
+}
+
 // The form for any head size and alignment: one block per (node, head), tiles
 // of 256 positions, a position per thread for the scores and an element of the
 // head per thread for the sums, with the running maximum and sum.
@@ -48,7 +53,7 @@ __global__ __launch_bounds__(256) void attn_tree_any_kernel(TreeAttnArgs a) {
     for (int e = t; e < a.hd; e += 256) out[e] = __builtin_nanf("");
     return;
   }
-  const int lo = a.window && s.past + mydepth >= a.window ? min(s.past + mydepth - a.window + 1, s.past) : 0;
+  const int lo = window_lo(a.window, s.past, mydepth);
   const int end = s.past + s.n;
   const size_t kv = (size_t)a.KVH * a.hd, base = (size_t)s.slot * a.t.C * kv + (size_t)kvh * a.hd;
   for (int e = t; e < a.hd; e += 256) q[e] = a.q[m * a.ldq + (size_t)h * a.hd + e];
@@ -94,13 +99,437 @@ __global__ __launch_bounds__(256) void attn_tree_any_kernel(TreeAttnArgs a) {
   }
 }
 
+// The matrix-core form (head sizes 32, 64, 96, 128).  One KV head serves G = H /
+// KVH query heads of n nodes: R = n G rows that share its keys and values.  A
+// block of four waves takes 64 RT rows of one KV head and a part of the
+// positions, 64 at a time: keys and values go from the cache straight into LDS,
+// the next tile while the waves work on one.
+//
+// Products run transposed, K Q^T and V^T P^T, so that a lane keeps one row
+// (lane & 15): the scores' accumulators hold 16 positions of it, its maximum and
+// sum need two exchanges with the other three groups of 16 lanes, and the
+// weights are the second product's operand as they stand: a matrix
+// instruction's 32 positions may come in any order that both operands share, so
+// lane group g takes 4 g .. 4 g + 3 of two runs of 16.  The values, rows of the
+// cache, are read for it by the transposing LDS load.
+//
+// fp32 by two 16-bit parts: q = hi + lo under a power of two that brings the
+// row's largest to 2^14 (22 bits and more of every element), weights = hi + lo
+// below 2^14; keys and values are 16 bits as they are, so two products give
+// each sum to about 2^-22.  The running maximum is raised when a score passes it
+// by 2^10 (the parts' room): nearly never after the first tile, and the
+// accumulated outputs are scaled only then.
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+
+constexpr int kTp = 64;          // positions per tile
+constexpr float kRoom = 10.0f;   // how far scores may pass the running maximum (powers of two)
+constexpr float kLift = 4.0f;    // weights are 2^kLift times e^(x - m)
+
+// chunk c (16 bytes) of a tile's row r is at chunk c ^ swz(r): the 16-byte reads
+// of one chunk by 8 consecutive rows fall on distinct banks
+template <int HD>
+__device__ __forceinline__ int swz(int r) {
+  return HD % 64 == 0 ? r & 7 : (r >> 1) & 3;
+}
+
+// the part of a sequence's tiles that split s of ns takes
+__device__ __forceinline__ int split_at(int tiles, int s, int ns) { return (int)((int64_t)tiles * s / ns); }
+
+struct TreeGrid {
+  int ns, rb, units;  // splits, row blocks per KV head, (split, sequence, KV head) triples
+};
+
+template <int HD, int RT>
+__global__ __launch_bounds__(256, 2) void attn_tree_kernel(TreeAttnArgs a, TreeGrid gr) {
+  constexpr int CPR = HD / 8, KS = HD / 32, DT = HD / 16, LPT = kTp * CPR / 256;
+  typedef __attribute__((address_space(1))) const void gvoid;
+  typedef __attribute__((address_space(3))) void lvoid;
+  typedef __attribute__((address_space(3))) v4s lv4s;
+  extern __shared__ __attribute__((aligned(16))) _Float16 lds[];  // [2 buffers][K, V][kTp][HD]
+  const int t = threadIdx.x, lane = t & 63, lr = lane & 15, lg = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(t >> 6);
+  // blocks go to the 8 XCDs in turn: a unit's row blocks, which read the same
+  // rows of the cache, follow each other on one XCD
+  const int x = blockIdx.x, unit = ((x >> 3) / gr.rb) * 8 + (x & 7), rb = (x >> 3) % gr.rb;
+  if (unit >= gr.units) return;
+  const int kvh = unit % a.KVH, b = (unit / a.KVH) % a.t.B, split = unit / (a.KVH * a.t.B);
+  const int G = a.H / a.KVH;
+  const EcTreeSeq s = ec_tree_seq(&a.t, b);
+  bool ok = ec_tree_seq_ok(&a.t, s);
+  uint64_t anc = 0;
+  int depth = 0;
+  if (ok) {
+    const int p = tree_parent(a.t, b, s.n, &ok);
+    if (ok) {
+      anc = tree_ancestors(p, &depth);
+      if (a.window > 0 && a.window < EC_TREE_MAX)
+        for (int j = 0; j < s.n; j++)
+          if (depth - __shfl(depth, j, 64) >= a.window) anc &= ~(1ull << j);
+    }
+  }
+  const int rows = ec_tree_rows(&a.t, s) * G, r0 = rb * 64 * RT;
+  if (r0 >= rows) return;
+  const size_t m0 = (size_t)b * a.t.N;
+  if (!ok) {
+    if (gr.ns == 1)
+      for (int e = t; e < min(rows - r0, 64 * RT) * HD; e += 256) {
+        const int r = r0 + e / HD;
+        a.out[(m0 + r / G) * a.ldo + (size_t)(kvh * G + r % G) * HD + e % HD] = __builtin_nanf("");
+      }
+    return;
+  }
+  const int end = s.past + s.n, lo0 = window_lo(a.window, s.past, 0);
+  const int lo_all = window_lo(a.window, s.past, s.n - 1);
+  const int tiles = (end - lo0 + kTp - 1) / kTp;
+  const int tile0 = split_at(tiles, split, gr.ns), tile1 = split_at(tiles, split + 1, gr.ns);
+  if (tile0 == tile1) return;
+
+  // this lane's rows: their node's visible nodes, first position and q
+  const bool work = r0 + w * 16 * RT < rows;
+  uint64_t see[RT];
+  int lo[RT];
+  v8h qh[RT][KS], ql[RT][KS];
+  float c[RT];
+  size_t orow[RT];
+  bool live[RT];
+#pragma unroll
+  for (int i = 0; i < RT; i++) {
+    const int r = r0 + (w * RT + i) * 16 + lr, node = r / G, h = kvh * G + (r - node * G);
+    live[i] = r < rows;
+    const int src = min(node, EC_TREE_MAX - 1);
+    see[i] = ((uint64_t)(uint32_t)__shfl((int)(uint32_t)(anc >> 32), src, 64) << 32) |
+             (uint32_t)__shfl((int)(uint32_t)anc, src, 64);
+    lo[i] = window_lo(a.window, s.past, __shfl(depth, src, 64));
+    if (!live[i]) see[i] = 0, lo[i] = s.past;
+    orow[i] = (m0 + node) * a.H + h;
+    const float *q = a.q + (m0 + node) * a.ldq + (size_t)h * HD + 8 * lg;
+    float v[KS][8], big = 0.0f;
+#pragma unroll
+    for (int k = 0; k < KS; k++) {
+      float4 u0 = {0.0f, 0.0f, 0.0f, 0.0f}, u1 = u0;
+      if (live[i]) {
+        u0 = *reinterpret_cast<const float4 *>(q + 32 * k);
+        u1 = *reinterpret_cast<const float4 *>(q + 32 * k + 4);
+      }
+      v[k][0] = u0.x, v[k][1] = u0.y, v[k][2] = u0.z, v[k][3] = u0.w;
+      v[k][4] = u1.x, v[k][5] = u1.y, v[k][6] = u1.z, v[k][7] = u1.w;
+#pragma unroll
+      for (int j = 0; j < 8; j++) big = fmaxf(big, fabsf(v[k][j]));
+    }
+    big = fmaxf(big, __shfl_xor(big, 16, 64));
+    big = fmaxf(big, __shfl_xor(big, 32, 64));
+    // the power of two 2^e that brings the largest to [2^14, 2^15)
+    const int e = min(14 - ((int)(__float_as_uint(big) >> 23) - 127), 127);
+    const float up = __uint_as_float((uint32_t)(e + 127) << 23);
+    c[i] = (float)((double)a.scale * 1.4426950408889634 * __builtin_ldexp(1.0, -e));
+#pragma unroll
+    for (int k = 0; k < KS; k++)
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const float f = v[k][j] * up;
+        const _Float16 hi = (_Float16)f;
+        qh[i][k][j] = hi;
+        ql[i][k][j] = (_Float16)(f - (float)hi);
+      }
+  }
+
+  // the tiles' way into LDS: a wave's instruction fills 64 chunks, lane l the
+  // l-th of them, with the chunk that the swizzle puts there
+  const size_t kv = (size_t)a.KVH * HD, base = (size_t)s.slot * a.t.C * kv + (size_t)kvh * HD;
+  const uint16_t *Kc = a.kc + base, *Vc = a.vc + base;
+  auto load = [&](int tile, int buf) {
+    const int p0 = lo0 + tile * kTp;
+#pragma unroll
+    for (int u = 0; u < LPT; u++) {
+      const int first = (w * LPT + u) * 64, ch = first + lane, r = ch / CPR, cc = (ch - r * CPR) ^ swz<HD>(r);
+      const size_t off = (size_t)min(p0 + r, end - 1) * kv + 8 * cc;
+      _Float16 *dst = lds + (size_t)buf * 2 * kTp * HD + first * 8;
+      __builtin_amdgcn_global_load_lds((gvoid *)(Kc + off), (lvoid *)dst, 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((gvoid *)(Vc + off), (lvoid *)(dst + kTp * HD), 16, 0, 0);
+    }
+  };
+
+  v4f o[DT][RT];
+  float mx[RT], sum[RT];
+#pragma unroll
+  for (int i = 0; i < RT; i++) {
+    mx[i] = -FLT_MAX;
+    sum[i] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < DT; d++) o[d][i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+
+  load(tile0, 0);
+  for (int tile = tile0; tile < tile1; tile++) {
+    const int buf = (tile - tile0) & 1, p0 = lo0 + tile * kTp;
+    // this tile has landed, and every wave is done with the one before it
+    __builtin_amdgcn_s_waitcnt(0);
+    asm volatile("s_barrier" ::: "memory");
+    if (tile + 1 < tile1) load(tile + 1, buf ^ 1);
+    _Float16 *K = lds + (size_t)buf * 2 * kTp * HD, *V = K + kTp * HD;
+    // a tile that some rows see in part: what they do not see has weight 0, and
+    // its values must be finite for that to be nothing
+    const bool mixed = p0 + kTp > s.past || p0 < lo_all;
+    bool inf = false;
+    if (mixed) {
+      for (int ch = t; ch < kTp * CPR; ch += 256) {
+        uint16_t *v = reinterpret_cast<uint16_t *>(V) + ch * 8;
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+          if ((v[j] & 0x7C00u) == 0x7C00u) {
+            v[j] = 0;
+            inf = true;
+          }
+      }
+      inf = __syncthreads_or(inf);
+    }
+    if (!work) continue;
+
+    // ---- scores: sc[pt][i][r] of position 16 pt + 4 lg + r ----
+    v4f sc[4][RT];
+#pragma unroll
+    for (int pt = 0; pt < 4; pt++) {
+#pragma unroll
+      for (int i = 0; i < RT; i++) sc[pt][i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int k = 0; k < KS; k++) {
+        const int r = 16 * pt + lr;
+        const v8h kf = *reinterpret_cast<const v8h *>(K + r * HD + ((4 * k + lg) ^ swz<HD>(r)) * 8);
+#pragma unroll
+        for (int i = 0; i < RT; i++) {
+          sc[pt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[i][k], sc[pt][i], 0, 0, 0);
+          sc[pt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[i][k], sc[pt][i], 0, 0, 0);
+        }
+      }
+    }
+
+    // ---- weights ----
+    v8h ph[2][RT], pl[2][RT];
+#pragma unroll
+    for (int i = 0; i < RT; i++) {
+      float top = -FLT_MAX;
+      uint32_t seen = 0xFFFFu;  // bit 4 pt + r
+      if (mixed) {
+        seen = 0;
+#pragma unroll
+        for (int pt = 0; pt < 4; pt++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            const int p = p0 + 16 * pt + 4 * lg + r, j = p - s.past;
+            const bool on = j < 0 ? p >= lo[i] : j < s.n && ((see[i] >> j) & 1);
+            seen |= (uint32_t)on << (4 * pt + r);
+          }
+#pragma unroll
+        for (int pt = 0; pt < 4; pt++)
+#pragma unroll
+          for (int r = 0; r < 4; r++)
+            if ((seen >> (4 * pt + r)) & 1) top = fmaxf(top, sc[pt][i][r]);
+      } else {
+#pragma unroll
+        for (int pt = 0; pt < 4; pt++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) top = fmaxf(top, sc[pt][i][r]);
+      }
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64)) * c[i];
+      if (__ballot(top > mx[i] + kRoom)) {
+        const float m = fmaxf(mx[i], top), back = __builtin_amdgcn_exp2f(mx[i] - m);
+        mx[i] = m;
+        sum[i] *= back;
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) o[d][i][r] *= back;
+      }
+      const float off = kLift - mx[i];
+#pragma unroll
+      for (int pt = 0; pt < 4; pt++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[pt][i][r], c[i], off));
+          if (mixed && !((seen >> (4 * pt + r)) & 1)) p = 0.0f;
+          sum[i] += p;
+          const _Float16 hi = (_Float16)p;
+          ph[pt >> 1][i][4 * (pt & 1) + r] = hi;
+          pl[pt >> 1][i][4 * (pt & 1) + r] = (_Float16)(p - (float)hi);
+        }
+    }
+
+    // ---- outputs: o[d][i][r] of element 16 d + 4 lg + r ----
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+#pragma unroll
+      for (int d = 0; d < DT; d++) {
+        // lane l of a group of 16 names the 8 bytes of row (l / 4), elements 4 (l % 4)
+        v8h vf;
+#pragma unroll
+        for (int q = 0; q < 2; q++) {
+          const int r = 32 * u + 16 * q + 4 * lg + (lr >> 2);
+          _Float16 *at = V + r * HD + ((2 * d + ((lr & 3) >> 1)) ^ swz<HD>(r)) * 8 + 4 * (lr & 1);
+          const v4h part = __builtin_bit_cast(v4h, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lv4s *)at));
+#pragma unroll
+          for (int j = 0; j < 4; j++) vf[4 * q + j] = part[j];
+        }
+#pragma unroll
+        for (int i = 0; i < RT; i++) {
+          o[d][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[u][i], o[d][i], 0, 0, 0);
+          o[d][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[u][i], o[d][i], 0, 0, 0);
+        }
+      }
+
+    // values that are not finite, for the rows that see them, one by one
+    if (inf) {
+      for (int pp = 0; pp < kTp; pp++) {
+        const int p = p0 + pp, j = p - s.past;
+        if (p >= end) break;
+        const int from = (((pp & 15) >> 2) << 4) | lr;  // the lane that has this row's weight of it
+#pragma unroll
+        for (int i = 0; i < RT; i++) {
+          float wgt = 0.0f;
+#pragma unroll
+          for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+              if (32 * u + 16 * (e >> 2) + (e & 3) == (pp & ~12)) wgt = (float)ph[u][i][e] + (float)pl[u][i][e];
+          wgt = __shfl(wgt, from, 64);
+          const bool on = j < 0 ? p >= lo[i] : (see[i] >> j) & 1;
+          if (on) {
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+              for (int r = 0; r < 4; r++) {
+                const uint16_t v = Vc[(size_t)p * kv + 16 * d + 4 * lg + r];
+                if ((v & 0x7C00u) == 0x7C00u) o[d][i][r] += wgt * h2f(v);
+              }
+          }
+        }
+      }
+    }
+  }
+  if (!work) return;
+
+#pragma unroll
+  for (int i = 0; i < RT; i++) {
+    float l = sum[i];
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    if (!live[i]) continue;
+    if (gr.ns == 1) {
+      const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+      const size_t m = orow[i] / a.H;
+      float *out = a.out + m * a.ldo + (orow[i] - m * a.H) * HD + 4 * lg;
+#pragma unroll
+      for (int d = 0; d < DT; d++)
+        *reinterpret_cast<float4 *>(out + 16 * d) =
+            make_float4(o[d][i][0] * inv, o[d][i][1] * inv, o[d][i][2] * inv, o[d][i][3] * inv);
+    } else {
+      const size_t all = (size_t)a.t.B * a.t.N * a.H, at = (size_t)split * all + orow[i];
+      float *po = (float *)a.ws + at * HD + 4 * lg;
+#pragma unroll
+      for (int d = 0; d < DT; d++)
+        *reinterpret_cast<float4 *>(po + 16 * d) = make_float4(o[d][i][0], o[d][i][1], o[d][i][2], o[d][i][3]);
+      if (lg == 0) ((float2 *)((float *)a.ws + (size_t)gr.ns * all * HD))[at] = make_float2(mx[i], l);
+    }
+  }
+}
+
+// Joins the splits' outputs: per row the largest of their maxima, the sums and
+// outputs brought to it, HD / 4 lanes a row.
+template <int HD>
+__global__ __launch_bounds__(256) void attn_tree_join_kernel(TreeAttnArgs a, int ns) {
+  constexpr int LPR = HD / 4, RPB = 256 / LPR;
+  const int t = threadIdx.x, b = blockIdx.y;
+  const EcTreeSeq s = ec_tree_seq(&a.t, b);
+  bool ok = ec_tree_seq_ok(&a.t, s);
+  if (ok) tree_parent(a.t, b, s.n, &ok);
+  const int r = blockIdx.x * RPB + t / LPR, d = 4 * (t % LPR);
+  if (t / LPR >= RPB || r >= ec_tree_rows(&a.t, s) * a.H) return;
+  const size_t all = (size_t)a.t.B * a.t.N * a.H, row = (size_t)b * a.t.N * a.H + r;
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (ok) {
+    const float *po = (const float *)a.ws + d;
+    const float2 *ml = (const float2 *)((const float *)a.ws + (size_t)ns * all * HD);
+    const int tiles = (s.past + s.n - window_lo(a.window, s.past, 0) + kTp - 1) / kTp;
+    float m = -FLT_MAX, l = 0.0f;
+    // splits beyond the tiles are empty: with fewer tiles than splits, the others
+    for (int i = 0; i < ns; i++)
+      if (split_at(tiles, i, ns) != split_at(tiles, i + 1, ns)) m = fmaxf(m, ml[i * all + row].x);
+    for (int i = 0; i < ns; i++)
+      if (split_at(tiles, i, ns) != split_at(tiles, i + 1, ns)) {
+        const float2 u = ml[i * all + row];
+        const float4 v = *reinterpret_cast<const float4 *>(po + (i * all + row) * HD);
+        const float f = __builtin_amdgcn_exp2f(u.x - m);
+        l = __builtin_fmaf(u.y, f, l);
+        o.x = __builtin_fmaf(v.x, f, o.x);
+        o.y = __builtin_fmaf(v.y, f, o.y);
+        o.z = __builtin_fmaf(v.z, f, o.z);
+        o.w = __builtin_fmaf(v.w, f, o.w);
+      }
+    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+    o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+  } else {
+    o.x = o.y = o.z = o.w = __builtin_nanf("");
+  }
+  const int node = r / a.H;
+  *reinterpret_cast<float4 *>(a.out + ((size_t)b * a.t.N + node) * a.ldo + (size_t)(r - node * a.H) * HD + d) = o;
+}
+
+// rows that the matrix-core form's 16-byte accesses can take
+bool tiles_ok(const TreeAttnArgs &a) {
+  const uintptr_t p = (uintptr_t)a.q | (uintptr_t)a.kc | (uintptr_t)a.vc | (uintptr_t)a.out;
+  return (a.hd == 32 || a.hd == 64 || a.hd == 96 || a.hd == 128) && !(p & 15) && a.ldq % 4 == 0 && a.ldo % 4 == 0;
+}
+
+// row tiles per wave, row blocks and splits.  Enough blocks for two on each CU,
+// of at least one tile each.
+int tree_rt(const TreeAttnArgs &a) { return (long)a.t.N * (a.H / a.KVH) <= 64 ? 1 : 2; }
+TreeGrid tree_grid(const TreeAttnArgs &a) {
+  TreeGrid g;
+  const int per = 64 * tree_rt(a);
+  g.rb = (int)(((long)a.t.N * (a.H / a.KVH) + per - 1) / per);
+  long span = (long)a.t.max_past + a.t.N;
+  if (a.window > 0 && (long)a.window + a.t.N < span) span = (long)a.window + a.t.N;
+  const long tiles = (span + kTp - 1) / kTp, units = (long)a.t.B * a.KVH, blocks = units * g.rb;
+  const long want = (512 + blocks - 1) / blocks;
+  g.ns = (int)(want < tiles ? want : tiles);
+  g.units = (int)(units * g.ns);
+  return g;
+}
+
+template <int HD>
+hipError_t launch_tree(const TreeAttnArgs &a, hipStream_t st) {
+  const TreeGrid g = tree_grid(a);
+  const dim3 grid((g.units + 7) / 8 * 8 * g.rb);
+  const uint32_t lds = 4 * kTp * HD * 2;
+  if (tree_rt(a) == 1) klaunch((attn_tree_kernel<HD, 1>), grid, dim3(256), lds, st, a, g);
+  else klaunch((attn_tree_kernel<HD, 2>), grid, dim3(256), lds, st, a, g);
+  if (g.ns > 1) {
+    constexpr int rpb = 256 / (HD / 4);
+    klaunch((attn_tree_join_kernel<HD>), dim3((a.t.N * a.H + rpb - 1) / rpb, a.t.B), dim3(256), 0, st, a, g.ns);
+  }
+  return hipGetLastError();
+}
+
 }  // namespace
 
 int attention_tree_max_hd() { return kTreeMaxHd; }
 
-size_t attention_tree_workspace(const TreeAttnArgs &) { return 0; }
+size_t attention_tree_workspace(const TreeAttnArgs &a) {
+  if (!tiles_ok(a)) return 0;
+  const TreeGrid g = tree_grid(a);
+  return g.ns > 1 ? (size_t)g.ns * a.t.B * a.t.N * a.H * (a.hd + 2) * sizeof(float) : 0;
+}
 
 hipError_t attention_tree(const TreeAttnArgs &a, hipStream_t st) {
+  if (tiles_ok(a)) {
+    if (a.hd == 64) return launch_tree<64>(a, st);
+    if (a.hd == 128) return launch_tree<128>(a, st);
+    if (a.hd == 96) return launch_tree<96>(a, st);
+    return launch_tree<32>(a, st);
+  }
   klaunch(attn_tree_any_kernel, dim3(a.t.B * a.t.N, a.H), dim3(256), 0, st, a);
   return hipGetLastError();
 }
