@@ -120,8 +120,6 @@ __global__ __launch_bounds__(256) void attn_tree_any_kernel(TreeAttnArgs a) {
 // by 2^10 (the parts' room): nearly never after the first tile, and the
 // accumulated outputs are scaled only then.
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-typedef _Float16 v4h __attribute__((ext_vector_type(4)));
-typedef short v4s __attribute__((ext_vector_type(4)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 
 constexpr int kTp = 64;          // positions per tile
@@ -135,19 +133,62 @@ __device__ __forceinline__ int swz(int r) {
   return HD % 64 == 0 ? r & 7 : (r >> 1) & 3;
 }
 
-// the part of a sequence's tiles that split s of ns takes
-__device__ __forceinline__ int split_at(int tiles, int s, int ns) { return (int)((int64_t)tiles * s / ns); }
+// where split s of a sequence's tiles starts: the first min(ns, tiles) splits
+// have some, the others none
+__device__ __forceinline__ int split_at(int tiles, int s, int ns) {
+  const int n = min(ns, tiles);
+  return s >= n ? tiles : (int)((int64_t)tiles * s / n);
+}
 
 struct TreeGrid {
   int ns, rb, units;  // splits, row blocks per KV head, (split, sequence, KV head) triples
 };
+
+__device__ __forceinline__ v4f mma(v4u a, v4u b, v4f c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+}
+
+// two values in two 16-bit parts each: hi the nearest, lo what is left of them.
+// minus_one is -1 from a register that the compiler cannot see into: the
+// difference and its rounding are then one instruction (v_fma_mixlo_f16).
+struct Parts {
+  uint32_t hi, lo;
+};
+__device__ __forceinline__ Parts split2(float x, float y, float minus_one) {
+  typedef float v2f __attribute__((ext_vector_type(2)));
+  typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+  const v2h hi = __builtin_convertvector((v2f{x, y}), v2h);
+  const v2h lo = {(_Float16)__builtin_fmaf((float)hi.x, minus_one, x), (_Float16)__builtin_fmaf((float)hi.y, minus_one, y)};
+  return Parts{__builtin_bit_cast(uint32_t, hi), __builtin_bit_cast(uint32_t, lo)};
+}
+__device__ __forceinline__ float half_of(v4u v, int e) { return h2f((uint16_t)(v[e >> 1] >> (16 * (e & 1)))); }
+
+// Operands of two groups of 16 elements, from rows 32 u .. 32 u + 31 of the
+// tile: lane l of 16 names 8 bytes of row l / 4 and gets element l of the four
+// rows.  The builtin would wait for every load that is on its way into LDS, the
+// next tile's too.
+template <int HD>
+__device__ __forceinline__ void read_v2(uint32_t at0, uint32_t at1, int u, v4u (&v)[2]) {
+  typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+  v2u x[4];
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %4 offset:%6\n\t"
+      "ds_read_b64_tr_b16 %1, %4 offset:%7\n\t"
+      "ds_read_b64_tr_b16 %2, %5 offset:%6\n\t"
+      "ds_read_b64_tr_b16 %3, %5 offset:%7\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3])
+      : "v"(at0), "v"(at1), "i"(64 * HD * u), "i"(64 * HD * u + 32 * HD)
+      : "memory");
+#pragma unroll
+  for (int e = 0; e < 2; e++) v[e] = v4u{x[2 * e].x, x[2 * e].y, x[2 * e + 1].x, x[2 * e + 1].y};
+}
 
 template <int HD, int RT>
 __global__ __launch_bounds__(256, 2) void attn_tree_kernel(TreeAttnArgs a, TreeGrid gr) {
   constexpr int CPR = HD / 8, KS = HD / 32, DT = HD / 16, LPT = kTp * CPR / 256;
   typedef __attribute__((address_space(1))) const void gvoid;
   typedef __attribute__((address_space(3))) void lvoid;
-  typedef __attribute__((address_space(3))) v4s lv4s;
   extern __shared__ __attribute__((aligned(16))) _Float16 lds[];  // [2 buffers][K, V][kTp][HD]
   const int t = threadIdx.x, lane = t & 63, lr = lane & 15, lg = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -187,11 +228,13 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(TreeAttnArgs a, TreeG
   const int tile0 = split_at(tiles, split, gr.ns), tile1 = split_at(tiles, split + 1, gr.ns);
   if (tile0 == tile1) return;
 
+  float minus_one = -1.0f;
+  asm volatile("" : "+s"(minus_one));
   // this lane's rows: their node's visible nodes, first position and q
   const bool work = r0 + w * 16 * RT < rows;
   uint64_t see[RT];
   int lo[RT];
-  v8h qh[RT][KS], ql[RT][KS];
+  v4u qh[RT][KS], ql[RT][KS];
   float c[RT];
   size_t orow[RT];
   bool live[RT];
@@ -224,15 +267,14 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(TreeAttnArgs a, TreeG
     // the power of two 2^e that brings the largest to [2^14, 2^15)
     const int e = min(14 - ((int)(__float_as_uint(big) >> 23) - 127), 127);
     const float up = __uint_as_float((uint32_t)(e + 127) << 23);
-    c[i] = (float)((double)a.scale * 1.4426950408889634 * __builtin_ldexp(1.0, -e));
+    c[i] = fmaxf((float)((double)a.scale * 1.4426950408889634 * __builtin_ldexp(1.0, -e)), FLT_MIN);
 #pragma unroll
     for (int k = 0; k < KS; k++)
 #pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const float f = v[k][j] * up;
-        const _Float16 hi = (_Float16)f;
-        qh[i][k][j] = hi;
-        ql[i][k][j] = (_Float16)(f - (float)hi);
+      for (int j = 0; j < 4; j++) {
+        const Parts f = split2(v[k][2 * j] * up, v[k][2 * j + 1] * up, minus_one);
+        qh[i][k][j] = f.hi;
+        ql[i][k][j] = f.lo;
       }
   }
 
@@ -251,6 +293,16 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(TreeAttnArgs a, TreeG
       __builtin_amdgcn_global_load_lds((gvoid *)(Vc + off), (lvoid *)(dst + kTp * HD), 16, 0, 0);
     }
   };
+
+  // the values' LDS addresses in a buffer's first 32 rows (rows 16 and 32 further
+  // on have the same swizzle)
+  const uint32_t vbase = (uint32_t)(uintptr_t)(lvoid *)lds + 2 * kTp * HD;
+  uint32_t vcol[DT];
+#pragma unroll
+  for (int d = 0; d < DT; d++) {
+    const int r = 4 * lg + (lr >> 2);
+    vcol[d] = (uint32_t)(r * HD + ((2 * d + ((lr & 3) >> 1)) ^ swz<HD>(r)) * 8 + 4 * (lr & 1)) * 2;
+  }
 
   v4f o[DT][RT];
   float mx[RT], sum[RT];
@@ -297,42 +349,34 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(TreeAttnArgs a, TreeG
 #pragma unroll
       for (int k = 0; k < KS; k++) {
         const int r = 16 * pt + lr;
-        const v8h kf = *reinterpret_cast<const v8h *>(K + r * HD + ((4 * k + lg) ^ swz<HD>(r)) * 8);
+        const v4u kf = *reinterpret_cast<const v4u *>(K + r * HD + ((4 * k + lg) ^ swz<HD>(r)) * 8);
 #pragma unroll
         for (int i = 0; i < RT; i++) {
-          sc[pt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[i][k], sc[pt][i], 0, 0, 0);
-          sc[pt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[i][k], sc[pt][i], 0, 0, 0);
+          sc[pt][i] = mma(kf, qh[i][k], sc[pt][i]);
+          sc[pt][i] = mma(kf, ql[i][k], sc[pt][i]);
         }
       }
     }
 
     // ---- weights ----
-    v8h ph[2][RT], pl[2][RT];
+    v4u ph[2][RT], pl[2][RT];
 #pragma unroll
     for (int i = 0; i < RT; i++) {
-      float top = -FLT_MAX;
-      uint32_t seen = 0xFFFFu;  // bit 4 pt + r
       if (mixed) {
-        seen = 0;
 #pragma unroll
         for (int pt = 0; pt < 4; pt++)
 #pragma unroll
           for (int r = 0; r < 4; r++) {
             const int p = p0 + 16 * pt + 4 * lg + r, j = p - s.past;
-            const bool on = j < 0 ? p >= lo[i] : j < s.n && ((see[i] >> j) & 1);
-            seen |= (uint32_t)on << (4 * pt + r);
+            const bool on = j < 0 ? p >= lo[i] : j < s.n && ((see[i] >> (j & 63)) & 1);
+            if (!on) sc[pt][i][r] = -__builtin_inff();
           }
-#pragma unroll
-        for (int pt = 0; pt < 4; pt++)
-#pragma unroll
-          for (int r = 0; r < 4; r++)
-            if ((seen >> (4 * pt + r)) & 1) top = fmaxf(top, sc[pt][i][r]);
-      } else {
-#pragma unroll
-        for (int pt = 0; pt < 4; pt++)
-#pragma unroll
-          for (int r = 0; r < 4; r++) top = fmaxf(top, sc[pt][i][r]);
       }
+      float top = -FLT_MAX;
+#pragma unroll
+      for (int pt = 0; pt < 4; pt++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) top = fmaxf(top, sc[pt][i][r]);
       top = fmaxf(top, __shfl_xor(top, 16, 64));
       top = fmaxf(top, __shfl_xor(top, 32, 64)) * c[i];
       if (__ballot(top > mx[i] + kRoom)) {
@@ -346,38 +390,37 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(TreeAttnArgs a, TreeG
       }
       const float off = kLift - mx[i];
 #pragma unroll
-      for (int pt = 0; pt < 4; pt++)
+      for (int pt = 0; pt < 4; pt++) {
+        float p[4];
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-          float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[pt][i][r], c[i], off));
-          if (mixed && !((seen >> (4 * pt + r)) & 1)) p = 0.0f;
-          sum[i] += p;
-          const _Float16 hi = (_Float16)p;
-          ph[pt >> 1][i][4 * (pt & 1) + r] = hi;
-          pl[pt >> 1][i][4 * (pt & 1) + r] = (_Float16)(p - (float)hi);
+          p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[pt][i][r], c[i], off));
+          sum[i] += p[r];
         }
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+          const Parts f = split2(p[2 * r], p[2 * r + 1], minus_one);
+          ph[pt >> 1][i][2 * (pt & 1) + r] = f.hi;
+          pl[pt >> 1][i][2 * (pt & 1) + r] = f.lo;
+        }
+      }
     }
 
     // ---- outputs: o[d][i][r] of element 16 d + 4 lg + r ----
+    const uint32_t vat = vbase + (uint32_t)buf * (4 * kTp * HD);
 #pragma unroll
     for (int u = 0; u < 2; u++)
 #pragma unroll
-      for (int d = 0; d < DT; d++) {
-        // lane l of a group of 16 names the 8 bytes of row (l / 4), elements 4 (l % 4)
-        v8h vf;
+      for (int d = 0; d < DT; d += 2) {
+        v4u vf[2];
+        read_v2<HD>(vat + vcol[d], vat + vcol[d + 1], u, vf);
 #pragma unroll
-        for (int q = 0; q < 2; q++) {
-          const int r = 32 * u + 16 * q + 4 * lg + (lr >> 2);
-          _Float16 *at = V + r * HD + ((2 * d + ((lr & 3) >> 1)) ^ swz<HD>(r)) * 8 + 4 * (lr & 1);
-          const v4h part = __builtin_bit_cast(v4h, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lv4s *)at));
+        for (int e = 0; e < 2; e++)
 #pragma unroll
-          for (int j = 0; j < 4; j++) vf[4 * q + j] = part[j];
-        }
-#pragma unroll
-        for (int i = 0; i < RT; i++) {
-          o[d][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[u][i], o[d][i], 0, 0, 0);
-          o[d][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[u][i], o[d][i], 0, 0, 0);
-        }
+          for (int i = 0; i < RT; i++) {
+            o[d + e][i] = mma(vf[e], ph[u][i], o[d + e][i]);
+            o[d + e][i] = mma(vf[e], pl[u][i], o[d + e][i]);
+          }
       }
 
     // values that are not finite, for the rows that see them, one by one
@@ -393,7 +436,7 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(TreeAttnArgs a, TreeG
           for (int u = 0; u < 2; u++)
 #pragma unroll
             for (int e = 0; e < 8; e++)
-              if (32 * u + 16 * (e >> 2) + (e & 3) == (pp & ~12)) wgt = (float)ph[u][i][e] + (float)pl[u][i][e];
+              if (32 * u + 16 * (e >> 2) + (e & 3) == (pp & ~12)) wgt = half_of(ph[u][i], e) + half_of(pl[u][i], e);
           wgt = __shfl(wgt, from, 64);
           const bool on = j < 0 ? p >= lo[i] : (see[i] >> j) & 1;
           if (on) {
@@ -437,44 +480,46 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(TreeAttnArgs a, TreeG
 }
 
 // Joins the splits' outputs: per row the largest of their maxima, the sums and
-// outputs brought to it, HD / 4 lanes a row.
+// outputs brought to it.  HD / 4 lanes a row (a power of two of them: 24 of 32 at
+// 96); the maxima and sums are read by all lanes of a row at once.
 template <int HD>
 __global__ __launch_bounds__(256) void attn_tree_join_kernel(TreeAttnArgs a, int ns) {
-  constexpr int LPR = HD / 4, RPB = 256 / LPR;
-  const int t = threadIdx.x, b = blockIdx.y;
+  constexpr int LPR = HD == 96 ? 32 : HD / 4, RPB = 256 / LPR;
+  const int t = threadIdx.x, b = blockIdx.y, li = t % LPR;
   const EcTreeSeq s = ec_tree_seq(&a.t, b);
   bool ok = ec_tree_seq_ok(&a.t, s);
   if (ok) tree_parent(a.t, b, s.n, &ok);
-  const int r = blockIdx.x * RPB + t / LPR, d = 4 * (t % LPR);
-  if (t / LPR >= RPB || r >= ec_tree_rows(&a.t, s) * a.H) return;
-  const size_t all = (size_t)a.t.B * a.t.N * a.H, row = (size_t)b * a.t.N * a.H + r;
+  const int r = blockIdx.x * RPB + t / LPR, rows = ec_tree_rows(&a.t, s) * a.H;
+  if (blockIdx.x * RPB >= rows) return;
+  const size_t all = (size_t)a.t.B * a.t.N * a.H, row = (size_t)b * a.t.N * a.H + min(r, rows - 1);
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   if (ok) {
-    const float *po = (const float *)a.ws + d;
-    const float2 *ml = (const float2 *)((const float *)a.ws + (size_t)ns * all * HD);
-    const int tiles = (s.past + s.n - window_lo(a.window, s.past, 0) + kTp - 1) / kTp;
+    const int tiles = (s.past + s.n - window_lo(a.window, s.past, 0) + kTp - 1) / kTp, n = min(ns, tiles);
+    const float *po = (const float *)a.ws + row * HD + 4 * min(li, HD / 4 - 1);
+    const float2 *ml = (const float2 *)((const float *)a.ws + (size_t)ns * all * HD) + row;
     float m = -FLT_MAX, l = 0.0f;
-    // splits beyond the tiles are empty: with fewer tiles than splits, the others
-    for (int i = 0; i < ns; i++)
-      if (split_at(tiles, i, ns) != split_at(tiles, i + 1, ns)) m = fmaxf(m, ml[i * all + row].x);
-    for (int i = 0; i < ns; i++)
-      if (split_at(tiles, i, ns) != split_at(tiles, i + 1, ns)) {
-        const float2 u = ml[i * all + row];
-        const float4 v = *reinterpret_cast<const float4 *>(po + (i * all + row) * HD);
-        const float f = __builtin_amdgcn_exp2f(u.x - m);
-        l = __builtin_fmaf(u.y, f, l);
-        o.x = __builtin_fmaf(v.x, f, o.x);
-        o.y = __builtin_fmaf(v.y, f, o.y);
-        o.z = __builtin_fmaf(v.z, f, o.z);
-        o.w = __builtin_fmaf(v.w, f, o.w);
-      }
+    for (int i = li; i < n; i += LPR) m = fmaxf(m, ml[i * all].x);
+#pragma unroll
+    for (int k = LPR / 2; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor(m, k, 64));
+#pragma unroll 8
+    for (int i = 0; i < n; i++) {
+      const float2 u = ml[i * all];
+      const float4 v = *reinterpret_cast<const float4 *>(po + (size_t)i * all * HD);
+      const float f = __builtin_amdgcn_exp2f(u.x - m);
+      l = __builtin_fmaf(u.y, f, l);
+      o.x = __builtin_fmaf(v.x, f, o.x);
+      o.y = __builtin_fmaf(v.y, f, o.y);
+      o.z = __builtin_fmaf(v.z, f, o.z);
+      o.w = __builtin_fmaf(v.w, f, o.w);
+    }
     const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
     o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
   } else {
     o.x = o.y = o.z = o.w = __builtin_nanf("");
   }
   const int node = r / a.H;
-  *reinterpret_cast<float4 *>(a.out + ((size_t)b * a.t.N + node) * a.ldo + (size_t)(r - node * a.H) * HD + d) = o;
+  if (r < rows && li < HD / 4)
+    *reinterpret_cast<float4 *>(a.out + ((size_t)b * a.t.N + node) * a.ldo + (size_t)(r - node * a.H) * HD + 4 * li) = o;
 }
 
 // rows that the matrix-core form's 16-byte accesses can take
@@ -507,7 +552,7 @@ hipError_t launch_tree(const TreeAttnArgs &a, hipStream_t st) {
   if (tree_rt(a) == 1) klaunch((attn_tree_kernel<HD, 1>), grid, dim3(256), lds, st, a, g);
   else klaunch((attn_tree_kernel<HD, 2>), grid, dim3(256), lds, st, a, g);
   if (g.ns > 1) {
-    constexpr int rpb = 256 / (HD / 4);
+    constexpr int rpb = 256 / (HD == 96 ? 32 : HD / 4);
     klaunch((attn_tree_join_kernel<HD>), dim3((a.t.N * a.H + rpb - 1) / rpb, a.t.B), dim3(256), 0, st, a, g.ns);
   }
   return hipGetLastError();
