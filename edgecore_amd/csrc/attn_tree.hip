@@ -140,6 +140,17 @@ __device__ __forceinline__ int split_at(int tiles, int s, int ns) {
   return s >= n ? tiles : (int)((int64_t)tiles * s / n);
 }
 
+// the bits 0 .. n - 1 (n up to 64, below 0 none)
+__device__ __forceinline__ uint64_t low_bits(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0 : (1ull << n) - 1; }
+
+// which of the positions p0 .. p0 + 63 a row sees: those of the text from lo on,
+// and the nodes of `see` behind it
+__device__ __forceinline__ uint64_t tile_mask(int p0, int lo, int past, uint64_t see) {
+  const int d = past - p0;
+  const uint64_t nodes = d >= 64 ? 0 : d >= 0 ? see << d : d > -64 ? see >> -d : 0;
+  return (low_bits(d) & ~low_bits(lo - p0)) | nodes;
+}
+
 struct TreeGrid {
   int ns, rb, units;  // splits, row blocks per KV head, (split, sequence, KV head) triples
 };
@@ -148,18 +159,33 @@ __device__ __forceinline__ v4f mma(v4u a, v4u b, v4f c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
 
-// two values in two 16-bit parts each: hi the nearest, lo what is left of them.
-// minus_one is -1 from a register that the compiler cannot see into: the
-// difference and its rounding are then one instruction (v_fma_mixlo_f16).
+// the maximum and the sum over the four lanes lr, lr + 16, lr + 32, lr + 48: the
+// halves, then the odd and the even rows of 16 change places
+__device__ __forceinline__ float row_max(float v) {
+  typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+  v2u x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(x.x), __uint_as_float(x.y));
+  x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(x.x), __uint_as_float(x.y));
+}
+__device__ __forceinline__ float row_sum(float v) {
+  typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+  v2u x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(x.x) + __uint_as_float(x.y);
+  x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(x.x) + __uint_as_float(x.y);
+}
+
+// two values in two 16-bit parts each: hi their leading 11 bits, lo the rest.
+// (The nearest 16-bit value and a mixed-precision difference would be three
+// instructions, not six, but those take 8 cycles each, these 2.)
 struct Parts {
   uint32_t hi, lo;
 };
-__device__ __forceinline__ Parts split2(float x, float y, float minus_one) {
-  typedef float v2f __attribute__((ext_vector_type(2)));
-  typedef _Float16 v2h __attribute__((ext_vector_type(2)));
-  const v2h hi = __builtin_convertvector((v2f{x, y}), v2h);
-  const v2h lo = {(_Float16)__builtin_fmaf((float)hi.x, minus_one, x), (_Float16)__builtin_fmaf((float)hi.y, minus_one, y)};
-  return Parts{__builtin_bit_cast(uint32_t, hi), __builtin_bit_cast(uint32_t, lo)};
+__device__ __forceinline__ Parts split2(float x, float y) {
+  const float hx = __uint_as_float(__float_as_uint(x) & 0xFFFFE000u), hy = __uint_as_float(__float_as_uint(y) & 0xFFFFE000u);
+  return Parts{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(hx, hy)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x - hx, y - hy))};
 }
 __device__ __forceinline__ float half_of(v4u v, int e) { return h2f((uint16_t)(v[e >> 1] >> (16 * (e & 1)))); }
 
@@ -184,9 +210,9 @@ __device__ __forceinline__ void read_v2(uint32_t at0, uint32_t at1, int u, v4u (
   for (int e = 0; e < 2; e++) v[e] = v4u{x[2 * e].x, x[2 * e].y, x[2 * e + 1].x, x[2 * e + 1].y};
 }
 
-template <int HD, int RT>
-__global__ __launch_bounds__(256, 2) void attn_tree_kernel(TreeAttnArgs a, TreeGrid gr) {
-  constexpr int CPR = HD / 8, KS = HD / 32, DT = HD / 16, LPT = kTp * CPR / 256;
+template <int HD, int NW, int OCC>
+__global__ __launch_bounds__(NW * 64, OCC) void attn_tree_kernel(TreeAttnArgs a, TreeGrid gr) {
+  constexpr int CPR = HD / 8, KS = HD / 32, DT = HD / 16, NT = NW * 64, LPT = (kTp * CPR + NT - 1) / NT;
   typedef __attribute__((address_space(1))) const void gvoid;
   typedef __attribute__((address_space(3))) void lvoid;
   extern __shared__ __attribute__((aligned(16))) _Float16 lds[];  // [2 buffers][K, V][kTp][HD]
@@ -197,12 +223,58 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(TreeAttnArgs a, TreeG
   const int x = blockIdx.x, unit = ((x >> 3) / gr.rb) * 8 + (x & 7), rb = (x >> 3) % gr.rb;
   if (unit >= gr.units) return;
   const int kvh = unit % a.KVH, b = (unit / a.KVH) % a.t.B, split = unit / (a.KVH * a.t.B);
-  const int G = a.H / a.KVH;
+  const int G = a.H / a.KVH, r0 = rb * 16 * NW;
+  const size_t m0 = (size_t)b * a.t.N;
+
+  // what depends on no other load is read first: the sequence's numbers, this
+  // lane's row of q (of a node that there is), then the first tile, and the
+  // parents while that is on its way
   const EcTreeSeq s = ec_tree_seq(&a.t, b);
+  const int row = r0 + w * 16 + lr, node = row / G, head = kvh * G + (row - node * G);
+  float4 qr[KS][2];
+  {
+    const float *q = a.q + (m0 + min(node, a.t.N - 1)) * a.ldq + (size_t)head * HD + 8 * lg;
+#pragma unroll
+    for (int k = 0; k < KS; k++) {
+      qr[k][0] = *reinterpret_cast<const float4 *>(q + 32 * k);
+      qr[k][1] = *reinterpret_cast<const float4 *>(q + 32 * k + 4);
+    }
+  }
   bool ok = ec_tree_seq_ok(&a.t, s);
+  const int rows = ec_tree_rows(&a.t, s) * G;
+  if (r0 >= rows) return;
+  const int end = s.past + s.n, lo0 = window_lo(a.window, s.past, 0);
+  const int lo_all = window_lo(a.window, s.past, s.n - 1);
+  const int tiles = ok ? (end - lo0 + kTp - 1) / kTp : 1;
+  const int tile0 = split_at(tiles, split, gr.ns), tile1 = split_at(tiles, split + 1, gr.ns);
+  if (tile0 == tile1) return;
+
+  // the tiles' way into LDS: a wave's instruction fills 64 chunks, lane l the
+  // l-th of them, with the chunk that the swizzle puts there
+  const size_t kv = (size_t)a.KVH * HD, base = ok ? (size_t)s.slot * a.t.C * kv + (size_t)kvh * HD : 0;
+  const uint16_t *Kc = a.kc + base, *Vc = a.vc + base;
+  auto load = [&](int tile, int buf) {
+    const int p0 = lo0 + tile * kTp;
+    const uint16_t *Kt = Kc + (size_t)p0 * kv, *Vt = Vc + (size_t)p0 * kv;
+#pragma unroll
+    for (int u = 0; u < LPT; u++) {
+      const int first = (w * LPT + u) * 64;
+      if (kTp * CPR % NT && first >= kTp * CPR) break;
+      const int ch = first + lane, r = ch / CPR, cc = (ch - r * CPR) ^ swz<HD>(r);
+      // rows behind the nodes: the last node's again (no row sees them)
+      const size_t off = (size_t)min(r, end - 1 - p0) * kv + 8 * cc;
+      _Float16 *dst = lds + (size_t)buf * 2 * kTp * HD + first * 8;
+      __builtin_amdgcn_global_load_lds((gvoid *)(Kt + off), (lvoid *)dst, 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((gvoid *)(Vt + off), (lvoid *)(dst + kTp * HD), 16, 0, 0);
+    }
+  };
+  if (ok) load(tile0, 0);
+
+  // the nodes' ancestors, where a tile of this block has rows that not all see
+  // (with one split the only check of the parents)
   uint64_t anc = 0;
   int depth = 0;
-  if (ok) {
+  if (ok && (gr.ns == 1 || lo0 + tile1 * kTp > s.past || lo0 + tile0 * kTp < lo_all)) {
     const int p = tree_parent(a.t, b, s.n, &ok);
     if (ok) {
       anc = tree_ancestors(p, &depth);
@@ -211,88 +283,56 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(TreeAttnArgs a, TreeG
           if (depth - __shfl(depth, j, 64) >= a.window) anc &= ~(1ull << j);
     }
   }
-  const int rows = ec_tree_rows(&a.t, s) * G, r0 = rb * 64 * RT;
-  if (r0 >= rows) return;
-  const size_t m0 = (size_t)b * a.t.N;
-  if (!ok) {
+  if (!ok) {  // the join marks the rows, or this block does
+    __builtin_amdgcn_s_waitcnt(0);
     if (gr.ns == 1)
-      for (int e = t; e < min(rows - r0, 64 * RT) * HD; e += 256) {
+      for (int e = t; e < min(rows - r0, 16 * NW) * HD; e += NT) {
         const int r = r0 + e / HD;
         a.out[(m0 + r / G) * a.ldo + (size_t)(kvh * G + r % G) * HD + e % HD] = __builtin_nanf("");
       }
     return;
   }
-  const int end = s.past + s.n, lo0 = window_lo(a.window, s.past, 0);
-  const int lo_all = window_lo(a.window, s.past, s.n - 1);
-  const int tiles = (end - lo0 + kTp - 1) / kTp;
-  const int tile0 = split_at(tiles, split, gr.ns), tile1 = split_at(tiles, split + 1, gr.ns);
-  if (tile0 == tile1) return;
 
-  float minus_one = -1.0f;
-  asm volatile("" : "+s"(minus_one));
-  // this lane's rows: their node's visible nodes, first position and q
-  const bool work = r0 + w * 16 * RT < rows;
-  uint64_t see[RT];
-  int lo[RT];
-  v4u qh[RT][KS], ql[RT][KS];
-  float c[RT];
-  size_t orow[RT];
-  bool live[RT];
-#pragma unroll
-  for (int i = 0; i < RT; i++) {
-    const int r = r0 + (w * RT + i) * 16 + lr, node = r / G, h = kvh * G + (r - node * G);
-    live[i] = r < rows;
-    const int src = min(node, EC_TREE_MAX - 1);
-    see[i] = ((uint64_t)(uint32_t)__shfl((int)(uint32_t)(anc >> 32), src, 64) << 32) |
-             (uint32_t)__shfl((int)(uint32_t)anc, src, 64);
-    lo[i] = window_lo(a.window, s.past, __shfl(depth, src, 64));
-    if (!live[i]) see[i] = 0, lo[i] = s.past;
-    orow[i] = (m0 + node) * a.H + h;
-    const float *q = a.q + (m0 + node) * a.ldq + (size_t)h * HD + 8 * lg;
+  const bool work = r0 + w * 16 < rows, live = row < rows;
+  const int src = min(node, EC_TREE_MAX - 1);
+  const uint64_t see = ((uint64_t)(uint32_t)__shfl((int)(uint32_t)(anc >> 32), src, 64) << 32) |
+                       (uint32_t)__shfl((int)(uint32_t)anc, src, 64);
+  const int lo = window_lo(a.window, s.past, __shfl(depth, src, 64));
+  // q in units of log2, so that a product is an exponent.  A row is brought
+  // into the parts' range by a power of two where its largest is outside [2^-2,
+  // 2^15) (below, the low parts' steps of 2^-24 would count).
+  v4u qh[KS], ql[KS];
+  float up, down;
+  bool plain;  // no row of the wave scaled
+  {
     float v[KS][8], big = 0.0f;
 #pragma unroll
     for (int k = 0; k < KS; k++) {
-      float4 u0 = {0.0f, 0.0f, 0.0f, 0.0f}, u1 = u0;
-      if (live[i]) {
-        u0 = *reinterpret_cast<const float4 *>(q + 32 * k);
-        u1 = *reinterpret_cast<const float4 *>(q + 32 * k + 4);
-      }
+      const float4 u0 = qr[k][0], u1 = qr[k][1];
       v[k][0] = u0.x, v[k][1] = u0.y, v[k][2] = u0.z, v[k][3] = u0.w;
       v[k][4] = u1.x, v[k][5] = u1.y, v[k][6] = u1.z, v[k][7] = u1.w;
 #pragma unroll
-      for (int j = 0; j < 8; j++) big = fmaxf(big, fabsf(v[k][j]));
+      for (int j = 0; j < 8; j++) {
+        v[k][j] *= a.scale * 1.44269504f;
+        big = fmaxf(big, fabsf(v[k][j]));
+      }
     }
-    big = fmaxf(big, __shfl_xor(big, 16, 64));
-    big = fmaxf(big, __shfl_xor(big, 32, 64));
-    // the power of two 2^e that brings the largest to [2^14, 2^15)
-    const int e = min(14 - ((int)(__float_as_uint(big) >> 23) - 127), 127);
-    const float up = __uint_as_float((uint32_t)(e + 127) << 23);
-    c[i] = fmaxf((float)((double)a.scale * 1.4426950408889634 * __builtin_ldexp(1.0, -e)), FLT_MIN);
+    big = row_max(big);
+    int e = 0;
+    if (!(big >= 0.25f && big < 32768.0f) && big > 0.0f)
+      e = min(max(14 - ((int)(__float_as_uint(big) >> 23) - 127), -126), 100);
+    up = __uint_as_float((uint32_t)(e + 127) << 23);
+    down = __uint_as_float((uint32_t)(127 - e) << 23);
+    plain = __ballot(e != 0) == 0;
 #pragma unroll
     for (int k = 0; k < KS; k++)
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const Parts f = split2(v[k][2 * j] * up, v[k][2 * j + 1] * up, minus_one);
-        qh[i][k][j] = f.hi;
-        ql[i][k][j] = f.lo;
+        const Parts f = split2(v[k][2 * j] * up, v[k][2 * j + 1] * up);
+        qh[k][j] = f.hi;
+        ql[k][j] = f.lo;
       }
   }
-
-  // the tiles' way into LDS: a wave's instruction fills 64 chunks, lane l the
-  // l-th of them, with the chunk that the swizzle puts there
-  const size_t kv = (size_t)a.KVH * HD, base = (size_t)s.slot * a.t.C * kv + (size_t)kvh * HD;
-  const uint16_t *Kc = a.kc + base, *Vc = a.vc + base;
-  auto load = [&](int tile, int buf) {
-    const int p0 = lo0 + tile * kTp;
-#pragma unroll
-    for (int u = 0; u < LPT; u++) {
-      const int first = (w * LPT + u) * 64, ch = first + lane, r = ch / CPR, cc = (ch - r * CPR) ^ swz<HD>(r);
-      const size_t off = (size_t)min(p0 + r, end - 1) * kv + 8 * cc;
-      _Float16 *dst = lds + (size_t)buf * 2 * kTp * HD + first * 8;
-      __builtin_amdgcn_global_load_lds((gvoid *)(Kc + off), (lvoid *)dst, 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((gvoid *)(Vc + off), (lvoid *)(dst + kTp * HD), 16, 0, 0);
-    }
-  };
 
   // the values' LDS addresses in a buffer's first 32 rows (rows 16 and 32 further
   // on have the same swizzle)
@@ -304,19 +344,14 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(TreeAttnArgs a, TreeG
     vcol[d] = (uint32_t)(r * HD + ((2 * d + ((lr & 3) >> 1)) ^ swz<HD>(r)) * 8 + 4 * (lr & 1)) * 2;
   }
 
-  v4f o[DT][RT];
-  float mx[RT], sum[RT];
+  v4f o[DT], from = {0.0f, 0.0f, 0.0f, 0.0f};  // from: what the row's products start at
+  float mx = -FLT_MAX, lim = -FLT_MAX, sum = 0.0f;
 #pragma unroll
-  for (int i = 0; i < RT; i++) {
-    mx[i] = -FLT_MAX;
-    sum[i] = 0.0f;
-#pragma unroll
-    for (int d = 0; d < DT; d++) o[d][i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-  }
+  for (int d = 0; d < DT; d++) o[d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 
-  load(tile0, 0);
-  for (int tile = tile0; tile < tile1; tile++) {
-    const int buf = (tile - tile0) & 1, p0 = lo0 + tile * kTp;
+  int buf = 0;
+  for (int tile = tile0; tile < tile1; tile++, buf ^= 1) {
+    const int p0 = lo0 + tile * kTp;
     // this tile has landed, and every wave is done with the one before it
     __builtin_amdgcn_s_waitcnt(0);
     asm volatile("s_barrier" ::: "memory");
@@ -327,86 +362,100 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(TreeAttnArgs a, TreeG
     const bool mixed = p0 + kTp > s.past || p0 < lo_all;
     bool inf = false;
     if (mixed) {
-      for (int ch = t; ch < kTp * CPR; ch += 256) {
-        uint16_t *v = reinterpret_cast<uint16_t *>(V) + ch * 8;
+      for (int ch = t; ch < kTp * CPR; ch += NT) {
+        v4u *at = reinterpret_cast<v4u *>(V) + ch, v = *at;
+        uint32_t hit = 0;
 #pragma unroll
-        for (int j = 0; j < 8; j++)
-          if ((v[j] & 0x7C00u) == 0x7C00u) {
-            v[j] = 0;
-            inf = true;
-          }
+        for (int j = 0; j < 4; j++) {
+          // an exponent of all ones carries out of its field
+          const uint32_t e = v[j] & 0x7C007C00u;
+          const uint32_t bad = ((e & 0x7C00u) + 0x0400u) & 0x8000u, bad2 = ((e >> 16) + 0x0400u) & 0x8000u;
+          v[j] &= ~((bad ? 0xFFFFu : 0u) | (bad2 ? 0xFFFF0000u : 0u));
+          hit |= bad | bad2;
+        }
+        if (hit) {
+          *at = v;
+          inf = true;
+        }
       }
       inf = __syncthreads_or(inf);
     }
     if (!work) continue;
 
-    // ---- scores: sc[pt][i][r] of position 16 pt + 4 lg + r ----
-    v4f sc[4][RT];
+    // ---- scores: sc[pt][r] of position 16 pt + 4 lg + r ----
+    v4f sc[4];
 #pragma unroll
     for (int pt = 0; pt < 4; pt++) {
-#pragma unroll
-      for (int i = 0; i < RT; i++) sc[pt][i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+      sc[pt] = from;
 #pragma unroll
       for (int k = 0; k < KS; k++) {
         const int r = 16 * pt + lr;
         const v4u kf = *reinterpret_cast<const v4u *>(K + r * HD + ((4 * k + lg) ^ swz<HD>(r)) * 8);
-#pragma unroll
-        for (int i = 0; i < RT; i++) {
-          sc[pt][i] = mma(kf, qh[i][k], sc[pt][i]);
-          sc[pt][i] = mma(kf, ql[i][k], sc[pt][i]);
-        }
+        sc[pt] = mma(kf, qh[k], sc[pt]);
+        sc[pt] = mma(kf, ql[k], sc[pt]);
       }
     }
 
     // ---- weights ----
-    v4u ph[2][RT], pl[2][RT];
-#pragma unroll
-    for (int i = 0; i < RT; i++) {
-      if (mixed) {
-#pragma unroll
-        for (int pt = 0; pt < 4; pt++)
-#pragma unroll
-          for (int r = 0; r < 4; r++) {
-            const int p = p0 + 16 * pt + 4 * lg + r, j = p - s.past;
-            const bool on = j < 0 ? p >= lo[i] : j < s.n && ((see[i] >> (j & 63)) & 1);
-            if (!on) sc[pt][i][r] = -__builtin_inff();
-          }
-      }
-      float top = -FLT_MAX;
+    if (mixed) {
+      const uint64_t on = tile_mask(p0, lo, s.past, see) >> (4 * lg);
 #pragma unroll
       for (int pt = 0; pt < 4; pt++)
 #pragma unroll
-        for (int r = 0; r < 4; r++) top = fmaxf(top, sc[pt][i][r]);
-      top = fmaxf(top, __shfl_xor(top, 16, 64));
-      top = fmaxf(top, __shfl_xor(top, 32, 64)) * c[i];
-      if (__ballot(top > mx[i] + kRoom)) {
-        const float m = fmaxf(mx[i], top), back = __builtin_amdgcn_exp2f(mx[i] - m);
-        mx[i] = m;
-        sum[i] *= back;
+        for (int r = 0; r < 4; r++)
+          if (!((on >> (16 * pt + r)) & 1)) sc[pt][r] = -__builtin_inff();
+    }
+    if (!plain) {
 #pragma unroll
-        for (int d = 0; d < DT; d++)
+      for (int pt = 0; pt < 4; pt++)
 #pragma unroll
-          for (int r = 0; r < 4; r++) o[d][i][r] *= back;
+        for (int r = 0; r < 4; r++) sc[pt][r] *= down;
+    }
+    // exponents of the weights already (the sums began at kLift - mx): above kLift
+    // + kRoom the maximum moves
+    float top = -FLT_MAX;
+#pragma unroll
+    for (int pt = 0; pt < 4; pt++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) top = fmaxf(top, sc[pt][r]);
+    if (__ballot(top > lim)) {
+      const float big = row_max(top);
+      const bool first = mx == -FLT_MAX, move = big > (first ? -FLT_MAX : kLift);
+      const float by = move ? big - kLift : 0.0f, back = first ? 0.0f : __builtin_amdgcn_exp2f(-by);
+      if (move) {
+        mx = first ? big : mx + by;
+        lim = kLift + kRoom;
       }
-      const float off = kLift - mx[i];
+      const float f = move || !first ? (kLift - mx) * up : 0.0f;
+      from = v4f{f, f, f, f};
+      sum *= back;
 #pragma unroll
-      for (int pt = 0; pt < 4; pt++) {
-        float p[4];
+      for (int d = 0; d < DT; d++)
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-          p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[pt][i][r], c[i], off));
-          sum[i] += p[r];
-        }
+        for (int r = 0; r < 4; r++) o[d][r] *= back;
 #pragma unroll
-        for (int r = 0; r < 2; r++) {
-          const Parts f = split2(p[2 * r], p[2 * r + 1], minus_one);
-          ph[pt >> 1][i][2 * (pt & 1) + r] = f.hi;
-          pl[pt >> 1][i][2 * (pt & 1) + r] = f.lo;
-        }
+      for (int pt = 0; pt < 4; pt++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) sc[pt][r] -= by;
+    }
+    v4u ph[2], pl[2];
+#pragma unroll
+    for (int pt = 0; pt < 4; pt++) {
+      float p[4];
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        p[r] = __builtin_amdgcn_exp2f(sc[pt][r]);
+        sum += p[r];
+      }
+#pragma unroll
+      for (int r = 0; r < 2; r++) {
+        const Parts f = split2(p[2 * r], p[2 * r + 1]);
+        ph[pt >> 1][2 * (pt & 1) + r] = f.hi;
+        pl[pt >> 1][2 * (pt & 1) + r] = f.lo;
       }
     }
 
-    // ---- outputs: o[d][i][r] of element 16 d + 4 lg + r ----
+    // ---- outputs: o[d][r] of element 16 d + 4 lg + r ----
     const uint32_t vat = vbase + (uint32_t)buf * (4 * kTp * HD);
 #pragma unroll
     for (int u = 0; u < 2; u++)
@@ -415,67 +464,51 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(TreeAttnArgs a, TreeG
         v4u vf[2];
         read_v2<HD>(vat + vcol[d], vat + vcol[d + 1], u, vf);
 #pragma unroll
-        for (int e = 0; e < 2; e++)
-#pragma unroll
-          for (int i = 0; i < RT; i++) {
-            o[d + e][i] = mma(vf[e], ph[u][i], o[d + e][i]);
-            o[d + e][i] = mma(vf[e], pl[u][i], o[d + e][i]);
-          }
+        for (int e = 0; e < 2; e++) {
+          o[d + e] = mma(vf[e], ph[u], o[d + e]);
+          o[d + e] = mma(vf[e], pl[u], o[d + e]);
+        }
       }
 
     // values that are not finite, for the rows that see them, one by one
     if (inf) {
-      for (int pp = 0; pp < kTp; pp++) {
-        const int p = p0 + pp, j = p - s.past;
-        if (p >= end) break;
-        const int from = (((pp & 15) >> 2) << 4) | lr;  // the lane that has this row's weight of it
+      const uint64_t on = tile_mask(p0, lo, s.past, see);
+      for (int pp = 0; pp < kTp && p0 + pp < end; pp++) {
+        float wgt = 0.0f;
 #pragma unroll
-        for (int i = 0; i < RT; i++) {
-          float wgt = 0.0f;
+        for (int u = 0; u < 2; u++)
 #pragma unroll
-          for (int u = 0; u < 2; u++)
+          for (int e = 0; e < 8; e++)
+            if (32 * u + 16 * (e >> 2) + (e & 3) == (pp & ~12)) wgt = half_of(ph[u], e) + half_of(pl[u], e);
+        wgt = __shfl(wgt, (((pp & 15) >> 2) << 4) | lr, 64);  // from the lane that has this row's weight of it
+        if ((on >> pp) & 1) {
 #pragma unroll
-            for (int e = 0; e < 8; e++)
-              if (32 * u + 16 * (e >> 2) + (e & 3) == (pp & ~12)) wgt = half_of(ph[u][i], e) + half_of(pl[u][i], e);
-          wgt = __shfl(wgt, from, 64);
-          const bool on = j < 0 ? p >= lo[i] : (see[i] >> j) & 1;
-          if (on) {
+          for (int d = 0; d < DT; d++)
 #pragma unroll
-            for (int d = 0; d < DT; d++)
-#pragma unroll
-              for (int r = 0; r < 4; r++) {
-                const uint16_t v = Vc[(size_t)p * kv + 16 * d + 4 * lg + r];
-                if ((v & 0x7C00u) == 0x7C00u) o[d][i][r] += wgt * h2f(v);
-              }
-          }
+            for (int r = 0; r < 4; r++) {
+              const uint16_t v = Vc[(size_t)(p0 + pp) * kv + 16 * d + 4 * lg + r];
+              if ((v & 0x7C00u) == 0x7C00u) o[d][r] += wgt * h2f(v);
+            }
         }
       }
     }
   }
-  if (!work) return;
 
+  const float l = row_sum(sum);
+  if (!live) return;
+  if (gr.ns == 1) {
+    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+    float *out = a.out + (m0 + node) * a.ldo + (size_t)head * HD + 4 * lg;
 #pragma unroll
-  for (int i = 0; i < RT; i++) {
-    float l = sum[i];
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
-    if (!live[i]) continue;
-    if (gr.ns == 1) {
-      const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-      const size_t m = orow[i] / a.H;
-      float *out = a.out + m * a.ldo + (orow[i] - m * a.H) * HD + 4 * lg;
+    for (int d = 0; d < DT; d++)
+      *reinterpret_cast<float4 *>(out + 16 * d) =
+          make_float4(o[d][0] * inv, o[d][1] * inv, o[d][2] * inv, o[d][3] * inv);
+  } else {
+    const size_t all = (size_t)a.t.B * a.t.N * a.H, at = (size_t)split * all + (m0 + node) * a.H + head;
+    float *po = (float *)a.ws + at * HD + 4 * lg;
 #pragma unroll
-      for (int d = 0; d < DT; d++)
-        *reinterpret_cast<float4 *>(out + 16 * d) =
-            make_float4(o[d][i][0] * inv, o[d][i][1] * inv, o[d][i][2] * inv, o[d][i][3] * inv);
-    } else {
-      const size_t all = (size_t)a.t.B * a.t.N * a.H, at = (size_t)split * all + orow[i];
-      float *po = (float *)a.ws + at * HD + 4 * lg;
-#pragma unroll
-      for (int d = 0; d < DT; d++)
-        *reinterpret_cast<float4 *>(po + 16 * d) = make_float4(o[d][i][0], o[d][i][1], o[d][i][2], o[d][i][3]);
-      if (lg == 0) ((float2 *)((float *)a.ws + (size_t)gr.ns * all * HD))[at] = make_float2(mx[i], l);
-    }
+    for (int d = 0; d < DT; d++) *reinterpret_cast<float4 *>(po + 16 * d) = make_float4(o[d][0], o[d][1], o[d][2], o[d][3]);
+    if (lg == 0) ((float2 *)((float *)a.ws + (size_t)gr.ns * all * HD))[at] = make_float2(mx, l);
   }
 }
 
@@ -528,17 +561,19 @@ bool tiles_ok(const TreeAttnArgs &a) {
   return (a.hd == 32 || a.hd == 64 || a.hd == 96 || a.hd == 128) && !(p & 15) && a.ldq % 4 == 0 && a.ldo % 4 == 0;
 }
 
-// row tiles per wave, row blocks and splits.  Enough blocks for two on each CU,
-// of at least one tile each.
-int tree_rt(const TreeAttnArgs &a) { return (long)a.t.N * (a.H / a.KVH) <= 64 ? 1 : 2; }
+// Waves per block: 4 (64 rows) or 8 (128), by the rows that share a KV head.
+int tree_waves(const TreeAttnArgs &a) { return (long)a.t.N * (a.H / a.KVH) <= 64 ? 4 : 8; }
+
+// Row blocks and splits: as many blocks as the CUs hold at a time (two of them, one of 8
+// waves at head sizes above 64), of at least a tile each.
 TreeGrid tree_grid(const TreeAttnArgs &a) {
   TreeGrid g;
-  const int per = 64 * tree_rt(a);
+  const int waves = tree_waves(a), per = 16 * waves;
   g.rb = (int)(((long)a.t.N * (a.H / a.KVH) + per - 1) / per);
   long span = (long)a.t.max_past + a.t.N;
   if (a.window > 0 && (long)a.window + a.t.N < span) span = (long)a.window + a.t.N;
   const long tiles = (span + kTp - 1) / kTp, units = (long)a.t.B * a.KVH, blocks = units * g.rb;
-  const long want = (512 + blocks - 1) / blocks;
+  const long full = waves == 8 && a.hd > 64 ? 256 : 512, want = (full + blocks - 1) / blocks;
   g.ns = (int)(want < tiles ? want : tiles);
   g.units = (int)(units * g.ns);
   return g;
@@ -548,9 +583,9 @@ template <int HD>
 hipError_t launch_tree(const TreeAttnArgs &a, hipStream_t st) {
   const TreeGrid g = tree_grid(a);
   const dim3 grid((g.units + 7) / 8 * 8 * g.rb);
-  const uint32_t lds = 4 * kTp * HD * 2;
-  if (tree_rt(a) == 1) klaunch((attn_tree_kernel<HD, 1>), grid, dim3(256), lds, st, a, g);
-  else klaunch((attn_tree_kernel<HD, 2>), grid, dim3(256), lds, st, a, g);
+  const uint32_t lds = 2 * 4 * kTp * HD;
+  if (tree_waves(a) == 4) klaunch((attn_tree_kernel<HD, 4, HD <= 64 ? 4 : 2>), grid, dim3(256), lds, st, a, g);
+  else klaunch((attn_tree_kernel<HD, 8, HD <= 64 ? 4 : 2>), grid, dim3(512), lds, st, a, g);
   if (g.ns > 1) {
     constexpr int rpb = 256 / (HD == 96 ? 32 : HD / 4);
     klaunch((attn_tree_join_kernel<HD>), dim3((a.t.N * a.H + rpb - 1) / rpb, a.t.B), dim3(256), 0, st, a, g.ns);
