@@ -481,7 +481,8 @@ struct SampleArgs {
   int *token;
   float *prob;
 };
-hipError_t sample_rows(const SampleArgs &a, hipStream_t st);
+size_t sample_workspace(int rows, int V);  // bytes of ws
+hipError_t sample_rows(const SampleArgs &a, void *ws, hipStream_t st);
 
 // rows of drafted tokens (tree_rows.hip, attn_tree.hip): ec_tree.h's batch
 struct NormRopeArgs {

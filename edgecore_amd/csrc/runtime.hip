@@ -453,7 +453,7 @@ struct W16Buf {
   void *retired[64] = {};
   int nretired = 0;
 };
-static W16Buf g_w16_parts, g_w16_rs, g_tree_ws;
+static W16Buf g_w16_parts, g_w16_rs, g_tree_ws, g_sample_ws;
 
 static int w16_grow(W16Buf &b, size_t bytes, const char *fn = "gemm") {
   if (bytes <= b.n) return 0;
@@ -2390,7 +2390,8 @@ extern "C" int ec_sample_dev(const float *logits, int rows, int vocab, int ld, c
   if (!logits || !u || !token) return set_err(-1, "ec_sample_dev: null pointer");
   EC_INIT();
   const SampleArgs a{logits, rows, vocab, ld, temp, top_k, top_p, min_p, u, token, prob};
-  EC_LAUNCH("sample", 4.0 * rows * vocab, sample_rows(a, g_stream));
+  if (const int r = w16_grow(g_sample_ws, sample_workspace(rows, vocab), "ec_sample_dev")) return r;
+  EC_LAUNCH("sample", 4.0 * rows * vocab, sample_rows(a, g_sample_ws.p, g_stream));
   return 0;
 }
 
@@ -2498,7 +2499,7 @@ extern "C" int ec_release(void) {
     if (g_kept_host.p) EC_HIP(hipHostFree(g_kept_host.p));
     g_kept_dev = g_kept_host = Staging{};
   }
-  for (W16Buf *b : {&g_w16_parts, &g_w16_rs, &g_tree_ws}) {
+  for (W16Buf *b : {&g_w16_parts, &g_w16_rs, &g_tree_ws, &g_sample_ws}) {
     if (b->p) EC_HIP(hipFree(b->p));
     for (int i = 0; i < b->nretired; i++) EC_HIP(hipFree(b->retired[i]));
     *b = W16Buf{};

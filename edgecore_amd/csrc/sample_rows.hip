@@ -10,14 +10,26 @@
 // T not above 0: the largest logit.  NaN counts as -inf, -inf is never drawn, a
 // row of nothing else gives -1.
 //
-// Nothing is sorted.  A place in the order is a border (Border below): the keys
-// above a key, and the first of those that equal it.  It is found by fixing the
-// key's bits from the top, 8 at a time, from a histogram of counts or of sums
-// over the elements that agree in the bits so far.  Sums are of w in steps of
-// 2^-44 in 64-bit integers: the order of the additions does not change them, so
-// a row gives the same token every time (2^18 tokens of w = 1 stay below 2^62;
-// a sum of 150000 is off by about 2^-27 of one token's largest weight at the
-// very most, by 2^-36 where the roundings fall at random).
+// Sums are of w in steps of 2^-44 in 64-bit integers: the order of the additions
+// does not change them, so a row gives the same token every time (2^18 tokens of
+// w = 1 stay below 2^62; a sum of 150000 is off by about 2^-27 of one token's
+// largest weight at the very most, by 2^-36 where the roundings fall at random).
+//
+// Nothing is sorted.  A place in the order is a border: the keys above a key, and
+// the first of those that equal it (Border).  Three launches:
+//
+//   sample_top_kernel: per chunk of 4096 logits the largest (with its index) and
+//     the smallest;
+//   sample_bins_kernel: per chunk the logits by value into 512 bins between the
+//     row's largest and smallest (or 32 T below, where w rounds to 0): their
+//     number and sum of w per bin, keys and indices in the bins' order;
+//   sample_pick_kernel: a block per row adds the chunks' bins up and finds the
+//     bin of each border; that bin's elements come from their chunks into LDS,
+//     where the border is found by fixing the key's bits from the top, 8 at a
+//     time, from a histogram of those that agree so far.
+//
+// A bin of more than kCap elements (equal logits mostly) is searched by the same
+// steps over the whole row.
 #include "ec_device.h"
 #include "ec_kernels.h"
 
@@ -28,6 +40,10 @@ namespace {
 typedef unsigned long long u64;
 
 constexpr double kOne = 17592186044416.0;  // 2^44: w = 1
+constexpr int kChunk = 4096, kBins = 512, kCap = 4096, kBinThreads = 512;
+constexpr int kMaxChunks = (1 << 18) / kChunk;  // one per lane of a wave
+static_assert(kMaxChunks <= 64 && kChunk <= 65535, "chunks per lane, counts in 16 bits");
+constexpr double kNats = 32.0;  // e^-32 is 0 in steps of 2^-44
 
 // an order-preserving image of the logit; NaN as -inf, -0 as +0
 __device__ __forceinline__ uint32_t key_of(float v) {
@@ -48,186 +64,570 @@ __device__ __forceinline__ u64 weight(uint32_t key, uint32_t top, double inv_t) 
   return (u64)__double2ll_rn(exp(x) * kOne);
 }
 
-// The elements before a place in the order: those with a key above `key`, and
-// the first `ties` of the `equal` ones that have it; `sum`: the weights of the
-// keys above.
-struct Border {
-  uint32_t key;
-  int ties, above;
-  u64 sum;
+// A row's bins: number (max - l) * per of the 512, the last one open.
+struct Bins {
+  uint32_t top;
+  double max, per;
 };
-
-struct RowBlock {
-  u64 hist[256];
-  int count[256];
-  u64 scan_sum;
-  int scan_bin, scan_count, found;
-};
-
-// The border of the place where the running count reaches `want` elements
-// (BY_SUM false), or where the running sum passes `target` (true), within the
-// elements before `lim`.  Every thread of the block calls it.
-template <bool BY_SUM>
-__device__ Border find_border(RowBlock &s, const float *l, int V, uint32_t top, double inv_t, int want, double target,
-                              const Border &lim) {
-  uint32_t prefix = 0;
-  u64 sum = 0;
-  int cnt = 0, equal = 0;
-  const int t = threadIdx.x;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (t < 256) {
-      s.hist[t] = 0;
-      s.count[t] = 0;
-    }
-    __syncthreads();
-    for (int i = t; i < V; i += 1024) {
-      const uint32_t k = key_of(l[i]);
-      if (k < lim.key || (k == lim.key && !lim.ties) || (shift < 24 && (k >> (shift + 8)) != prefix)) continue;
-      const int bin = (k >> shift) & 255;
-      atomicAdd(&s.count[bin], 1);
-      atomicAdd(&s.hist[bin], weight(k, top, inv_t));
-    }
-    __syncthreads();
-    if (t == 0) {
-      int bin = 255, c = cnt, last = -1;
-      u64 w = sum;
-      int at_c = cnt;
-      u64 at_w = sum;
-      for (; bin >= 0; bin--) {
-        if (BY_SUM ? s.hist[bin] != 0 : s.count[bin] != 0) {
-          last = bin;
-          at_c = c;
-          at_w = w;
-          c += s.count[bin];
-          w += s.hist[bin];
-          if (BY_SUM ? (double)w > target : c >= want) break;
-        }
-      }
-      // never passed: the last element
-      s.scan_bin = last;
-      s.scan_count = at_c;
-      s.scan_sum = at_w;
-      s.found = last < 0 ? 0 : s.count[last];
-    }
-    __syncthreads();
-    prefix = (prefix << 8) | (uint32_t)s.scan_bin;
-    cnt = s.scan_count;
-    sum = s.scan_sum;
-    equal = s.found;
-    __syncthreads();
-  }
-  if (prefix == lim.key) equal = min(equal, lim.ties);
-  Border b;
-  b.key = prefix;
-  b.above = cnt;
-  b.sum = sum;
-  if (!BY_SUM) {
-    b.ties = min(equal, want - cnt);
-  } else {
-    const u64 w = weight(prefix, top, inv_t);
-    const double r = w ? floor((target - (double)sum) / (double)w) : (double)equal;
-    b.ties = r < 0.0 ? 0 : r < (double)equal ? (int)r : equal - 1;  // elements of this key before the one that passes
-  }
+__device__ __forceinline__ Bins bins_of(uint32_t top, uint32_t low, double T) {
+  Bins b;
+  b.top = top;
+  b.max = (double)key_value(top);
+  const double span = fmin(b.max - (double)key_value(low), kNats * T);
+  b.per = span > 0.0 ? kBins / span : 0.0;
   return b;
 }
+__device__ __forceinline__ int bin_of(const Bins &b, uint32_t key) {
+  if (b.top == kPosInf) return key == b.top ? 0 : kBins - 1;
+  const double x = (b.max - (double)key_value(key)) * b.per;
+  return x < (double)(kBins - 1) ? (int)x : kBins - 1;
+}
 
-__global__ __launch_bounds__(1024) void sample_rows_kernel(SampleArgs a) {
-  __shared__ RowBlock s;
-  __shared__ uint32_t s_max[16];
-  __shared__ u64 s_sum[16];
-  __shared__ int s_cnt[16], s_token;
-  const int t = threadIdx.x, lane = t & 63, w = t >> 6, row = blockIdx.x;
-  const float *l = a.logits + (size_t)row * a.ld;
-  uint32_t mx = 0;
-  for (int i = t; i < a.V; i += 1024) mx = max(mx, key_of(l[i]));
-  for (int o = 32; o > 0; o >>= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, o, 64));
-  if (lane == 0) s_max[w] = mx;
-  __syncthreads();
-  uint32_t top = s_max[0];
-  for (int j = 1; j < 16; j++) top = max(top, s_max[j]);
-  const float T = a.temp ? a.temp[row] : 1.0f;
-  const bool none = top == kNegInf, greedy = !(T > 0.0f);
-  Border at{top, 0, 0, 0};
-  double p = 1.0;
-  if (!none && !greedy) {
-    const double inv_t = 1.0 / (double)T;
-    // what stays: at first all but -inf
-    Border keep{kNegInf, 0, 0, 0};
-    const int k = a.top_k ? a.top_k[row] : 0;
-    if (k > 0 && k < a.V) keep = find_border<false>(s, l, a.V, top, inv_t, k, 0.0, keep);
-    auto sum_of = [&](const Border &b) {
-      u64 sum = 0;
-      for (int i = t; i < a.V; i += 1024) {
-        const uint32_t key = key_of(l[i]);
-        if (key > b.key) sum += weight(key, top, inv_t);
-      }
-      for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-      __syncthreads();
-      if (lane == 0) s_sum[w] = sum;
-      __syncthreads();
-      sum = 0;
-      for (int j = 0; j < 16; j++) sum += s_sum[j];
-      return sum + (u64)b.ties * weight(b.key, top, inv_t);
-    };
-    u64 total = sum_of(keep);
-    const float tp = a.top_p ? a.top_p[row] : 1.0f, mp = a.min_p ? a.min_p[row] : 0.0f;
-    if (tp < 1.0f) {
-      // the element at which the sum reaches top_p of it is the last one that stays
-      const double target = (double)tp * (double)total;
-      // of the elements up to the one that passes the target that one stays too, if it starts below it
-      keep = find_border<true>(s, l, a.V, top, inv_t, 0, target, keep);
-      const u64 wb = weight(keep.key, top, inv_t);
-      if ((double)(keep.sum + (u64)keep.ties * wb) < target || keep.ties + keep.above == 0) keep.ties++;
-      total = sum_of(keep);
-    }
-    if (mp > 0.0f) {
-      // the smallest key whose weight reaches min_p, by its bits
-      uint32_t thr = 0;
-      for (int bit = 31; bit >= 0; bit--) {
-        const uint32_t c = thr | ((1u << bit) - 1u);  // the largest key with this bit clear
-        double x = ((double)key_value(c) - (double)key_value(top)) * inv_t;
-        const bool reaches = c >= top || (c > kNegInf && exp(x) >= (double)mp);  // min_p above 1: the largest alone
-        if (!reaches) thr |= 1u << bit;
-      }
-      thr = min(thr, top);
-      if (thr > keep.key) {
-        keep = Border{thr - 1, 0, 0, 0};
-        total = sum_of(keep);
-      }
-    }
-    at = find_border<true>(s, l, a.V, top, inv_t, 0, a.u[row] * (double)total, keep);
-    p = (double)weight(at.key, top, inv_t) / (double)total;
+// scratch of a batch of rows, in bytes (each part a multiple of 16)
+struct Scratch {
+  u64 *top;        // [rows][chunks] key << 32 | ~index of the largest
+  uint32_t *low;   // [rows][chunks] key of the smallest above -inf
+  u64 *sum;        // [rows][chunks][kBins]
+  uint16_t *start; // [rows][chunks][kBins]: a bin's first place in the chunk's order
+  uint16_t *count; // [rows][chunks][kBins]
+  uint32_t *key;   // [rows][chunks][kChunk] in the bins' order
+  uint16_t *at;    // [rows][chunks][kChunk]: index within the chunk
+};
+size_t scratch_row(int nb) {
+  return (size_t)nb * (16 + kBins * (8 + 2 + 2) + kChunk * (4 + 2));
+}
+Scratch scratch_of(void *p, int rows, int nb) {
+  const size_t n = (size_t)rows * nb;
+  Scratch s;
+  char *c = (char *)p;
+  s.sum = (u64 *)c, c += n * kBins * 8;
+  s.top = (u64 *)c, c += n * 8;
+  s.low = (uint32_t *)c, c += n * 8;
+  s.key = (uint32_t *)c, c += n * kChunk * 4;
+  s.start = (uint16_t *)c, c += n * kBins * 2;
+  s.count = (uint16_t *)c, c += n * kBins * 2;
+  s.at = (uint16_t *)c;
+  return s;
+}
+
+__device__ __forceinline__ u64 wave_max64(u64 v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const u64 x = __shfl_xor(v, o, 64);
+    v = x > v ? x : v;
   }
-  // the element number at.ties of those that have the key, by index
-  int left = at.ties;
-  if (t == 0) s_token = -1;
-  for (int i0 = 0; i0 < a.V; i0 += 1024) {
-    const int i = i0 + t;
-    const bool hit = i < a.V && key_of(l[i]) == at.key;
-    const uint64_t m = __ballot(hit);
-    __syncthreads();
-    if (lane == 0) s_cnt[w] = __popcll(m);
-    __syncthreads();
-    int before = 0, all = 0;
-    for (int j = 0; j < 16; j++) {
-      if (j < w) before += s_cnt[j];
-      all += s_cnt[j];
-    }
-    if (hit && before + __popcll(m & ((1ull << lane) - 1)) == left) s_token = i;
-    if (left < all) break;
-    left -= all;
+  return v;
+}
+__device__ __forceinline__ uint32_t wave_min32(uint32_t v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = min(v, (uint32_t)__shfl_xor((int)v, o, 64));
+  return v;
+}
+
+__global__ __launch_bounds__(256) void sample_top_kernel(SampleArgs a, Scratch s, int row0) {
+  __shared__ u64 s_top[4];
+  __shared__ uint32_t s_low[4];
+  const int t = threadIdx.x, c0 = blockIdx.x * kChunk, nb = gridDim.x;
+  const float *l = a.logits + (size_t)(row0 + blockIdx.y) * a.ld;
+  u64 top = 0;
+  uint32_t low = ~0u;
+  float v[kChunk / 256];
+#pragma unroll
+  for (int j = 0; j < kChunk / 256; j++) v[j] = l[min(c0 + t + 256 * j, a.V - 1)];
+#pragma unroll
+  for (int j = 0; j < kChunk / 256; j++) {
+    const int i = min(c0 + t + 256 * j, a.V - 1);
+    const uint32_t k = key_of(v[j]);
+    const u64 e = ((u64)k << 32) | (uint32_t)~i;
+    top = e > top ? e : top;
+    if (k > kNegInf) low = min(low, k);
+  }
+  top = wave_max64(top);
+  low = wave_min32(low);
+  if ((t & 63) == 0) {
+    s_top[t >> 6] = top;
+    s_low[t >> 6] = low;
   }
   __syncthreads();
   if (t == 0) {
-    a.token[row] = none ? -1 : s_token;
-    if (a.prob) a.prob[row] = none ? 0.0f : (float)p;
+    for (int i = 1; i < 4; i++) {
+      top = s_top[i] > top ? s_top[i] : top;
+      low = min(low, s_low[i]);
+    }
+    s.top[(size_t)blockIdx.y * nb + blockIdx.x] = top;
+    s.low[(size_t)blockIdx.y * nb + blockIdx.x] = low;
   }
 }
 
+// the row's largest (key << 32 | ~index) and smallest, by every wave
+__device__ __forceinline__ void row_ends(const Scratch &s, int row, int nb, u64 *top, uint32_t *low) {
+  const int lane = threadIdx.x & 63;
+  const size_t at = (size_t)row * nb + min(lane, nb - 1);
+  *top = wave_max64(s.top[at]);
+  *low = wave_min32(s.low[at]);
+}
+
+__device__ __forceinline__ float temp_of(const SampleArgs &a, int row) { return a.temp ? a.temp[row] : 1.0f; }
+
+// exclusive sum over the wave's lanes; *all: over all of them
+__device__ __forceinline__ int wave_scan(int v, int *all) {
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(x, o, 64);
+    if ((int)(threadIdx.x & 63) >= o) x += y;
+  }
+  *all = __shfl(x, 63, 64);
+  return x - v;
+}
+__device__ __forceinline__ u64 wave_scan64(u64 v) {  // inclusive
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const u64 y = __shfl_up(v, o, 64);
+    if ((int)(threadIdx.x & 63) >= o) v += y;
+  }
+  return v;
+}
+
+__global__ __launch_bounds__(kBinThreads) void sample_bins_kernel(SampleArgs a, Scratch s, int row0) {
+  constexpr int PT = kChunk / kBinThreads;
+  __shared__ u64 s_sum[kBins];
+  __shared__ int s_cnt[kBins], s_at[kBins], s_wave[kBinThreads / 64];
+  __shared__ uint32_t s_key[kChunk];
+  __shared__ uint16_t s_idx[kChunk];
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6, row = blockIdx.y, c0 = blockIdx.x * kChunk, nb = gridDim.x;
+  const float *l = a.logits + (size_t)(row0 + row) * a.ld;
+  float v[PT];
+#pragma unroll
+  for (int j = 0; j < PT; j++) v[j] = l[min(c0 + t + kBinThreads * j, a.V - 1)];
+  const float T = temp_of(a, row0 + row);
+  u64 top;
+  uint32_t low;
+  row_ends(s, row, nb, &top, &low);
+  const uint32_t tk = (uint32_t)(top >> 32);
+  if (!(T > 0.0f) || tk == kNegInf) return;  // the largest logit, or none: nothing to weigh
+  const double inv_t = 1.0 / (double)T;
+  const Bins bins = bins_of(tk, low, (double)T);
+  s_sum[t] = 0;
+  s_cnt[t] = 0;
+  __syncthreads();
+  uint32_t key[PT];
+  int bin[PT], place[PT];
+#pragma unroll
+  for (int j = 0; j < PT; j++) {
+    key[j] = key_of(v[j]);
+    bin[j] = -1;
+    if (c0 + t + kBinThreads * j < a.V && key[j] > kNegInf) {
+      bin[j] = bin_of(bins, key[j]);
+      place[j] = atomicAdd(&s_cnt[bin[j]], 1);
+      const u64 x = weight(key[j], tk, inv_t);
+      if (x) atomicAdd(&s_sum[bin[j]], x);
+    }
+  }
+  __syncthreads();
+  static_assert(kBins == kBinThreads, "a bin per thread");
+  int all;
+  const int mine = s_cnt[t];
+  const int before = wave_scan(mine, &all);
+  if (lane == 0) s_wave[w] = all;
+  __syncthreads();
+  int first = before, total = 0;
+  for (int i = 0; i < kBinThreads / 64; i++) {
+    if (i < w) first += s_wave[i];
+    total += s_wave[i];
+  }
+  s_at[t] = first;
+  const size_t ch = (size_t)row * nb + blockIdx.x;
+  s.sum[ch * kBins + t] = s_sum[t];
+  s.start[ch * kBins + t] = (uint16_t)first;
+  s.count[ch * kBins + t] = (uint16_t)mine;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < PT; j++)
+    if (bin[j] >= 0) {
+      const int p = s_at[bin[j]] + place[j];
+      s_key[p] = key[j];
+      s_idx[p] = (uint16_t)(t + kBinThreads * j);
+    }
+  __syncthreads();
+  for (int i = t; i < total; i += kBinThreads) {
+    s.key[ch * kChunk + i] = s_key[i];
+    s.at[ch * kChunk + i] = s_idx[i];
+  }
+}
+
+// A place in the order: behind the elements with a key above `key` (their number,
+// the sum of their weights) and the first `ties` of the `equal` that have it.
+struct Border {
+  uint32_t key;
+  int equal, above;
+  u64 sum;
+  int ties;
+};
+
+struct Pick {
+  // bins of the whole row: number and sum of those before a bin
+  int cnt[kBins + 1];
+  u64 sum[kBins + 1];
+  // the elements of one bin
+  uint32_t key[kCap], idx[kCap];
+  u64 w[kCap];
+  int seg[kMaxChunks];
+  // a step's histogram, and what it found
+  int hc[256];
+  u64 hw[256];
+  int found, found_cnt, found_equal;
+  u64 found_sum;
+  int wave_c[16];
+  u64 wave_w[16];
+  uint32_t differ;
+};
+
+// One row's elements and what is known of them.
+struct Row {
+  const float *l;
+  const Scratch *s;
+  size_t ch0;  // the row's first chunk in the scratch
+  int V, nb;
+  uint32_t top;
+  double inv_t;
+  Bins bins;
+  int loaded, n;  // the bin in LDS (-1: none) and its elements
+};
+
+// loads bin b's elements, in the order of their chunks; false where they are too many
+__device__ bool load_bin(Pick &k, Row &r, int b) {
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
+  const int n = k.cnt[b + 1] - k.cnt[b];
+  if (n > kCap) return false;
+  if (r.loaded == b) return true;
+  __syncthreads();
+  if (w == 0) {
+    int all;
+    const int c = lane < r.nb ? r.s->count[(r.ch0 + lane) * kBins + b] : 0;
+    k.seg[lane] = wave_scan(c, &all);
+  }
+  if (t == 0) k.differ = 0;
+  __syncthreads();
+  for (int c = w; c < r.nb; c += 16) {
+    const size_t ch = r.ch0 + c;
+    const int first = r.s->start[ch * kBins + b], to = k.seg[c];
+    const int m = (c + 1 < r.nb ? k.seg[c + 1] : n) - to;
+    for (int i = lane; i < m; i += 64) {
+      const uint32_t key = r.s->key[ch * kChunk + first + i];
+      k.key[to + i] = key;
+      k.idx[to + i] = (uint32_t)(c * kChunk + r.s->at[ch * kChunk + first + i]);
+      k.w[to + i] = weight(key, r.top, r.inv_t);
+    }
+  }
+  __syncthreads();
+  uint32_t d = 0;
+  for (int i = t; i < n; i += 1024) d |= k.key[i] ^ k.key[0];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) d |= (uint32_t)__shfl_xor((int)d, o, 64);
+  if (lane == 0 && d) atomicOr(&k.differ, d);
+  __syncthreads();
+  r.loaded = b;
+  r.n = n;
+  return true;
+}
+
+// Fixes the bits of a key below `bits`, 8 at a time, until the element is found at
+// which the running count reaches want (BY_SUM false) or the running sum passes
+// target, over the elements that each(f) hands to f(key, weight) and whose upper
+// bits are prefix's.  cnt, sum: what comes before them all.
+template <bool BY_SUM, class Each>
+__device__ Border fix_bits(Pick &k, const Each &each, uint32_t prefix, int bits, int cnt, u64 sum, int want, u64 target) {
+  const int t = threadIdx.x, lane = t & 63;
+  int equal = 0;
+  while (bits > 0) {
+    const int take = bits < 8 ? bits : 8, shift = bits - take;
+    __syncthreads();
+    if (t < 256) {
+      k.hc[t] = 0;
+      k.hw[t] = 0;
+    }
+    __syncthreads();
+    each([&](uint32_t key, u64 w) {
+      if (bits < 32 && (key >> bits) != prefix) return;
+      const int bin = (key >> shift) & ((1 << take) - 1);
+      atomicAdd(&k.hc[bin], 1);
+      if (w) atomicAdd(&k.hw[bin], w);
+    });
+    __syncthreads();
+    if (t < 64) {
+      // four bins a lane, the largest first
+      int c[4], call = 0;
+      u64 w[4], wall = 0;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        c[j] = k.hc[255 - 4 * lane - j];
+        w[j] = k.hw[255 - 4 * lane - j];
+        call += c[j];
+        wall += w[j];
+      }
+      int all;
+      int cb = cnt + wave_scan(call, &all);
+      u64 wb = sum + wave_scan64(wall) - wall;
+      int hit = -1, hc = 0, he = 0;
+      u64 hw = 0;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        if (hit < 0 && (BY_SUM ? wb + w[j] > target : cb + c[j] >= want)) hit = 255 - 4 * lane - j, hc = cb, hw = wb, he = c[j];
+        cb += c[j];
+        wb += w[j];
+      }
+      const uint64_t m = __ballot(hit >= 0);
+      if (m && lane == __ffsll((unsigned long long)m) - 1) {
+        k.found = hit;
+        k.found_cnt = hc;
+        k.found_sum = hw;
+        k.found_equal = he;
+      }
+    }
+    __syncthreads();
+    prefix = (prefix << take) | (uint32_t)k.found;
+    cnt = k.found_cnt;
+    sum = k.found_sum;
+    equal = k.found_equal;
+    bits = shift;
+  }
+  return Border{prefix, equal, cnt, sum, 0};
+}
+
+// The element at which the running count of the row reaches want, or its running
+// sum passes target (there is one): its key, what comes before that key, and in
+// `ties` the elements of the key before this one.
+template <bool BY_SUM>
+__device__ Border find_border(Pick &k, Row &r, int want, u64 target) {
+  const int t = threadIdx.x;
+  __syncthreads();
+  if (t < kBins) {
+    const bool hit = BY_SUM ? k.sum[t] <= target && k.sum[t + 1] > target : k.cnt[t] < want && k.cnt[t + 1] >= want;
+    if (hit) k.found = t;
+  }
+  __syncthreads();
+  const int b = k.found;
+  Border at;
+  if (load_bin(k, r, b)) {
+    const int bits = k.differ ? 32 - __clz(k.differ) : 0;
+    if (bits == 0) {
+      at = Border{k.key[0], r.n, k.cnt[b], k.sum[b], 0};
+    } else {
+      at = fix_bits<BY_SUM>(
+          k,
+          [&](auto f) {
+            for (int i = t; i < r.n; i += 1024) f(k.key[i], k.w[i]);
+          },
+          bits < 32 ? k.key[0] >> bits : 0, bits, k.cnt[b], k.sum[b], want, target);
+    }
+  } else {
+    at = fix_bits<BY_SUM>(
+        k,
+        [&](auto f) {
+          for (int i = t; i < r.V; i += 1024) {
+            const uint32_t key = key_of(r.l[i]);
+            if (key > kNegInf && bin_of(r.bins, key) == b) f(key, weight(key, r.top, r.inv_t));
+          }
+        },
+        0, 32, k.cnt[b], k.sum[b], want, target);
+  }
+  // of the elements with the key
+  if (!BY_SUM) {
+    at.ties = want - at.above - 1;
+  } else {
+    const u64 w = weight(at.key, r.top, r.inv_t);
+    const u64 before = w ? (target - at.sum) / w : 0;
+    at.ties = before < (u64)at.equal ? (int)before : at.equal - 1;
+  }
+  return at;
+}
+
+// the smallest key whose weight reaches min_p (at most the largest one's)
+__device__ uint32_t least_key(uint32_t top, double inv_t, double min_p) {
+  const double max = (double)key_value(top);
+  auto reaches = [&](uint32_t c) {
+    return c >= top || (c > kNegInf && top != kPosInf && exp(((double)key_value(c) - max) * inv_t) >= min_p);
+  };
+  // near max + T log min_p: 64 keys at a time
+  const int lane = threadIdx.x & 63;
+  const float guess = (float)(max + log(min_p) / inv_t);
+  const uint32_t g = key_of(guess);
+  if (g > kNegInf + 64 && g < top) {
+    const uint64_t m = __ballot(reaches(g - 32 + lane));
+    if (m && !(m & 1)) return g - 32 + (uint32_t)__ffsll((unsigned long long)m) - 1;
+  }
+  uint32_t thr = 0;
+  for (int bit = 31; bit >= 0; bit--)
+    if (!reaches(thr | ((1u << bit) - 1u))) thr |= 1u << bit;
+  return thr;
+}
+
+__global__ __launch_bounds__(1024) void sample_pick_kernel(SampleArgs a, Scratch s, int row0, int nb) {
+  __shared__ Pick k;
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6, row = row0 + blockIdx.x;
+  u64 top;
+  uint32_t low;
+  row_ends(s, blockIdx.x, nb, &top, &low);
+  Row r;
+  r.top = (uint32_t)(top >> 32);
+  const float T = temp_of(a, row);
+  if (r.top == kNegInf || !(T > 0.0f)) {
+    if (t == 0) {
+      const bool none = r.top == kNegInf;
+      a.token[row] = none ? -1 : (int)~(uint32_t)top;
+      if (a.prob) a.prob[row] = none ? 0.0f : 1.0f;
+    }
+    return;
+  }
+  r.l = a.logits + (size_t)row * a.ld;
+  r.s = &s;
+  r.ch0 = (size_t)blockIdx.x * nb;
+  r.V = a.V;
+  r.nb = nb;
+  r.inv_t = 1.0 / (double)T;
+  r.bins = bins_of(r.top, low, (double)T);
+  r.loaded = -1;
+  r.n = 0;
+  const int top_k = a.top_k ? a.top_k[row] : 0;
+  const float top_p = a.top_p ? a.top_p[row] : 1.0f, min_p = a.min_p ? a.min_p[row] : 0.0f;
+  const double u = a.u[row];
+
+  // the chunks' bins, added up: half of the chunks per thread
+  {
+    const int b = t & (kBins - 1);
+    u64 sum = 0;
+    int cnt = 0;
+#pragma unroll 8
+    for (int c = t / kBins; c < nb; c += 1024 / kBins) {
+      sum += s.sum[(r.ch0 + c) * kBins + b];
+      cnt += s.count[(r.ch0 + c) * kBins + b];
+    }
+    static_assert(kBins == 512, "two threads a bin");
+    if (t >= kBins) {
+      k.sum[b] = sum;
+      k.cnt[b] = cnt;
+    }
+    __syncthreads();
+    if (t < kBins) {
+      sum += k.sum[b];
+      cnt += k.cnt[b];
+    }
+    int call;
+    const int cb = wave_scan(cnt, &call);
+    const u64 wi = wave_scan64(sum);
+    if (lane == 63) {
+      k.wave_c[w] = call;
+      k.wave_w[w] = wi;
+    }
+    __syncthreads();
+    if (t < kBins) {
+      int c = cb + cnt;
+      u64 x = wi;
+      for (int i = 0; i < w; i++) {
+        c += k.wave_c[i];
+        x += k.wave_w[i];
+      }
+      k.cnt[b + 1] = c;
+      k.sum[b + 1] = x;
+      if (t == 0) k.cnt[0] = 0, k.sum[0] = 0;
+    }
+    __syncthreads();
+  }
+  const int live = k.cnt[kBins];  // above -inf
+  u64 total = k.sum[kBins];
+  // the sum of those that stay and, where some do not, the border
+  if (top_k > 0 && top_k < live) {
+    const Border b = find_border<false>(k, r, top_k, 0);
+    total = b.sum + (u64)(b.ties + 1) * weight(b.key, r.top, r.inv_t);
+  }
+  if (top_p < 1.0f) {
+    // up to the element at which the sum reaches top_p of it: passes ceil(top_p sum) - 1
+    const double x = ceil((double)top_p * (double)total) - 1.0;
+    u64 target = x > 0.0 ? (u64)x : 0;
+    if (target >= total) target = total - 1;
+    const Border b = find_border<true>(k, r, 0, target);
+    total = b.sum + (u64)(b.ties + 1) * weight(b.key, r.top, r.inv_t);
+  }
+  if (min_p > 0.0f) {
+    // those from the least key on, as far as they are among those that stay
+    const uint32_t thr = least_key(r.top, r.inv_t, (double)min_p);
+    const int b = bin_of(r.bins, thr);
+    u64 sum = 0;
+    if (load_bin(k, r, b)) {
+      for (int i = t; i < r.n; i += 1024)
+        if (k.key[i] >= thr) sum += k.w[i];
+    } else {
+      for (int i = t; i < r.V; i += 1024) {
+        const uint32_t key = key_of(r.l[i]);
+        if (key >= thr && bin_of(r.bins, key) == b) sum += weight(key, r.top, r.inv_t);
+      }
+    }
+    sum = wave_scan64(sum);
+    __syncthreads();
+    if (lane == 63) k.wave_w[w] = sum;
+    __syncthreads();
+    sum = k.sum[b];
+    for (int i = 0; i < 16; i++) sum += k.wave_w[i];
+    total = sum < total ? sum : total;
+  }
+  // the draw: running sum above u total
+  const double x = u * (double)total;
+  u64 target = x > 0.0 ? x < (double)total ? (u64)x : total - 1 : u == u ? 0 : total - 1;
+  if (target >= total) target = total - 1;
+  const Border at = find_border<true>(k, r, 0, target);
+  // of the elements that have the key, number at.ties by index: the largest
+  // complement of the index but for so many
+  const bool listed = r.loaded >= 0 && bin_of(r.bins, at.key) == r.loaded;
+  int token = 0;
+  if (listed && at.equal == 1) {
+    __syncthreads();
+    for (int i = t; i < r.n; i += 1024)
+      if (k.key[i] == at.key) k.found = (int)k.idx[i];
+    __syncthreads();
+    token = k.found;
+  } else {
+    constexpr int kIdxBits = 18;
+    constexpr uint32_t kIdx = (1u << kIdxBits) - 1;
+    static_assert(kMaxChunks * kChunk <= 1 << kIdxBits, "an index's bits");
+    const Border i = fix_bits<false>(
+        k,
+        [&](auto f) {
+          if (listed) {
+            for (int j = t; j < r.n; j += 1024)
+              if (k.key[j] == at.key) f(~k.idx[j] & kIdx, 0);
+          } else {
+            for (int j = t; j < r.V; j += 1024)
+              if (key_of(r.l[j]) == at.key) f(~(uint32_t)j & kIdx, 0);
+          }
+        },
+        0, kIdxBits, 0, 0, at.ties + 1, 0);
+    token = (int)(~i.key & kIdx);
+  }
+  if (t == 0) {
+    a.token[row] = token;
+    if (a.prob) a.prob[row] = (float)((double)weight(at.key, r.top, r.inv_t) / (double)total);
+  }
+}
+
+// rows per batch: enough chunks for every CU, a bounded scratch
+constexpr int kBatch = 64;
+
 }  // namespace
 
-hipError_t sample_rows(const SampleArgs &a, hipStream_t st) {
-  klaunch(sample_rows_kernel, dim3(a.rows), dim3(1024), 0, st, a);
+size_t sample_workspace(int rows, int V) {
+  return scratch_row((V + kChunk - 1) / kChunk) * (rows < kBatch ? rows : kBatch);
+}
+
+hipError_t sample_rows(const SampleArgs &a, void *ws, hipStream_t st) {
+  const int nb = (a.V + kChunk - 1) / kChunk;
+  for (int r0 = 0; r0 < a.rows; r0 += kBatch) {
+    const int n = a.rows - r0 < kBatch ? a.rows - r0 : kBatch;
+    const Scratch s = scratch_of(ws, n, nb);
+    klaunch(sample_top_kernel, dim3(nb, n), dim3(256), 0, st, a, s, r0);
+    klaunch(sample_bins_kernel, dim3(nb, n), dim3(kBinThreads), 0, st, a, s, r0);
+    klaunch(sample_pick_kernel, dim3(n), dim3(1024), 0, st, a, s, r0, nb);
+  }
   return hipGetLastError();
 }
 
