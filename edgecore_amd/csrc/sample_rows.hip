@@ -22,7 +22,7 @@
 //     the smallest;
 //   sample_bins_kernel: per chunk the logits by value into 512 bins between the
 //     row's largest and smallest (or 32 T below, where w rounds to 0): their
-//     number and sum of w per bin, keys and indices in the bins' order;
+//     number and sum of w per bin, and their indices in the bins' order;
 //   sample_pick_kernel: a block per row adds the chunks' bins up and finds the
 //     bin of each border; that bin's elements come from their chunks into LDS,
 //     where the border is found by fixing the key's bits from the top, 8 at a
@@ -31,6 +31,7 @@
 // A bin of more than kCap elements (equal logits mostly) is searched by the same
 // steps over the whole row.
 #include "ec_device.h"
+#include "ec_expf.h"
 #include "ec_kernels.h"
 
 namespace ec {
@@ -40,7 +41,7 @@ namespace {
 typedef unsigned long long u64;
 
 constexpr double kOne = 17592186044416.0;  // 2^44: w = 1
-constexpr int kChunk = 4096, kBins = 512, kCap = 4096, kBinThreads = 512;
+constexpr int kChunk = 4096, kBins = 512, kCap = 4096, kSorted = 256, kBinThreads = 512;
 constexpr int kMaxChunks = (1 << 18) / kChunk;  // one per lane of a wave
 static_assert(kMaxChunks <= 64 && kChunk <= 65535, "chunks per lane, counts in 16 bits");
 constexpr double kNats = 32.0;  // e^-32 is 0 in steps of 2^-44
@@ -56,12 +57,35 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 }
 constexpr uint32_t kNegInf = 0x007FFFFFu, kPosInf = 0xFF800000u;  // key_of(-inf), key_of(inf)
 
+// e^x in steps of 2^-44, rounded to nearest, for x <= 0: x = k ln2 / 32 + r with
+// |r| <= ln2 / 64, 2^(k / 32) from the table (ec_exp2_32, a copy in LDS) and e^r by
+// its series to r^5 (r^6 / 720 is 2^-49 of it).  About 15 instructions where the
+// library's exp and conversion take 60.
+__device__ __forceinline__ u64 exp_steps(double x, const uint64_t *tab) {
+  constexpr double kInv = 46.16624130844683;                // 32 / ln2
+  constexpr double kHi = 0x1.62e42fef8p-6, kLo = 0x1.1cf79abc9e3b4p-41;  // ln2 / 32 in two parts
+  constexpr double kShift = 0x1.8p52;
+  x = fmax(x, -40.0);
+  double kd = __builtin_fma(x, kInv, kShift);
+  const uint64_t ki = __builtin_bit_cast(uint64_t, kd);
+  kd -= kShift;
+  double r = __builtin_fma(-kd, kHi, x);
+  r = __builtin_fma(-kd, kLo, r);
+  double p = __builtin_fma(r, 1.0 / 120.0, 1.0 / 24.0);
+  p = __builtin_fma(p, r, 1.0 / 6.0);
+  p = __builtin_fma(p, r, 0.5);
+  p = __builtin_fma(p, r, 1.0);
+  p = __builtin_fma(p, r, 1.0);
+  // the table's entries leave out the exponent that k's low bits add; 2^44 on top
+  const double s = __builtin_bit_cast(double, tab[ki % 32] + (ki << 47) + (44ull << 52));
+  return __builtin_bit_cast(uint64_t, __builtin_fma(s, p, kShift)) - __builtin_bit_cast(uint64_t, kShift);
+}
+
 // a logit's weight in steps of 2^-44
-__device__ __forceinline__ u64 weight(uint32_t key, uint32_t top, double inv_t) {
-  if (key == top) return (u64)kOne;
-  if (key <= kNegInf || top == kPosInf) return 0;
+__device__ __forceinline__ u64 weight(uint32_t key, uint32_t top, double inv_t, const uint64_t *tab) {
   const double x = ((double)key_value(key) - (double)key_value(top)) * inv_t;
-  return (u64)__double2ll_rn(exp(x) * kOne);
+  const u64 w = exp_steps(x, tab);
+  return key == top ? (u64)kOne : key <= kNegInf || top == kPosInf ? 0 : w;
 }
 
 // A row's bins: number (max - l) * per of the 512, the last one open.
@@ -83,29 +107,25 @@ __device__ __forceinline__ int bin_of(const Bins &b, uint32_t key) {
   return x < (double)(kBins - 1) ? (int)x : kBins - 1;
 }
 
-// scratch of a batch of rows, in bytes (each part a multiple of 16)
+// scratch of a batch of rows
 struct Scratch {
-  u64 *top;        // [rows][chunks] key << 32 | ~index of the largest
-  uint32_t *low;   // [rows][chunks] key of the smallest above -inf
-  u64 *sum;        // [rows][chunks][kBins]
-  uint16_t *start; // [rows][chunks][kBins]: a bin's first place in the chunk's order
-  uint16_t *count; // [rows][chunks][kBins]
-  uint32_t *key;   // [rows][chunks][kChunk] in the bins' order
-  uint16_t *at;    // [rows][chunks][kChunk]: index within the chunk
+  u64 *sum;         // [rows][chunks][kBins]
+  u64 *top;         // [rows][chunks] key << 32 | ~index of the largest
+  uint32_t *low;    // [rows][chunks] key of the smallest above -inf
+  uint32_t *live;   // [rows][chunks] elements above -inf
+  uint16_t *start;  // [rows][chunks][kBins]: a bin's first place in the chunk's order
+  uint16_t *at;     // [rows][chunks][kChunk]: indices within the chunk in the bins' order
 };
-size_t scratch_row(int nb) {
-  return (size_t)nb * (16 + kBins * (8 + 2 + 2) + kChunk * (4 + 2));
-}
+size_t scratch_row(int nb) { return (size_t)nb * (8 + 4 + 4 + kBins * (8 + 2) + kChunk * 2); }
 Scratch scratch_of(void *p, int rows, int nb) {
   const size_t n = (size_t)rows * nb;
   Scratch s;
   char *c = (char *)p;
   s.sum = (u64 *)c, c += n * kBins * 8;
   s.top = (u64 *)c, c += n * 8;
-  s.low = (uint32_t *)c, c += n * 8;
-  s.key = (uint32_t *)c, c += n * kChunk * 4;
+  s.low = (uint32_t *)c, c += n * 4;
+  s.live = (uint32_t *)c, c += n * 4;
   s.start = (uint16_t *)c, c += n * kBins * 2;
-  s.count = (uint16_t *)c, c += n * kBins * 2;
   s.at = (uint16_t *)c;
   return s;
 }
@@ -169,23 +189,24 @@ __device__ __forceinline__ void row_ends(const Scratch &s, int row, int nb, u64 
 
 __device__ __forceinline__ float temp_of(const SampleArgs &a, int row) { return a.temp ? a.temp[row] : 1.0f; }
 
-// exclusive sum over the wave's lanes; *all: over all of them
-__device__ __forceinline__ int wave_scan(int v, int *all) {
-  int x = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(x, o, 64);
-    if ((int)(threadIdx.x & 63) >= o) x += y;
-  }
-  *all = __shfl(x, 63, 64);
-  return x - v;
+// inclusive sums over the wave's lanes, by DPP: within rows of 16 (shifts of 1, 2,
+// 4 and 8), then a row's last lane into the next row, then into the upper half
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_rows(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
 }
-__device__ __forceinline__ u64 wave_scan64(u64 v) {  // inclusive
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const u64 y = __shfl_up(v, o, 64);
-    if ((int)(threadIdx.x & 63) >= o) v += y;
-  }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 dpp_rows(u64 v) {
+  return ((u64)dpp_rows<CTRL, ROWS>((uint32_t)(v >> 32)) << 32) | dpp_rows<CTRL, ROWS>((uint32_t)v);
+}
+template <class T>
+__device__ __forceinline__ T wave_scan(T v) {
+  v += dpp_rows<0x111, 0xF>(v);
+  v += dpp_rows<0x112, 0xF>(v);
+  v += dpp_rows<0x114, 0xF>(v);
+  v += dpp_rows<0x118, 0xF>(v);
+  v += dpp_rows<0x142, 0xA>(v);  // row_bcast15, rows 1 and 3
+  v += dpp_rows<0x143, 0xC>(v);  // row_bcast31, rows 2 and 3
   return v;
 }
 
@@ -193,8 +214,8 @@ __global__ __launch_bounds__(kBinThreads) void sample_bins_kernel(SampleArgs a, 
   constexpr int PT = kChunk / kBinThreads;
   __shared__ u64 s_sum[kBins];
   __shared__ int s_cnt[kBins], s_at[kBins], s_wave[kBinThreads / 64];
-  __shared__ uint32_t s_key[kChunk];
-  __shared__ uint16_t s_idx[kChunk];
+  __shared__ __attribute__((aligned(4))) uint16_t s_idx[kChunk];
+  __shared__ uint64_t s_tab[32];
   const int t = threadIdx.x, lane = t & 63, w = t >> 6, row = blockIdx.y, c0 = blockIdx.x * kChunk, nb = gridDim.x;
   const float *l = a.logits + (size_t)(row0 + row) * a.ld;
   float v[PT];
@@ -210,6 +231,7 @@ __global__ __launch_bounds__(kBinThreads) void sample_bins_kernel(SampleArgs a, 
   const Bins bins = bins_of(tk, low, (double)T);
   s_sum[t] = 0;
   s_cnt[t] = 0;
+  if (t < 32) s_tab[t] = ec_exp2_32[t];
   __syncthreads();
   uint32_t key[PT];
   int bin[PT], place[PT];
@@ -220,18 +242,16 @@ __global__ __launch_bounds__(kBinThreads) void sample_bins_kernel(SampleArgs a, 
     if (c0 + t + kBinThreads * j < a.V && key[j] > kNegInf) {
       bin[j] = bin_of(bins, key[j]);
       place[j] = atomicAdd(&s_cnt[bin[j]], 1);
-      const u64 x = weight(key[j], tk, inv_t);
+      const u64 x = weight(key[j], tk, inv_t, s_tab);
       if (x) atomicAdd(&s_sum[bin[j]], x);
     }
   }
   __syncthreads();
   static_assert(kBins == kBinThreads, "a bin per thread");
-  int all;
-  const int mine = s_cnt[t];
-  const int before = wave_scan(mine, &all);
-  if (lane == 0) s_wave[w] = all;
+  const int mine = s_cnt[t], upto = (int)wave_scan((uint32_t)mine);
+  if (lane == 63) s_wave[w] = upto;
   __syncthreads();
-  int first = before, total = 0;
+  int first = upto - mine, total = 0;
   for (int i = 0; i < kBinThreads / 64; i++) {
     if (i < w) first += s_wave[i];
     total += s_wave[i];
@@ -240,50 +260,40 @@ __global__ __launch_bounds__(kBinThreads) void sample_bins_kernel(SampleArgs a, 
   const size_t ch = (size_t)row * nb + blockIdx.x;
   s.sum[ch * kBins + t] = s_sum[t];
   s.start[ch * kBins + t] = (uint16_t)first;
-  s.count[ch * kBins + t] = (uint16_t)mine;
+  if (t == 0) s.live[ch] = (uint32_t)total;
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < PT; j++)
-    if (bin[j] >= 0) {
-      const int p = s_at[bin[j]] + place[j];
-      s_key[p] = key[j];
-      s_idx[p] = (uint16_t)(t + kBinThreads * j);
-    }
+    if (bin[j] >= 0) s_idx[s_at[bin[j]] + place[j]] = (uint16_t)(t + kBinThreads * j);
   __syncthreads();
-  for (int i = t; i < total; i += kBinThreads) {
-    s.key[ch * kChunk + i] = s_key[i];
-    s.at[ch * kChunk + i] = s_idx[i];
-  }
+  // two indices a store (one past the end at most, in the chunk's own room)
+  for (int i = 2 * t; i < total; i += 2 * kBinThreads)
+    *reinterpret_cast<uint32_t *>(s.at + ch * kChunk + i) = *reinterpret_cast<const uint32_t *>(s_idx + i);
 }
 
-// A place in the order: behind the elements with a key above `key` (their number,
-// the sum of their weights) and the first `ties` of the `equal` that have it.
-struct Border {
-  uint32_t key;
-  int equal, above;
-  u64 sum;
-  int ties;
-};
-
+// A block's LDS for a row.
 struct Pick {
-  // bins of the whole row: number and sum of those before a bin
+  // the row's bins: number and sum of w of the elements before a bin
   int cnt[kBins + 1];
   u64 sum[kBins + 1];
-  // the elements of one bin
+  uint16_t start[kMaxChunks][kBins];  // a bin's first place in each chunk's order
+  int live[kMaxChunks];
+  // the elements of a run of bins, in any order; up to kSorted of them in order
+  // instead, with the sum of w up to each
   uint32_t key[kCap], idx[kCap];
-  u64 w[kCap];
-  int seg[kMaxChunks];
+  u64 w[kCap], upto[kSorted];
+  int seg[kMaxChunks], first[kMaxChunks];
   // a step's histogram, and what it found
   int hc[256];
   u64 hw[256];
   int found, found_cnt, found_equal;
   u64 found_sum;
-  int wave_c[16];
   u64 wave_w[16];
   uint32_t differ;
+  uint64_t tab[32];
 };
 
-// One row's elements and what is known of them.
+// One row, and which of its bins are in LDS: lo .. hi, n elements.
 struct Row {
   const float *l;
   const Scratch *s;
@@ -292,45 +302,97 @@ struct Row {
   uint32_t top;
   double inv_t;
   Bins bins;
-  int loaded, n;  // the bin in LDS (-1: none) and its elements
+  int lo, hi, n;
 };
 
-// loads bin b's elements, in the order of their chunks; false where they are too many
-__device__ bool load_bin(Pick &k, Row &r, int b) {
-  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
-  const int n = k.cnt[b + 1] - k.cnt[b];
-  if (n > kCap) return false;
-  if (r.loaded == b) return true;
-  __syncthreads();
-  if (w == 0) {
-    int all;
-    const int c = lane < r.nb ? r.s->count[(r.ch0 + lane) * kBins + b] : 0;
-    k.seg[lane] = wave_scan(c, &all);
+// Up to kSorted listed elements into their order, with running sums: four threads
+// count the elements before each.
+__device__ void sort_list(Pick &k, const Row &r) {
+  const int t = threadIdx.x, i = t >> 2;
+  auto order = [&](int j) { return ((u64)k.key[j] << 32) | ~k.idx[j]; };
+  uint32_t key = 0, idx = 0;
+  u64 w = 0;
+  int before = 0;
+  if (i < r.n) {
+    key = k.key[i], idx = k.idx[i], w = k.w[i];
+    const u64 mine = order(i);
+    for (int j = t & 3; j < r.n; j += 4) before += order(j) > mine;
   }
-  if (t == 0) k.differ = 0;
+  before += dpp_mov<0xB1>(before);
+  before += dpp_mov<0x4E>(before);
   __syncthreads();
-  for (int c = w; c < r.nb; c += 16) {
-    const size_t ch = r.ch0 + c;
-    const int first = r.s->start[ch * kBins + b], to = k.seg[c];
-    const int m = (c + 1 < r.nb ? k.seg[c + 1] : n) - to;
-    for (int i = lane; i < m; i += 64) {
-      const uint32_t key = r.s->key[ch * kChunk + first + i];
-      k.key[to + i] = key;
-      k.idx[to + i] = (uint32_t)(c * kChunk + r.s->at[ch * kChunk + first + i]);
-      k.w[to + i] = weight(key, r.top, r.inv_t);
+  if (i < r.n && (t & 3) == 0) k.key[before] = key, k.idx[before] = idx, k.w[before] = w;
+  __syncthreads();
+  static_assert(kSorted == 256, "four a lane");
+  if (t < 64) {
+    u64 v[4], all = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      v[j] = 4 * t + j < r.n ? k.w[4 * t + j] : 0;
+      all += v[j];
+    }
+    u64 x = k.sum[r.lo] + wave_scan(all) - all;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      x += v[j];
+      k.upto[4 * t + j] = x;
     }
   }
   __syncthreads();
-  uint32_t d = 0;
-  for (int i = t; i < n; i += 1024) d |= k.key[i] ^ k.key[0];
+}
+
+// Bin b's elements into LDS, with those of all bins before it where they are few
+// (the next border is among them then); false where b's are too many.
+__device__ bool load_bin(Pick &k, Row &r, int b) {
+  const int t = threadIdx.x, lane = t & 63;
+  if (r.lo <= b && b <= r.hi) return true;
+  if (k.cnt[b + 1] - k.cnt[b] > kCap) return false;
+  r.lo = k.cnt[b + 1] <= kSorted ? 0 : b;
+  r.hi = b;
+  r.n = k.cnt[b + 1] - k.cnt[r.lo];
+  __syncthreads();
+  if (t < 64) {
+    const int c = min(lane, r.nb - 1), from = k.start[c][r.lo];
+    const int m = lane < r.nb ? (b + 1 < kBins ? k.start[c][b + 1] : k.live[c]) - from : 0;
+    k.seg[lane] = (int)wave_scan((uint32_t)m) - m;
+    k.first[lane] = from;
+    if (t == 0) k.differ = 0;
+  }
+  __syncthreads();
+  uint32_t d = 0, first = 0;
+  for (int i = t; i < r.n; i += 1024) {
+    int c = 0;  // the last chunk whose elements start at i or before it
+#pragma unroll
+    for (int step = 32; step > 0; step >>= 1)
+      if (c + step < r.nb && k.seg[c + step] <= i) c += step;
+    const int at = c * kChunk + r.s->at[(r.ch0 + c) * kChunk + k.first[c] + (i - k.seg[c])];
+    const uint32_t key = key_of(r.l[at]);
+    k.key[i] = key;
+    k.idx[i] = (uint32_t)at;
+    k.w[i] = weight(key, r.top, r.inv_t, k.tab);
+    if (i == t) first = key;
+    d |= key ^ first;
+  }
+  // bits in which any two keys differ: from the wave's first key, and that from the list's
+  const uint32_t lead = (uint32_t)__shfl((int)first, 0, 64);
+  if (t < r.n) d |= first ^ lead;
+  __syncthreads();
+  if ((t & ~63) < r.n) d |= lead ^ k.key[0];
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) d |= (uint32_t)__shfl_xor((int)d, o, 64);
   if (lane == 0 && d) atomicOr(&k.differ, d);
   __syncthreads();
-  r.loaded = b;
-  r.n = n;
+  if (r.n <= kSorted) sort_list(k, r);
   return true;
 }
+
+// A key with what is before it in the order: their number and sum of w; and how
+// many have it.
+struct Border {
+  uint32_t key;
+  int equal, above;
+  u64 sum;
+};
 
 // Fixes the bits of a key below `bits`, 8 at a time, until the element is found at
 // which the running count reaches want (BY_SUM false) or the running sum passes
@@ -366,9 +428,8 @@ __device__ Border fix_bits(Pick &k, const Each &each, uint32_t prefix, int bits,
         call += c[j];
         wall += w[j];
       }
-      int all;
-      int cb = cnt + wave_scan(call, &all);
-      u64 wb = sum + wave_scan64(wall) - wall;
+      int cb = cnt + (int)wave_scan((uint32_t)call) - call;
+      u64 wb = sum + wave_scan(wall) - wall;
       int hit = -1, hc = 0, he = 0;
       u64 hw = 0;
 #pragma unroll
@@ -392,14 +453,20 @@ __device__ Border fix_bits(Pick &k, const Each &each, uint32_t prefix, int bits,
     equal = k.found_equal;
     bits = shift;
   }
-  return Border{prefix, equal, cnt, sum, 0};
+  return Border{prefix, equal, cnt, sum};
 }
 
-// The element at which the running count of the row reaches want, or its running
-// sum passes target (there is one): its key, what comes before that key, and in
-// `ties` the elements of the key before this one.
-template <bool BY_SUM>
-__device__ Border find_border(Pick &k, Row &r, int want, u64 target) {
+// An element of the row: the sum of w up to it and itself, its weight, and (TOKEN)
+// its index.
+struct Place {
+  u64 upto, w;
+  int token;
+};
+
+// The element at which the running count reaches want, or the running sum passes
+// target (there is one).
+template <bool BY_SUM, bool TOKEN>
+__device__ Place find_place(Pick &k, Row &r, int want, u64 target) {
   const int t = threadIdx.x;
   __syncthreads();
   if (t < kBins) {
@@ -408,11 +475,26 @@ __device__ Border find_border(Pick &k, Row &r, int want, u64 target) {
   }
   __syncthreads();
   const int b = k.found;
+  Place p{0, 0, 0};
+  const bool listed = load_bin(k, r, b);
+  if (listed && r.n <= kSorted) {
+    __syncthreads();
+    if (t < r.n) {
+      const u64 before = t ? k.upto[t - 1] : k.sum[r.lo];
+      if (BY_SUM ? before <= target && k.upto[t] > target : k.cnt[r.lo] + t + 1 == want) k.found = t;
+    }
+    __syncthreads();
+    const int i = k.found;
+    p.upto = k.upto[i];
+    p.w = k.w[i];
+    p.token = (int)k.idx[i];
+    return p;
+  }
   Border at;
-  if (load_bin(k, r, b)) {
+  if (listed) {
     const int bits = k.differ ? 32 - __clz(k.differ) : 0;
     if (bits == 0) {
-      at = Border{k.key[0], r.n, k.cnt[b], k.sum[b], 0};
+      at = Border{k.key[0], r.n, k.cnt[b], k.sum[b]};
     } else {
       at = fix_bits<BY_SUM>(
           k,
@@ -427,20 +509,46 @@ __device__ Border find_border(Pick &k, Row &r, int want, u64 target) {
         [&](auto f) {
           for (int i = t; i < r.V; i += 1024) {
             const uint32_t key = key_of(r.l[i]);
-            if (key > kNegInf && bin_of(r.bins, key) == b) f(key, weight(key, r.top, r.inv_t));
+            if (key > kNegInf && bin_of(r.bins, key) == b) f(key, weight(key, r.top, r.inv_t, k.tab));
           }
         },
         0, 32, k.cnt[b], k.sum[b], want, target);
   }
-  // of the elements with the key
-  if (!BY_SUM) {
-    at.ties = want - at.above - 1;
-  } else {
-    const u64 w = weight(at.key, r.top, r.inv_t);
-    const u64 before = w ? (target - at.sum) / w : 0;
-    at.ties = before < (u64)at.equal ? (int)before : at.equal - 1;
+  // of the elements with the key, the number of those before this one
+  p.w = weight(at.key, r.top, r.inv_t, k.tab);
+  int ties = want - at.above - 1;
+  if (BY_SUM) {
+    const u64 before = p.w ? (target - at.sum) / p.w : 0;
+    ties = before < (u64)at.equal ? (int)before : at.equal - 1;
   }
-  return at;
+  p.upto = at.sum + (u64)(ties + 1) * p.w;
+  if (!TOKEN) return p;
+  if (listed && at.equal == 1) {
+    __syncthreads();
+    for (int i = t; i < r.n; i += 1024)
+      if (k.key[i] == at.key) k.found = (int)k.idx[i];
+    __syncthreads();
+    p.token = k.found;
+    return p;
+  }
+  // number `ties` by index: the largest complement of the index but for so many
+  constexpr int kIdxBits = 18;
+  constexpr uint32_t kIdx = (1u << kIdxBits) - 1;
+  static_assert(kMaxChunks * kChunk <= 1 << kIdxBits, "an index's bits");
+  const Border i = fix_bits<false>(
+      k,
+      [&](auto f) {
+        if (listed) {
+          for (int j = t; j < r.n; j += 1024)
+            if (k.key[j] == at.key) f(~k.idx[j] & kIdx, 0);
+        } else {
+          for (int j = t; j < r.V; j += 1024)
+            if (key_of(r.l[j]) == at.key) f(~(uint32_t)j & kIdx, 0);
+        }
+      },
+      0, kIdxBits, 0, 0, ties + 1, 0);
+  p.token = (int)(~i.key & kIdx);
+  return p;
 }
 
 // the smallest key whose weight reaches min_p (at most the largest one's)
@@ -487,87 +595,98 @@ __global__ __launch_bounds__(1024) void sample_pick_kernel(SampleArgs a, Scratch
   r.nb = nb;
   r.inv_t = 1.0 / (double)T;
   r.bins = bins_of(r.top, low, (double)T);
-  r.loaded = -1;
+  r.lo = 0;
+  r.hi = -1;
   r.n = 0;
   const int top_k = a.top_k ? a.top_k[row] : 0;
   const float top_p = a.top_p ? a.top_p[row] : 1.0f, min_p = a.min_p ? a.min_p[row] : 0.0f;
   const double u = a.u[row];
 
-  // the chunks' bins, added up: half of the chunks per thread
+  // The chunks' bins, added up: half of the chunks per thread, kRead of them read
+  // at a time (the chunks' blocks ran on other XCDs, so every read goes past this
+  // one's L2).  A bin's first place, added over the chunks, is the number of elements
+  // before it.
   {
-    const int b = t & (kBins - 1);
-    u64 sum = 0;
-    int cnt = 0;
-#pragma unroll 8
-    for (int c = t / kBins; c < nb; c += 1024 / kBins) {
-      sum += s.sum[(r.ch0 + c) * kBins + b];
-      cnt += s.count[(r.ch0 + c) * kBins + b];
-    }
+    constexpr int kRead = 20;
+    const int b = t & (kBins - 1), half = t / kBins;
     static_assert(kBins == 512, "two threads a bin");
-    if (t >= kBins) {
-      k.sum[b] = sum;
-      k.cnt[b] = cnt;
-    }
-    __syncthreads();
-    if (t < kBins) {
-      sum += k.sum[b];
-      cnt += k.cnt[b];
-    }
-    int call;
-    const int cb = wave_scan(cnt, &call);
-    const u64 wi = wave_scan64(sum);
-    if (lane == 63) {
-      k.wave_c[w] = call;
-      k.wave_w[w] = wi;
-    }
-    __syncthreads();
-    if (t < kBins) {
-      int c = cb + cnt;
-      u64 x = wi;
-      for (int i = 0; i < w; i++) {
-        c += k.wave_c[i];
-        x += k.wave_w[i];
+    u64 sum = 0;
+    int before = 0;
+    for (int c0 = half; c0 < nb; c0 += 2 * kRead) {
+      u64 x[kRead];
+      uint16_t y[kRead];
+#pragma unroll
+      for (int i = 0; i < kRead; i++) {
+        const size_t ch = r.ch0 + min(c0 + 2 * i, nb - 1);
+        x[i] = s.sum[ch * kBins + b];
+        y[i] = s.start[ch * kBins + b];
       }
-      k.cnt[b + 1] = c;
-      k.sum[b + 1] = x;
-      if (t == 0) k.cnt[0] = 0, k.sum[0] = 0;
+#pragma unroll
+      for (int i = 0; i < kRead; i++)
+        if (c0 + 2 * i < nb) {
+          sum += x[i];
+          before += y[i];
+          k.start[c0 + 2 * i][b] = y[i];
+        }
+    }
+    if (t < 64) {
+      const int n = t < nb ? (int)s.live[r.ch0 + t] : 0;
+      k.live[t] = n;
+      const int all = (int)wave_scan((uint32_t)n);
+      if (t == 63) k.cnt[kBins] = all;
+    }
+    if (t < 32) k.tab[t] = ec_exp2_32[t];
+    if (half) {
+      k.sum[b] = sum;
+      k.cnt[b] = before;
+    }
+    __syncthreads();
+    u64 upto = 0;
+    if (!half) {
+      upto = wave_scan(sum + k.sum[b]);
+      before += k.cnt[b];
+      if (lane == 63) k.wave_w[w] = upto;
+    }
+    __syncthreads();
+    if (!half) {
+      for (int i = 0; i < w; i++) upto += k.wave_w[i];
+      k.sum[b + 1] = upto;
+      k.cnt[b] = before;
+      if (t == 0) k.sum[0] = 0;
     }
     __syncthreads();
   }
-  const int live = k.cnt[kBins];  // above -inf
+  // the sum of those that stay
   u64 total = k.sum[kBins];
-  // the sum of those that stay and, where some do not, the border
-  if (top_k > 0 && top_k < live) {
-    const Border b = find_border<false>(k, r, top_k, 0);
-    total = b.sum + (u64)(b.ties + 1) * weight(b.key, r.top, r.inv_t);
-  }
+  if (top_k > 0 && top_k < k.cnt[kBins]) total = find_place<false, false>(k, r, top_k, 0).upto;
   if (top_p < 1.0f) {
     // up to the element at which the sum reaches top_p of it: passes ceil(top_p sum) - 1
     const double x = ceil((double)top_p * (double)total) - 1.0;
     u64 target = x > 0.0 ? (u64)x : 0;
     if (target >= total) target = total - 1;
-    const Border b = find_border<true>(k, r, 0, target);
-    total = b.sum + (u64)(b.ties + 1) * weight(b.key, r.top, r.inv_t);
+    total = find_place<true, false>(k, r, 0, target).upto;
   }
   if (min_p > 0.0f) {
     // those from the least key on, as far as they are among those that stay
     const uint32_t thr = least_key(r.top, r.inv_t, (double)min_p);
     const int b = bin_of(r.bins, thr);
     u64 sum = 0;
+    int from = b;
     if (load_bin(k, r, b)) {
       for (int i = t; i < r.n; i += 1024)
         if (k.key[i] >= thr) sum += k.w[i];
+      from = r.lo;
     } else {
       for (int i = t; i < r.V; i += 1024) {
         const uint32_t key = key_of(r.l[i]);
-        if (key >= thr && bin_of(r.bins, key) == b) sum += weight(key, r.top, r.inv_t);
+        if (key >= thr && bin_of(r.bins, key) == b) sum += weight(key, r.top, r.inv_t, k.tab);
       }
     }
-    sum = wave_scan64(sum);
+    sum = wave_scan(sum);
     __syncthreads();
     if (lane == 63) k.wave_w[w] = sum;
     __syncthreads();
-    sum = k.sum[b];
+    sum = k.sum[from];
     for (int i = 0; i < 16; i++) sum += k.wave_w[i];
     total = sum < total ? sum : total;
   }
@@ -575,43 +694,15 @@ __global__ __launch_bounds__(1024) void sample_pick_kernel(SampleArgs a, Scratch
   const double x = u * (double)total;
   u64 target = x > 0.0 ? x < (double)total ? (u64)x : total - 1 : u == u ? 0 : total - 1;
   if (target >= total) target = total - 1;
-  const Border at = find_border<true>(k, r, 0, target);
-  // of the elements that have the key, number at.ties by index: the largest
-  // complement of the index but for so many
-  const bool listed = r.loaded >= 0 && bin_of(r.bins, at.key) == r.loaded;
-  int token = 0;
-  if (listed && at.equal == 1) {
-    __syncthreads();
-    for (int i = t; i < r.n; i += 1024)
-      if (k.key[i] == at.key) k.found = (int)k.idx[i];
-    __syncthreads();
-    token = k.found;
-  } else {
-    constexpr int kIdxBits = 18;
-    constexpr uint32_t kIdx = (1u << kIdxBits) - 1;
-    static_assert(kMaxChunks * kChunk <= 1 << kIdxBits, "an index's bits");
-    const Border i = fix_bits<false>(
-        k,
-        [&](auto f) {
-          if (listed) {
-            for (int j = t; j < r.n; j += 1024)
-              if (k.key[j] == at.key) f(~k.idx[j] & kIdx, 0);
-          } else {
-            for (int j = t; j < r.V; j += 1024)
-              if (key_of(r.l[j]) == at.key) f(~(uint32_t)j & kIdx, 0);
-          }
-        },
-        0, kIdxBits, 0, 0, at.ties + 1, 0);
-    token = (int)(~i.key & kIdx);
-  }
+  const Place p = find_place<true, true>(k, r, 0, target);
   if (t == 0) {
-    a.token[row] = token;
-    if (a.prob) a.prob[row] = (float)((double)weight(at.key, r.top, r.inv_t) / (double)total);
+    a.token[row] = p.token;
+    if (a.prob) a.prob[row] = (float)((double)p.w / (double)total);
   }
 }
 
 // rows per batch: enough chunks for every CU, a bounded scratch
-constexpr int kBatch = 64;
+constexpr int kBatch = 128;
 
 }  // namespace
 
