@@ -28,40 +28,52 @@ __device__ __forceinline__ float2 rope_cs(int pos, double f, float factor) {
   return make_float2(c * factor, s * factor);
 }
 
-// One block per token.  A wave takes a head at a time, its elements through
-// the wave's row in LDS.
-constexpr int kRopeMaxHd = 512;
-__global__ __launch_bounds__(256) void qk_norm_rope_kernel(NormRopeArgs a) {
-  __shared__ float row[4][kRopeMaxHd];
-  __shared__ float2 cs[kRopeMaxHd / 2];
-  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
-  const int b = blockIdx.x / a.t.N, i = blockIdx.x - b * a.t.N;
+// What a row's threads know of it: its cache row, and the position it stands at.
+struct RopeRow {
+  bool mine, ok;  // a node's row; of a sequence that takes part
+  int pos;
+  size_t crow;  // first element in the caches
+};
+__device__ __forceinline__ RopeRow rope_row(const NormRopeArgs &a, int m) {
+  const int b = m / a.t.N, i = m - b * a.t.N;
   const EcTreeSeq s = ec_tree_seq(&a.t, b);
-  if (i >= ec_tree_rows(&a.t, s)) return;
-  bool ok = ec_tree_seq_ok(&a.t, s);
+  RopeRow r;
+  r.mine = i < ec_tree_rows(&a.t, s);
+  r.ok = r.mine && ec_tree_seq_ok(&a.t, s);
   int depth = i;
-  if (ok && a.t.parent) {
-    bool pok;
-    const int p = tree_parent(a.t, b, s.n, &pok);
-    ok = pok;
-    if (ok) {
+  if (r.ok && a.t.parent) {
+    const int p = tree_parent(a.t, b, s.n, &r.ok);
+    if (r.ok) {
       int d;
       tree_ancestors(p, &d);
       depth = __shfl(d, i, 64);
     }
   }
-  ok = ok && !tree_clashes(a.t, b, s);
+  r.ok = r.ok && !tree_clashes(a.t, b, s);
+  r.pos = s.past + depth;
+  r.crow = r.ok ? ((size_t)s.slot * a.t.C + (s.past + i)) * ((size_t)a.KVH * a.hd) : 0;
+  return r;
+}
+
+// The form for any head size and alignment: one block per token, a wave a head at
+// a time, its elements through the wave's row in LDS.
+constexpr int kRopeMaxHd = 512;
+__global__ __launch_bounds__(256) void qk_norm_rope_any_kernel(NormRopeArgs a) {
+  __shared__ float row[4][kRopeMaxHd];
+  __shared__ float2 cs[kRopeMaxHd / 2];
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
+  const RopeRow rr = rope_row(a, blockIdx.x);
+  if (!rr.mine) return;
   const size_t m = blockIdx.x;
   float *q = a.q + m * a.ldq;
-  if (!ok) {
+  if (!rr.ok) {
     for (int e = t; e < a.H * a.hd; e += 256) q[e] = __builtin_nanf("");
     return;
   }
   const int half = a.rot >> 1;
-  for (int e = t; e < half; e += 256) cs[e] = rope_cs(s.past + depth, a.inv_freq[e], a.factor);
+  for (int e = t; e < half; e += 256) cs[e] = rope_cs(rr.pos, a.inv_freq[e], a.factor);
   __syncthreads();
   const float *x = a.x + m * a.ldx;
-  const size_t crow = ((size_t)s.slot * a.t.C + (s.past + i)) * ((size_t)a.KVH * a.hd);
   // a uniform count of rounds: the waves meet at barriers in each
   for (int h0 = 0; h0 < a.H + 2 * a.KVH; h0 += 4) {
     const int h = h0 + w;
@@ -92,11 +104,129 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(NormRopeArgs a) {
           y = second ? o * cs[f].y + y * cs[f].x : y * cs[f].x - o * cs[f].y;
         }
         if (isq) q[(size_t)h * a.hd + e] = y;
-        else if (isv) a.vc[crow + (size_t)(h - a.H - a.KVH) * a.hd + e] = f2h(y);
-        else a.kc[crow + (size_t)(h - a.H) * a.hd + e] = f2h(y);
+        else if (isv) a.vc[rr.crow + (size_t)(h - a.H - a.KVH) * a.hd + e] = f2h(y);
+        else a.kc[rr.crow + (size_t)(h - a.H) * a.hd + e] = f2h(y);
       }
     }
     __syncthreads();
+  }
+}
+
+// The form for head sizes that are multiples of 4 up to 256 and rows of whole
+// 16-byte chunks: LPH lanes a head, four elements a lane, `rows` rows of the call a
+// block.  The norm's sum goes over the head's lanes; a pair's other element is in
+// the same lane (layout 1) or in lane +- rot / 8, which holds its four (layout 0,
+// rot a multiple of 8).  Bound by memory, every element read and written once;
+// what counts is the chain before the first store (a sequence's numbers, its
+// tree, the angles): a block goes through it once for its rows, with kAhead heads
+// a lane already on their way.
+constexpr int kRopeRows = 4, kAhead = 4;
+template <int LPH>
+__global__ __launch_bounds__(256) void qk_norm_rope_kernel(NormRopeArgs a, int rows) {
+  __shared__ float4 cs[kRopeRows][64];  // four cosines, then four sines, of four frequencies
+  __shared__ RopeRow info[kRopeRows];
+  constexpr int kGroups = 256 / LPH;
+  const int t = threadIdx.x, li = t % LPH, e = 4 * li, heads = a.H + 2 * a.KVH;
+  const int m0 = blockIdx.x * rows, n = min(rows, a.t.B * a.t.N - m0), items = n * heads;
+  const int half = a.rot >> 1;
+  const bool in = e < a.hd;
+  float4 v[kAhead];
+  int it = t / LPH;
+  auto read = [&](int i) {
+    float4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (in && i < items) {
+      const int r = i / heads, h = i - r * heads;
+      x = *reinterpret_cast<const float4 *>(a.x + (size_t)(m0 + r) * a.ldx + (size_t)h * a.hd + e);
+    }
+    return x;
+  };
+#pragma unroll
+  for (int j = 0; j < kAhead; j++) v[j] = read(it + j * kGroups);
+  double f = 0.0;
+  if (half) f = a.inv_freq[t % half];
+  {
+    const int w = t >> 6;
+    static_assert(kRopeRows == 4, "a wave per row");
+    if (w < n) {
+      const RopeRow rr = rope_row(a, m0 + w);
+      if ((t & 63) == 0) info[w] = rr;
+    }
+  }
+  __syncthreads();
+  for (int j = t; j < n * half; j += 256) {
+    const int r = j / half, i = j - r * half;
+    const float2 c = rope_cs(info[r].pos, j == t ? f : a.inv_freq[i], a.factor);
+    float *p = reinterpret_cast<float *>(cs[r] + 2 * (i >> 2)) + (i & 3);
+    p[0] = c.x;
+    p[4] = c.y;
+  }
+  __syncthreads();
+  // a uniform count of rounds: the lanes of a wave exchange their elements in each
+  for (int i0 = 0; i0 < items; i0 += kAhead * kGroups) {
+#pragma unroll
+    for (int j = 0; j < kAhead; j++) {
+      const int i = i0 + j * kGroups + it;
+      const int r = min(i, items - 1) / heads, h = min(i, items - 1) - r * heads;
+      float4 x = v[j];
+      v[j] = read(i + kAhead * kGroups);
+      const bool isq = h < a.H, isv = h >= a.H + a.KVH;
+      const float *gamma = isq ? a.q_gamma : isv ? nullptr : a.k_gamma;
+      float sum = x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w;
+#pragma unroll
+      for (int o = LPH / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+      if (gamma && in) {
+        const float s = 1.0f / sqrtf(sum / (float)a.hd + a.eps);
+        const float4 g = *reinterpret_cast<const float4 *>(gamma + e);
+        x.x = x.x * s * g.x;
+        x.y = x.y * s * g.y;
+        x.z = x.z * s * g.z;
+        x.w = x.w * s * g.w;
+      }
+      if (a.layout) {
+        if (!isv && e < a.rot) {
+          // frequencies 2 li and 2 li + 1; where rot ends inside the lane, the first alone
+          const float *c = reinterpret_cast<const float *>(cs[r] + 2 * (li >> 1)) + 2 * (li & 1);
+          const float a0 = x.x, b0 = x.y, a1 = x.z, b1 = x.w;
+          x.x = a0 * c[0] - b0 * c[4];
+          x.y = a0 * c[4] + b0 * c[0];
+          if (e + 2 < a.rot) {
+            x.z = a1 * c[1] - b1 * c[5];
+            x.w = a1 * c[5] + b1 * c[1];
+          }
+        }
+      } else if (a.rot) {
+        const int far = half >> 2;  // lanes from an element to its pair's other one
+        const bool first = li < far;
+        const int src = ((t & 63) + (first ? far : -far)) & 63;
+        float4 o;
+        o.x = __shfl(x.x, src, 64);
+        o.y = __shfl(x.y, src, 64);
+        o.z = __shfl(x.z, src, 64);
+        o.w = __shfl(x.w, src, 64);
+        if (!isv && e < a.rot) {
+          const int k = first ? li : li - far;
+          const float4 c = cs[r][2 * k], s = cs[r][2 * k + 1];
+          const float sg = first ? -1.0f : 1.0f;
+          x.x = x.x * c.x + sg * (o.x * s.x);
+          x.y = x.y * c.y + sg * (o.y * s.y);
+          x.z = x.z * c.z + sg * (o.z * s.z);
+          x.w = x.w * c.w + sg * (o.w * s.w);
+        }
+      }
+      const RopeRow &rr = info[r];
+      if (!in || i >= items || !rr.mine) continue;
+      if (isq) {
+        const float nan = __builtin_nanf("");
+        if (!rr.ok) x = make_float4(nan, nan, nan, nan);
+        *reinterpret_cast<float4 *>(a.q + (size_t)(m0 + r) * a.ldq + (size_t)h * a.hd + e) = x;
+      } else if (rr.ok) {
+        uint16_t *to = isv ? a.vc + rr.crow + (size_t)(h - a.H - a.KVH) * a.hd + e : a.kc + rr.crow + (size_t)(h - a.H) * a.hd + e;
+        uint2 p;
+        p.x = (uint32_t)f2h(x.x) | (uint32_t)f2h(x.y) << 16;
+        p.y = (uint32_t)f2h(x.z) | (uint32_t)f2h(x.w) << 16;
+        *reinterpret_cast<uint2 *>(to) = p;
+      }
+    }
   }
 }
 
@@ -163,8 +293,28 @@ __global__ __launch_bounds__(256) void tree_accept_kernel(AcceptArgs a, int cols
 
 int qk_norm_rope_max_hd() { return kRopeMaxHd; }
 
+// rows that the vector form's 16-byte (caches: 8-byte) accesses can take
+static bool rope_vector_ok(const NormRopeArgs &a) {
+  const uintptr_t p = (uintptr_t)a.x | (uintptr_t)a.q | (uintptr_t)a.q_gamma | (uintptr_t)a.k_gamma;
+  return a.hd % 4 == 0 && a.hd <= 256 && a.ldx % 4 == 0 && a.ldq % 4 == 0 && !(p & 15) &&
+         !(((uintptr_t)a.kc | (uintptr_t)a.vc) & 7) && (a.layout || a.rot % 8 == 0);
+}
+
+template <int LPH>
+static void launch_rope(const NormRopeArgs &a, hipStream_t st) {
+  // rows a block: as many as its lanes hold ahead, while two blocks per CU are left
+  const int m = a.t.B * a.t.N, hold = kAhead * (256 / LPH) / (a.H + 2 * a.KVH), spread = m / 512;
+  int rows = hold < spread ? hold : spread;
+  rows = rows < 1 ? 1 : rows > kRopeRows ? kRopeRows : rows;
+  klaunch(qk_norm_rope_kernel<LPH>, dim3((m + rows - 1) / rows), dim3(256), 0, st, a, rows);
+}
+
 hipError_t qk_norm_rope(const NormRopeArgs &a, hipStream_t st) {
-  klaunch(qk_norm_rope_kernel, dim3(a.t.B * a.t.N), dim3(256), 0, st, a);
+  if (!rope_vector_ok(a)) klaunch(qk_norm_rope_any_kernel, dim3(a.t.B * a.t.N), dim3(256), 0, st, a);
+  else if (a.hd <= 32) launch_rope<8>(a, st);
+  else if (a.hd <= 64) launch_rope<16>(a, st);
+  else if (a.hd <= 128) launch_rope<32>(a, st);
+  else launch_rope<64>(a, st);
   return hipGetLastError();
 }
 
