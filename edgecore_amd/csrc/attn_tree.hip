@@ -514,36 +514,61 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_tree_kernel(TreeAttnArgs a,
 
 // Joins the splits' outputs: per row the largest of their maxima, the sums and
 // outputs brought to it.  HD / 4 lanes a row (a power of two of them: 24 of 32 at
-// 96); the maxima and sums are read by all lanes of a row at once.
+// 96).  Latency is all of it: the reads do not wait for the sequence's numbers.
 template <int HD>
 __global__ __launch_bounds__(256) void attn_tree_join_kernel(TreeAttnArgs a, int ns) {
   constexpr int LPR = HD == 96 ? 32 : HD / 4, RPB = 256 / LPR;
+  constexpr int kRead = 16;  // splits read at a time
   const int t = threadIdx.x, b = blockIdx.y, li = t % LPR;
+  const int r = blockIdx.x * RPB + t / LPR;
+  const size_t all = (size_t)a.t.B * a.t.N * a.H, row = (size_t)b * a.t.N * a.H + min(r, a.t.N * a.H - 1);
+  const float *po = (const float *)a.ws + row * HD + 4 * min(li, HD / 4 - 1);
+  const float2 *ml = (const float2 *)((const float *)a.ws + (size_t)ns * all * HD) + row;
+  // the first splits are read before it is known how many of them there are
+  float2 u[kRead];
+  float4 v[kRead];
+#pragma unroll
+  for (int i = 0; i < kRead; i++) {
+    const size_t at = (size_t)min(i, ns - 1) * all;
+    u[i] = ml[at];
+    v[i] = *reinterpret_cast<const float4 *>(po + at * HD);
+  }
   const EcTreeSeq s = ec_tree_seq(&a.t, b);
   bool ok = ec_tree_seq_ok(&a.t, s);
   if (ok) tree_parent(a.t, b, s.n, &ok);
-  const int r = blockIdx.x * RPB + t / LPR, rows = ec_tree_rows(&a.t, s) * a.H;
+  const int rows = ec_tree_rows(&a.t, s) * a.H;
   if (blockIdx.x * RPB >= rows) return;
-  const size_t all = (size_t)a.t.B * a.t.N * a.H, row = (size_t)b * a.t.N * a.H + min(r, rows - 1);
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   if (ok) {
     const int tiles = (s.past + s.n - window_lo(a.window, s.past, 0) + kTp - 1) / kTp, n = min(ns, tiles);
-    const float *po = (const float *)a.ws + row * HD + 4 * min(li, HD / 4 - 1);
-    const float2 *ml = (const float2 *)((const float *)a.ws + (size_t)ns * all * HD) + row;
     float m = -FLT_MAX, l = 0.0f;
-    for (int i = li; i < n; i += LPR) m = fmaxf(m, ml[i * all].x);
+    for (int i0 = 0; i0 < n; i0 += kRead) {
+      if (i0) {
 #pragma unroll
-    for (int k = LPR / 2; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor(m, k, 64));
-#pragma unroll 8
-    for (int i = 0; i < n; i++) {
-      const float2 u = ml[i * all];
-      const float4 v = *reinterpret_cast<const float4 *>(po + (size_t)i * all * HD);
-      const float f = __builtin_amdgcn_exp2f(u.x - m);
-      l = __builtin_fmaf(u.y, f, l);
-      o.x = __builtin_fmaf(v.x, f, o.x);
-      o.y = __builtin_fmaf(v.y, f, o.y);
-      o.z = __builtin_fmaf(v.z, f, o.z);
-      o.w = __builtin_fmaf(v.w, f, o.w);
+        for (int i = 0; i < kRead; i++) {
+          const size_t at = (size_t)min(i0 + i, ns - 1) * all;
+          u[i] = ml[at];
+          v[i] = *reinterpret_cast<const float4 *>(po + at * HD);
+        }
+      }
+      float big = m;
+#pragma unroll
+      for (int i = 0; i < kRead; i++)
+        if (i0 + i < n) big = fmaxf(big, u[i].x);
+      const float back = __builtin_amdgcn_exp2f(m - big);
+      m = big;
+      l *= back;
+      o = make_float4(o.x * back, o.y * back, o.z * back, o.w * back);
+#pragma unroll
+      for (int i = 0; i < kRead; i++)
+        if (i0 + i < n) {
+          const float f = __builtin_amdgcn_exp2f(u[i].x - m);
+          l = __builtin_fmaf(u[i].y, f, l);
+          o.x = __builtin_fmaf(v[i].x, f, o.x);
+          o.y = __builtin_fmaf(v[i].y, f, o.y);
+          o.z = __builtin_fmaf(v[i].z, f, o.z);
+          o.w = __builtin_fmaf(v[i].w, f, o.w);
+        }
     }
     const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
     o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
