@@ -189,30 +189,49 @@ __device__ __forceinline__ Parts split2(float x, float y) {
 }
 __device__ __forceinline__ float half_of(v4u v, int e) { return h2f((uint16_t)(v[e >> 1] >> (16 * (e & 1)))); }
 
-// Operands of two groups of 16 elements, from rows 32 u .. 32 u + 31 of the
+// Operands of ND groups of 16 elements, from rows 32 u .. 32 u + 31 of the
 // tile: lane l of 16 names 8 bytes of row l / 4 and gets element l of the four
 // rows.  The builtin would wait for every load that is on its way into LDS, the
 // next tile's too.
-template <int HD>
-__device__ __forceinline__ void read_v2(uint32_t at0, uint32_t at1, int u, v4u (&v)[2]) {
+template <int HD, int ND>
+__device__ __forceinline__ void read_v(const uint32_t *at, uint32_t base, int u, v4u (&v)[ND]) {
   typedef uint32_t v2u __attribute__((ext_vector_type(2)));
-  v2u x[4];
-  asm volatile(
-      "ds_read_b64_tr_b16 %0, %4 offset:%6\n\t"
-      "ds_read_b64_tr_b16 %1, %4 offset:%7\n\t"
-      "ds_read_b64_tr_b16 %2, %5 offset:%6\n\t"
-      "ds_read_b64_tr_b16 %3, %5 offset:%7\n\t"
-      "s_waitcnt lgkmcnt(0)"
-      : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3])
-      : "v"(at0), "v"(at1), "i"(64 * HD * u), "i"(64 * HD * u + 32 * HD)
-      : "memory");
+  static_assert(ND == 2 || ND == 4, "groups of elements");
+  v2u x[2 * ND];
+  if constexpr (ND == 2) {
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %4 offset:%6\n\t"
+        "ds_read_b64_tr_b16 %1, %4 offset:%7\n\t"
+        "ds_read_b64_tr_b16 %2, %5 offset:%6\n\t"
+        "ds_read_b64_tr_b16 %3, %5 offset:%7\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3])
+        : "v"(base + at[0]), "v"(base + at[1]), "i"(64 * HD * u), "i"(64 * HD * u + 32 * HD)
+        : "memory");
+  } else {
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %8 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %2, %9 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %4, %10 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %6, %11 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(x[4]), "=&v"(x[5]), "=&v"(x[6]), "=&v"(x[7])
+        : "v"(base + at[0]), "v"(base + at[1]), "v"(base + at[2]), "v"(base + at[3]), "i"(64 * HD * u),
+          "i"(64 * HD * u + 32 * HD)
+        : "memory");
+  }
 #pragma unroll
-  for (int e = 0; e < 2; e++) v[e] = v4u{x[2 * e].x, x[2 * e].y, x[2 * e + 1].x, x[2 * e + 1].y};
+  for (int e = 0; e < ND; e++) v[e] = v4u{x[2 * e].x, x[2 * e].y, x[2 * e + 1].x, x[2 * e + 1].y};
 }
 
 template <int HD, int NW, int OCC>
 __global__ __launch_bounds__(NW * 64, OCC) void attn_tree_kernel(TreeAttnArgs a, TreeGrid gr) {
-  constexpr int CPR = HD / 8, KS = HD / 32, DT = HD / 16, NT = NW * 64, LPT = (kTp * CPR + NT - 1) / NT;
+  constexpr int CPR = HD / 8, KS = HD / 32, DT = HD / 16, NT = NW * 64, LPT = (kTp * CPR + NT - 1) / NT,
+                ND = DT % 4 ? 2 : 4;
   typedef __attribute__((address_space(1))) const void gvoid;
   typedef __attribute__((address_space(3))) void lvoid;
   extern __shared__ __attribute__((aligned(16))) _Float16 lds[];  // [2 buffers][K, V][kTp][HD]
@@ -460,11 +479,11 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_tree_kernel(TreeAttnArgs a,
 #pragma unroll
     for (int u = 0; u < 2; u++)
 #pragma unroll
-      for (int d = 0; d < DT; d += 2) {
-        v4u vf[2];
-        read_v2<HD>(vat + vcol[d], vat + vcol[d + 1], u, vf);
+      for (int d = 0; d < DT; d += ND) {
+        v4u vf[ND];
+        read_v<HD, ND>(vcol + d, vat, u, vf);
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
+        for (int e = 0; e < ND; e++) {
           o[d + e] = mma(vf[e], ph[u], o[d + e]);
           o[d + e] = mma(vf[e], pl[u], o[d + e]);
         }
@@ -611,10 +630,13 @@ hipError_t launch_tree(const TreeAttnArgs &a, hipStream_t st) {
   const uint32_t lds = 2 * 4 * kTp * HD;
   if (tree_waves(a) == 4) klaunch((attn_tree_kernel<HD, 4, HD <= 64 ? 4 : 2>), grid, dim3(256), lds, st, a, g);
   else klaunch((attn_tree_kernel<HD, 8, HD <= 64 ? 4 : 2>), grid, dim3(512), lds, st, a, g);
-  if (g.ns > 1) {
-    constexpr int rpb = 256 / (HD == 96 ? 32 : HD / 4);
-    klaunch((attn_tree_join_kernel<HD>), dim3((a.t.N * a.H + rpb - 1) / rpb, a.t.B), dim3(256), 0, st, a, g.ns);
-  }
+  return hipGetLastError();
+}
+
+template <int HD>
+hipError_t launch_join(const TreeAttnArgs &a, hipStream_t st) {
+  constexpr int rpb = 256 / (HD == 96 ? 32 : HD / 4);
+  klaunch((attn_tree_join_kernel<HD>), dim3((a.t.N * a.H + rpb - 1) / rpb, a.t.B), dim3(256), 0, st, a, tree_grid(a).ns);
   return hipGetLastError();
 }
 
@@ -623,9 +645,7 @@ hipError_t launch_tree(const TreeAttnArgs &a, hipStream_t st) {
 int attention_tree_max_hd() { return kTreeMaxHd; }
 
 size_t attention_tree_workspace(const TreeAttnArgs &a) {
-  if (!tiles_ok(a)) return 0;
-  const TreeGrid g = tree_grid(a);
-  return g.ns > 1 ? (size_t)g.ns * a.t.B * a.t.N * a.H * (a.hd + 2) * sizeof(float) : 0;
+  return attention_tree_joins(a) ? (size_t)tree_grid(a).ns * a.t.B * a.t.N * a.H * (a.hd + 2) * sizeof(float) : 0;
 }
 
 hipError_t attention_tree(const TreeAttnArgs &a, hipStream_t st) {
@@ -637,6 +657,15 @@ hipError_t attention_tree(const TreeAttnArgs &a, hipStream_t st) {
   }
   klaunch(attn_tree_any_kernel, dim3(a.t.B * a.t.N, a.H), dim3(256), 0, st, a);
   return hipGetLastError();
+}
+
+bool attention_tree_joins(const TreeAttnArgs &a) { return tiles_ok(a) && tree_grid(a).ns > 1; }
+
+hipError_t attention_tree_join(const TreeAttnArgs &a, hipStream_t st) {
+  if (a.hd == 64) return launch_join<64>(a, st);
+  if (a.hd == 128) return launch_join<128>(a, st);
+  if (a.hd == 96) return launch_join<96>(a, st);
+  return launch_join<32>(a, st);
 }
 
 }  // namespace ec

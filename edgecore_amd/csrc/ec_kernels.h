@@ -481,8 +481,12 @@ struct SampleArgs {
   int *token;
   float *prob;
 };
+// in batches of sample_batch rows, three launches each, which share ws
+int sample_batch(int V);
 size_t sample_workspace(int rows, int V);  // bytes of ws
-hipError_t sample_rows(const SampleArgs &a, void *ws, hipStream_t st);
+hipError_t sample_top(const SampleArgs &a, void *ws, int row0, int n, hipStream_t st);
+hipError_t sample_bins(const SampleArgs &a, void *ws, int row0, int n, hipStream_t st);
+hipError_t sample_pick(const SampleArgs &a, void *ws, int row0, int n, hipStream_t st);
 
 // rows of drafted tokens (tree_rows.hip, attn_tree.hip): ec_tree.h's batch
 struct NormRopeArgs {
@@ -516,6 +520,8 @@ struct TreeAttnArgs {
 int attention_tree_max_hd();
 size_t attention_tree_workspace(const TreeAttnArgs &a);  // bytes of ws
 hipError_t attention_tree(const TreeAttnArgs &a, hipStream_t st);
+bool attention_tree_joins(const TreeAttnArgs &a);  // whether a join follows
+hipError_t attention_tree_join(const TreeAttnArgs &a, hipStream_t st);
 
 struct AcceptArgs {
   EcTreeBatch t;

@@ -2364,14 +2364,52 @@ extern "C" int ec_attention_dev(const float *q, int ldq, const uint16_t *kc, con
 
 // What these entry points share.  Arguments are checked before the device is
 // opened; what device arrays hold is checked in the kernels (ec_tree.h).
-constexpr long kMaxRows = 1L << 22;  // rows of a call (grids and row offsets stay in 32 bits)
+constexpr long kMaxRows = 1L << 22;       // rows of a call (grids and row offsets stay in 32 bits)
+constexpr int kMaxCacheRows = 1 << 30;    // of a slot
+
+// A range of memory; an empty or null one overlaps nothing.
+struct Span {
+  const void *p;
+  size_t n;
+  bool overlaps(const Span &o) const {
+    const uintptr_t a = (uintptr_t)p, b = (uintptr_t)o.p;
+    return p && o.p && a < b + o.n && b < a + n;
+  }
+};
+// whether one of the outputs overlaps an input or another output
+template <size_t NI, size_t NO>
+static bool spans_clash(const Span (&in)[NI], const Span (&out)[NO]) {
+  for (size_t i = 0; i < NO; i++) {
+    for (const Span &s : in)
+      if (out[i].overlaps(s)) return true;
+    for (size_t j = 0; j < i; j++)
+      if (out[i].overlaps(out[j])) return true;
+  }
+  return false;
+}
+static Span rows_span(const void *p, long rows, int ld, int width, size_t elem) {
+  return Span{p, ((size_t)(rows - 1) * ld + width) * elem};
+}
+
+// The library's device for the length of a call: a thread's own may be another.
+struct DeviceScope {
+  int before = -1;
+  DeviceScope() {
+    if (hipGetDevice(&before) != hipSuccess || before == g_device) before = -1;
+    else (void)hipSetDevice(g_device);
+  }
+  ~DeviceScope() {
+    if (before >= 0) (void)hipSetDevice(before);
+  }
+};
 
 static int tree_check(const char *fn, const EcTreeBatch &t, bool wide) {
   if (t.B < 1 || t.N < 1 || t.B > 65535 || (long)t.B * t.N > kMaxRows)
     return set_err(-1, "%s: B=%d sequences of N=%d rows (up to 65535, and %ld rows together)", fn, t.B, t.N, kMaxRows);
   if (t.N > EC_TREE_MAX && (t.parent || !wide))
     return set_err(-1, "%s: N=%d, more than the %d nodes of a tree", fn, t.N, EC_TREE_MAX);
-  if (t.nslots < 1 || t.C < 1) return set_err(-1, "%s: a cache of %d slots of %d rows", fn, t.nslots, t.C);
+  if (t.nslots < 1 || t.C < 1 || t.C > kMaxCacheRows)
+    return set_err(-1, "%s: a cache of %d slots of %d rows (up to %d)", fn, t.nslots, t.C, kMaxCacheRows);
   if (!t.past) return set_err(-1, "%s: null pointer", fn);
   return 0;
 }
@@ -2388,10 +2426,22 @@ extern "C" int ec_sample_dev(const float *logits, int rows, int vocab, int ld, c
     return set_err(-1, "ec_sample_dev: rows=%d vocab=%d (up to %d) ld=%d", rows, vocab, 1 << 18, ld);
   if (rows == 0) return 0;
   if (!logits || !u || !token) return set_err(-1, "ec_sample_dev: null pointer");
+  {
+    const size_t n = (size_t)rows * 4;
+    const Span in[] = {rows_span(logits, rows, ld, vocab, 4), {temp, n}, {top_k, n}, {top_p, n}, {min_p, n}, {u, 2 * n}};
+    const Span out[] = {{token, n}, {prob, n}};
+    if (spans_clash(in, out)) return set_err(-1, "ec_sample_dev: an output overlaps another array");
+  }
   EC_INIT();
+  const DeviceScope dev;
   const SampleArgs a{logits, rows, vocab, ld, temp, top_k, top_p, min_p, u, token, prob};
   if (const int r = w16_grow(g_sample_ws, sample_workspace(rows, vocab), "ec_sample_dev")) return r;
-  EC_LAUNCH("sample", 4.0 * rows * vocab, sample_rows(a, g_sample_ws.p, g_stream));
+  for (int r0 = 0; r0 < rows; r0 += sample_batch(vocab)) {
+    const int n = rows - r0 < sample_batch(vocab) ? rows - r0 : sample_batch(vocab);
+    EC_LAUNCH("sample_top", 4.0 * n * vocab, sample_top(a, g_sample_ws.p, r0, n, g_stream));
+    EC_LAUNCH("sample_bins", 4.0 * n * vocab, sample_bins(a, g_sample_ws.p, r0, n, g_stream));
+    EC_LAUNCH("sample_pick", 32.0 * n, sample_pick(a, g_sample_ws.p, r0, n, g_stream));
+  }
   return 0;
 }
 
@@ -2408,7 +2458,11 @@ extern "C" int ec_qk_norm_rope_dev(const float *qkv, int ldx, float *q, int ldq,
   if (rot < 0 || rot > hd || rot % 2 || layout < 0 || layout > 1 || !(eps >= 0.0))
     return set_err(-1, "%s: rot=%d (even, up to hd) layout=%d (0 half, 1 interleaved) eps=%g", fn, rot, layout, eps);
   if (!qkv || !q || !kc || !vc || (rot > 0 && !inv_freq)) return set_err(-1, "%s: null pointer", fn);
+  if (!(q == qkv && ldq == ldx) &&
+      rows_span(q, (long)B * N, ldq, H * hd, 4).overlaps(rows_span(qkv, (long)B * N, ldx, (H + 2 * KVH) * hd, 4)))
+    return set_err(-1, "%s: q overlaps qkv and is not its first columns", fn);
   EC_INIT();
+  const DeviceScope dev;
   const NormRopeArgs a{t, qkv, ldx, q, ldq, kc, vc, H, KVH, hd, q_gamma, k_gamma, (float)eps, inv_freq, rot, layout,
                        (float)factor};
   EC_LAUNCH("qk_norm_rope", (double)B * N * hd * (8.0 * H + 12.0 * KVH), qk_norm_rope(a, g_stream));
@@ -2425,12 +2479,17 @@ extern "C" int ec_attention_tree_dev(const float *q, int ldq, const uint16_t *kc
   if ((long)ldq < (long)H * hd || (long)ldo < (long)H * hd || window < 0 || max_past < 0 || max_past > C)
     return set_err(-1, "%s: ldq=%d ldo=%d window=%d max_past=%d (C=%d)", fn, ldq, ldo, window, max_past, C);
   if (!q || !kc || !vc || !out) return set_err(-1, "%s: null pointer", fn);
+  if (!(out == q && ldo == ldq) &&
+      rows_span(out, (long)B * N, ldo, H * hd, 4).overlaps(rows_span(q, (long)B * N, ldq, H * hd, 4)))
+    return set_err(-1, "%s: out overlaps q and is not q", fn);
   EC_INIT();
+  const DeviceScope dev;
   TreeAttnArgs a{t, q, ldq, kc, vc, H, KVH, hd, window, (float)(1.0 / sqrt((double)hd)), out, ldo, nullptr};
   const size_t need = attention_tree_workspace(a);
   if (need && (r = w16_grow(g_tree_ws, need, fn))) return r;
   a.ws = g_tree_ws.p;
   EC_LAUNCH("attention_tree", 4.0 * B * (max_past + N) * KVH * hd, attention_tree(a, g_stream));
+  if (attention_tree_joins(a)) EC_LAUNCH("attention_tree_join", (double)need, attention_tree_join(a, g_stream));
   return 0;
 }
 
@@ -2444,11 +2503,14 @@ extern "C" int ec_tree_accept_dev(uint16_t *kc, uint16_t *vc, int layers, int ns
   if (layers < 1 || kv < 1) return set_err(-1, "%s: %d layers of rows of %d", fn, layers, kv);
   if (!kc || !vc || !token || !sampled || !path || !npath || !next || !new_past)
     return set_err(-1, "%s: null pointer", fn);
-  const int *in[] = {slot, past, nodes};
-  for (const int *p : in)
-    for (int *o : {npath, next, new_past})
-      if (p && p < o + B && o < p + B) return set_err(-1, "%s: an output overlaps slot, past or nodes", fn);
+  {
+    const size_t b4 = (size_t)B * 4, n4 = b4 * N;
+    const Span in[] = {{slot, b4}, {past, b4}, {nodes, b4}, {parent, n4}, {token, n4}, {sampled, n4}};
+    const Span out[] = {{path, n4}, {npath, b4}, {next, b4}, {new_past, b4}};
+    if (spans_clash(in, out)) return set_err(-1, "%s: an output overlaps another array", fn);
+  }
   EC_INIT();
+  const DeviceScope dev;
   const AcceptArgs a{t, kc, vc, layers, kv, token, sampled, path, npath, next, new_past};
   EC_LAUNCH("tree_accept", 8.0 * layers * B * kv, tree_accept(a, g_stream));
   return 0;

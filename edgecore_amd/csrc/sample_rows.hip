@@ -81,30 +81,29 @@ __device__ __forceinline__ u64 exp_steps(double x, const uint64_t *tab) {
   return __builtin_bit_cast(uint64_t, __builtin_fma(s, p, kShift)) - __builtin_bit_cast(uint64_t, kShift);
 }
 
-// a logit's weight in steps of 2^-44
-__device__ __forceinline__ u64 weight(uint32_t key, uint32_t top, double inv_t, const uint64_t *tab) {
-  const double x = ((double)key_value(key) - (double)key_value(top)) * inv_t;
-  const u64 w = exp_steps(x, tab);
-  return key == top ? (u64)kOne : key <= kNegInf || top == kPosInf ? 0 : w;
-}
-
-// A row's bins: number (max - l) * per of the 512, the last one open.
-struct Bins {
-  uint32_t top;
-  double max, per;
+// What a row's weights and bins are made of.  A logit's bin is number (max - l) *
+// per of the 512, the last one open.
+struct Scale {
+  uint32_t top;  // key of the largest
+  double max, neg_inv_t, per;
 };
-__device__ __forceinline__ Bins bins_of(uint32_t top, uint32_t low, double T) {
-  Bins b;
+__device__ __forceinline__ Scale scale_of(uint32_t top, uint32_t low, double T) {
+  Scale b;
   b.top = top;
   b.max = (double)key_value(top);
+  b.neg_inv_t = -1.0 / T;  // T is 2^-149 at least
   const double span = fmin(b.max - (double)key_value(low), kNats * T);
   b.per = span > 0.0 ? kBins / span : 0.0;
   return b;
 }
-__device__ __forceinline__ int bin_of(const Bins &b, uint32_t key) {
-  if (b.top == kPosInf) return key == b.top ? 0 : kBins - 1;
-  const double x = (b.max - (double)key_value(key)) * b.per;
-  return x < (double)(kBins - 1) ? (int)x : kBins - 1;
+// of a value above -inf; where the largest is infinite it alone weighs
+__device__ __forceinline__ u64 weight(const Scale &b, float v, const uint64_t *tab) {
+  if (b.top == kPosInf) return v == __builtin_inff() ? (u64)kOne : 0;
+  return exp_steps((b.max - (double)v) * b.neg_inv_t, tab);
+}
+__device__ __forceinline__ int bin_of(const Scale &b, float v) {
+  if (b.top == kPosInf) return v == __builtin_inff() ? 0 : kBins - 1;
+  return (int)fmin((b.max - (double)v) * b.per, (double)(kBins - 1));
 }
 
 // scratch of a batch of rows
@@ -149,19 +148,18 @@ __global__ __launch_bounds__(256) void sample_top_kernel(SampleArgs a, Scratch s
   __shared__ uint32_t s_low[4];
   const int t = threadIdx.x, c0 = blockIdx.x * kChunk, nb = gridDim.x;
   const float *l = a.logits + (size_t)(row0 + blockIdx.y) * a.ld;
-  u64 top = 0;
-  uint32_t low = ~0u;
+  uint32_t low = ~0u, big = 0;
+  int at = 0;
   float v[kChunk / 256];
 #pragma unroll
   for (int j = 0; j < kChunk / 256; j++) v[j] = l[min(c0 + t + 256 * j, a.V - 1)];
 #pragma unroll
   for (int j = 0; j < kChunk / 256; j++) {
-    const int i = min(c0 + t + 256 * j, a.V - 1);
     const uint32_t k = key_of(v[j]);
-    const u64 e = ((u64)k << 32) | (uint32_t)~i;
-    top = e > top ? e : top;
+    if (k > big) big = k, at = j;  // the first of equal ones
     if (k > kNegInf) low = min(low, k);
   }
+  u64 top = ((u64)big << 32) | (uint32_t)~min(c0 + t + 256 * at, a.V - 1);
   top = wave_max64(top);
   low = wave_min32(low);
   if ((t & 63) == 0) {
@@ -227,22 +225,19 @@ __global__ __launch_bounds__(kBinThreads) void sample_bins_kernel(SampleArgs a, 
   row_ends(s, row, nb, &top, &low);
   const uint32_t tk = (uint32_t)(top >> 32);
   if (!(T > 0.0f) || tk == kNegInf) return;  // the largest logit, or none: nothing to weigh
-  const double inv_t = 1.0 / (double)T;
-  const Bins bins = bins_of(tk, low, (double)T);
+  const Scale sc = scale_of(tk, low, (double)T);
   s_sum[t] = 0;
   s_cnt[t] = 0;
   if (t < 32) s_tab[t] = ec_exp2_32[t];
   __syncthreads();
-  uint32_t key[PT];
   int bin[PT], place[PT];
 #pragma unroll
   for (int j = 0; j < PT; j++) {
-    key[j] = key_of(v[j]);
     bin[j] = -1;
-    if (c0 + t + kBinThreads * j < a.V && key[j] > kNegInf) {
-      bin[j] = bin_of(bins, key[j]);
+    if (c0 + t + kBinThreads * j < a.V && v[j] > -__builtin_inff()) {
+      bin[j] = bin_of(sc, v[j]);
       place[j] = atomicAdd(&s_cnt[bin[j]], 1);
-      const u64 x = weight(key[j], tk, inv_t, s_tab);
+      const u64 x = weight(sc, v[j], s_tab);
       if (x) atomicAdd(&s_sum[bin[j]], x);
     }
   }
@@ -299,9 +294,7 @@ struct Row {
   const Scratch *s;
   size_t ch0;  // the row's first chunk in the scratch
   int V, nb;
-  uint32_t top;
-  double inv_t;
-  Bins bins;
+  Scale sc;
   int lo, hi, n;
 };
 
@@ -366,10 +359,11 @@ __device__ bool load_bin(Pick &k, Row &r, int b) {
     for (int step = 32; step > 0; step >>= 1)
       if (c + step < r.nb && k.seg[c + step] <= i) c += step;
     const int at = c * kChunk + r.s->at[(r.ch0 + c) * kChunk + k.first[c] + (i - k.seg[c])];
-    const uint32_t key = key_of(r.l[at]);
+    const float v = r.l[at];
+    const uint32_t key = key_of(v);
     k.key[i] = key;
     k.idx[i] = (uint32_t)at;
-    k.w[i] = weight(key, r.top, r.inv_t, k.tab);
+    k.w[i] = weight(r.sc, v, k.tab);
     if (i == t) first = key;
     d |= key ^ first;
   }
@@ -508,14 +502,14 @@ __device__ Place find_place(Pick &k, Row &r, int want, u64 target) {
         k,
         [&](auto f) {
           for (int i = t; i < r.V; i += 1024) {
-            const uint32_t key = key_of(r.l[i]);
-            if (key > kNegInf && bin_of(r.bins, key) == b) f(key, weight(key, r.top, r.inv_t, k.tab));
+            const float v = r.l[i];
+            if (v > -__builtin_inff() && bin_of(r.sc, v) == b) f(key_of(v), weight(r.sc, v, k.tab));
           }
         },
         0, 32, k.cnt[b], k.sum[b], want, target);
   }
   // of the elements with the key, the number of those before this one
-  p.w = weight(at.key, r.top, r.inv_t, k.tab);
+  p.w = weight(r.sc, key_value(at.key), k.tab);
   int ties = want - at.above - 1;
   if (BY_SUM) {
     const u64 before = p.w ? (target - at.sum) / p.w : 0;
@@ -552,16 +546,14 @@ __device__ Place find_place(Pick &k, Row &r, int want, u64 target) {
 }
 
 // the smallest key whose weight reaches min_p (at most the largest one's)
-__device__ uint32_t least_key(uint32_t top, double inv_t, double min_p) {
-  const double max = (double)key_value(top);
+__device__ uint32_t least_key(const Scale &sc, double min_p) {
   auto reaches = [&](uint32_t c) {
-    return c >= top || (c > kNegInf && top != kPosInf && exp(((double)key_value(c) - max) * inv_t) >= min_p);
+    return c >= sc.top || (c > kNegInf && sc.top != kPosInf && exp((sc.max - (double)key_value(c)) * sc.neg_inv_t) >= min_p);
   };
   // near max + T log min_p: 64 keys at a time
   const int lane = threadIdx.x & 63;
-  const float guess = (float)(max + log(min_p) / inv_t);
-  const uint32_t g = key_of(guess);
-  if (g > kNegInf + 64 && g < top) {
+  const uint32_t g = key_of((float)(sc.max - log(min_p) / sc.neg_inv_t));
+  if (g > kNegInf + 64 && g < sc.top) {
     const uint64_t m = __ballot(reaches(g - 32 + lane));
     if (m && !(m & 1)) return g - 32 + (uint32_t)__ffsll((unsigned long long)m) - 1;
   }
@@ -577,24 +569,23 @@ __global__ __launch_bounds__(1024) void sample_pick_kernel(SampleArgs a, Scratch
   u64 top;
   uint32_t low;
   row_ends(s, blockIdx.x, nb, &top, &low);
-  Row r;
-  r.top = (uint32_t)(top >> 32);
+  const uint32_t tk = (uint32_t)(top >> 32);
   const float T = temp_of(a, row);
-  if (r.top == kNegInf || !(T > 0.0f)) {
+  if (tk == kNegInf || !(T > 0.0f)) {
     if (t == 0) {
-      const bool none = r.top == kNegInf;
+      const bool none = tk == kNegInf;
       a.token[row] = none ? -1 : (int)~(uint32_t)top;
       if (a.prob) a.prob[row] = none ? 0.0f : 1.0f;
     }
     return;
   }
+  Row r;
   r.l = a.logits + (size_t)row * a.ld;
   r.s = &s;
   r.ch0 = (size_t)blockIdx.x * nb;
   r.V = a.V;
   r.nb = nb;
-  r.inv_t = 1.0 / (double)T;
-  r.bins = bins_of(r.top, low, (double)T);
+  r.sc = scale_of(tk, low, (double)T);
   r.lo = 0;
   r.hi = -1;
   r.n = 0;
@@ -668,8 +659,8 @@ __global__ __launch_bounds__(1024) void sample_pick_kernel(SampleArgs a, Scratch
   }
   if (min_p > 0.0f) {
     // those from the least key on, as far as they are among those that stay
-    const uint32_t thr = least_key(r.top, r.inv_t, (double)min_p);
-    const int b = bin_of(r.bins, thr);
+    const uint32_t thr = least_key(r.sc, (double)min_p);
+    const int b = bin_of(r.sc, key_value(thr));
     u64 sum = 0;
     int from = b;
     if (load_bin(k, r, b)) {
@@ -678,8 +669,8 @@ __global__ __launch_bounds__(1024) void sample_pick_kernel(SampleArgs a, Scratch
       from = r.lo;
     } else {
       for (int i = t; i < r.V; i += 1024) {
-        const uint32_t key = key_of(r.l[i]);
-        if (key >= thr && bin_of(r.bins, key) == b) sum += weight(key, r.top, r.inv_t, k.tab);
+        const float v = r.l[i];
+        if (key_of(v) >= thr && bin_of(r.sc, v) == b) sum += weight(r.sc, v, k.tab);
       }
     }
     sum = wave_scan(sum);
@@ -701,24 +692,33 @@ __global__ __launch_bounds__(1024) void sample_pick_kernel(SampleArgs a, Scratch
   }
 }
 
-// rows per batch: enough chunks for every CU, a bounded scratch
-constexpr int kBatch = 128;
+int chunks_of(int V) { return (V + kChunk - 1) / kChunk; }
 
 }  // namespace
 
+// rows of a batch: some rounds of chunks for every CU, a scratch of about 110 MB at most
+int sample_batch(int V) { return 8192 / chunks_of(V); }
+
 size_t sample_workspace(int rows, int V) {
-  return scratch_row((V + kChunk - 1) / kChunk) * (rows < kBatch ? rows : kBatch);
+  const int n = sample_batch(V);
+  return scratch_row(chunks_of(V)) * (rows < n ? rows : n);
 }
 
-hipError_t sample_rows(const SampleArgs &a, void *ws, hipStream_t st) {
-  const int nb = (a.V + kChunk - 1) / kChunk;
-  for (int r0 = 0; r0 < a.rows; r0 += kBatch) {
-    const int n = a.rows - r0 < kBatch ? a.rows - r0 : kBatch;
-    const Scratch s = scratch_of(ws, n, nb);
-    klaunch(sample_top_kernel, dim3(nb, n), dim3(256), 0, st, a, s, r0);
-    klaunch(sample_bins_kernel, dim3(nb, n), dim3(kBinThreads), 0, st, a, s, r0);
-    klaunch(sample_pick_kernel, dim3(n), dim3(1024), 0, st, a, s, r0, nb);
-  }
+hipError_t sample_top(const SampleArgs &a, void *ws, int row0, int n, hipStream_t st) {
+  const int nb = chunks_of(a.V);
+  klaunch(sample_top_kernel, dim3(nb, n), dim3(256), 0, st, a, scratch_of(ws, n, nb), row0);
+  return hipGetLastError();
+}
+
+hipError_t sample_bins(const SampleArgs &a, void *ws, int row0, int n, hipStream_t st) {
+  const int nb = chunks_of(a.V);
+  klaunch(sample_bins_kernel, dim3(nb, n), dim3(kBinThreads), 0, st, a, scratch_of(ws, n, nb), row0);
+  return hipGetLastError();
+}
+
+hipError_t sample_pick(const SampleArgs &a, void *ws, int row0, int n, hipStream_t st) {
+  const int nb = chunks_of(a.V);
+  klaunch(sample_pick_kernel, dim3(n), dim3(1024), 0, st, a, scratch_of(ws, n, nb), row0, nb);
   return hipGetLastError();
 }
 

@@ -251,9 +251,12 @@ __device__ __forceinline__ int accept_walk(const AcceptArgs &a, int b, int n, in
   }
 }
 
-// One block per (layer, sequence).  Every thread owns columns of the rows and
-// moves them in the path's order: row j's source is at j or behind it, and the
-// sources ascend, so no row is written before it has been read.
+// One block per (layer, sequence).  Every thread owns columns of the rows (16
+// bytes where the rows allow it) and moves them in the path's order, kMoves rows
+// read before they are written: row j's source is at j or behind it, and the
+// sources ascend, so no row is written before it has been read.  Bound by latency:
+// the sequence's numbers, the tree, the rows, one after the other.
+constexpr int kMoves = 8;
 template <typename T>
 __global__ __launch_bounds__(256) void tree_accept_kernel(AcceptArgs a, int cols) {
   __shared__ int path[EC_TREE_MAX];
@@ -282,10 +285,16 @@ __global__ __launch_bounds__(256) void tree_accept_kernel(AcceptArgs a, int cols
   const int len = s_len;
   if (len < 2) return;
   const size_t base = (((size_t)layer * a.t.nslots + s.slot) * a.t.C + s.past) * cols;
-  for (int c = t; c < 2 * cols; c += 256) {
+  for (int c = t; c < 2 * cols; c += blockDim.x) {
     T *rows = c < cols ? (T *)a.kc + base + c : (T *)a.vc + base + (c - cols);
-    for (int j = 1; j < len; j++)
-      if (path[j] != j) rows[(size_t)j * cols] = rows[(size_t)path[j] * cols];
+    for (int j = 1; j < len; j += kMoves) {
+      T v[kMoves];
+#pragma unroll
+      for (int i = 0; i < kMoves; i++) v[i] = rows[(size_t)path[min(j + i, len - 1)] * cols];
+#pragma unroll
+      for (int i = 0; i < kMoves; i++)
+        if (j + i < len && path[j + i] != j + i) rows[(size_t)(j + i) * cols] = v[i];
+    }
   }
 }
 
@@ -319,7 +328,12 @@ hipError_t qk_norm_rope(const NormRopeArgs &a, hipStream_t st) {
 }
 
 hipError_t tree_accept(const AcceptArgs &a, hipStream_t st) {
-  klaunch(tree_accept_kernel<uint16_t>, dim3(a.layers, a.t.B), dim3(256), 0, st, a, a.kv);
+  const dim3 grid(a.layers, a.t.B);
+  auto block = [](int cols) { return dim3(2 * cols <= 64 ? 64 : 2 * cols <= 128 ? 128 : 256); };
+  if (a.kv % 8 == 0 && !(((uintptr_t)a.kc | (uintptr_t)a.vc) & 15))
+    klaunch(tree_accept_kernel<v4u>, grid, block(a.kv / 8), 0, st, a, a.kv / 8);
+  else
+    klaunch(tree_accept_kernel<uint16_t>, grid, block(a.kv), 0, st, a, a.kv);
   return hipGetLastError();
 }
 

@@ -427,8 +427,8 @@ int ec_sample_candidates(const float *vals, const int *idx, int ncand, int vocab
  * or a negative error code (ec_last_error()) and may be captured there.
  * Arguments are checked before anything is launched.
  *
- * The batch: B sequences of N rows each (B <= 65535, B * N <= 2^22), row b * N
- * + i being node i of sequence b.
+ * The batch: B sequences of N rows each (B <= 65535, B * N <= 2^22; slots of up
+ * to 2^30 rows), row b * N + i being node i of sequence b.
  *   slot [B]       the sequence's cache slot; NULL: b
  *   past [B]       rows of the slot that are cached already
  *   nodes [B]      how many of the N rows are nodes; NULL: N.  The rows behind
@@ -446,7 +446,7 @@ int ec_sample_candidates(const float *vals, const int *idx, int ncand, int vocab
  * earlier one of the call. */
 
 /* Rows of q | k | v (fp32, H + 2 KVH heads of hd <= 512, row stride ldx) into
- * q (fp32, row stride ldq; it may be qkv itself) and the fp16 caches kc, vc
+ * q (fp32, row stride ldq; it may be qkv itself, with ldx) and the fp16 caches kc, vc
  * [nslots][C][KVH*hd] of one layer: per head of q and k
  *   y = x / sqrt(mean(x^2) + eps) * gamma    (a NULL gamma: y = x)
  * then the first rot elements (even; 0: none) rotated by the angles position *
@@ -470,7 +470,9 @@ int ec_rope_inv_freq(int rope_type, int dim, double theta, double factor, double
  * [H*hd] (row stride ldq), out likewise (ldo); q head h reads KV head h * KVH /
  * H.  max_past: the largest past of the call (it sizes the launch; a sequence
  * with a larger one takes no part).  Rows that a node does not see do not
- * reach it, whatever they hold.  Uses the library's workspace: a captured call
+ * reach it, whatever they hold.  out may be q itself, but overlap
+ * it in no other way.  A key or query with an infinity among finite ones gives
+ * NaN to the nodes that see it.  Uses the library's workspace: a captured call
  * needs one of its size before the capture, as the matrix-core GEMMs do. */
 int ec_attention_tree_dev(const float *q, int ldq, const uint16_t *kc, const uint16_t *vc, int nslots, int C, int H,
                           int KVH, int hd, const int *slot, const int *past, const int *nodes, const int *parent, int B,
@@ -488,7 +490,8 @@ int ec_attention_tree_dev(const float *q, int ldq, const uint16_t *kc, const uin
  * not drawn, a row of nothing else gives -1.  prob [rows] (nullable): the
  * drawn token's share of the sum, 1 for the largest logit, 0 for -1.  Weights
  * and sums are 64-bit in an order-independent form: equal calls give equal
- * tokens. */
+ * tokens.  Uses the library's workspace (as ec_attention_tree_dev); token and
+ * prob overlap no other array. */
 int ec_sample_dev(const float *logits, int rows, int vocab, int ld, const float *temp, const int *top_k,
                   const float *top_p, const float *min_p, const double *u, int *token, float *prob);
 
@@ -499,7 +502,7 @@ int ec_sample_dev(const float *logits, int rows, int vocab, int ld, const float 
  * token, new_past [B] past + npath, and in every layer of kc, vc
  * [layers][nslots][C][kv] the rows past + path[j] move to past + j.  No nodes,
  * or a sequence that takes no part: npath 0, next -1, new_past = past.  N <=
- * 64.  The outputs may not overlap slot, past or nodes. */
+ * 64.  The outputs overlap no other array of the call. */
 int ec_tree_accept_dev(uint16_t *kc, uint16_t *vc, int layers, int nslots, int C, int kv, const int *slot,
                        const int *past, const int *nodes, const int *parent, const int *token, const int *sampled,
                        int B, int N, int *path, int *npath, int *next, int *new_past);

@@ -171,6 +171,19 @@ def test_sample_stride_and_repeats():
     assert np.array_equal(a[0], b[0]) and np.array_equal(a[1].view(np.uint32), b[1].view(np.uint32))
 
 
+def test_sample_many_rows():
+    """More rows than a batch takes."""
+    rng = np.random.default_rng(17)
+    V = 9000  # 3 chunks: 2730 rows a batch
+    x = np.tile(rng.normal(0, 2, (60, V)).astype(np.float32), (50, 1))
+    u = rng.random(len(x))
+    T = rng.uniform(0.2, 1.5, len(x)).astype(np.float32)
+    tok, prob = ec.sample_dev(x, u, T)
+    for r in [*range(0, 60), *range(2700, 2760), *range(2990, 3000)]:
+        want = ref_sample(x[r], u[r], T[r])
+        assert tok[r] == want[0] and abs(prob[r] - want[1]) <= 2 * U * want[1] + 1e-12
+
+
 def test_sample_as_the_driver():
     """With top_k alone and the driver's number the driver's token."""
     rng = np.random.default_rng(12)
@@ -416,6 +429,21 @@ def test_attention_strides_and_alignment(H, KVH, hd):
     finally:
         for b in bufs:
             b.close()
+
+
+@pytest.mark.parametrize("H,KVH,hd,past", [(14, 2, 64, [900, 5]), (14, 2, 64, [9, 5]), (5, 1, 7, [90, 5])])
+def test_attention_in_place(H, KVH, hd, past):
+    """out = q, with splits and without."""
+    c = attn_case(42, H, KVH, hd, 2, 6, past)
+    want = check_attention(c)
+    with ec._Call() as k:
+        q, kc, vc = k.put("q", c["q"], np.float32), k.put("kc", c["kc"], np.uint16), k.put("vc", c["vc"], np.uint16)
+        nslots, Cr, _ = c["kc"].shape
+        E = H * hd
+        rc = ec.lib().ec_attention_tree_dev(q, E, kc, vc, nslots, Cr, H, KVH, hd, *k.tree(c["slot"], c["past"], None, c["parent"]),
+                                            2, 6, Cr, 0, q, E)
+        assert rc == 0 and ec.lib().ec_sync() == 0
+        assert np.array_equal(k.get("q", np.float32, (12, E)), want)
 
 
 def test_attention_past_32_bits():
@@ -679,6 +707,18 @@ def test_accept_bad_numbers(name, at, value):
         check_accept(c, bad=(1,))
 
 
+@pytest.mark.parametrize("kv", [128, 12])
+def test_accept_long_moves(kv):
+    """Paths of 32 and 63 rows of which every one moves."""
+    c = accept_case(21, 2, kv, 2, 64, [7, 30])
+    c["parent"][0] = np.maximum(np.arange(64) - 2, np.where(np.arange(64) == 0, -1, 0))
+    c["parent"][1] = np.where(np.arange(64) == 2, 0, np.arange(64) - 1)
+    c["token"][:], c["sampled"][:] = 5, 5
+    c["token"][:, 1] = 6
+    got = check_accept(c)
+    assert list(got[1]) == [32, 63]
+
+
 def test_accept_same_rows_twice():
     c = accept_case(14, 2, 64, 3, 8, [50, 57, 58], C=100)
     c["slot"][:] = 1
@@ -878,6 +918,7 @@ def test_profiled_calls():
         buf = C.create_string_buffer(1 << 16)
         assert L.ec_prof_stop(buf, len(buf)) > 0
         names = {r["kernel"] for r in json.loads(buf.value.decode())}
-        assert {"qk_norm_rope", "attention_tree", "sample", "tree_accept"} <= names
+        assert {"qk_norm_rope", "attention_tree", "attention_tree_join", "sample_top", "sample_bins", "sample_pick",
+                "tree_accept"} <= names
     finally:
         s.k.__exit__()

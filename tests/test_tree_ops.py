@@ -21,13 +21,14 @@ def refused(rc, *words):
 
 
 def sample(**k):
-    a = dict(logits=P, rows=2, vocab=100, ld=100, temp=None, top_k=None, top_p=None, min_p=None, u=P, token=P, prob=None)
+    a = dict(logits=P, rows=2, vocab=100, ld=100, temp=None, top_k=None, top_p=None, min_p=None, u=1 << 16, token=1 << 17,
+             prob=None)
     a.update(k)
     return ec.lib().ec_sample_dev(*a.values())
 
 
 def rope(**k):
-    a = dict(qkv=P, ldx=4 * 64, q=P, ldq=128, kc=P, vc=P, nslots=2, C=100, H=2, KVH=1, hd=64, qg=None, kg=None, eps=1e-6,
+    a = dict(qkv=P, ldx=4 * 64, q=1 << 17, ldq=128, kc=P, vc=P, nslots=2, C=100, H=2, KVH=1, hd=64, qg=None, kg=None, eps=1e-6,
              inv_freq=P, rot=64, layout=0, factor=1.0, slot=None, past=P, nodes=None, parent=None, B=2, N=3)
     a.update(k)
     return ec.lib().ec_qk_norm_rope_dev(*a.values())
@@ -35,20 +36,22 @@ def rope(**k):
 
 def attention(**k):
     a = dict(q=P, ldq=128, kc=P, vc=P, nslots=2, C=100, H=2, KVH=1, hd=64, slot=None, past=P, nodes=None, parent=None,
-             B=2, N=3, max_past=50, window=0, out=P, ldo=128)
+             B=2, N=3, max_past=50, window=0, out=1 << 17, ldo=128)
     a.update(k)
     return ec.lib().ec_attention_tree_dev(*a.values())
 
 
 def accept(**k):
-    a = dict(kc=P, vc=P, layers=2, nslots=2, C=100, kv=128, slot=None, past=P, nodes=None, parent=P, token=P, sampled=P,
+    a = dict(kc=P, vc=P, layers=2, nslots=2, C=100, kv=128, slot=None, past=P, nodes=None, parent=P, token=P + 64, sampled=P + 128,
              B=2, N=3, path=P + 1024, npath=P + 2048, next=P + 2100, new_past=P + 2200)
     a.update(k)
     return ec.lib().ec_tree_accept_dev(*a.values())
 
 
 @pytest.mark.parametrize("k", [dict(rows=-1), dict(vocab=0), dict(vocab=(1 << 18) + 1, ld=1 << 19), dict(ld=99),
-                               dict(rows=(1 << 22) + 1), dict(logits=None), dict(u=None), dict(token=None)])
+                               dict(rows=(1 << 22) + 1), dict(logits=None), dict(u=None), dict(token=None),
+                               dict(token=P + 2 * 400 - 4), dict(u=1 << 20, token=(1 << 20) + 12),
+                               dict(temp=1 << 20, token=1 << 20), dict(token=1 << 20, prob=(1 << 20) + 4)])
 def test_sample_refuses(k):
     refused(sample(**k), "ec_sample_dev")
 
@@ -65,14 +68,16 @@ BATCH = [dict(B=0), dict(N=0), dict(B=-1), dict(N=-1), dict(B=65536), dict(B=655
                                        dict(hd=513, ldx=1 << 20, ldq=1 << 20), dict(ldx=255), dict(ldq=127), dict(rot=63),
                                        dict(rot=66), dict(rot=-2), dict(layout=2), dict(layout=-1), dict(eps=-1e-6),
                                        dict(eps=math.nan), dict(qkv=None), dict(q=None), dict(kc=None), dict(vc=None),
-                                       dict(inv_freq=None)])
+                                       dict(inv_freq=None), dict(C=(1 << 30) + 1), dict(q=P), dict(q=P + 256, ldq=256),
+                                       dict(q=P + 4 * (5 * 256 + 255))])
 def test_rope_refuses(k):
     refused(rope(**k), "ec_qk_norm_rope_dev")
 
 
 @pytest.mark.parametrize("k", BATCH + [dict(N=65), dict(H=3, KVH=2), dict(hd=513, ldq=2000, ldo=2000), dict(ldq=127),
                                        dict(ldo=127), dict(window=-1), dict(max_past=-1), dict(max_past=101),
-                                       dict(q=None), dict(kc=None), dict(vc=None), dict(out=None)])
+                                       dict(q=None), dict(kc=None), dict(vc=None), dict(out=None), dict(out=P, ldo=256),
+                                       dict(out=P + 512)])
 def test_attention_refuses(k):
     refused(attention(**k), "ec_attention_tree_dev")
 
@@ -80,7 +85,9 @@ def test_attention_refuses(k):
 @pytest.mark.parametrize("k", BATCH + [dict(N=65), dict(layers=0), dict(kv=0), dict(kc=None), dict(vc=None),
                                        dict(token=None), dict(sampled=None), dict(path=None), dict(npath=None),
                                        dict(next=None), dict(new_past=None), dict(new_past=P), dict(npath=P + 4),
-                                       dict(slot=P + 2096), dict(nodes=P + 2204)])
+                                       dict(slot=P + 2096), dict(nodes=P + 2204),
+                                       dict(parent=P + 1040), dict(token=P + 2048), dict(sampled=P + 1024),
+                                       dict(npath=P + 2104), dict(next=P + 1044)])
 def test_accept_refuses(k):
     refused(accept(**k), "ec_tree_accept_dev")
 
