@@ -8,6 +8,7 @@
 // in fp32 (a row that sees nothing gives 0).  What a row does not see does not
 // reach it, finite or not.
 #include <cfloat>
+#include <type_traits>
 
 #include "ec_device.h"
 #include "ec_kernels.h"
@@ -262,32 +263,39 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_tree_kernel(TreeAttnArgs a,
   bool ok = ec_tree_seq_ok(&a.t, s);
   const int rows = ec_tree_rows(&a.t, s) * G;
   if (r0 >= rows) return;
-  const int end = s.past + s.n, lo0 = window_lo(a.window, s.past, 0);
-  const int lo_all = window_lo(a.window, s.past, s.n - 1);
+  const int end = ok ? s.past + s.n : 1, lo0 = ok ? window_lo(a.window, s.past, 0) : 0;
+  const int lo_all = ok ? window_lo(a.window, s.past, s.n - 1) : 0;
   const int tiles = ok ? (end - lo0 + kTp - 1) / kTp : 1;
   const int tile0 = split_at(tiles, split, gr.ns), tile1 = split_at(tiles, split + 1, gr.ns);
   if (tile0 == tile1) return;
 
-  // the tiles' way into LDS: a wave's instruction fills 64 chunks, lane l the
-  // l-th of them, with the chunk that the swizzle puts there
+  // The tiles' way into LDS: a wave's instruction fills 64 chunks, lane l the l-th
+  // of them, with the chunk that the swizzle puts there.  In the sequence's last
+  // tile the rows behind the nodes are the last node's again (no row sees them).
   const size_t kv = (size_t)a.KVH * HD, base = ok ? (size_t)s.slot * a.t.C * kv + (size_t)kvh * HD : 0;
-  const uint16_t *Kc = a.kc + base, *Vc = a.vc + base;
-  auto load = [&](int tile, int buf) {
-    const int p0 = lo0 + tile * kTp;
-    const uint16_t *Kt = Kc + (size_t)p0 * kv, *Vt = Vc + (size_t)p0 * kv;
+  const int rest = end - lo0 - (tiles - 1) * kTp;  // rows of the last tile
+  uint32_t off[LPT], off_last[LPT];
+#pragma unroll
+  for (int u = 0; u < LPT; u++) {
+    const int ch = (w * LPT + u) * 64 + lane, r = ch / CPR, cc = 8 * ((ch - r * CPR) ^ swz<HD>(r));
+    off[u] = (uint32_t)r * (uint32_t)kv + cc;
+    off_last[u] = (uint32_t)min(r, rest - 1) * (uint32_t)kv + cc;
+  }
+  constexpr int kBuf = 2 * kTp * HD;  // elements of a buffer: K, then V
+  const uint16_t *kn = a.kc + base + (size_t)(lo0 + tile0 * kTp) * kv, *vn = a.vc + base + (size_t)(lo0 + tile0 * kTp) * kv;
+  auto load = [&](bool last, int to) {
 #pragma unroll
     for (int u = 0; u < LPT; u++) {
       const int first = (w * LPT + u) * 64;
       if (kTp * CPR % NT && first >= kTp * CPR) break;
-      const int ch = first + lane, r = ch / CPR, cc = (ch - r * CPR) ^ swz<HD>(r);
-      // rows behind the nodes: the last node's again (no row sees them)
-      const size_t off = (size_t)min(r, end - 1 - p0) * kv + 8 * cc;
-      _Float16 *dst = lds + (size_t)buf * 2 * kTp * HD + first * 8;
-      __builtin_amdgcn_global_load_lds((gvoid *)(Kt + off), (lvoid *)dst, 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((gvoid *)(Vt + off), (lvoid *)(dst + kTp * HD), 16, 0, 0);
+      const uint32_t o = last ? off_last[u] : off[u];
+      __builtin_amdgcn_global_load_lds((gvoid *)(kn + o), (lvoid *)(lds + to + first * 8), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((gvoid *)(vn + o), (lvoid *)(lds + to + kTp * HD + first * 8), 16, 0, 0);
     }
+    kn += kTp * kv;
+    vn += kTp * kv;
   };
-  if (ok) load(tile0, 0);
+  if (ok) load(tile0 + 1 == tiles, 0);
 
   // the nodes' ancestors, where a tile of this block has rows that not all see
   // (with one split the only check of the parents)
@@ -368,19 +376,21 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_tree_kernel(TreeAttnArgs a,
 #pragma unroll
   for (int d = 0; d < DT; d++) o[d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 
-  int buf = 0;
-  for (int tile = tile0; tile < tile1; tile++, buf ^= 1) {
+  int buf = 0;  // of this tile: 0 or kBuf
+  // One tile.  EDGE: one that some rows see in part: what they do not see has weight
+  // 0, and its values must be finite for that to be nothing.
+  auto step = [&](auto edge, int tile) {
+    constexpr bool EDGE = decltype(edge)::value;
     const int p0 = lo0 + tile * kTp;
     // this tile has landed, and every wave is done with the one before it
     __builtin_amdgcn_s_waitcnt(0);
     asm volatile("s_barrier" ::: "memory");
-    if (tile + 1 < tile1) load(tile + 1, buf ^ 1);
-    _Float16 *K = lds + (size_t)buf * 2 * kTp * HD, *V = K + kTp * HD;
-    // a tile that some rows see in part: what they do not see has weight 0, and
-    // its values must be finite for that to be nothing
-    const bool mixed = p0 + kTp > s.past || p0 < lo_all;
+    if (tile + 1 < tile1) load(tile + 2 == tiles, kBuf - buf);
+    _Float16 *K = lds + buf, *V = K + kTp * HD;
+    const uint32_t vat = vbase + 2 * (uint32_t)buf;
+    buf = kBuf - buf;
     bool inf = false;
-    if (mixed) {
+    if constexpr (EDGE) {
       for (int ch = t; ch < kTp * CPR; ch += NT) {
         v4u *at = reinterpret_cast<v4u *>(V) + ch, v = *at;
         uint32_t hit = 0;
@@ -399,7 +409,7 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_tree_kernel(TreeAttnArgs a,
       }
       inf = __syncthreads_or(inf);
     }
-    if (!work) continue;
+    if (!work) return;
 
     // ---- scores: sc[pt][r] of position 16 pt + 4 lg + r ----
     v4f sc[4];
@@ -416,7 +426,7 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_tree_kernel(TreeAttnArgs a,
     }
 
     // ---- weights ----
-    if (mixed) {
+    if constexpr (EDGE) {
       const uint64_t on = tile_mask(p0, lo, s.past, see) >> (4 * lg);
 #pragma unroll
       for (int pt = 0; pt < 4; pt++)
@@ -424,7 +434,7 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_tree_kernel(TreeAttnArgs a,
         for (int r = 0; r < 4; r++)
           if (!((on >> (16 * pt + r)) & 1)) sc[pt][r] = -__builtin_inff();
     }
-    if (!plain) {
+    if (__builtin_expect(!plain, 0)) {
 #pragma unroll
       for (int pt = 0; pt < 4; pt++)
 #pragma unroll
@@ -437,7 +447,7 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_tree_kernel(TreeAttnArgs a,
     for (int pt = 0; pt < 4; pt++)
 #pragma unroll
       for (int r = 0; r < 4; r++) top = fmaxf(top, sc[pt][r]);
-    if (__ballot(top > lim)) {
+    if (__builtin_expect(__ballot(top > lim) != 0, 0)) {
       const float big = row_max(top);
       const bool first = mx == -FLT_MAX, move = big > (first ? -FLT_MAX : kLift);
       const float by = move ? big - kLift : 0.0f, back = first ? 0.0f : __builtin_amdgcn_exp2f(-by);
@@ -475,7 +485,6 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_tree_kernel(TreeAttnArgs a,
     }
 
     // ---- outputs: o[d][r] of element 16 d + 4 lg + r ----
-    const uint32_t vat = vbase + (uint32_t)buf * (4 * kTp * HD);
 #pragma unroll
     for (int u = 0; u < 2; u++)
 #pragma unroll
@@ -490,7 +499,7 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_tree_kernel(TreeAttnArgs a,
       }
 
     // values that are not finite, for the rows that see them, one by one
-    if (inf) {
+    if (EDGE && __builtin_expect(inf, 0)) {
       const uint64_t on = tile_mask(p0, lo, s.past, see);
       for (int pp = 0; pp < kTp && p0 + pp < end; pp++) {
         float wgt = 0.0f;
@@ -505,13 +514,19 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_tree_kernel(TreeAttnArgs a,
           for (int d = 0; d < DT; d++)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-              const uint16_t v = Vc[(size_t)(p0 + pp) * kv + 16 * d + 4 * lg + r];
+              const uint16_t v = a.vc[base + (size_t)(p0 + pp) * kv + 16 * d + 4 * lg + r];
               if ((v & 0x7C00u) == 0x7C00u) o[d][r] += wgt * h2f(v);
             }
         }
       }
     }
-  }
+  };
+  // the tiles that every row sees whole, and those in front of and behind them
+  const int whole0 = min(max(lo_all - lo0 + kTp - 1, 0) / kTp, tile1), whole1 = max(s.past - lo0, 0) / kTp;
+  int tile = tile0;
+  for (; tile < whole0; tile++) step(std::true_type{}, tile);
+  for (; tile < min(whole1, tile1); tile++) step(std::false_type{}, tile);
+  for (; tile < tile1; tile++) step(std::true_type{}, tile);
 
   const float l = row_sum(sum);
   if (!live) return;
