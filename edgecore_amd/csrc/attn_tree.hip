@@ -326,7 +326,7 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_tree_kernel(TreeAttnArgs a,
                        (uint32_t)__shfl((int)(uint32_t)anc, src, 64);
   const int lo = window_lo(a.window, s.past, __shfl(depth, src, 64));
   // q in units of log2, so that a product is an exponent.  A row is brought
-  // into the parts' range by a power of two where its largest is outside [2^-2,
+  // into the parts' range by a power of two where its largest is outside [2^-4,
   // 2^15) (below, the low parts' steps of 2^-24 would count).
   v4u qh[KS], ql[KS];
   float up, down;
@@ -346,7 +346,7 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_tree_kernel(TreeAttnArgs a,
     }
     big = row_max(big);
     int e = 0;
-    if (!(big >= 0.25f && big < 32768.0f) && big > 0.0f)
+    if (!(big >= 0.0625f && big < 32768.0f) && big > 0.0f)
       e = min(max(14 - ((int)(__float_as_uint(big) >> 23) - 127), -126), 100);
     up = __uint_as_float((uint32_t)(e + 127) << 23);
     down = __uint_as_float((uint32_t)(127 - e) << 23);

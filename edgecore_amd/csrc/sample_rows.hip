@@ -177,13 +177,16 @@ __global__ __launch_bounds__(256) void sample_top_kernel(SampleArgs a, Scratch s
   }
 }
 
-// the row's largest (key << 32 | ~index) and smallest, by every wave
-__device__ __forceinline__ void row_ends(const Scratch &s, int row, int nb, u64 *top, uint32_t *low) {
-  const int lane = threadIdx.x & 63;
-  const size_t at = (size_t)row * nb + min(lane, nb - 1);
-  *top = wave_max64(s.top[at]);
-  *low = wave_min32(s.low[at]);
+// the row's largest (key << 32 | ~index) and smallest, by every wave: read, then joined
+struct Ends {
+  u64 top;
+  uint32_t low;
+};
+__device__ __forceinline__ Ends read_ends(const Scratch &s, int row, int nb) {
+  const size_t at = (size_t)row * nb + min((int)(threadIdx.x & 63), nb - 1);
+  return Ends{s.top[at], s.low[at]};
 }
+__device__ __forceinline__ Ends row_ends(Ends e) { return Ends{wave_max64(e.top), wave_min32(e.low)}; }
 
 __device__ __forceinline__ float temp_of(const SampleArgs &a, int row) { return a.temp ? a.temp[row] : 1.0f; }
 
@@ -220,12 +223,10 @@ __global__ __launch_bounds__(kBinThreads) void sample_bins_kernel(SampleArgs a, 
 #pragma unroll
   for (int j = 0; j < PT; j++) v[j] = l[min(c0 + t + kBinThreads * j, a.V - 1)];
   const float T = temp_of(a, row0 + row);
-  u64 top;
-  uint32_t low;
-  row_ends(s, row, nb, &top, &low);
-  const uint32_t tk = (uint32_t)(top >> 32);
+  const Ends ends = row_ends(read_ends(s, row, nb));
+  const uint32_t tk = (uint32_t)(ends.top >> 32);
   if (!(T > 0.0f) || tk == kNegInf) return;  // the largest logit, or none: nothing to weigh
-  const Scale sc = scale_of(tk, low, (double)T);
+  const Scale sc = scale_of(tk, ends.low, (double)T);
   s_sum[t] = 0;
   s_cnt[t] = 0;
   if (t < 32) s_tab[t] = ec_exp2_32[t];
@@ -271,7 +272,7 @@ struct Pick {
   // the row's bins: number and sum of w of the elements before a bin
   int cnt[kBins + 1];
   u64 sum[kBins + 1];
-  uint16_t start[kMaxChunks][kBins];  // a bin's first place in each chunk's order
+  __attribute__((aligned(4))) uint16_t start[kMaxChunks][kBins];  // a bin's first place in each chunk's order
   int live[kMaxChunks];
   // the elements of a run of bins, in any order; up to kSorted of them in order
   // instead, with the sum of w up to each
@@ -566,15 +567,32 @@ __device__ uint32_t least_key(const Scale &sc, double min_p) {
 __global__ __launch_bounds__(1024) void sample_pick_kernel(SampleArgs a, Scratch s, int row0, int nb) {
   __shared__ Pick k;
   const int t = threadIdx.x, lane = t & 63, w = t >> 6, row = row0 + blockIdx.x;
-  u64 top;
-  uint32_t low;
-  row_ends(s, blockIdx.x, nb, &top, &low);
-  const uint32_t tk = (uint32_t)(top >> 32);
+  // The chunks' bins: two of them a thread, every fourth chunk, kRead chunks read at
+  // a time (the chunks' blocks ran on other XCDs, so every read goes past this one's
+  // L2), and the row's ends before them.
+  constexpr int kRead = 10, kGroups = 1024 / (kBins / 2);
+  const int b2 = 2 * (t & (kBins / 2 - 1)), group = t / (kBins / 2);
+  const size_t ch0 = (size_t)blockIdx.x * nb;
+  typedef u64 u64x2 __attribute__((ext_vector_type(2)));
+  u64x2 x[kRead];
+  uint32_t y[kRead];
+  auto read = [&](int c0) {
+#pragma unroll
+    for (int i = 0; i < kRead; i++) {
+      const size_t ch = ch0 + min(c0 + kGroups * i, nb - 1);
+      x[i] = *reinterpret_cast<const u64x2 *>(s.sum + ch * kBins + b2);
+      y[i] = *reinterpret_cast<const uint32_t *>(s.start + ch * kBins + b2);
+    }
+  };
+  const Ends part = read_ends(s, blockIdx.x, nb);
   const float T = temp_of(a, row);
+  read(group);
+  const Ends ends = row_ends(part);
+  const uint32_t tk = (uint32_t)(ends.top >> 32);
   if (tk == kNegInf || !(T > 0.0f)) {
     if (t == 0) {
       const bool none = tk == kNegInf;
-      a.token[row] = none ? -1 : (int)~(uint32_t)top;
+      a.token[row] = none ? -1 : (int)~(uint32_t)ends.top;
       if (a.prob) a.prob[row] = none ? 0.0f : 1.0f;
     }
     return;
@@ -582,10 +600,10 @@ __global__ __launch_bounds__(1024) void sample_pick_kernel(SampleArgs a, Scratch
   Row r;
   r.l = a.logits + (size_t)row * a.ld;
   r.s = &s;
-  r.ch0 = (size_t)blockIdx.x * nb;
+  r.ch0 = ch0;
   r.V = a.V;
   r.nb = nb;
-  r.sc = scale_of(tk, low, (double)T);
+  r.sc = scale_of(tk, ends.low, (double)T);
   r.lo = 0;
   r.hi = -1;
   r.n = 0;
@@ -593,33 +611,31 @@ __global__ __launch_bounds__(1024) void sample_pick_kernel(SampleArgs a, Scratch
   const float top_p = a.top_p ? a.top_p[row] : 1.0f, min_p = a.min_p ? a.min_p[row] : 0.0f;
   const double u = a.u[row];
 
-  // The chunks' bins, added up: half of the chunks per thread, kRead of them read
-  // at a time (the chunks' blocks ran on other XCDs, so every read goes past this
-  // one's L2).  A bin's first place, added over the chunks, is the number of elements
+  // Added up.  A bin's first place, added over the chunks, is the number of elements
   // before it.
   {
-    constexpr int kRead = 20;
-    const int b = t & (kBins - 1), half = t / kBins;
-    static_assert(kBins == 512, "two threads a bin");
-    u64 sum = 0;
-    int before = 0;
-    for (int c0 = half; c0 < nb; c0 += 2 * kRead) {
-      u64 x[kRead];
-      uint16_t y[kRead];
-#pragma unroll
-      for (int i = 0; i < kRead; i++) {
-        const size_t ch = r.ch0 + min(c0 + 2 * i, nb - 1);
-        x[i] = s.sum[ch * kBins + b];
-        y[i] = s.start[ch * kBins + b];
-      }
+    u64 sum0 = 0, sum1 = 0;
+    int before0 = 0, before1 = 0;
+    for (int c0 = group; c0 < nb; c0 += kGroups * kRead) {
+      if (c0 != group) read(c0);
 #pragma unroll
       for (int i = 0; i < kRead; i++)
-        if (c0 + 2 * i < nb) {
-          sum += x[i];
-          before += y[i];
-          k.start[c0 + 2 * i][b] = y[i];
+        if (c0 + kGroups * i < nb) {
+          sum0 += x[i].x;
+          sum1 += x[i].y;
+          before0 += (int)(y[i] & 0xFFFFu);
+          before1 += (int)(y[i] >> 16);
+          *reinterpret_cast<uint32_t *>(&k.start[c0 + kGroups * i][b2]) = y[i];
         }
     }
+    // the groups' sums in the place of the elements, which come later
+    u64(*part_sum)[kBins] = reinterpret_cast<u64(*)[kBins]>(k.w);
+    int(*part_cnt)[kBins] = reinterpret_cast<int(*)[kBins]>(k.key);
+    static_assert(kGroups * kBins <= kCap, "room for them");
+    part_sum[group][b2] = sum0;
+    part_sum[group][b2 + 1] = sum1;
+    part_cnt[group][b2] = before0;
+    part_cnt[group][b2 + 1] = before1;
     if (t < 64) {
       const int n = t < nb ? (int)s.live[r.ch0 + t] : 0;
       k.live[t] = n;
@@ -627,22 +643,23 @@ __global__ __launch_bounds__(1024) void sample_pick_kernel(SampleArgs a, Scratch
       if (t == 63) k.cnt[kBins] = all;
     }
     if (t < 32) k.tab[t] = ec_exp2_32[t];
-    if (half) {
-      k.sum[b] = sum;
-      k.cnt[b] = before;
-    }
     __syncthreads();
-    u64 upto = 0;
-    if (!half) {
-      upto = wave_scan(sum + k.sum[b]);
-      before += k.cnt[b];
+    u64 sum = 0, upto = 0;
+    int before = 0;
+    if (t < kBins) {
+#pragma unroll
+      for (int g = 0; g < kGroups; g++) {
+        sum += part_sum[g][t];
+        before += part_cnt[g][t];
+      }
+      upto = wave_scan(sum);
       if (lane == 63) k.wave_w[w] = upto;
     }
     __syncthreads();
-    if (!half) {
+    if (t < kBins) {
       for (int i = 0; i < w; i++) upto += k.wave_w[i];
-      k.sum[b + 1] = upto;
-      k.cnt[b] = before;
+      k.sum[t + 1] = upto;
+      k.cnt[t] = before;
       if (t == 0) k.sum[0] = 0;
     }
     __syncthreads();
@@ -652,8 +669,8 @@ __global__ __launch_bounds__(1024) void sample_pick_kernel(SampleArgs a, Scratch
   if (top_k > 0 && top_k < k.cnt[kBins]) total = find_place<false, false>(k, r, top_k, 0).upto;
   if (top_p < 1.0f) {
     // up to the element at which the sum reaches top_p of it: passes ceil(top_p sum) - 1
-    const double x = ceil((double)top_p * (double)total) - 1.0;
-    u64 target = x > 0.0 ? (u64)x : 0;
+    const double at = ceil((double)top_p * (double)total) - 1.0;
+    u64 target = at > 0.0 ? (u64)at : 0;
     if (target >= total) target = total - 1;
     total = find_place<true, false>(k, r, 0, target).upto;
   }
@@ -682,8 +699,8 @@ __global__ __launch_bounds__(1024) void sample_pick_kernel(SampleArgs a, Scratch
     total = sum < total ? sum : total;
   }
   // the draw: running sum above u total
-  const double x = u * (double)total;
-  u64 target = x > 0.0 ? x < (double)total ? (u64)x : total - 1 : u == u ? 0 : total - 1;
+  const double at = u * (double)total;
+  u64 target = at > 0.0 ? at < (double)total ? (u64)at : total - 1 : u == u ? 0 : total - 1;
   if (target >= total) target = total - 1;
   const Place p = find_place<true, true>(k, r, 0, target);
   if (t == 0) {
