@@ -297,26 +297,29 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_tree_kernel(TreeAttnArgs a,
   };
   if (ok) load(tile0 + 1 == tiles, 0);
 
-  // the nodes' ancestors, where a tile of this block has rows that not all see
-  // (with one split the only check of the parents)
+  // the parents, and the nodes' ancestors where a tile of this block has rows that
+  // not all see
   uint64_t anc = 0;
   int depth = 0;
-  if (ok && (gr.ns == 1 || lo0 + tile1 * kTp > s.past || lo0 + tile0 * kTp < lo_all)) {
+  if (ok) {
     const int p = tree_parent(a.t, b, s.n, &ok);
-    if (ok) {
+    if (ok && (lo0 + tile1 * kTp > s.past || lo0 + tile0 * kTp < lo_all)) {
       anc = tree_ancestors(p, &depth);
       if (a.window > 0 && a.window < EC_TREE_MAX)
         for (int j = 0; j < s.n; j++)
           if (depth - __shfl(depth, j, 64) >= a.window) anc &= ~(1ull << j);
     }
   }
-  if (!ok) {  // the join marks the rows, or this block does
+  const size_t all = (size_t)a.t.B * a.t.N * a.H, part = (size_t)split * all;  // rows of a split's results
+  float2 *const ml = (float2 *)((float *)a.ws + (size_t)gr.ns * all * HD) + part;
+  if (!ok) {  // NaN as a row's sum, or the row itself
     __builtin_amdgcn_s_waitcnt(0);
-    if (gr.ns == 1)
-      for (int e = t; e < min(rows - r0, 16 * NW) * HD; e += NT) {
-        const int r = r0 + e / HD;
-        a.out[(m0 + r / G) * a.ldo + (size_t)(kvh * G + r % G) * HD + e % HD] = __builtin_nanf("");
-      }
+    for (int e = t; e < min(rows - r0, 16 * NW) * HD; e += NT) {
+      const int r = r0 + e / HD;
+      const size_t node = m0 + r / G, h = kvh * G + r % G;
+      if (gr.ns == 1) a.out[node * a.ldo + h * HD + e % HD] = __builtin_nanf("");
+      else if (e % HD == 0) ml[node * a.H + h] = make_float2(0.0f, __builtin_nanf(""));
+    }
     return;
   }
 
@@ -538,11 +541,11 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_tree_kernel(TreeAttnArgs a,
       *reinterpret_cast<float4 *>(out + 16 * d) =
           make_float4(o[d][0] * inv, o[d][1] * inv, o[d][2] * inv, o[d][3] * inv);
   } else {
-    const size_t all = (size_t)a.t.B * a.t.N * a.H, at = (size_t)split * all + (m0 + node) * a.H + head;
-    float *po = (float *)a.ws + at * HD + 4 * lg;
+    const size_t at = (m0 + node) * a.H + head;
+    float *po = (float *)a.ws + (part + at) * HD + 4 * lg;
 #pragma unroll
     for (int d = 0; d < DT; d++) *reinterpret_cast<float4 *>(po + 16 * d) = make_float4(o[d][0], o[d][1], o[d][2], o[d][3]);
-    if (lg == 0) ((float2 *)((float *)a.ws + (size_t)gr.ns * all * HD))[at] = make_float2(mx, l);
+    if (lg == 0) ml[at] = make_float2(mx, l);
   }
 }
 
@@ -568,8 +571,7 @@ __global__ __launch_bounds__(256) void attn_tree_join_kernel(TreeAttnArgs a, int
     v[i] = *reinterpret_cast<const float4 *>(po + at * HD);
   }
   const EcTreeSeq s = ec_tree_seq(&a.t, b);
-  bool ok = ec_tree_seq_ok(&a.t, s);
-  if (ok) tree_parent(a.t, b, s.n, &ok);
+  const bool ok = ec_tree_seq_ok(&a.t, s);  // (bad parents: the splits' sums are NaN)
   const int rows = ec_tree_rows(&a.t, s) * a.H;
   if (blockIdx.x * RPB >= rows) return;
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
