@@ -50,13 +50,14 @@ __device__ __forceinline__ RopeRow rope_row(const NormRopeArgs &a, int m) {
     }
   }
   r.ok = r.ok && !tree_clashes(a.t, b, s);
-  r.pos = s.past + depth;
+  r.pos = r.ok ? s.past + depth : 0;
   r.crow = r.ok ? ((size_t)s.slot * a.t.C + (s.past + i)) * ((size_t)a.KVH * a.hd) : 0;
   return r;
 }
 
 // The form for any head size and alignment: one block per token, a wave a head at
-// a time, its elements through the wave's row in LDS.
+// a time, its elements through the wave's row in LDS.  333 rows of 10 + 2 x 5 heads of
+// 80 take 9.7 us here, 5.9 in the form below.
 constexpr int kRopeMaxHd = 512;
 __global__ __launch_bounds__(256) void qk_norm_rope_any_kernel(NormRopeArgs a) {
   __shared__ float row[4][kRopeMaxHd];
@@ -113,119 +114,107 @@ __global__ __launch_bounds__(256) void qk_norm_rope_any_kernel(NormRopeArgs a) {
 }
 
 // The form for head sizes that are multiples of 4 up to 256 and rows of whole
-// 16-byte chunks: LPH lanes a head, four elements a lane, `rows` rows of the call a
-// block.  The norm's sum goes over the head's lanes; a pair's other element is in
-// the same lane (layout 1) or in lane +- rot / 8, which holds its four (layout 0,
-// rot a multiple of 8).  Bound by memory, every element read and written once;
-// what counts is the chain before the first store (a sequence's numbers, its
-// tree, the angles): a block goes through it once for its rows, with kAhead heads
-// a lane already on their way.
-constexpr int kRopeRows = 4, kAhead = 4;
+// 16-byte chunks: a block per row, LPH lanes a head, four elements a lane, the next
+// head's on their way while one is worked on.  The norm's sum goes over the head's
+// lanes; a pair's other element is in the same lane (layout 1) or in lane +- rot / 8,
+// which holds its four (layout 0, rot a multiple of 8).  Every element is read and
+// written once: 2048 rows of 12 + 2 x 2 heads of 128, 27.5 MB, take 8.7 us (3.2 TB/s;
+// a copy of as much 5.4), 128 rows of 14 + 2 x 2 of 64 take 5.0, a launch and the
+// chain before the first store (a sequence's numbers, its tree, the angles), which
+// blocks of their own overlap best: with two rows a block the prompt's rows took 3%
+// longer, with four 24%, with four heads of a lane ahead 14%.  The form for any size
+// takes 17.3 and 8.2.
 template <int LPH>
-__global__ __launch_bounds__(256) void qk_norm_rope_kernel(NormRopeArgs a, int rows) {
-  __shared__ float4 cs[kRopeRows][64];  // four cosines, then four sines, of four frequencies
-  __shared__ RopeRow info[kRopeRows];
-  constexpr int kGroups = 256 / LPH;
-  const int t = threadIdx.x, li = t % LPH, e = 4 * li, heads = a.H + 2 * a.KVH;
-  const int m0 = blockIdx.x * rows, n = min(rows, a.t.B * a.t.N - m0), items = n * heads;
+__global__ __launch_bounds__(256) void qk_norm_rope_kernel(NormRopeArgs a) {
+  __shared__ float4 cs[64];  // four cosines, then four sines, of four frequencies
+  __shared__ RopeRow info;
+  const int t = threadIdx.x, li = t % LPH, e = 4 * li, heads = a.H + 2 * a.KVH, groups = blockDim.x / LPH;
+  const size_t m = blockIdx.x;
   const int half = a.rot >> 1;
   const bool in = e < a.hd;
-  float4 v[kAhead];
-  int it = t / LPH;
-  auto read = [&](int i) {
+  const float *row = a.x + m * a.ldx + e;
+  auto read = [&](int h) {
     float4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (in && i < items) {
-      const int r = i / heads, h = i - r * heads;
-      x = *reinterpret_cast<const float4 *>(a.x + (size_t)(m0 + r) * a.ldx + (size_t)h * a.hd + e);
-    }
+    if (in && h < heads) x = *reinterpret_cast<const float4 *>(row + (size_t)h * a.hd);
     return x;
   };
-#pragma unroll
-  for (int j = 0; j < kAhead; j++) v[j] = read(it + j * kGroups);
+  int h = t / LPH;
+  float4 next = read(h);
   double f = 0.0;
-  if (half) f = a.inv_freq[t % half];
-  {
-    const int w = t >> 6;
-    static_assert(kRopeRows == 4, "a wave per row");
-    if (w < n) {
-      const RopeRow rr = rope_row(a, m0 + w);
-      if ((t & 63) == 0) info[w] = rr;
-    }
+  if (t < half) f = a.inv_freq[t];
+  if (t < 64) {
+    const RopeRow rr = rope_row(a, blockIdx.x);
+    if (t == 0) info = rr;
   }
   __syncthreads();
-  for (int j = t; j < n * half; j += 256) {
-    const int r = j / half, i = j - r * half;
-    const float2 c = rope_cs(info[r].pos, j == t ? f : a.inv_freq[i], a.factor);
-    float *p = reinterpret_cast<float *>(cs[r] + 2 * (i >> 2)) + (i & 3);
+  const RopeRow rr = info;
+  if (!rr.mine) return;
+  for (int j = t; j < half; j += blockDim.x) {
+    const float2 c = rope_cs(rr.pos, j == t ? f : a.inv_freq[j], a.factor);
+    float *p = reinterpret_cast<float *>(cs + 2 * (j >> 2)) + (j & 3);
     p[0] = c.x;
     p[4] = c.y;
   }
   __syncthreads();
   // a uniform count of rounds: the lanes of a wave exchange their elements in each
-  for (int i0 = 0; i0 < items; i0 += kAhead * kGroups) {
+  for (int h0 = 0; h0 < heads; h0 += groups, h += groups) {
+    float4 x = next;
+    next = read(h + groups);
+    const bool isq = h < a.H, isv = h >= a.H + a.KVH;
+    const float *gamma = isq ? a.q_gamma : isv ? nullptr : a.k_gamma;
+    float sum = x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w;
 #pragma unroll
-    for (int j = 0; j < kAhead; j++) {
-      const int i = i0 + j * kGroups + it;
-      const int r = min(i, items - 1) / heads, h = min(i, items - 1) - r * heads;
-      float4 x = v[j];
-      v[j] = read(i + kAhead * kGroups);
-      const bool isq = h < a.H, isv = h >= a.H + a.KVH;
-      const float *gamma = isq ? a.q_gamma : isv ? nullptr : a.k_gamma;
-      float sum = x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w;
-#pragma unroll
-      for (int o = LPH / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-      if (gamma && in) {
-        const float s = 1.0f / sqrtf(sum / (float)a.hd + a.eps);
-        const float4 g = *reinterpret_cast<const float4 *>(gamma + e);
-        x.x = x.x * s * g.x;
-        x.y = x.y * s * g.y;
-        x.z = x.z * s * g.z;
-        x.w = x.w * s * g.w;
-      }
-      if (a.layout) {
-        if (!isv && e < a.rot) {
-          // frequencies 2 li and 2 li + 1; where rot ends inside the lane, the first alone
-          const float *c = reinterpret_cast<const float *>(cs[r] + 2 * (li >> 1)) + 2 * (li & 1);
-          const float a0 = x.x, b0 = x.y, a1 = x.z, b1 = x.w;
-          x.x = a0 * c[0] - b0 * c[4];
-          x.y = a0 * c[4] + b0 * c[0];
-          if (e + 2 < a.rot) {
-            x.z = a1 * c[1] - b1 * c[5];
-            x.w = a1 * c[5] + b1 * c[1];
-          }
-        }
-      } else if (a.rot) {
-        const int far = half >> 2;  // lanes from an element to its pair's other one
-        const bool first = li < far;
-        const int src = ((t & 63) + (first ? far : -far)) & 63;
-        float4 o;
-        o.x = __shfl(x.x, src, 64);
-        o.y = __shfl(x.y, src, 64);
-        o.z = __shfl(x.z, src, 64);
-        o.w = __shfl(x.w, src, 64);
-        if (!isv && e < a.rot) {
-          const int k = first ? li : li - far;
-          const float4 c = cs[r][2 * k], s = cs[r][2 * k + 1];
-          const float sg = first ? -1.0f : 1.0f;
-          x.x = x.x * c.x + sg * (o.x * s.x);
-          x.y = x.y * c.y + sg * (o.y * s.y);
-          x.z = x.z * c.z + sg * (o.z * s.z);
-          x.w = x.w * c.w + sg * (o.w * s.w);
+    for (int o = LPH / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    if (gamma && in) {
+      const float s = 1.0f / sqrtf(sum / (float)a.hd + a.eps);
+      const float4 g = *reinterpret_cast<const float4 *>(gamma + e);
+      x.x = x.x * s * g.x;
+      x.y = x.y * s * g.y;
+      x.z = x.z * s * g.z;
+      x.w = x.w * s * g.w;
+    }
+    if (a.layout) {
+      if (!isv && e < a.rot) {
+        // frequencies 2 li and 2 li + 1; where rot ends inside the lane, the first alone
+        const float *c = reinterpret_cast<const float *>(cs + 2 * (li >> 1)) + 2 * (li & 1);
+        const float a0 = x.x, b0 = x.y, a1 = x.z, b1 = x.w;
+        x.x = a0 * c[0] - b0 * c[4];
+        x.y = a0 * c[4] + b0 * c[0];
+        if (e + 2 < a.rot) {
+          x.z = a1 * c[1] - b1 * c[5];
+          x.w = a1 * c[5] + b1 * c[1];
         }
       }
-      const RopeRow &rr = info[r];
-      if (!in || i >= items || !rr.mine) continue;
-      if (isq) {
-        const float nan = __builtin_nanf("");
-        if (!rr.ok) x = make_float4(nan, nan, nan, nan);
-        *reinterpret_cast<float4 *>(a.q + (size_t)(m0 + r) * a.ldq + (size_t)h * a.hd + e) = x;
-      } else if (rr.ok) {
-        uint16_t *to = isv ? a.vc + rr.crow + (size_t)(h - a.H - a.KVH) * a.hd + e : a.kc + rr.crow + (size_t)(h - a.H) * a.hd + e;
-        uint2 p;
-        p.x = (uint32_t)f2h(x.x) | (uint32_t)f2h(x.y) << 16;
-        p.y = (uint32_t)f2h(x.z) | (uint32_t)f2h(x.w) << 16;
-        *reinterpret_cast<uint2 *>(to) = p;
+    } else if (a.rot) {
+      const int far = half >> 2;  // lanes from an element to its pair's other one
+      const bool first = li < far;
+      const int src = ((t & 63) + (first ? far : -far)) & 63;
+      float4 o;
+      o.x = __shfl(x.x, src, 64);
+      o.y = __shfl(x.y, src, 64);
+      o.z = __shfl(x.z, src, 64);
+      o.w = __shfl(x.w, src, 64);
+      if (!isv && e < a.rot) {
+        const int k = first ? li : li - far;
+        const float4 c = cs[2 * k], s = cs[2 * k + 1];
+        const float sg = first ? -1.0f : 1.0f;
+        x.x = x.x * c.x + sg * (o.x * s.x);
+        x.y = x.y * c.y + sg * (o.y * s.y);
+        x.z = x.z * c.z + sg * (o.z * s.z);
+        x.w = x.w * c.w + sg * (o.w * s.w);
       }
+    }
+    if (!in || h >= heads) continue;
+    if (isq) {
+      const float nan = __builtin_nanf("");
+      if (!rr.ok) x = make_float4(nan, nan, nan, nan);
+      *reinterpret_cast<float4 *>(a.q + m * a.ldq + (size_t)h * a.hd + e) = x;
+    } else if (rr.ok) {
+      uint16_t *to = isv ? a.vc + rr.crow + (size_t)(h - a.H - a.KVH) * a.hd + e : a.kc + rr.crow + (size_t)(h - a.H) * a.hd + e;
+      uint2 p;
+      p.x = (uint32_t)f2h(x.x) | (uint32_t)f2h(x.y) << 16;
+      p.y = (uint32_t)f2h(x.z) | (uint32_t)f2h(x.w) << 16;
+      *reinterpret_cast<uint2 *>(to) = p;
     }
   }
 }
@@ -255,7 +244,9 @@ __device__ __forceinline__ int accept_walk(const AcceptArgs &a, int b, int n, in
 // bytes where the rows allow it) and moves them in the path's order, kMoves rows
 // read before they are written: row j's source is at j or behind it, and the
 // sources ascend, so no row is written before it has been read.  Bound by latency:
-// the sequence's numbers, the tree, the rows, one after the other.
+// the sequence's numbers, the tree, the rows, one after the other: 3.8 us for one
+// sequence's 8 nodes in 24 layers, 5.4 for 16 wide trees in 28 (3.7 MB at most); 6.1
+// with one row at a time, 6.7 with 2-byte columns.
 constexpr int kMoves = 8;
 template <typename T>
 __global__ __launch_bounds__(256) void tree_accept_kernel(AcceptArgs a, int cols) {
@@ -311,11 +302,9 @@ static bool rope_vector_ok(const NormRopeArgs &a) {
 
 template <int LPH>
 static void launch_rope(const NormRopeArgs &a, hipStream_t st) {
-  // rows a block: as many as its lanes hold ahead, while two blocks per CU are left
-  const int m = a.t.B * a.t.N, hold = kAhead * (256 / LPH) / (a.H + 2 * a.KVH), spread = m / 512;
-  int rows = hold < spread ? hold : spread;
-  rows = rows < 1 ? 1 : rows > kRopeRows ? kRopeRows : rows;
-  klaunch(qk_norm_rope_kernel<LPH>, dim3((m + rows - 1) / rows), dim3(256), 0, st, a, rows);
+  const long threads = (long)(a.H + 2 * a.KVH) * LPH;
+  const int block = threads >= 256 ? 256 : (int)(threads + 63) / 64 * 64;
+  klaunch(qk_norm_rope_kernel<LPH>, dim3(a.t.B * a.t.N), dim3(block), 0, st, a);
 }
 
 hipError_t qk_norm_rope(const NormRopeArgs &a, hipStream_t st) {
