@@ -24,7 +24,10 @@ __device__ __forceinline__ int window_lo(int window, int past, int depth) {
 
 // The form for any head size and alignment: one block per (node, head), tiles
 // of 256 positions, a position per thread for the scores and an element of the
-// head per thread for the sums, with the running maximum and sum.
+// head per thread for the sums, with the running maximum and sum.  Every query head
+// reads its keys and values anew, a thread a whole key: 8 nodes of 14 / 2 heads of 64
+// over 700 rows take 42 us (the matrix-core form and its join 10.6), 16 one-token
+// sequences of 12 / 12 heads over 1000 rows 91 (18).
 constexpr int kTreeMaxHd = 512;
 __global__ __launch_bounds__(256) void attn_tree_any_kernel(TreeAttnArgs a) {
   __shared__ float q[kTreeMaxHd], p_s[256], red[4];
@@ -102,9 +105,9 @@ __global__ __launch_bounds__(256) void attn_tree_any_kernel(TreeAttnArgs a) {
 
 // The matrix-core form (head sizes 32, 64, 96, 128).  One KV head serves G = H /
 // KVH query heads of n nodes: R = n G rows that share its keys and values.  A
-// block of four waves takes 64 RT rows of one KV head and a part of the
-// positions, 64 at a time: keys and values go from the cache straight into LDS,
-// the next tile while the waves work on one.
+// block of NW waves takes 16 NW rows of one KV head and a part of the positions, 64
+// at a time: keys and values go from the cache straight into LDS, the next tile
+// while the waves work on one.
 //
 // Products run transposed, K Q^T and V^T P^T, so that a lane keeps one row
 // (lane & 15): the scores' accumulators hold 16 positions of it, its maximum and
@@ -114,12 +117,24 @@ __global__ __launch_bounds__(256) void attn_tree_any_kernel(TreeAttnArgs a) {
 // lane group g takes 4 g .. 4 g + 3 of two runs of 16.  The values, rows of the
 // cache, are read for it by the transposing LDS load.
 //
-// fp32 by two 16-bit parts: q = hi + lo under a power of two that brings the
-// row's largest to 2^14 (22 bits and more of every element), weights = hi + lo
-// below 2^14; keys and values are 16 bits as they are, so two products give
-// each sum to about 2^-22.  The running maximum is raised when a score passes it
-// by 2^10 (the parts' room): nearly never after the first tile, and the
-// accumulated outputs are scaled only then.
+// fp32 by two 16-bit parts: q = hi + lo (a row whose largest is outside [2^-4, 2^15)
+// under a power of two that brings it to 2^14: its low part's steps of 2^-24 are below
+// 2^-20 of the largest at worst, and a part is cut, not rounded, so that it is two
+// instructions less), weights = hi + lo below 2^14; keys and values are 16 bits as
+// they are, so two products give each sum to about 2^-21.  The running maximum is
+// raised only when a score passes it by a factor of 2^10 (the parts' room), and the
+// accumulated outputs are scaled only then: mostly in a split's first tile.
+//
+// What bounds it.  Two sequences of 64 nodes, 14 / 2 heads of 64, over 32600 rows: 38
+// us, 23 GFLOP of matrix products in two parts, 0.6 PFLOP/s.  The matrix cores are
+// busy 41% of it, the vector ALUs (16 exponentials, maxima, sums and the weights'
+// parts, 110 instructions a tile and wave) 47%; the two overlap in part only, and
+// every wave waits for its LDS reads in four places a tile.  Half of the products left
+// out (the low parts') would save 8 us, the exponentials 2, the loads none.  Slower or
+// no faster: two tiles of rows a wave, a third buffer, the next tile's keys read or
+// multiplied ahead, operands of all products read first (registers), priorities.
+// One-token sequences are bound by memory: 16 of 12 / 12 heads over 1000 rows, 43
+// MB, take 14 us, 3.1 TB/s (a plain sum reads 4.0).
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 
@@ -551,7 +566,10 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_tree_kernel(TreeAttnArgs a,
 
 // Joins the splits' outputs: per row the largest of their maxima, the sums and
 // outputs brought to it.  HD / 4 lanes a row (a power of two of them: 24 of 32 at
-// 96).  Latency is all of it: the reads do not wait for the sequence's numbers.
+// 96).  Latency is all of it: the reads do not wait for the sequence's numbers (3.5 us
+// for 8 nodes, 5.7 for the 32 splits of 2 x 64 nodes).  The last block of a row's
+// splits could join them, without this launch; but what it counts arrivals with lives
+// from call to call, and a run that ends half way would leave it wrong for good.
 template <int HD>
 __global__ __launch_bounds__(256) void attn_tree_join_kernel(TreeAttnArgs a, int ns) {
   constexpr int LPR = HD == 96 ? 32 : HD / 4, RPB = 256 / LPR;
@@ -616,17 +634,25 @@ __global__ __launch_bounds__(256) void attn_tree_join_kernel(TreeAttnArgs a, int
     *reinterpret_cast<float4 *>(a.out + ((size_t)b * a.t.N + node) * a.ldo + (size_t)(r - node * a.H) * HD + 4 * li) = o;
 }
 
-// rows that the matrix-core form's 16-byte accesses can take
+// heads and rows that the matrix-core form's tiles and 16-byte accesses can take (both
+// sides' times stand at the form for any size)
 bool tiles_ok(const TreeAttnArgs &a) {
   const uintptr_t p = (uintptr_t)a.q | (uintptr_t)a.kc | (uintptr_t)a.vc | (uintptr_t)a.out;
   return (a.hd == 32 || a.hd == 64 || a.hd == 96 || a.hd == 128) && !(p & 15) && a.ldq % 4 == 0 && a.ldo % 4 == 0;
 }
 
-// Waves per block: 4 (64 rows) or 8 (128), by the rows that share a KV head.
+// Waves per block: 4 (64 rows) or 8 (128), by the rows that share a KV head.  Up to 64
+// rows, 8 waves would load faster but for more blocks' places: 16.8 instead of 14 us
+// for the one-token sequences above.  Over 64, 4 waves read the cache twice as often:
+// 48 instead of 38 us for the two long contexts, 18.4 instead of 17.5 for 8 trees of
+// 16 nodes, 12 / 2 heads of 128, over 4000 rows.
 int tree_waves(const TreeAttnArgs &a) { return (long)a.t.N * (a.H / a.KVH) <= 64 ? 4 : 8; }
 
-// Row blocks and splits: as many blocks as the CUs hold at a time (two of them, one of 8
-// waves at head sizes above 64), of at least a tile each.
+// Row blocks and splits: two blocks a CU, one of 8 waves at head sizes above 64 (its LDS
+// and registers leave room for no second), of at least a tile each.  Three and four a
+// CU take 41 and 42 us instead of 38 for the long contexts (the joins 8 and 10 instead
+// of 6), two of the wide ones 22 instead of 17.5 for the trees over 4000 rows; with no
+// split these take 101, 8 nodes over 700 rows 16 instead of 7 + 3.5.
 TreeGrid tree_grid(const TreeAttnArgs &a) {
   TreeGrid g;
   const int waves = tree_waves(a), per = 16 * waves;

@@ -2366,6 +2366,7 @@ extern "C" int ec_attention_dev(const float *q, int ldq, const uint16_t *kc, con
 // opened; what device arrays hold is checked in the kernels (ec_tree.h).
 constexpr long kMaxRows = 1L << 22;       // rows of a call (grids and row offsets stay in 32 bits)
 constexpr int kMaxCacheRows = 1 << 30;    // of a slot
+constexpr int kMaxKv = 1 << 28;           // elements of a cache row (twice as many columns count in an int)
 
 // A range of memory; an empty or null one overlaps nothing.
 struct Span {
@@ -2389,6 +2390,11 @@ static bool spans_clash(const Span (&in)[NI], const Span (&out)[NO]) {
 }
 static Span rows_span(const void *p, long rows, int ld, int width, size_t elem) {
   return Span{p, ((size_t)(rows - 1) * ld + width) * elem};
+}
+// a cache of fp16; one larger than any memory counts as 2^62 bytes
+static Span cache_span(const void *p, int layers, const EcTreeBatch &t, size_t kv) {
+  const double n = 2.0 * layers * t.nslots * t.C * (double)kv;
+  return Span{p, n < 0x1p62 ? (size_t)2 * layers * t.nslots * t.C * kv : (size_t)1 << 62};
 }
 
 // The library's device for the length of a call: a thread's own may be another.
@@ -2461,6 +2467,14 @@ extern "C" int ec_qk_norm_rope_dev(const float *qkv, int ldx, float *q, int ldq,
   if (!(q == qkv && ldq == ldx) &&
       rows_span(q, (long)B * N, ldq, H * hd, 4).overlaps(rows_span(qkv, (long)B * N, ldx, (H + 2 * KVH) * hd, 4)))
     return set_err(-1, "%s: q overlaps qkv and is not its first columns", fn);
+  {
+    const size_t b4 = (size_t)B * 4, n4 = b4 * N, h4 = (size_t)hd * 4, kv = (size_t)KVH * hd;
+    const Span x = rows_span(qkv, (long)B * N, ldx, (H + 2 * KVH) * hd, 4);
+    const Span in[] = {{q_gamma, h4}, {k_gamma, h4}, {inv_freq, (size_t)rot * 4}, {slot, b4}, {past, b4}, {nodes, b4}, {parent, n4}};
+    const Span out[] = {rows_span(q, (long)B * N, ldq, H * hd, 4), cache_span(kc, 1, t, kv), cache_span(vc, 1, t, kv)};
+    if (spans_clash(in, out) || x.overlaps(out[1]) || x.overlaps(out[2]))
+      return set_err(-1, "%s: q, kc or vc overlaps another array", fn);
+  }
   EC_INIT();
   const DeviceScope dev;
   const NormRopeArgs a{t, qkv, ldx, q, ldq, kc, vc, H, KVH, hd, q_gamma, k_gamma, (float)eps, inv_freq, rot, layout,
@@ -2482,6 +2496,12 @@ extern "C" int ec_attention_tree_dev(const float *q, int ldq, const uint16_t *kc
   if (!(out == q && ldo == ldq) &&
       rows_span(out, (long)B * N, ldo, H * hd, 4).overlaps(rows_span(q, (long)B * N, ldq, H * hd, 4)))
     return set_err(-1, "%s: out overlaps q and is not q", fn);
+  {
+    const size_t b4 = (size_t)B * 4, n4 = b4 * N, kv = (size_t)KVH * hd;
+    const Span in[] = {cache_span(kc, 1, t, kv), cache_span(vc, 1, t, kv), {slot, b4}, {past, b4}, {nodes, b4}, {parent, n4}};
+    const Span o[] = {rows_span(out, (long)B * N, ldo, H * hd, 4)};
+    if (spans_clash(in, o)) return set_err(-1, "%s: out overlaps another array", fn);
+  }
   EC_INIT();
   const DeviceScope dev;
   TreeAttnArgs a{t, q, ldq, kc, vc, H, KVH, hd, window, (float)(1.0 / sqrt((double)hd)), out, ldo, nullptr};
@@ -2500,14 +2520,16 @@ extern "C" int ec_tree_accept_dev(uint16_t *kc, uint16_t *vc, int layers, int ns
   const EcTreeBatch t{B, N, slot, past, nodes, parent, nslots, C, C};
   int r;
   if ((r = tree_check(fn, t, false))) return r;
-  if (layers < 1 || kv < 1) return set_err(-1, "%s: %d layers of rows of %d", fn, layers, kv);
+  if (layers < 1 || kv < 1 || kv > kMaxKv)
+    return set_err(-1, "%s: %d layers of rows of %d (up to %d)", fn, layers, kv, kMaxKv);
   if (!kc || !vc || !token || !sampled || !path || !npath || !next || !new_past)
     return set_err(-1, "%s: null pointer", fn);
   {
     const size_t b4 = (size_t)B * 4, n4 = b4 * N;
     const Span in[] = {{slot, b4}, {past, b4}, {nodes, b4}, {parent, n4}, {token, n4}, {sampled, n4}};
-    const Span out[] = {{path, n4}, {npath, b4}, {next, b4}, {new_past, b4}};
-    if (spans_clash(in, out)) return set_err(-1, "%s: an output overlaps another array", fn);
+    const Span out[] = {{path, n4}, {npath, b4}, {next, b4}, {new_past, b4}, cache_span(kc, layers, t, kv),
+                        cache_span(vc, layers, t, kv)};
+    if (spans_clash(in, out)) return set_err(-1, "%s: an output or a cache overlaps another array", fn);
   }
   EC_INIT();
   const DeviceScope dev;

@@ -424,8 +424,8 @@ int ec_sample_candidates(const float *vals, const int *idx, int ncand, int vocab
  * and the rows that these tokens confirm stay (ec_tree_accept_dev).
  *
  * All arrays are device pointers; the calls enqueue on ec_stream(), return 0
- * or a negative error code (ec_last_error()) and may be captured there.
- * Arguments are checked before anything is launched.
+ * or a negative error code (ec_last_error()) and may be captured and replayed
+ * there.  Arguments are checked before anything is launched.
  *
  * The batch: B sequences of N rows each (B <= 65535, B * N <= 2^22; slots of up
  * to 2^30 rows), row b * N + i being node i of sequence b.
@@ -452,7 +452,8 @@ int ec_sample_candidates(const float *vals, const int *idx, int ncand, int vocab
  * then the first rot elements (even; 0: none) rotated by the angles position *
  * inv_freq[rot / 2] (device, fp64), cosine and sine times factor: pairs (i, i
  * + rot / 2) for layout 0, (2 i, 2 i + 1) for layout 1.  v is copied.  Without
- * parents N is any number: prompts. */
+ * parents N is any number: prompts.  The caches overlap no other array, nor
+ * does q but as above. */
 int ec_qk_norm_rope_dev(const float *qkv, int ldx, float *q, int ldq, uint16_t *kc, uint16_t *vc, int nslots, int C,
                         int H, int KVH, int hd, const float *q_gamma, const float *k_gamma, double eps,
                         const double *inv_freq, int rot, int layout, double factor, const int *slot, const int *past,
@@ -470,10 +471,11 @@ int ec_rope_inv_freq(int rope_type, int dim, double theta, double factor, double
  * [H*hd] (row stride ldq), out likewise (ldo); q head h reads KV head h * KVH /
  * H.  max_past: the largest past of the call (it sizes the launch; a sequence
  * with a larger one takes no part).  Rows that a node does not see do not
- * reach it, whatever they hold.  out may be q itself, but overlap
- * it in no other way.  A key or query with an infinity among finite ones gives
- * NaN to the nodes that see it.  Uses the library's workspace: a captured call
- * needs one of its size before the capture, as the matrix-core GEMMs do. */
+ * reach it, whatever they hold.  out may be q itself, but overlaps no other
+ * array.  A key or query with an infinity among finite ones gives NaN to the
+ * nodes that see it, an infinite value NaN or an infinity.  Uses the library's
+ * workspace: a captured call needs one of its size before the capture, as the
+ * matrix-core GEMMs do. */
 int ec_attention_tree_dev(const float *q, int ldq, const uint16_t *kc, const uint16_t *vc, int nslots, int C, int H,
                           int KVH, int hd, const int *slot, const int *past, const int *nodes, const int *parent, int B,
                           int N, int max_past, int window, float *out, int ldo);
@@ -502,7 +504,7 @@ int ec_sample_dev(const float *logits, int rows, int vocab, int ld, const float 
  * token, new_past [B] past + npath, and in every layer of kc, vc
  * [layers][nslots][C][kv] the rows past + path[j] move to past + j.  No nodes,
  * or a sequence that takes no part: npath 0, next -1, new_past = past.  N <=
- * 64.  The outputs overlap no other array of the call. */
+ * 64, kv <= 2^28.  The outputs and caches overlap no other array of the call. */
 int ec_tree_accept_dev(uint16_t *kc, uint16_t *vc, int layers, int nslots, int C, int kv, const int *slot,
                        const int *past, const int *nodes, const int *parent, const int *token, const int *sampled,
                        int B, int N, int *path, int *npath, int *next, int *new_past);

@@ -141,6 +141,27 @@ def test_sample_special_values():
         check_sample(x, u, T=np.zeros(12, np.float32))
 
 
+@pytest.mark.parametrize("V", [64, 4096, 4100, 12289])
+def test_sample_few_left(V):
+    """Masks of -inf (or NaN) that leave one lane's tokens, a few or whole chunks; low
+    temperatures, at which most weights are 0."""
+    rng = np.random.default_rng(V + 3)
+    x = rng.normal(0, 2, (8, V)).astype(np.float32)
+    at = np.arange(V)
+    x[0, at % 64 != 5] = -np.inf
+    x[1, at % 64 != 63] = np.nan
+    x[2, at != V - 1] = -np.inf
+    x[3, :V // 2] = -np.inf
+    x[4, V // 2:] = np.nan
+    x[5, rng.random(V) < 0.999] = -np.inf
+    x[5, 3] = 0.0
+    x[6] *= 40.0
+    T = np.array([1, 1, 1, 0.7, 0.7, 1, 1, 0.01], np.float32)
+    for u in (0.0, 0.3, 0.9999):
+        check_sample(x, np.full(8, u), T)
+        check_sample(x, np.full(8, u), T, np.full(8, 3, np.int32), np.full(8, 0.9, np.float32), np.full(8, 0.01, np.float32))
+
+
 @pytest.mark.parametrize("V", [37, 6000])
 def test_sample_extreme_settings(V):
     rng = np.random.default_rng(V + 2)
@@ -363,6 +384,40 @@ def test_attention_unseen_values(H, KVH, hd):
     check_attention(c, window=20)
 
 
+@pytest.mark.parametrize("H,KVH,hd", [(14, 2, 64), (12, 2, 128), (8, 1, 32), (5, 1, 7)])
+def test_attention_seen_values(H, KVH, hd):
+    """One element of a value that is not finite, in the text: the outputs of that
+    element and its KV head are not finite, all others are as they were; of a key:
+    the KV head's."""
+    c = attn_case(22, H, KVH, hd, 2, 5, [700, 90])
+    clean = check_attention(c)
+    s, at, e = c["slot"][0], 300, (KVH - 1) * hd + hd // 2
+    for cache, bad in ((c["vc"], NAN16), (c["vc"], INF16), (c["kc"], NAN16)):
+        kept = cache[s, at, e]
+        cache[s, at, e] = bad
+        got = ec.attention_tree_dev(c["q"], c["kc"], c["vc"], H, KVH, c["past"], 5, c["slot"], None, c["parent"])
+        cache[s, at, e] = kept
+        hit = np.zeros((10, KVH, H // KVH, hd), bool)
+        if cache is c["vc"]:
+            hit[:5, -1, :, hd // 2] = True
+        else:
+            hit[:5, -1] = True
+        hit = hit.reshape(10, H * hd)
+        assert not np.isfinite(got[hit]).any() and np.array_equal(got[~hit], clean[~hit])
+
+
+@pytest.mark.parametrize("at,value", [((1, 0), 0), ((1, 3), 3), ((1, 7), -2), ((1, 7), 2 ** 31 - 1)])
+@pytest.mark.parametrize("window", [0, 100])
+def test_attention_bad_parents_in_a_long_text(at, value, window):
+    """Splits whose tiles hold no node mark their rows too."""
+    c = attn_case(32, 14, 2, 64, 3, 8, [2000, 3000, 700])
+    want = check_attention(c, window, rows=[(0, 0), (2, 7)])
+    c["parent"][at] = value
+    got = ec.attention_tree_dev(c["q"], c["kc"], c["vc"], 14, 2, c["past"], 8, c["slot"], None, c["parent"], window)
+    assert np.isnan(got[8:16]).all()
+    assert np.array_equal(got[:8], want[:8]) and np.array_equal(got[16:], want[16:])
+
+
 def test_attention_wide_scores():
     """Scores of thousands (one position takes all) and equal ones."""
     c = attn_case(4, 12, 2, 128, 2, 5, [300, 64])
@@ -562,6 +617,15 @@ def test_rope_trees_and_padding(hd):
     check_rope(c, ec.rope_inv_freq(hd // 2 * 2, 1e6), 0)
     c["parent"][0] = -1
     check_rope(c, ec.rope_inv_freq(hd // 2 * 2, 1e6), 1)
+
+
+@pytest.mark.parametrize("H,KVH,hd", [(1, 1, 4), (1, 1, 8), (2, 1, 16), (5, 5, 12), (3, 1, 64), (64, 8, 128)])
+def test_rope_narrow_and_wide_rows(H, KVH, hd):
+    """Blocks of one wave to four, rows of fewer heads than a block has groups and of
+    many more."""
+    c = rope_case(8, H, KVH, hd, 3, 9, [10, 0, 300], nodes=[9, 4, 1], tree=True)
+    for rot, layout in ((0, 0), (hd // 8 * 8, 0), (hd // 2 * 2, 1), (2, 1)):
+        check_rope(c, ec.rope_inv_freq(rot, 1e4) if rot else None, layout)
 
 
 def test_rope_prompts():

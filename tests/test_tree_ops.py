@@ -92,6 +92,37 @@ def test_accept_refuses(k):
     refused(accept(**k), "ec_tree_accept_dev")
 
 
+APART = dict(kc=1 << 24, vc=1 << 26)  # caches of their own
+CACHE = 2 * 2 * 100 * 64              # bytes of one of rope() or attention()
+
+
+@pytest.mark.parametrize("k", [dict(vc=(1 << 24) + CACHE - 2), dict(vc=1 << 24), dict(q=(1 << 24) + CACHE - 4),
+                               dict(qkv=(1 << 26) - 4 * (5 * 256 + 256) + 4, past=P + 4), dict(past=1 << 17),
+                               dict(qg=(1 << 26) + CACHE - 4), dict(kg=(1 << 17) + 4), dict(inv_freq=(1 << 26) - 252),
+                               dict(slot=1 << 24), dict(nodes=(1 << 26) + 8), dict(parent=(1 << 17) - 20),
+                               dict(nslots=2 ** 31 - 1, C=1 << 30, q=1 << 40)])
+def test_rope_refuses_overlaps(k):
+    refused(rope(**{**APART, "past": P * 4, **k}), "ec_qk_norm_rope_dev", "overlaps another array")
+
+
+@pytest.mark.parametrize("k", [dict(out=(1 << 24) + CACHE - 4), dict(out=(1 << 26) - 4 * (5 * 128 + 128) + 4), dict(past=1 << 17),
+                               dict(slot=(1 << 17) + 4), dict(nodes=(1 << 17) + 1000), dict(parent=(1 << 17) - 20),
+                               dict(nslots=2 ** 31 - 1, C=1 << 30, out=1 << 40)])
+def test_attention_refuses_overlaps(k):
+    refused(attention(**{**APART, "past": P * 4, **k}), "ec_attention_tree_dev", "overlaps another array")
+
+
+@pytest.mark.parametrize("k", [dict(vc=(1 << 24) + 2 * 2 * 2 * 100 * 128 - 2), dict(vc=1 << 24), dict(path=(1 << 24) - 4 * 6 + 4),
+                               dict(npath=1 << 26), dict(token=(1 << 26) + 8), dict(parent=(1 << 24) + 400), dict(past=1 << 24),
+                               dict(layers=2 ** 31 - 1, nslots=2 ** 31 - 1, next=1 << 40)])
+def test_accept_refuses_overlaps(k):
+    refused(accept(**{**APART, **k}), "ec_tree_accept_dev", "overlaps another array")
+
+
+def test_accept_refuses_wide_rows():
+    refused(accept(**APART, kv=(1 << 28) + 1), "ec_tree_accept_dev", "rows of")
+
+
 def test_device_array_checks(tmp_path):
     exe = tmp_path / "tree_check"
     src = REPO / "tests" / "c" / "tree_check.c"
