@@ -43,7 +43,7 @@ __global__ __launch_bounds__(256) void attn_tree_any_kernel(TreeAttnArgs a) {
   uint64_t see = 0;
   int depth = 0, mydepth = 0;
   if (ok) {
-    const int p = tree_parent(a.t, b, s.n, &ok);
+    const int p = tree_parent(tree_parent_read(a.t, b), s.n, &ok);
     if (ok) {
       const uint64_t anc = tree_ancestors(p, &depth);
       see = ((uint64_t)(uint32_t)__shfl((int)(uint32_t)(anc >> 32), i, 64) << 32) |
@@ -149,12 +149,8 @@ __device__ __forceinline__ int swz(int r) {
   return HD % 64 == 0 ? r & 7 : (r >> 1) & 3;
 }
 
-// where split s of a sequence's tiles starts: the first min(ns, tiles) splits
-// have some, the others none
-__device__ __forceinline__ int split_at(int tiles, int s, int ns) {
-  const int n = min(ns, tiles);
-  return s >= n ? tiles : (int)((int64_t)tiles * s / n);
-}
+// where part i of a sequence's n parts starts, of its tiles
+__device__ __forceinline__ int part_at(int tiles, int i, int n) { return (int)((int64_t)tiles * i / n); }
 
 // the bits 0 .. n - 1 (n up to 64, below 0 none)
 __device__ __forceinline__ uint64_t low_bits(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0 : (1ull << n) - 1; }
@@ -167,9 +163,71 @@ __device__ __forceinline__ uint64_t tile_mask(int p0, int lo, int past, uint64_t
   return (low_bits(d) & ~low_bits(lo - p0)) | nodes;
 }
 
+// How the positions are split: `parts` blocks per KV head and row block, of which a
+// sequence has as many as its tiles ask for, up to `most`.
 struct TreeGrid {
-  int ns, rb, units;  // splits, row blocks per KV head, (split, sequence, KV head) triples
+  int parts, most, rb, shift;  // rb: row blocks per KV head; tiles >> shift add up in 31 bits
 };
+
+// a sequence's tiles (one where it takes no part)
+__device__ __forceinline__ int tree_tiles(const TreeAttnArgs &a, const EcTreeSeq &s) {
+  return ec_tree_seq_ok(&a.t, s) ? (s.past + s.n - window_lo(a.window, s.past, 0) + kTp - 1) / kTp : 1;
+}
+
+// A sequence's parts: one, and of those left (parts - B) those between its tiles' share
+// of the running sum of all sequences' and the next one's; of these as many as it has
+// tiles, up to `most`.  By a wave, a sequence per lane.  Part i of the grid gets its
+// sequence, its place j among the sequence's parts and their number n (b is -1 where
+// it is none of them).
+struct TreePart {
+  int b, j, n;
+  EcTreeSeq s;
+};
+__device__ __forceinline__ TreePart tree_part(const TreeAttnArgs &a, const TreeGrid &gr, int i) {
+  const int lane = threadIdx.x & 63, B = a.t.B;
+  const auto tiles_of = [&](int c, EcTreeSeq &s) {
+    s = ec_tree_seq(&a.t, min(c, B - 1));
+    return c < B ? tree_tiles(a, s) : 0;
+  };
+  EcTreeSeq s0, s;
+  const int tiles0 = tiles_of(lane, s0);
+  uint32_t all = 0;
+  for (int c0 = 0; c0 < B; c0 += 64)
+    all += readlane(wave_scan((uint32_t)((c0 ? tiles_of(c0 + lane, s) : tiles0) >> gr.shift)), 63);
+  // exact: the products stay below 2^53, the quotients' steps above 2^-40
+  const double left = (double)(gr.parts - B), per = (double)max(all, 1u);
+  uint32_t sum = 0;
+  for (int c0 = 0; c0 < B; c0 += 64) {
+    s = s0;
+    const int c = c0 + lane, tiles = c0 ? tiles_of(c, s) : tiles0;
+    const uint32_t w = (uint32_t)(tiles >> gr.shift), upto = sum + wave_scan(w);
+    const int first = c + (int)(left * (double)(upto - w) / per), next = c + 1 + (int)(left * (double)upto / per);
+    const uint64_t hit = __ballot(c < B && first <= i && i < next);
+    if (hit) {
+      const int at = __ffsll((unsigned long long)hit) - 1, j = i - readlane(first, at);
+      const int n = readlane(min(min(next - first, tiles), gr.most), at);
+      return TreePart{j < n ? c0 + at : -1, j, n, EcTreeSeq{readlane(s.slot, at), readlane(s.past, at), readlane(s.n, at)}};
+    }
+    sum = readlane(upto, 63);
+  }
+  return TreePart{-1, 0, 0, {0, 0, 0}};
+}
+// The parts' results: outputs, then maxima and sums, [most][rows of the call], and each
+// sequence's number of parts.
+struct PartRows {
+  float *o;
+  float2 *ml;
+  int *n;
+  size_t all;
+};
+__device__ __forceinline__ PartRows part_rows(const TreeAttnArgs &a, const TreeGrid &gr, int hd) {
+  PartRows p;
+  p.all = (size_t)a.t.B * a.t.N * a.H;
+  p.o = (float *)a.ws;
+  p.ml = (float2 *)(p.o + gr.most * p.all * hd);
+  p.n = (int *)(p.ml + gr.most * p.all);
+  return p;
+}
 
 __device__ __forceinline__ v4f mma(v4u a, v4u b, v4f c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
@@ -253,18 +311,45 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_tree_kernel(TreeAttnArgs a,
   extern __shared__ __attribute__((aligned(16))) _Float16 lds[];  // [2 buffers][K, V][kTp][HD]
   const int t = threadIdx.x, lane = t & 63, lr = lane & 15, lg = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(t >> 6);
-  // blocks go to the 8 XCDs in turn: a unit's row blocks, which read the same
-  // rows of the cache, follow each other on one XCD
+  // blocks go to the 8 XCDs in turn: a part's row blocks, which read the same rows
+  // of the cache, follow each other on one XCD
   const int x = blockIdx.x, unit = ((x >> 3) / gr.rb) * 8 + (x & 7), rb = (x >> 3) % gr.rb;
-  if (unit >= gr.units) return;
-  const int kvh = unit % a.KVH, b = (unit / a.KVH) % a.t.B, split = unit / (a.KVH * a.t.B);
+  if (unit >= gr.parts * a.KVH) return;
+  const int kvh = unit % a.KVH, part = unit / a.KVH;
   const int G = a.H / a.KVH, r0 = rb * 16 * NW;
+  const bool joins = gr.parts > a.t.B;
+  TreePart tp{part, 0, 1, {0, 0, 0}};
+  if (joins && a.t.B > 1) {
+    tp = tree_part(a, gr, part);
+  } else if (joins) {
+    tp.s = ec_tree_seq(&a.t, 0);
+    tp.n = min(gr.most, tree_tiles(a, tp.s));
+    tp.b = part < tp.n ? 0 : -1;
+    tp.j = part;
+  } else {
+    tp.s = ec_tree_seq(&a.t, part);
+  }
+  const int b = tp.b;
+  if (b < 0) return;
+  const EcTreeSeq s = tp.s;
   const size_t m0 = (size_t)b * a.t.N;
+  const int rows = ec_tree_rows(&a.t, s) * G;
+  if (r0 >= rows) return;
+  if (!ec_tree_seq_ok(&a.t, s)) {  // NaN, here or by the join
+    if (!joins)
+      for (int e = t; e < min(rows - r0, 16 * NW) * HD; e += NT) {
+        const int r = r0 + e / HD;
+        a.out[(m0 + r / G) * a.ldo + (size_t)(kvh * G + r % G) * HD + e % HD] = __builtin_nanf("");
+      }
+    return;
+  }
+  const int end = s.past + s.n, lo0 = window_lo(a.window, s.past, 0), lo_all = window_lo(a.window, s.past, s.n - 1);
+  const int tiles = (end - lo0 + kTp - 1) / kTp;
+  const int tile0 = part_at(tiles, tp.j, tp.n), tile1 = part_at(tiles, tp.j + 1, tp.n);
 
-  // what depends on no other load is read first: the sequence's numbers, this
-  // lane's row of q (of a node that there is), then the first tile, and the
-  // parents while that is on its way
-  const EcTreeSeq s = ec_tree_seq(&a.t, b);
+  // the parents and this lane's row of q (of a node that there is), both before the
+  // first tile
+  const int parent = tree_parent_read(a.t, b);
   const int row = r0 + w * 16 + lr, node = row / G, head = kvh * G + (row - node * G);
   float4 qr[KS][2];
   {
@@ -275,19 +360,11 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_tree_kernel(TreeAttnArgs a,
       qr[k][1] = *reinterpret_cast<const float4 *>(q + 32 * k + 4);
     }
   }
-  bool ok = ec_tree_seq_ok(&a.t, s);
-  const int rows = ec_tree_rows(&a.t, s) * G;
-  if (r0 >= rows) return;
-  const int end = ok ? s.past + s.n : 1, lo0 = ok ? window_lo(a.window, s.past, 0) : 0;
-  const int lo_all = ok ? window_lo(a.window, s.past, s.n - 1) : 0;
-  const int tiles = ok ? (end - lo0 + kTp - 1) / kTp : 1;
-  const int tile0 = split_at(tiles, split, gr.ns), tile1 = split_at(tiles, split + 1, gr.ns);
-  if (tile0 == tile1) return;
 
   // The tiles' way into LDS: a wave's instruction fills 64 chunks, lane l the l-th
   // of them, with the chunk that the swizzle puts there.  In the sequence's last
   // tile the rows behind the nodes are the last node's again (no row sees them).
-  const size_t kv = (size_t)a.KVH * HD, base = ok ? (size_t)s.slot * a.t.C * kv + (size_t)kvh * HD : 0;
+  const size_t kv = (size_t)a.KVH * HD, base = (size_t)s.slot * a.t.C * kv + (size_t)kvh * HD;
   const int rest = end - lo0 - (tiles - 1) * kTp;  // rows of the last tile
   uint32_t off[LPT], off_last[LPT];
 #pragma unroll
@@ -310,32 +387,19 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_tree_kernel(TreeAttnArgs a,
     kn += kTp * kv;
     vn += kTp * kv;
   };
-  if (ok) load(tile0 + 1 == tiles, 0);
+  load(tile0 + 1 == tiles, 0);
 
-  // the parents, and the nodes' ancestors where a tile of this block has rows that
-  // not all see
+  // the nodes' ancestors, where a tile of this block has rows that not all see (from
+  // parents that are not valid some mask: the rows are NaN in the end)
   uint64_t anc = 0;
   int depth = 0;
-  if (ok) {
-    const int p = tree_parent(a.t, b, s.n, &ok);
-    if (ok && (lo0 + tile1 * kTp > s.past || lo0 + tile0 * kTp < lo_all)) {
-      anc = tree_ancestors(p, &depth);
-      if (a.window > 0 && a.window < EC_TREE_MAX)
-        for (int j = 0; j < s.n; j++)
-          if (depth - __shfl(depth, j, 64) >= a.window) anc &= ~(1ull << j);
-    }
-  }
-  const size_t all = (size_t)a.t.B * a.t.N * a.H, part = (size_t)split * all;  // rows of a split's results
-  float2 *const ml = (float2 *)((float *)a.ws + (size_t)gr.ns * all * HD) + part;
-  if (!ok) {  // NaN as a row's sum, or the row itself
-    __builtin_amdgcn_s_waitcnt(0);
-    for (int e = t; e < min(rows - r0, 16 * NW) * HD; e += NT) {
-      const int r = r0 + e / HD;
-      const size_t node = m0 + r / G, h = kvh * G + r % G;
-      if (gr.ns == 1) a.out[node * a.ldo + h * HD + e % HD] = __builtin_nanf("");
-      else if (e % HD == 0) ml[node * a.H + h] = make_float2(0.0f, __builtin_nanf(""));
-    }
-    return;
+  bool ok = true;
+  const bool edges = lo0 + tile1 * kTp > s.past || lo0 + tile0 * kTp < lo_all;
+  if (edges) {
+    anc = tree_ancestors(tree_parent(parent, s.n, &ok), &depth);
+    if (a.window > 0 && a.window < EC_TREE_MAX)
+      for (int j = 0; j < s.n; j++)
+        if (depth - __shfl(depth, j, 64) >= a.window) anc &= ~(1ull << j);
   }
 
   const bool work = r0 + w * 16 < rows, live = row < rows;
@@ -546,9 +610,10 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_tree_kernel(TreeAttnArgs a,
   for (; tile < min(whole1, tile1); tile++) step(std::false_type{}, tile);
   for (; tile < tile1; tile++) step(std::true_type{}, tile);
 
-  const float l = row_sum(sum);
+  if (!edges) tree_parent(parent, s.n, &ok);
+  const float l = ok ? row_sum(sum) : __builtin_nanf("");
   if (!live) return;
-  if (gr.ns == 1) {
+  if (!joins) {
     const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
     float *out = a.out + (m0 + node) * a.ldo + (size_t)head * HD + 4 * lg;
 #pragma unroll
@@ -556,59 +621,56 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_tree_kernel(TreeAttnArgs a,
       *reinterpret_cast<float4 *>(out + 16 * d) =
           make_float4(o[d][0] * inv, o[d][1] * inv, o[d][2] * inv, o[d][3] * inv);
   } else {
-    const size_t at = (m0 + node) * a.H + head;
-    float *po = (float *)a.ws + (part + at) * HD + 4 * lg;
+    const PartRows pr = part_rows(a, gr, HD);
+    const size_t at = tp.j * pr.all + (m0 + node) * a.H + head;
+    float *po = pr.o + at * HD + 4 * lg;
 #pragma unroll
     for (int d = 0; d < DT; d++) *reinterpret_cast<float4 *>(po + 16 * d) = make_float4(o[d][0], o[d][1], o[d][2], o[d][3]);
-    if (lg == 0) ml[at] = make_float2(mx, l);
+    if (lg == 0) pr.ml[at] = make_float2(mx, l);
+    if (tp.j == 0 && kvh == 0 && rb == 0 && t == 0) pr.n[b] = tp.n;
   }
 }
 
-// Joins the splits' outputs: per row the largest of their maxima, the sums and
-// outputs brought to it.  HD / 4 lanes a row (a power of two of them: 24 of 32 at
-// 96).  Latency is all of it: the reads do not wait for the sequence's numbers (3.5 us
-// for 8 nodes, 5.7 for the 32 splits of 2 x 64 nodes).  The last block of a row's
-// splits could join them, without this launch; but what it counts arrivals with lives
-// from call to call, and a run that ends half way would leave it wrong for good.
+// Joins the parts' outputs: per row the largest of their maxima, the sums and outputs
+// brought to it.  HD / 4 lanes a row (a power of two of them: 24 of 32 at 96).  Latency
+// is all of it: the reads do not wait for the sequence's numbers, and those of the next
+// parts do not for these (3.6 us for 8 nodes, 6.4 for the 30 to 34 parts of 2 x 64
+// nodes; one set of 16 parts 7.9).  The last block of a row's parts could join them,
+// without this launch; but what it counts arrivals with lives from call to call, and a
+// run that ends half way would leave it wrong for good.
 template <int HD>
-__global__ __launch_bounds__(256) void attn_tree_join_kernel(TreeAttnArgs a, int ns) {
+__global__ __launch_bounds__(256) void attn_tree_join_kernel(TreeAttnArgs a, TreeGrid gr) {
   constexpr int LPR = HD == 96 ? 32 : HD / 4, RPB = 256 / LPR;
-  constexpr int kRead = 16;  // splits read at a time
+  constexpr int kRead = 12;  // parts read at a time, in two sets by turns
   const int t = threadIdx.x, b = blockIdx.y, li = t % LPR;
   const int r = blockIdx.x * RPB + t / LPR;
-  const size_t all = (size_t)a.t.B * a.t.N * a.H, row = (size_t)b * a.t.N * a.H + min(r, a.t.N * a.H - 1);
-  const float *po = (const float *)a.ws + row * HD + 4 * min(li, HD / 4 - 1);
-  const float2 *ml = (const float2 *)((const float *)a.ws + (size_t)ns * all * HD) + row;
-  // the first splits are read before it is known how many of them there are
-  float2 u[kRead];
-  float4 v[kRead];
+  const PartRows pr = part_rows(a, gr, HD);
+  const size_t row = (size_t)b * a.t.N * a.H + min(r, a.t.N * a.H - 1);
+  struct Read {
+    float2 u[kRead];
+    float4 v[kRead];
+  } x[2];
+  const auto read = [&](Read &x, int j0, int n) {
 #pragma unroll
-  for (int i = 0; i < kRead; i++) {
-    const size_t at = (size_t)min(i, ns - 1) * all;
-    u[i] = ml[at];
-    v[i] = *reinterpret_cast<const float4 *>(po + at * HD);
-  }
+    for (int i = 0; i < kRead; i++) {
+      const size_t at = (size_t)min(j0 + i, n - 1) * pr.all + row;
+      x.u[i] = pr.ml[at];
+      x.v[i] = *reinterpret_cast<const float4 *>(pr.o + at * HD + 4 * min(li, HD / 4 - 1));
+    }
+  };
+  read(x[0], 0, gr.most);  // before it is known how many there are
   const EcTreeSeq s = ec_tree_seq(&a.t, b);
-  const bool ok = ec_tree_seq_ok(&a.t, s);  // (bad parents: the splits' sums are NaN)
-  const int rows = ec_tree_rows(&a.t, s) * a.H;
+  const bool ok = ec_tree_seq_ok(&a.t, s);  // (bad parents: the parts' sums are NaN)
+  const int rows = ec_tree_rows(&a.t, s) * a.H, n = pr.n[b];
   if (blockIdx.x * RPB >= rows) return;
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   if (ok) {
-    const int tiles = (s.past + s.n - window_lo(a.window, s.past, 0) + kTp - 1) / kTp, n = min(ns, tiles);
     float m = -FLT_MAX, l = 0.0f;
-    for (int i0 = 0; i0 < n; i0 += kRead) {
-      if (i0) {
-#pragma unroll
-        for (int i = 0; i < kRead; i++) {
-          const size_t at = (size_t)min(i0 + i, ns - 1) * all;
-          u[i] = ml[at];
-          v[i] = *reinterpret_cast<const float4 *>(po + at * HD);
-        }
-      }
+    const auto use = [&](const Read &x, int i0) {
       float big = m;
 #pragma unroll
       for (int i = 0; i < kRead; i++)
-        if (i0 + i < n) big = fmaxf(big, u[i].x);
+        if (i0 + i < n) big = fmaxf(big, x.u[i].x);
       const float back = __builtin_amdgcn_exp2f(m - big);
       m = big;
       l *= back;
@@ -616,13 +678,20 @@ __global__ __launch_bounds__(256) void attn_tree_join_kernel(TreeAttnArgs a, int
 #pragma unroll
       for (int i = 0; i < kRead; i++)
         if (i0 + i < n) {
-          const float f = __builtin_amdgcn_exp2f(u[i].x - m);
-          l = __builtin_fmaf(u[i].y, f, l);
-          o.x = __builtin_fmaf(v[i].x, f, o.x);
-          o.y = __builtin_fmaf(v[i].y, f, o.y);
-          o.z = __builtin_fmaf(v[i].z, f, o.z);
-          o.w = __builtin_fmaf(v[i].w, f, o.w);
+          const float f = __builtin_amdgcn_exp2f(x.u[i].x - m);
+          l = __builtin_fmaf(x.u[i].y, f, l);
+          o.x = __builtin_fmaf(x.v[i].x, f, o.x);
+          o.y = __builtin_fmaf(x.v[i].y, f, o.y);
+          o.z = __builtin_fmaf(x.v[i].z, f, o.z);
+          o.w = __builtin_fmaf(x.v[i].w, f, o.w);
         }
+    };
+    for (int i0 = 0; i0 < n; i0 += 2 * kRead) {
+      if (i0 + kRead < n) read(x[1], i0 + kRead, n);
+      use(x[0], i0);
+      if (i0 + kRead >= n) break;
+      if (i0 + 2 * kRead < n) read(x[0], i0 + 2 * kRead, n);
+      use(x[1], i0 + kRead);
     }
     const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
     o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
@@ -648,28 +717,35 @@ bool tiles_ok(const TreeAttnArgs &a) {
 // 16 nodes, 12 / 2 heads of 128, over 4000 rows.
 int tree_waves(const TreeAttnArgs &a) { return (long)a.t.N * (a.H / a.KVH) <= 64 ? 4 : 8; }
 
-// Row blocks and splits: two blocks a CU, one of 8 waves at head sizes above 64 (its LDS
-// and registers leave room for no second), of at least a tile each.  Three and four a
-// CU take 41 and 42 us instead of 38 for the long contexts (the joins 8 and 10 instead
-// of 6), two of the wide ones 22 instead of 17.5 for the trees over 4000 rows; with no
-// split these take 101, 8 nodes over 700 rows 16 instead of 7 + 3.5.
+// Row blocks and parts: blocks for the CUs' places, of at least a tile each.  Two a CU, at
+// head sizes above 64 with 8 waves one (LDS and registers leave room for no second:
+// two a CU, one after the other, take 22 instead of 17.5 us for the trees over 4000
+// rows), at those up to 64 with 4 waves three: 16 one-token sequences of 12 / 12 heads
+// over 1000 rows take 14.1 + 4.1 us (the join's) with two, 13.0 + 4.1 with three, 12.3 +
+// 4.7 with four, 32 of 14 / 2 heads over 2000 rows 13.1, 13.0 and 14.3 in all.  Three and
+// four a CU for 8 waves take 41 and 42 us instead of 38 for the long contexts.  With no
+// parts at all the trees take 101 us, 8 nodes over 700 rows 16 instead of 7 + 3.5.
 TreeGrid tree_grid(const TreeAttnArgs &a) {
   TreeGrid g;
   const int waves = tree_waves(a), per = 16 * waves;
   g.rb = (int)(((long)a.t.N * (a.H / a.KVH) + per - 1) / per);
   long span = (long)a.t.max_past + a.t.N;
   if (a.window > 0 && (long)a.window + a.t.N < span) span = (long)a.window + a.t.N;
-  const long tiles = (span + kTp - 1) / kTp, units = (long)a.t.B * a.KVH, blocks = units * g.rb;
-  const long full = waves == 8 && a.hd > 64 ? 256 : 512, want = (full + blocks - 1) / blocks;
-  g.ns = (int)(want < tiles ? want : tiles);
-  g.units = (int)(units * g.ns);
+  const long tiles = (span + kTp - 1) / kTp, full = a.hd <= 64 ? (waves == 4 ? 768 : 512) : waves == 4 ? 512 : 256;
+  const long want = full / ((long)a.KVH * g.rb), most = tiles * a.t.B;
+  g.parts = (int)(want < a.t.B ? a.t.B : want < most ? want : most);
+  // of a sequence, four times its even share at most: the join's rows have room for that
+  const long share = 4 * ((g.parts + a.t.B - 1) / a.t.B);
+  g.most = (int)(share < g.parts - a.t.B + 1 ? share : g.parts - a.t.B + 1);
+  g.shift = 0;
+  while ((tiles >> g.shift) * a.t.B >= 1L << 31) g.shift++;
   return g;
 }
 
 template <int HD>
 hipError_t launch_tree(const TreeAttnArgs &a, hipStream_t st) {
   const TreeGrid g = tree_grid(a);
-  const dim3 grid((g.units + 7) / 8 * 8 * g.rb);
+  const dim3 grid((unsigned)(((long)g.parts * a.KVH + 7) / 8 * 8 * g.rb));
   const uint32_t lds = 2 * 4 * kTp * HD;
   if (tree_waves(a) == 4) klaunch((attn_tree_kernel<HD, 4, HD <= 64 ? 4 : 2>), grid, dim3(256), lds, st, a, g);
   else klaunch((attn_tree_kernel<HD, 8, HD <= 64 ? 4 : 2>), grid, dim3(512), lds, st, a, g);
@@ -679,7 +755,7 @@ hipError_t launch_tree(const TreeAttnArgs &a, hipStream_t st) {
 template <int HD>
 hipError_t launch_join(const TreeAttnArgs &a, hipStream_t st) {
   constexpr int rpb = 256 / (HD == 96 ? 32 : HD / 4);
-  klaunch((attn_tree_join_kernel<HD>), dim3((a.t.N * a.H + rpb - 1) / rpb, a.t.B), dim3(256), 0, st, a, tree_grid(a).ns);
+  klaunch((attn_tree_join_kernel<HD>), dim3((a.t.N * a.H + rpb - 1) / rpb, a.t.B), dim3(256), 0, st, a, tree_grid(a));
   return hipGetLastError();
 }
 
@@ -688,7 +764,8 @@ hipError_t launch_join(const TreeAttnArgs &a, hipStream_t st) {
 int attention_tree_max_hd() { return kTreeMaxHd; }
 
 size_t attention_tree_workspace(const TreeAttnArgs &a) {
-  return attention_tree_joins(a) ? (size_t)tree_grid(a).ns * a.t.B * a.t.N * a.H * (a.hd + 2) * sizeof(float) : 0;
+  if (!attention_tree_joins(a)) return 0;
+  return (size_t)a.t.B * ((size_t)tree_grid(a).most * a.t.N * a.H * (a.hd + 2) * sizeof(float) + sizeof(int));
 }
 
 hipError_t attention_tree(const TreeAttnArgs &a, hipStream_t st) {
@@ -702,7 +779,7 @@ hipError_t attention_tree(const TreeAttnArgs &a, hipStream_t st) {
   return hipGetLastError();
 }
 
-bool attention_tree_joins(const TreeAttnArgs &a) { return tiles_ok(a) && tree_grid(a).ns > 1; }
+bool attention_tree_joins(const TreeAttnArgs &a) { return tiles_ok(a) && tree_grid(a).parts > a.t.B; }
 
 hipError_t attention_tree_join(const TreeAttnArgs &a, hipStream_t st) {
   if (a.hd == 64) return launch_join<64>(a, st);

@@ -275,6 +275,26 @@ __device__ __forceinline__ float wave_max_dpp(float v) {
   v = fmaxf(v, dpp_mov<0x140>(v));
   return fmaxf(fmaxf(readlane(v, 0), readlane(v, 16)), fmaxf(readlane(v, 32), readlane(v, 48)));
 }
+// inclusive sums over the wave's lanes, by DPP: within rows of 16 (shifts of 1, 2,
+// 4 and 8), then a row's last lane into the next row, then into the upper half
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_rows(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned long long dpp_rows(unsigned long long v) {
+  return ((unsigned long long)dpp_rows<CTRL, ROWS>((uint32_t)(v >> 32)) << 32) | dpp_rows<CTRL, ROWS>((uint32_t)v);
+}
+template <class T>
+__device__ __forceinline__ T wave_scan(T v) {
+  v += dpp_rows<0x111, 0xF>(v);
+  v += dpp_rows<0x112, 0xF>(v);
+  v += dpp_rows<0x114, 0xF>(v);
+  v += dpp_rows<0x118, 0xF>(v);
+  v += dpp_rows<0x142, 0xA>(v);  // row_bcast15, rows 1 and 3
+  v += dpp_rows<0x143, 0xC>(v);  // row_bcast31, rows 2 and 3
+  return v;
+}
 // Block reductions for blockDim.x == 256 with a single barrier.  `red` (4
 // slots) must not be written by another reduction until every thread has
 // passed one more barrier: callers alternate between slot sets or separate

@@ -88,12 +88,14 @@ __device__ __forceinline__ bool tree_clashes(const EcTreeBatch &t, int b, EcTree
   return false;
 }
 
-/* lane i's parent (-1 past the nodes); *ok: whether every node's is valid */
-__device__ __forceinline__ int tree_parent(const EcTreeBatch &t, int b, int n, bool *ok) {
+/* lane i's entry of the parents, read ahead of its check (any value behind the rows) */
+__device__ __forceinline__ int tree_parent_read(const EcTreeBatch &t, int b) {
   const int i = threadIdx.x & 63;
-  int p = i - 1;
-  if (t.parent && i < n) p = t.parent[(size_t)b * t.N + i];
-  if (i >= n) p = -1;
+  return t.parent ? t.parent[(size_t)b * t.N + min(i, t.N - 1)] : i - 1;
+}
+/* lane i's parent (-1 past the nodes) from what it read; *ok: whether every node's is valid */
+__device__ __forceinline__ int tree_parent(int read, int n, bool *ok) {
+  const int i = threadIdx.x & 63, p = i < n ? read : -1;
   *ok = __ballot(!ec_tree_parent_ok(p, i)) == 0;
   return p;
 }

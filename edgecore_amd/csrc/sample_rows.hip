@@ -208,27 +208,6 @@ __device__ __forceinline__ Ends row_ends(Ends e) { return Ends{wave_max64(e.top)
 
 __device__ __forceinline__ float temp_of(const SampleArgs &a, int row) { return a.temp ? a.temp[row] : 1.0f; }
 
-// inclusive sums over the wave's lanes, by DPP: within rows of 16 (shifts of 1, 2,
-// 4 and 8), then a row's last lane into the next row, then into the upper half
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint32_t dpp_rows(uint32_t v) {
-  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
-}
-template <int CTRL, int ROWS>
-__device__ __forceinline__ u64 dpp_rows(u64 v) {
-  return ((u64)dpp_rows<CTRL, ROWS>((uint32_t)(v >> 32)) << 32) | dpp_rows<CTRL, ROWS>((uint32_t)v);
-}
-template <class T>
-__device__ __forceinline__ T wave_scan(T v) {
-  v += dpp_rows<0x111, 0xF>(v);
-  v += dpp_rows<0x112, 0xF>(v);
-  v += dpp_rows<0x114, 0xF>(v);
-  v += dpp_rows<0x118, 0xF>(v);
-  v += dpp_rows<0x142, 0xA>(v);  // row_bcast15, rows 1 and 3
-  v += dpp_rows<0x143, 0xC>(v);  // row_bcast31, rows 2 and 3
-  return v;
-}
-
 // the keys alone, by DPP: within the row of 16 (lane pairs, quads, then mirrored halves
 // and rows), then the rows' by lane
 struct KeyEnds {

@@ -42,7 +42,7 @@ __device__ __forceinline__ RopeRow rope_row(const NormRopeArgs &a, int m) {
   r.ok = r.mine && ec_tree_seq_ok(&a.t, s);
   int depth = i;
   if (r.ok && a.t.parent) {
-    const int p = tree_parent(a.t, b, s.n, &r.ok);
+    const int p = tree_parent(tree_parent_read(a.t, b), s.n, &r.ok);
     if (r.ok) {
       int d;
       tree_ancestors(p, &d);
@@ -258,7 +258,7 @@ __global__ __launch_bounds__(256) void tree_accept_kernel(AcceptArgs a, int cols
     int len = 0, node = -1, next = -1;
     if (ec_tree_seq_ok(&a.t, s) && s.n > 0) {
       bool ok;
-      const int p = tree_parent(a.t, b, s.n, &ok);
+      const int p = tree_parent(tree_parent_read(a.t, b), s.n, &ok);
       if (ok && !tree_clashes(a.t, b, s)) len = accept_walk(a, b, s.n, p, &node, &next);
     }
     path[t] = node;

@@ -406,6 +406,26 @@ def test_attention_seen_values(H, KVH, hd):
         assert not np.isfinite(got[hit]).any() and np.array_equal(got[~hit], clean[~hit])
 
 
+@pytest.mark.parametrize("H,KVH,hd,B,N", [(2, 1, 64, 130, 2), (4, 1, 128, 65, 3), (2, 1, 32, 200, 1), (6, 2, 64, 64, 1)])
+@pytest.mark.parametrize("window", [0, 300])
+def test_attention_many_ragged_sequences(H, KVH, hd, B, N, window):
+    """More sequences than a wave has lanes, from empty to long ones, some of no
+    nodes, one that takes no part: each has its share of the blocks."""
+    rng = np.random.default_rng(B)
+    past = rng.integers(0, 200, B)
+    past[rng.integers(0, B, 5)] = [0, 3000, 1, 2047, 1500]
+    nodes = rng.integers(0, N + 1, B)
+    nodes[past > 1000] = N
+    c = attn_case(B, H, KVH, hd, B, N, past, nodes=nodes)
+    c["slot"][7], n7 = -1, int(c["nodes"][7])
+    n = np.where(np.arange(B) == 7, 0, c["nodes"])
+    got = ec.attention_tree_dev(c["q"], c["kc"], c["vc"], H, KVH, c["past"], N, c["slot"], c["nodes"], c["parent"], window,
+                                out=np.full_like(c["q"], 7.25))
+    assert np.isnan(got[7 * N:7 * N + n7]).all()
+    got[7 * N:8 * N] = 7.25
+    check_attention({**c, "nodes": n}, window, got=got)
+
+
 @pytest.mark.parametrize("at,value", [((1, 0), 0), ((1, 3), 3), ((1, 7), -2), ((1, 7), 2 ** 31 - 1)])
 @pytest.mark.parametrize("window", [0, 100])
 def test_attention_bad_parents_in_a_long_text(at, value, window):
