@@ -27,7 +27,7 @@ __device__ __forceinline__ int window_lo(int window, int past, int depth) {
 // head per thread for the sums, with the running maximum and sum.  Every query head
 // reads its keys and values anew, a thread a whole key: 8 nodes of 14 / 2 heads of 64
 // over 700 rows take 42 us (the matrix-core form and its join 10.6), 16 one-token
-// sequences of 12 / 12 heads over 1000 rows 91 (18).
+// sequences of 12 / 12 heads over 1000 rows 91 (17).
 constexpr int kTreeMaxHd = 512;
 __global__ __launch_bounds__(256) void attn_tree_any_kernel(TreeAttnArgs a) {
   __shared__ float q[kTreeMaxHd], p_s[256], red[4];
@@ -123,7 +123,7 @@ __global__ __launch_bounds__(256) void attn_tree_any_kernel(TreeAttnArgs a) {
 // instructions less), weights = hi + lo below 2^14; keys and values are 16 bits as
 // they are, so two products give each sum to about 2^-21.  The running maximum is
 // raised only when a score passes it by a factor of 2^10 (the parts' room), and the
-// accumulated outputs are scaled only then: mostly in a split's first tile.
+// accumulated outputs are scaled only then: mostly in a part's first tile.
 //
 // What bounds it.  Two sequences of 64 nodes, 14 / 2 heads of 64, over 32600 rows: 38
 // us, 23 GFLOP of matrix products in two parts, 0.6 PFLOP/s.  The matrix cores are
