@@ -74,15 +74,18 @@ namespace ec {
 
 /* Every lane of the wave calls the functions below. */
 
-/* whether sequence b's nodes share a row with those of an earlier sequence */
+/* whether sequence b's nodes share a row with those of an earlier sequence (never
+ * where every sequence has its own slot): four sequences a lane at a time, so that
+ * a round is one wait */
 __device__ __forceinline__ bool tree_clashes(const EcTreeBatch &t, int b, EcTreeSeq s) {
-  for (int c0 = 0; c0 < b; c0 += 64) {
-    const int c = c0 + (int)(threadIdx.x & 63);
+  if (!t.slot) return false;
+  for (int c0 = 0; c0 < b; c0 += 256) {
+    EcTreeSeq o[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) o[k] = ec_tree_seq(&t, min(c0 + 64 * k + (int)(threadIdx.x & 63), b - 1));
     bool hit = false;
-    if (c < b) {
-      const EcTreeSeq o = ec_tree_seq(&t, c);
-      hit = ec_tree_seq_ok(&t, o) && ec_tree_clash(s, o);
-    }
+#pragma unroll
+    for (int k = 0; k < 4; k++) hit |= ec_tree_seq_ok(&t, o[k]) && ec_tree_clash(s, o[k]);
     if (__ballot(hit)) return true;
   }
   return false;

@@ -705,6 +705,15 @@ def test_rope_same_rows_twice():
     check_rope(c, ec.rope_inv_freq(64, 1e4))
 
 
+def test_rope_same_rows_far_apart():
+    """Among 600 sequences: pairs that share a row, next to each other and far apart."""
+    c = rope_case(15, 2, 1, 16, 600, 2, [5] * 600)
+    for late, early in ((1, 0), (300, 43), (513, 256), (599, 3)):
+        c["slot"][late] = c["slot"][early]
+    c["past"][513] = 4
+    check_rope(c, ec.rope_inv_freq(16, 1e4), bad=(1, 300, 513, 599))
+
+
 # ---------------------------------------------------------------------------
 # accepted rows
 # ---------------------------------------------------------------------------
