@@ -145,18 +145,24 @@ Scratch scratch_of(void *p, int rows, int nb) {
   return s;
 }
 
+// f of all lanes' values, by DPP: within the row of 16 (lane pairs, quads, then mirrored
+// halves and rows), then the rows' by lane
+template <class T, class F>
+__device__ __forceinline__ T wave_join(T v, F f) {
+  v = f(v, dpp_mov<0xB1>(v));
+  v = f(v, dpp_mov<0x4E>(v));
+  v = f(v, dpp_mov<0x141>(v));
+  v = f(v, dpp_mov<0x140>(v));
+  return f(f(readlane(v, 0), readlane(v, 16)), f(readlane(v, 32), readlane(v, 48)));
+}
 __device__ __forceinline__ u64 wave_max64(u64 v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const u64 x = __shfl_xor(v, o, 64);
-    v = x > v ? x : v;
-  }
-  return v;
+  return wave_join(v, [](u64 x, u64 y) { return x > y ? x : y; });
+}
+__device__ __forceinline__ uint32_t wave_max32(uint32_t v) {
+  return wave_join(v, [](uint32_t x, uint32_t y) { return max(x, y); });
 }
 __device__ __forceinline__ uint32_t wave_min32(uint32_t v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = min(v, (uint32_t)__shfl_xor((int)v, o, 64));
-  return v;
+  return wave_join(v, [](uint32_t x, uint32_t y) { return min(x, y); });
 }
 
 // Bound by memory: 128 rows of 151936, 78 MB, in 15.4 us (5.0 TB/s).  One row is a launch
@@ -208,24 +214,13 @@ __device__ __forceinline__ Ends row_ends(Ends e) { return Ends{wave_max64(e.top)
 
 __device__ __forceinline__ float temp_of(const SampleArgs &a, int row) { return a.temp ? a.temp[row] : 1.0f; }
 
-// the keys alone, by DPP: within the row of 16 (lane pairs, quads, then mirrored halves
-// and rows), then the rows' by lane
+// the keys alone
 struct KeyEnds {
   uint32_t top, low;
 };
-template <class F>
-__device__ __forceinline__ uint32_t wave_join(uint32_t v, F f) {
-  v = f(v, dpp_mov<0xB1>(v));
-  v = f(v, dpp_mov<0x4E>(v));
-  v = f(v, dpp_mov<0x141>(v));
-  v = f(v, dpp_mov<0x140>(v));
-  const auto at = [&](int i) { return (uint32_t)__builtin_amdgcn_readlane((int)v, i); };
-  return f(f(at(0), at(16)), f(at(32), at(48)));
-}
 __device__ __forceinline__ KeyEnds key_ends(const Scratch &s, int row, int nb) {
   const size_t at = (size_t)row * nb + min((int)(threadIdx.x & 63), nb - 1);
-  return KeyEnds{wave_join(((const uint32_t *)s.top)[2 * at + 1], [](uint32_t x, uint32_t y) { return max(x, y); }),
-                 wave_join(s.low[at], [](uint32_t x, uint32_t y) { return min(x, y); })};
+  return KeyEnds{wave_max32(((const uint32_t *)s.top)[2 * at + 1]), wave_min32(s.low[at])};
 }
 
 // In straight code: what is not to be counted goes to a spare bin of its lane, whose
@@ -406,16 +401,19 @@ __device__ bool load_bin(Pick &k, Row &r, int b) {
     if (i == t) first = key;
     d |= key ^ first;
   }
+  if (r.n <= kSorted) {
+    __syncthreads();
+    sort_list(k, r);
+    return true;
+  }
   // bits in which any two keys differ: from the wave's first key, and that from the list's
-  const uint32_t lead = (uint32_t)__shfl((int)first, 0, 64);
+  const uint32_t lead = (uint32_t)readlane((int)first, 0);
   if (t < r.n) d |= first ^ lead;
   __syncthreads();
   if ((t & ~63) < r.n) d |= lead ^ k.key[0];
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) d |= (uint32_t)__shfl_xor((int)d, o, 64);
+  d = wave_join(d, [](uint32_t x, uint32_t y) { return x | y; });
   if (lane == 0 && d) atomicOr(&k.differ, d);
   __syncthreads();
-  if (r.n <= kSorted) sort_list(k, r);
   return true;
 }
 
