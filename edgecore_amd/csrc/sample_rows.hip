@@ -31,10 +31,9 @@
 // A bin of more than kCap elements (equal logits mostly; what a block's LDS has room
 // for) is searched by the same steps over the whole row.
 //
-// Rows of 151936: one with top-k and top-p takes 3.1 + 5.2 + 10.6 us in the three
-// kernels, 16 nuclei 4.1 + 9.8 + 18.9, 128 mixed ones 15.4 + 37 + 21.  Chunks of 8192
-// gave 3.7 + 7 + 9, 5 + 11 + 17.6 and 15.3 + 38 + 19.4: the same within 2%, with twice
-// the room for a row's tail.
+// Rows of 151936: one with top-k and top-p takes 3 + 5.2 + 9.5 us in the three kernels, 16
+// nuclei 4.4 + 9.9 + 16.1, 128 mixed ones 15 + 37 + 18.4.  Chunks of 8192 gave the same
+// within 2%, with twice the room for a row's tail.
 #include <type_traits>
 
 #include "ec_device.h"
@@ -48,7 +47,7 @@ namespace {
 typedef unsigned long long u64;
 
 constexpr double kOne = 17592186044416.0;  // 2^44: w = 1
-constexpr int kChunk = 4096, kBins = 512, kCap = 4096, kSorted = 256, kBinThreads = 512, kTopThreads = 256;
+constexpr int kChunk = 4096, kBins = 512, kCap = 4096, kSorted = 256, kFew = 32, kBinThreads = 512, kTopThreads = 256;
 constexpr int kMaxChunks = (1 << 18) / kChunk;  // one per lane of a wave
 static_assert(kMaxChunks <= 64 && kChunk <= 65535, "chunks per lane, counts in 16 bits");
 constexpr float kNats = 32.0f;  // e^-32 is 0 in steps of 2^-44
@@ -315,7 +314,7 @@ struct Pick {
   // a step's histogram, and what it found
   int hc[256];
   u64 hw[256];
-  int found, found_cnt, found_equal;
+  int found, found_cnt, found_equal, few, few_at[kFew];
   u64 found_sum;
   u64 wave_w[16];
   uint32_t differ;
@@ -343,7 +342,14 @@ __device__ void sort_list(Pick &k, const Row &r) {
   if (i < r.n) {
     key = k.key[i], idx = k.idx[i], w = k.w[i];
     const u64 mine = order(i);
-    for (int j = t & 3; j < r.n; j += 4) before += order(j) > mine;
+    // eight reads a round (behind the list, but in the arrays: not counted)
+    for (int j0 = t & 3; j0 < r.n; j0 += 32) {
+      u64 o[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++) o[j] = order(j0 + 4 * j);
+#pragma unroll
+      for (int j = 0; j < 8; j++) before += j0 + 4 * j < r.n && o[j] > mine;
+    }
   }
   before += dpp_mov<0xB1>(before);
   before += dpp_mov<0x4E>(before);
@@ -428,12 +434,14 @@ struct Border {
 // Fixes the bits of a key below `bits`, 8 at a time, until the element is found at
 // which the running count reaches want (BY_SUM false) or the running sum passes
 // target, over the elements that each(f) hands to f(key, weight) and whose upper
-// bits are prefix's.  cnt, sum: what comes before them all.
+// bits are prefix's.  cnt, sum: what comes before them all.  It ends when all bits are
+// fixed or at most `few` elements agree in those that are (bits: how many are not).
 template <bool BY_SUM, class Each>
-__device__ Border fix_bits(Pick &k, const Each &each, uint32_t prefix, int bits, int cnt, u64 sum, int want, u64 target) {
+__device__ Border fix_bits(Pick &k, const Each &each, uint32_t prefix, int &bits, int cnt, u64 sum, int want, u64 target,
+                           int few = 0) {
   const int t = threadIdx.x, lane = t & 63;
-  int equal = 0;
-  while (bits > 0) {
+  int equal = few + 1;
+  while (bits > 0 && equal > few) {
     const int take = bits < 8 ? bits : 8, shift = bits - take;
     __syncthreads();
     if (t < 256) {
@@ -494,6 +502,34 @@ struct Place {
   int token;
 };
 
+// The element among at.equal (kFew at most) of the list whose keys agree with at.key
+// above `bits`: a wave compares each with all.
+template <bool BY_SUM>
+__device__ Place find_few(Pick &k, const Row &r, const Border &at, int bits, int want, u64 target) {
+  const int t = threadIdx.x;
+  __syncthreads();
+  if (t == 0) k.few = 0;
+  __syncthreads();
+  for (int i = t; i < r.n; i += 1024)
+    if ((k.key[i] >> bits) == at.key) k.few_at[atomicAdd(&k.few, 1)] = i;
+  __syncthreads();
+  if (t < 64) {
+    const int i = t < at.equal ? k.few_at[t] : -1;
+    const u64 mine = i < 0 ? 0 : ((u64)k.key[i] << 32) | ~k.idx[i], w = i < 0 ? 0 : k.w[i];
+    int cnt = at.above;
+    u64 sum = at.sum;
+    for (int j = 0; j < at.equal; j++)
+      if (readlane(mine, j) > mine) cnt++, sum += readlane(w, j);
+    if (i >= 0 && (BY_SUM ? sum <= target && sum + w > target : cnt + 1 == want)) {
+      k.found = i;
+      k.found_sum = sum + w;
+    }
+  }
+  __syncthreads();
+  const int i = k.found;
+  return Place{k.found_sum, k.w[i], (int)k.idx[i]};
+}
+
 // The element at which the running count reaches want, or the running sum passes
 // target (there is one).
 template <bool BY_SUM, bool TOKEN>
@@ -523,7 +559,7 @@ __device__ Place find_place(Pick &k, Row &r, int want, u64 target) {
   }
   Border at;
   if (listed) {
-    const int bits = k.differ ? 32 - __clz(k.differ) : 0;
+    int bits = k.differ ? 32 - __clz(k.differ) : 0;
     if (bits == 0) {
       at = Border{k.key[0], r.n, k.cnt[b], k.sum[b]};
     } else {
@@ -532,9 +568,11 @@ __device__ Place find_place(Pick &k, Row &r, int want, u64 target) {
           [&](auto f) {
             for (int i = t; i < r.n; i += 1024) f(k.key[i], k.w[i]);
           },
-          bits < 32 ? k.key[0] >> bits : 0, bits, k.cnt[b], k.sum[b], want, target);
+          bits < 32 ? k.key[0] >> bits : 0, bits, k.cnt[b], k.sum[b], want, target, kFew);
+      if (at.equal <= kFew) return find_few<BY_SUM>(k, r, at, bits, want, target);
     }
   } else {
+    int bits = 32;
     at = fix_bits<BY_SUM>(
         k,
         [&](auto f) {
@@ -543,7 +581,7 @@ __device__ Place find_place(Pick &k, Row &r, int want, u64 target) {
             if (v > -__builtin_inff() && bin_of(r.sc, v) == b) f(key_of(v), weight(r.sc, v, k.tab));
           }
         },
-        0, 32, k.cnt[b], k.sum[b], want, target);
+        0, bits, k.cnt[b], k.sum[b], want, target);
   }
   // of the elements with the key, the number of those before this one
   p.w = weight(r.sc, key_value(at.key), k.tab);
@@ -554,18 +592,11 @@ __device__ Place find_place(Pick &k, Row &r, int want, u64 target) {
   }
   p.upto = at.sum + (u64)(ties + 1) * p.w;
   if (!TOKEN) return p;
-  if (listed && at.equal == 1) {
-    __syncthreads();
-    for (int i = t; i < r.n; i += 1024)
-      if (k.key[i] == at.key) k.found = (int)k.idx[i];
-    __syncthreads();
-    p.token = k.found;
-    return p;
-  }
   // number `ties` by index: the largest complement of the index but for so many
   constexpr int kIdxBits = 18;
   constexpr uint32_t kIdx = (1u << kIdxBits) - 1;
   static_assert(kMaxChunks * kChunk <= 1 << kIdxBits, "an index's bits");
+  int bits = kIdxBits;
   const Border i = fix_bits<false>(
       k,
       [&](auto f) {
@@ -577,7 +608,7 @@ __device__ Place find_place(Pick &k, Row &r, int want, u64 target) {
             if (key_of(r.l[j]) == at.key) f(~(uint32_t)j & kIdx, 0);
         }
       },
-      0, kIdxBits, 0, 0, ties + 1, 0);
+      0, bits, 0, 0, ties + 1, 0);
   p.token = (int)(~i.key & kIdx);
   return p;
 }
@@ -600,10 +631,10 @@ __device__ uint32_t least_key(const Scale &sc, double min_p) {
   return thr;
 }
 
-// Bound by latency, a block per row: the ends 1.5 us, the chunks' bins 2.5, then for each
-// border not among the elements already there its bin 2.3 (two dependent reads past
-// the L2) and the search, 0.4 in a sorted list, 0.9 a round of 8 bits; so 10 us for a
-// short top-k, 18 where two borders of a nucleus lie in bins of 800.
+// Bound by latency, a block per row: the ends 1.5 us, the chunks' bins 2.1, then for each
+// border not among the elements already there its bin 2.1 (two dependent reads past
+// the L2) and the search: 0.4 to 0.8 in a sorted list, else 0.9 a round of 8 bits and 0.5
+// for the few that are left (all 32 bits in rounds took 18.1 us for the nuclei).
 __global__ __launch_bounds__(1024) void sample_pick_kernel(SampleArgs a, Scratch s, int row0, int nb) {
   __shared__ Pick k;
   const int t = threadIdx.x, lane = t & 63, w = t >> 6, row = row0 + blockIdx.x;

@@ -113,6 +113,19 @@ def test_sample_ties(V):
     check_sample(x, rng.random(R), None, None, p, None)
 
 
+@pytest.mark.parametrize("V,step", [(60000, 2.0 ** -9), (60000, 2.0 ** -12), (151936, 2.0 ** -13), (151936, 2.0 ** -7)])
+def test_sample_ties_in_full_bins(V, step):
+    """Logits on a grid: bins of hundreds of elements, equal ones by a few to hundreds."""
+    rng = np.random.default_rng(int(V + 1 / step))
+    R = 12
+    x = (np.round(rng.normal(0, 1.5, (R, V)) / step) * step).astype(np.float32)
+    T = rng.uniform(0.8, 3.0, R).astype(np.float32)
+    check_sample(x, rng.random(R), T)
+    check_sample(x, rng.random(R), T, None, rng.uniform(0.3, 0.99, R).astype(np.float32))
+    check_sample(x, rng.random(R), T, rng.integers(V // 50, V // 2, R).astype(np.int32), None,
+                 np.where(rng.random(R) < 0.5, 1e-3, 0.0).astype(np.float32))
+
+
 def test_sample_special_values():
     rng = np.random.default_rng(3)
     V = 5003
