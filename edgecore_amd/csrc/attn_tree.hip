@@ -119,9 +119,9 @@ __global__ __launch_bounds__(256) void attn_tree_any_kernel(TreeAttnArgs a) {
 //
 // fp32 by two 16-bit parts: q = hi + lo (a row whose largest is outside [2^-4, 2^15)
 // under a power of two that brings it to 2^14: its low part's steps of 2^-24 are below
-// 2^-20 of the largest at worst, and a part is cut, not rounded, so that it is two
-// instructions less), weights = hi + lo below 2^14; keys and values are 16 bits as
-// they are, so two products give each sum to about 2^-21.  The running maximum is
+// 2^-20 of the largest at worst), weights = hi + lo below 2^14 (cut, not rounded, in
+// two instructions less: 2^-21 of a weight at most, as is a chain of fp32 sums); keys and
+// values are 16 bits as they are, so two products give each sum.  The running maximum is
 // raised only when a score passes it by a factor of 2^10 (the parts' room), and the
 // accumulated outputs are scaled only then: mostly in a part's first tile.
 //
@@ -437,9 +437,11 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_tree_kernel(TreeAttnArgs a,
     for (int k = 0; k < KS; k++)
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const Parts f = split2(v[k][2 * j] * up, v[k][2 * j + 1] * up);
+        const float x = v[k][2 * j] * up, y = v[k][2 * j + 1] * up;
+        const Parts f = split2(x, y);
         qh[k][j] = f.hi;
-        ql[k][j] = f.lo;
+        // once a block, so the low parts are the nearest here
+        ql[k][j] = (uint32_t)f2h(x - h2f((uint16_t)f.hi)) | (uint32_t)f2h(y - h2f((uint16_t)(f.hi >> 16))) << 16;
       }
   }
 
