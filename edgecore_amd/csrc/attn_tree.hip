@@ -119,9 +119,9 @@ __global__ __launch_bounds__(256) void attn_tree_any_kernel(TreeAttnArgs a) {
 //
 // fp32 by two 16-bit parts: q = hi + lo (a row whose largest is outside [2^-4, 2^15)
 // under a power of two that brings it to 2^14: its low part's steps of 2^-24 are below
-// 2^-20 of the largest at worst), weights = hi + lo below 2^14 (cut, not rounded, in
-// two instructions less: 2^-21 of a weight at most, as is a chain of fp32 sums); keys and
-// values are 16 bits as they are, so two products give each sum.  The running maximum is
+// 2^-20 of the largest at worst), weights = hi + lo below 2^14 (cut, not rounded, which
+// is two instructions less: off by 2^-21 of a weight at most); keys and values are 16
+// bits as they are, so two products give each sum.  The running maximum is
 // raised only when a score passes it by a factor of 2^10 (the parts' room), and the
 // accumulated outputs are scaled only then: mostly in a part's first tile.
 //
