@@ -848,6 +848,83 @@ def test_accept_unaligned_rows():
             assert np.array_equal(k.get(n, np.uint16, c[n].size + 1)[1:], w.ravel())
 
 
+@pytest.mark.parametrize("layers,kv,B,N", [(1, 1, 3, 4), (3, 7, 2, 64), (2, 8, 1, 2), (5, 520, 2, 9)])
+def test_accept_narrow_rows(layers, kv, B, N):
+    check_accept(accept_case(kv, layers, kv, B, N, range(3, 3 + B)))
+
+
+# ---------------------------------------------------------------------------
+# the largest batch, and arguments that may be missing
+# ---------------------------------------------------------------------------
+
+def test_largest_batch():
+    """65535 sequences of 64 rows through all of the cache's operators, checked at
+    the ends and in between."""
+    B, N, hd, Cr = 65535, 64, 4, 70
+    rng = np.random.default_rng(77)
+    x = rng.normal(0, 2, (B * N, 3 * hd)).astype(np.float32)
+    past = rng.integers(0, Cr - N + 1, B).astype(np.int32)
+    at = [0, 1, 255, 256, 32767, 32768, B - 2, B - 1]
+    kc = np.zeros((B, Cr, hd), np.uint16)
+    inv = ec.rope_inv_freq(hd, 1e4)
+    q, k, v = ec.qk_norm_rope_dev(x, kc, kc, 1, 1, past, N, inv_freq=inv)
+    for b in at:
+        one = ec.qk_norm_rope_dev(x[b * N:(b + 1) * N], kc[b:b + 1], kc[b:b + 1], 1, 1, past[b:b + 1], N, inv_freq=inv)
+        assert np.array_equal(q[b * N:(b + 1) * N], one[0])
+        assert np.array_equal(k[b], one[1][0]) and np.array_equal(v[b], one[2][0])
+    att = ec.attention_tree_dev(q, k, v, 1, 1, past, N)
+    for b in at:
+        check_attention(dict(H=1, KVH=1, past=past[b:b + 1], N=N, q=q[b * N:(b + 1) * N], kc=k[b:b + 1], vc=v[b:b + 1],
+                             slot=None, parent=None, nodes=None), got=att[b * N:(b + 1) * N])
+    token = rng.integers(0, 3, (B, N)).astype(np.int32)
+    path, npath, nxt, new, k2, _ = ec.tree_accept_dev(k[None], v[None], past, token, np.roll(token, -1, 1))
+    # a chain whose sampled tokens are the next node's: all of it stays but for what
+    # the last one's says
+    assert (npath == N).all() and (path == np.arange(N)).all() and np.array_equal(new, past + N)
+    assert np.array_equal(nxt, token[:, 0]) and np.array_equal(k2[0], k)
+
+
+def test_largest_batch_on_the_matrix_cores():
+    """As many rows for the form of tiles, one KV head of 32."""
+    B, N, hd, Cr = 65535, 64, 32, 65
+    rng = np.random.default_rng(78)
+    q = np.tile(rng.normal(0, 1, (N * 5, hd)).astype(np.float32), (B // 5, 1))
+    kc, vc = (f16(rng.normal(0, 1, (7, Cr, hd))) for _ in range(2))
+    slot, past = (np.arange(B) % 7).astype(np.int32), (np.arange(B) % 2).astype(np.int32)
+    got = ec.attention_tree_dev(q, kc, vc, 1, 1, past, N, slot)
+    for b in (0, 1, 4097, 32768, B - 1):
+        check_attention(dict(H=1, KVH=1, past=past[b:b + 1], N=N, q=q[b * N:(b + 1) * N], kc=kc, vc=vc, slot=slot[b:b + 1],
+                             parent=None, nodes=None), got=got[b * N:(b + 1) * N])
+    # equal inputs, equal outputs, all through the batch
+    assert np.array_equal(got[:70 * N], got[65450 * N:65520 * N])
+
+
+def test_one_norm_alone():
+    for name in ("qg", "kg"):
+        for hd in (64, 42):
+            c = rope_case(16, 4, 2, hd, 2, 3, [7, 0])
+            c[name] = None
+            check_rope(c, ec.rope_inv_freq(hd // 2 * 2, 1e4))
+
+
+def test_sample_without_probabilities():
+    rng = np.random.default_rng(18)
+    x, u = rng.normal(0, 2, (3, 700)).astype(np.float32), rng.random(3)
+    want, _ = ec.sample_dev(x, u)
+    with ec._Call() as k:
+        p = k.put("x", x, np.float32), k.put("u", u, np.float64), k.put("t", np.zeros(3), np.int32)
+        assert ec.lib().ec_sample_dev(p[0], 3, 700, 700, None, None, None, None, p[1], p[2], None) == 0
+        assert ec.lib().ec_sync() == 0
+        assert np.array_equal(k.get("t", np.int32, 3), want)
+
+
+def test_shared_slot():
+    """Two sequences that read one slot, at lengths of their own."""
+    c = attn_case(23, 6, 2, 64, 3, 1, [500, 90, 333], C=600)
+    c["slot"][:] = 2
+    check_attention(c)
+
+
 # ---------------------------------------------------------------------------
 # together
 # ---------------------------------------------------------------------------
