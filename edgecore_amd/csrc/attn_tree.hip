@@ -119,11 +119,13 @@ __global__ __launch_bounds__(256) void attn_tree_any_kernel(TreeAttnArgs a) {
 //
 // fp32 by two 16-bit parts: q = hi + lo (a row whose largest is outside [2^-4, 2^15)
 // under a power of two that brings it to 2^14: its low part's steps of 2^-24 are below
-// 2^-20 of the largest at worst), weights = hi + lo below 2^14 (cut, not rounded, which
-// is two instructions less: off by 2^-21 of a weight at most); keys and values are 16
-// bits as they are, so two products give each sum.  The running maximum is
-// raised only when a score passes it by a factor of 2^10 (the parts' room), and the
-// accumulated outputs are scaled only then: mostly in a part's first tile.
+// 2^-20 of the largest at worst), weights = hi + lo (off by 2^-23 of a weight or, below
+// 2^-1, by 2^-24 at most); keys and values are 16 bits as they are, so two products give
+// each sum.  The running maximum has weight 2^12, so that 2^-24 is 2^-36 of it: behind a
+// token that takes most of the weight stand thousands of small ones that matter
+// together.  It is raised only when a score passes it by a factor of 2^3 (the parts'
+// room), and the accumulated outputs are scaled only then: mostly in a part's first tile
+// (a lift of 2^4 and a room of 2^10 are no faster).
 //
 // What bounds it.  Two sequences of 64 nodes, 14 / 2 heads of 64, over 32600 rows: 38
 // us, 23 GFLOP of matrix products in two parts, 0.6 PFLOP/s.  The matrix cores are
@@ -139,8 +141,9 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 
 constexpr int kTp = 64;          // positions per tile
-constexpr float kRoom = 10.0f;   // how far scores may pass the running maximum (powers of two)
-constexpr float kLift = 4.0f;    // weights are 2^kLift times e^(x - m)
+constexpr float kRoom = 3.0f;    // how far scores may pass the running maximum (powers of two)
+constexpr float kLift = 12.0f;   // weights are 2^kLift times e^(x - m)
+static_assert(kLift + kRoom < 16.0f, "weights below 65504");
 
 // chunk c (16 bytes) of a tile's row r is at chunk c ^ swz(r): the 16-byte reads
 // of one chunk by 8 consecutive rows fall on distinct banks
@@ -250,16 +253,25 @@ __device__ __forceinline__ float row_sum(float v) {
   return __uint_as_float(x.x) + __uint_as_float(x.y);
 }
 
-// two values in two 16-bit parts each: hi their leading 11 bits, lo the rest.
-// (The nearest 16-bit value and a mixed-precision difference would be three
-// instructions, not six, but those take 8 cycles each, these 2.)
+// two values in two 16-bit parts each: hi their nearest 11 bits, lo the rest, both
+// stored as the nearest 16-bit value.  Nothing is cut: what is lost below the 16-bit
+// steps, and of lo's products in the sums that the largest weights have filled, goes
+// either way, so that many small weights lose nothing together (lo from cut bits, which
+// is one instruction a value less, is never negative: 1.4e-5 instead of 1.9e-6 off over
+// 32600 positions of which the first takes 0.99, and 2 of 42 us faster for the long
+// contexts).  The nearest 16-bit value and a mixed-precision difference would be three
+// instructions, not eight, but those take 8 cycles each, these 2: 43 us, and 20 instead
+// of 16.5 for the one-token sequences.
 struct Parts {
   uint32_t hi, lo;
 };
 __device__ __forceinline__ Parts split2(float x, float y) {
-  const float hx = __uint_as_float(__float_as_uint(x) & 0xFFFFE000u), hy = __uint_as_float(__float_as_uint(y) & 0xFFFFE000u);
-  return Parts{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(hx, hy)),
-               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x - hx, y - hy))};
+  typedef float v2f __attribute__((ext_vector_type(2)));
+  typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+  const float hx = __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xFFFFE000u),
+              hy = __uint_as_float((__float_as_uint(y) + 0x1000u) & 0xFFFFE000u);
+  return Parts{__builtin_bit_cast(uint32_t, __builtin_convertvector((v2f{hx, hy}), v2h)),
+               __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f{x - hx, y - hy}), v2h))};
 }
 __device__ __forceinline__ float half_of(v4u v, int e) { return h2f((uint16_t)(v[e >> 1] >> (16 * (e & 1)))); }
 
@@ -551,14 +563,17 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_tree_kernel(TreeAttnArgs a,
 #pragma unroll
         for (int r = 0; r < 4; r++) sc[pt][r] -= by;
     }
+    // the tile's weights are added up before they meet the sum so far: one by one, those
+    // below half a step of it would be lost
     v4u ph[2], pl[2];
+    float here = 0.0f;
 #pragma unroll
     for (int pt = 0; pt < 4; pt++) {
       float p[4];
 #pragma unroll
       for (int r = 0; r < 4; r++) {
         p[r] = __builtin_amdgcn_exp2f(sc[pt][r]);
-        sum += p[r];
+        here += p[r];
       }
 #pragma unroll
       for (int r = 0; r < 2; r++) {
@@ -567,6 +582,7 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_tree_kernel(TreeAttnArgs a,
         pl[pt >> 1][2 * (pt & 1) + r] = f.lo;
       }
     }
+    sum += here;
 
     // ---- outputs: o[d][r] of element 16 d + 4 lg + r ----
 #pragma unroll
