@@ -168,6 +168,7 @@ __device__ __forceinline__ uint64_t tile_mask(int p0, int lo, int past, uint64_t
 
 // How the positions are split: `parts` blocks per KV head and row block, of which a
 // sequence has as many as its tiles ask for, up to `most`.
+constexpr long kGridRow = 1L << 20;
 struct TreeGrid {
   int parts, most, rb, shift;  // rb: row blocks per KV head; tiles >> shift add up in 31 bits
 };
@@ -325,7 +326,7 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_tree_kernel(TreeAttnArgs a,
   const int w = __builtin_amdgcn_readfirstlane(t >> 6);
   // blocks go to the 8 XCDs in turn: a part's row blocks, which read the same rows
   // of the cache, follow each other on one XCD
-  const int x = blockIdx.x, unit = ((x >> 3) / gr.rb) * 8 + (x & 7), rb = (x >> 3) % gr.rb;
+  const int x = blockIdx.y * gridDim.x + blockIdx.x, unit = ((x >> 3) / gr.rb) * 8 + (x & 7), rb = (x >> 3) % gr.rb;
   if (unit >= gr.parts * a.KVH) return;
   const int kvh = unit % a.KVH, part = unit / a.KVH;
   const int G = a.H / a.KVH, r0 = rb * 16 * NW;
@@ -721,9 +722,11 @@ __global__ __launch_bounds__(256) void attn_tree_join_kernel(TreeAttnArgs a, Tre
     *reinterpret_cast<float4 *>(a.out + ((size_t)b * a.t.N + node) * a.ldo + (size_t)(r - node * a.H) * HD + 4 * li) = o;
 }
 
-// heads and rows that the matrix-core form's tiles and 16-byte accesses can take (both
-// sides' times stand at the form for any size)
+// heads and rows that the matrix-core form's tiles and 16-byte accesses can take, and
+// whose blocks (no more than query heads in all) count in an int (both sides' times stand
+// at the form for any size)
 bool tiles_ok(const TreeAttnArgs &a) {
+  if ((long)a.t.B * a.t.N * a.H > 1L << 30) return false;
   const uintptr_t p = (uintptr_t)a.q | (uintptr_t)a.kc | (uintptr_t)a.vc | (uintptr_t)a.out;
   return (a.hd == 32 || a.hd == 64 || a.hd == 96 || a.hd == 128) && !(p & 15) && a.ldq % 4 == 0 && a.ldo % 4 == 0;
 }
@@ -763,7 +766,10 @@ TreeGrid tree_grid(const TreeAttnArgs &a) {
 template <int HD>
 hipError_t launch_tree(const TreeAttnArgs &a, hipStream_t st) {
   const TreeGrid g = tree_grid(a);
-  const dim3 grid((unsigned)(((long)g.parts * a.KVH + 7) / 8 * 8 * g.rb));
+  // a multiple of 8 blocks in x (the XCDs' turns), as many as a dimension's 2^32 threads
+  // have room for
+  const long blocks = ((long)g.parts * a.KVH + 7) / 8 * 8 * g.rb, row = blocks < kGridRow ? blocks : kGridRow;
+  const dim3 grid((unsigned)row, (unsigned)((blocks + row - 1) / row));
   const uint32_t lds = 2 * 4 * kTp * HD;
   if (tree_waves(a) == 4) klaunch((attn_tree_kernel<HD, 4, HD <= 64 ? 4 : 2>), grid, dim3(256), lds, st, a, g);
   else klaunch((attn_tree_kernel<HD, 8, HD <= 64 ? 4 : 2>), grid, dim3(512), lds, st, a, g);

@@ -899,6 +899,23 @@ def test_largest_batch_on_the_matrix_cores():
     assert np.array_equal(got[:70 * N], got[65450 * N:65520 * N])
 
 
+def test_more_blocks_than_a_grid_dimension():
+    """65535 one-token sequences of 260 heads: blocks of 256 threads that are more than
+    2^32 threads in all."""
+    B, H, hd = 65535, 260, 32
+    assert B * H * 256 > 2 ** 32
+    rng = np.random.default_rng(79)
+    few = rng.normal(0, 1, (15, H * hd)).astype(np.float32)
+    kc, vc = (f16(rng.normal(0, 1, (7, 3, H * hd))) for _ in range(2))
+    slot, past = (np.arange(B) % 7).astype(np.int32), (np.arange(B) % 3).astype(np.int32)
+    got = ec.attention_tree_dev(np.tile(few, (B // 15, 1)), kc, vc, H, H, past, 1, slot, max_past=2)
+    for b in (0, 1, 32768, 65011, B - 2, B - 1):
+        check_attention(dict(H=H, KVH=H, past=past[b:b + 1], N=1, q=few[b % 15:b % 15 + 1], kc=kc, vc=vc, slot=slot[b:b + 1],
+                             parent=None, nodes=None), got=got[b:b + 1])
+    # equal inputs every 105 sequences, equal outputs all through the batch
+    assert np.array_equal(got[:-105], got[105:])
+
+
 def test_one_norm_alone():
     for name in ("qg", "kg"):
         for hd in (64, 42):
