@@ -2367,6 +2367,7 @@ extern "C" int ec_attention_dev(const float *q, int ldq, const uint16_t *kc, con
 constexpr long kMaxRows = 1L << 22;       // rows of a call (grids and row offsets stay in 32 bits)
 constexpr int kMaxCacheRows = 1 << 30;    // of a slot
 constexpr int kMaxKv = 1 << 28;           // elements of a cache row (twice as many columns count in an int)
+constexpr int kMaxLayers = 1 << 20;       // blocks of a grid's dimension
 
 // A range of memory; an empty or null one overlaps nothing.
 struct Span {
@@ -2531,6 +2532,7 @@ extern "C" int ec_tree_accept_dev(uint16_t *kc, uint16_t *vc, int layers, int ns
                         cache_span(vc, layers, t, kv)};
     if (spans_clash(in, out)) return set_err(-1, "%s: an output or a cache overlaps another array", fn);
   }
+  if (layers > kMaxLayers) return set_err(-1, "%s: %d layers (up to %d)", fn, layers, kMaxLayers);
   EC_INIT();
   const DeviceScope dev;
   const AcceptArgs a{t, kc, vc, layers, kv, token, sampled, path, npath, next, new_past};

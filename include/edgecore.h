@@ -504,7 +504,7 @@ int ec_sample_dev(const float *logits, int rows, int vocab, int ld, const float 
  * token, new_past [B] past + npath, and in every layer of kc, vc
  * [layers][nslots][C][kv] the rows past + path[j] move to past + j.  No nodes,
  * or a sequence that takes no part: npath 0, next -1, new_past = past.  N <=
- * 64, kv <= 2^28.  The outputs and caches overlap no other array of the call. */
+ * 64, kv <= 2^28, layers <= 2^20.  The outputs and caches overlap no other array of the call. */
 int ec_tree_accept_dev(uint16_t *kc, uint16_t *vc, int layers, int nslots, int C, int kv, const int *slot,
                        const int *past, const int *nodes, const int *parent, const int *token, const int *sampled,
                        int B, int N, int *path, int *npath, int *next, int *new_past);

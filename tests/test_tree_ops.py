@@ -123,6 +123,10 @@ def test_accept_refuses_wide_rows():
     refused(accept(**APART, kv=(1 << 28) + 1), "ec_tree_accept_dev", "rows of")
 
 
+def test_accept_refuses_more_layers_than_a_grid_has():
+    refused(accept(**APART, layers=(1 << 20) + 1, nslots=1, C=1, kv=1), "ec_tree_accept_dev", "layers")
+
+
 def test_device_array_checks(tmp_path):
     exe = tmp_path / "tree_check"
     src = REPO / "tests" / "c" / "tree_check.c"
