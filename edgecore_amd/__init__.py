@@ -493,6 +493,25 @@ def attention_dev(q: np.ndarray, kc: np.ndarray, vc: np.ndarray, pos, slot, H: i
 # drafted tokens over the slot cache, on host arrays copied to the device
 # ---------------------------------------------------------------------------
 
+def _sized(name: str, a, *shape) -> None:
+    """The kernels read as many elements as the call's numbers say: an array of another
+    shape (flat or not; None: absent) is refused."""
+    if a is not None and np.shape(a) != shape and np.shape(a) != (int(np.prod(shape)),):
+        raise ValueError(f"{name} has shape {np.shape(a)}, not {shape}")
+
+
+def _tree_sized(B: int, N: int, slot, past, nodes, parent) -> None:
+    for n, a, shape in (("slot", slot, (B,)), ("past", past, (B,)), ("nodes", nodes, (B,)), ("parent", parent, (B, N))):
+        _sized(n, a, *shape)
+
+
+def _caches(kc: np.ndarray, vc: np.ndarray, dims: int) -> tuple:
+    """The shape of a pair of caches, which hold fp16 bits."""
+    if kc.dtype != np.uint16 or vc.dtype != np.uint16 or kc.ndim != dims or kc.shape != vc.shape:
+        raise ValueError(f"caches of {kc.dtype} {kc.shape} and {vc.dtype} {vc.shape}, not two of uint16 and one shape")
+    return kc.shape
+
+
 class _Call:
     """Device copies of a call's arrays, freed at its end; None stays None."""
 
@@ -501,7 +520,10 @@ class _Call:
 
     def put(self, name: str, a, dtype):
         if a is not None:
-            self.bufs[name] = DeviceBuffer.from_array(np.ascontiguousarray(a, dtype))
+            b = np.ascontiguousarray(a, dtype)
+            if b.dtype == np.int32 and not np.array_equal(b, a):
+                raise ValueError(f"{name} has numbers that are no 32-bit integers")
+            self.bufs[name] = DeviceBuffer.from_array(b)
         return self.ptr(name)
 
     def ptr(self, name: str):
@@ -536,9 +558,14 @@ def qk_norm_rope_dev(qkv: np.ndarray, kc: np.ndarray, vc: np.ndarray, H: int, KV
     [nslots][C][KVH*hd] fp16 bits (uint16); returns (q [B*N][H*hd], kc, vc)
     after the call (q: what the padding rows hold)."""
     M, width = qkv.shape
-    nslots, Cr, kv = kc.shape
+    nslots, Cr, kv = _caches(kc, vc, 3)
     hd = kv // KVH
-    assert width == (H + 2 * KVH) * hd and M % N == 0
+    if kv % KVH or M % N:
+        raise ValueError(f"cache rows of {kv} for {KVH} heads, {M} rows for sequences of {N}")
+    for n, a, shape in (("qkv", qkv, (M, (H + 2 * KVH) * hd)), ("q", q, (M, H * hd)), ("q_gamma", q_gamma, (hd,)),
+                        ("k_gamma", k_gamma, (hd,))):
+        _sized(n, a, *shape)
+    _tree_sized(M // N, N, slot, past, nodes, parent)
     with _Call() as c:
         x = c.put("x", qkv, np.float32)
         qp = c.put("q", np.zeros((M, H * hd), np.float32) if q is None else q, np.float32)
@@ -547,7 +574,8 @@ def qk_norm_rope_dev(qkv: np.ndarray, kc: np.ndarray, vc: np.ndarray, H: int, KV
         f = c.put("f", inv_freq, np.float64)
         rot = 0 if inv_freq is None else 2 * len(inv_freq)
         _check(lib().ec_qk_norm_rope_dev(x, width, qp, H * hd, k, v, nslots, Cr, H, KVH, hd, *g, eps, f, rot, layout,
-                                         factor, *c.tree(slot, past, nodes, parent), M // N, N), "ec_qk_norm_rope_dev")
+                                         factor, *c.tree(slot, past, nodes, parent), M // N, N),
+               "ec_qk_norm_rope_dev")
         _check(lib().ec_sync(), "ec_sync")
         return (c.get("q", np.float32, (M, H * hd)), c.get("kc", np.uint16, kc.shape), c.get("vc", np.uint16, vc.shape))
 
@@ -559,7 +587,11 @@ def attention_tree_dev(q: np.ndarray, kc: np.ndarray, vc: np.ndarray, H: int, KV
     [nslots][C][KVH*hd] fp16 bits; returns out [B*N][H*hd] (out: what the
     padding rows hold; max_past: the cache's length by default)."""
     M, E = q.shape
-    nslots, Cr, _ = kc.shape
+    nslots, Cr, kv = _caches(kc, vc, 3)
+    if E % H or kv != KVH * (E // H) or M % N:
+        raise ValueError(f"q rows of {E} for {H} heads, cache rows of {kv} for {KVH}, {M} rows for sequences of {N}")
+    _sized("out", out, M, E)
+    _tree_sized(M // N, N, slot, past, nodes, parent)
     with _Call() as c:
         p = [c.put("q", q, np.float32), c.put("kc", kc, np.uint16), c.put("vc", vc, np.uint16)]
         o = c.put("out", np.zeros_like(q) if out is None else out, np.float32)
@@ -575,6 +607,8 @@ def sample_dev(logits: np.ndarray, u, temp=None, top_k=None, top_p=None, min_p=N
     """ec_sample_dev on host rows [rows][ld] (vocab: the columns that count);
     returns (token, prob) [rows]."""
     rows, ld = logits.shape
+    for n, a in (("u", u), ("temp", temp), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p)):
+        _sized(n, a, rows)
     with _Call() as c:
         x = c.put("x", logits, np.float32)
         p = [c.put("t", temp, np.float32), c.put("k", top_k, np.int32), c.put("p", top_p, np.float32),
@@ -589,8 +623,10 @@ def tree_accept_dev(kc: np.ndarray, vc: np.ndarray, past, token, sampled, slot=N
     """ec_tree_accept_dev on host arrays: kc / vc [layers][nslots][C][kv] fp16
     bits, token / sampled [B][N]; returns (path [B][N], npath, next, new_past
     [B], kc, vc) after the call."""
-    layers, nslots, Cr, kv = kc.shape
+    layers, nslots, Cr, kv = _caches(kc, vc, 4)
     B, N = np.shape(token)
+    _sized("sampled", sampled, B, N)
+    _tree_sized(B, N, slot, past, nodes, parent)
     with _Call() as c:
         k, v = c.put("kc", kc, np.uint16), c.put("vc", vc, np.uint16)
         t = [c.put("token", token, np.int32), c.put("sampled", sampled, np.int32)]

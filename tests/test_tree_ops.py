@@ -127,6 +127,41 @@ def test_accept_refuses_more_layers_than_a_grid_has():
     refused(accept(**APART, layers=(1 << 20) + 1, nslots=1, C=1, kv=1), "ec_tree_accept_dev", "layers")
 
 
+CACHE3, ROWS = np.zeros((2, 10, 64), np.uint16), np.zeros((6, 128), np.float32)
+GOOD = {
+    "rope": dict(qkv=np.zeros((6, 256), np.float32), kc=CACHE3, vc=CACHE3, H=2, KVH=1, past=[0, 1], N=3),
+    "attention": dict(q=ROWS, kc=CACHE3, vc=CACHE3, H=2, KVH=1, past=[0, 1], N=3),
+    "sample": dict(logits=ROWS, u=np.zeros(6)),
+    "accept": dict(kc=CACHE3[None], vc=CACHE3[None], past=[0, 1], token=np.zeros((2, 3), int), sampled=np.zeros((2, 3), int)),
+}
+TREE = [dict(past=[0]), dict(past=[0, 1, 2]), dict(slot=[0]), dict(nodes=[3, 3, 3]), dict(parent=[-1, 0, 1]),
+        dict(parent=np.zeros((3, 2), int)), dict(vc=CACHE3[:1]), dict(kc=CACHE3.astype(np.float16))]
+
+
+@pytest.mark.parametrize("fn,k", [(f, k) for f in ("rope", "attention", "accept") for k in TREE] + [
+    ("rope", dict(qkv=np.zeros((6, 255)))), ("rope", dict(qkv=np.zeros((7, 256)))), ("rope", dict(q=ROWS[:5])),
+    ("rope", dict(q_gamma=np.ones(63))), ("rope", dict(k_gamma=np.ones(1))), ("rope", dict(KVH=3)),
+    ("attention", dict(q=ROWS[:5])), ("attention", dict(H=3)), ("attention", dict(KVH=2)), ("attention", dict(out=ROWS[:5])),
+    ("sample", dict(u=np.zeros(5))), ("sample", dict(temp=np.ones(1))), ("sample", dict(top_k=[1, 2])),
+    ("sample", dict(top_p=np.ones(7))), ("sample", dict(min_p=np.ones((6, 2)))),
+    ("accept", dict(sampled=np.zeros((2, 2), int)))])
+def test_arrays_of_other_sizes(fn, k):
+    """The functions on host arrays refuse what the kernels would read past the end of."""
+    call = {"rope": ec.qk_norm_rope_dev, "attention": ec.attention_tree_dev, "sample": ec.sample_dev, "accept": ec.tree_accept_dev}[fn]
+    if fn == "accept":
+        k = {n: a[None] if n in ("kc", "vc") else a for n, a in k.items()}
+    with pytest.raises(ValueError):
+        call(**{**GOOD[fn], **k})
+
+
+def test_numbers_of_more_than_32_bits(monkeypatch):
+    monkeypatch.setattr(ec.DeviceBuffer, "from_array", classmethod(lambda cls, a: None))
+    with pytest.raises((ValueError, OverflowError)):
+        ec._Call().put("past", np.array([2 ** 32 + 5]), np.int32)
+    with pytest.raises(ValueError):
+        ec._Call().put("past", np.array([0.5]), np.int32)
+
+
 def test_device_array_checks(tmp_path):
     exe = tmp_path / "tree_check"
     src = REPO / "tests" / "c" / "tree_check.c"
