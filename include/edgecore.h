@@ -472,9 +472,9 @@ int ec_rope_inv_freq(int rope_type, int dim, double theta, double factor, double
  * H.  max_past: the largest past of the call (it sizes the launch; a sequence
  * with a larger one takes no part).  Rows that a node does not see do not
  * reach it, whatever they hold.  out may be q itself, but overlaps no other
- * array.  A key or query with an infinity among finite ones gives NaN to the
- * nodes that see it, an infinite value NaN or an infinity.  Uses the library's
- * workspace: a captured call needs one of its size before the capture, as the
+ * array.  Of what a node sees, a score of +inf or NaN gives NaN, a score of
+ * -inf (of an infinity in its key or query) weighs nothing or gives NaN, an
+ * infinite value gives NaN or an infinity.  Uses the library's workspace: a captured call needs one of its size before the capture, as the
  * matrix-core GEMMs do. */
 int ec_attention_tree_dev(const float *q, int ldq, const uint16_t *kc, const uint16_t *vc, int nslots, int C, int H,
                           int KVH, int hd, const int *slot, const int *past, const int *nodes, const int *parent, int B,

@@ -135,3 +135,48 @@ def test_first_token_in_and_out_of_a_window(window):
     for H, KVH, hd in ((14, 2, 64), (12, 2, 128)):
         for at in (0.0, 1.0 - window / 3000, 1.0 - (window - 4) / 3000):
             check(peaked(window, H, KVH, hd, 2, 9, 3000, at, 4.6), [(0, 0), (1, 8)], window)
+
+
+@pytest.mark.parametrize("H,KVH,hd", [(14, 2, 64), (12, 2, 128), (8, 1, 32), (5, 1, 40)])
+@pytest.mark.parametrize("at", [100, 703])
+def test_infinite_keys_and_queries(H, KVH, hd, at):
+    """One element of a key that is seen (in the text, among the nodes) is infinite: NaN
+    where the score is +inf; where it is -inf, NaN or the result without the key.  One
+    of a query: NaN in its own row and head."""
+    c = peaked(11, H, KVH, hd, 2, 5, 703, 0.3, 1.0)
+    c["parent"][:] = np.arange(5) - 1
+    call = lambda: ec.attention_tree_dev(c["q"], c["kc"], c["vc"], H, KVH, c["past"], 5, c["slot"], None, c["parent"])
+    clean = call().reshape(2, 5, KVH, H // KVH, hd)
+    e = hd // 2 + 3
+    kept = c["kc"][0, at].copy()
+    for sign in (1, -1):
+        c["kc"][0, at] = kept
+        c["kc"][0, at, e] = 0x7C00 if sign > 0 else 0xFC00
+        got = call().reshape(clean.shape)
+        up = c["q"].reshape(clean.shape)[0, :, 0, :, e] * sign > 0
+        assert up.any() and not up.all()
+        assert np.isnan(got[0, :, 0][up]).all()
+        # the same with a key whose score is far below all others
+        far = c["q"].reshape(clean.shape)[0, :, 0][~up]
+        for n, q in zip(np.argwhere(~up), far):
+            i, g = n
+            mine = got[0, i, 0, g]
+            if np.isnan(mine).all():
+                continue
+            keys, values = (c[m][0, :703 + i + 1, :hd].view(np.float16).astype(np.float64) for m in ("kc", "vc"))
+            with np.errstate(invalid="ignore"):
+                x = keys @ q.astype(np.float64) / math.sqrt(hd)
+            x[at] = -np.inf
+            # (7e2 positions, values of about 1: what plain fp32 is off by stays below 1e-5)
+            assert np.abs(mine - attend(x[None], values, np.float64)[0]).max() < 1e-5
+        assert np.array_equal(got[1], clean[1]) and np.array_equal(got[0, :, 1:], clean[0, :, 1:])
+    c["kc"][0, at] = kept
+    for bad in (np.inf, -np.inf, np.nan):
+        q = c["q"][3, hd + 1]
+        c["q"][3, hd + 1] = bad
+        got = call().reshape(10, H, hd)
+        c["q"][3, hd + 1] = q
+        assert np.isnan(got[3, 1]).all()
+        got[3, 1] = clean.reshape(10, H, hd)[3, 1]
+        # (when a row's maximum moves decides when its neighbours' do, by their room)
+        assert np.abs(got - clean.reshape(10, H, hd)).max() < 1e-5
