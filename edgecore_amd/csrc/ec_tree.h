@@ -74,8 +74,9 @@ namespace ec {
 
 /* Every lane of the wave calls the functions below. */
 
-/* whether sequence b's nodes share a row with those of an earlier sequence (never
- * where every sequence has its own slot): four sequences a lane at a time, so that
+/* whether sequence b's nodes share a row with those of an earlier sequence, written
+ * or not: what the earlier ones' parents and clashes are is not followed (never where
+ * every sequence has its own slot).  Four sequences a lane at a time, so that
  * a round is one wait */
 __device__ __forceinline__ bool tree_clashes(const EcTreeBatch &t, int b, EcTreeSeq s) {
   if (!t.slot) return false;

@@ -443,7 +443,9 @@ int ec_sample_candidates(const float *vals, const int *idx, int ncand, int vocab
  * before its node, takes no part.  Its rows of q / out are NaN (with nodes
  * outside [0, N]: all N), no cache row is written, its path is empty.  Where
  * rows are written, so it is for a sequence whose rows overlap those of an
- * earlier one of the call. */
+ * earlier one of the call, also where that one, by its parents or by a still
+ * earlier one, takes no part itself (one whose slot, past or nodes name no rows
+ * has none to overlap). */
 
 /* Rows of q | k | v (fp32, H + 2 KVH heads of hd <= 512, row stride ldx) into
  * q (fp32, row stride ldq; it may be qkv itself, with ldx) and the fp16 caches kc, vc

@@ -718,6 +718,17 @@ def test_rope_same_rows_twice():
     check_rope(c, ec.rope_inv_freq(64, 1e4))
 
 
+def test_rope_same_rows_as_one_that_writes_none():
+    """An earlier sequence with bad parents, or itself too late, still excludes a later
+    one; one that names no rows does not."""
+    c = rope_case(17, 4, 2, 64, 3, 8, [50, 57, 64], C=100, tree=True)
+    c["slot"][:] = 1
+    c["parent"][0, 3] = 5
+    check_rope(c, ec.rope_inv_freq(64, 1e4), bad=(0, 1, 2))
+    c["past"][0] = 93
+    check_rope(c, ec.rope_inv_freq(64, 1e4), bad=(0, 2))
+
+
 def test_rope_same_rows_far_apart():
     """Among 600 sequences: pairs that share a row, next to each other and far apart."""
     c = rope_case(15, 2, 1, 16, 600, 2, [5] * 600)
@@ -829,6 +840,16 @@ def test_accept_same_rows_twice():
     c = accept_case(14, 2, 64, 3, 8, [50, 57, 58], C=100)
     c["slot"][:] = 1
     check_accept(c, bad=(1, 2))
+
+
+def test_accept_same_rows_as_one_that_keeps_none():
+    """As for the appends: bad parents, too late itself, no rows."""
+    c = accept_case(17, 2, 64, 3, 8, [50, 57, 64], C=100)
+    c["slot"][:] = 1
+    c["parent"][0, 3] = 5
+    check_accept(c, bad=(0, 1, 2))
+    c["past"][0] = 93
+    check_accept(c, bad=(0, 2))
 
 
 def test_accept_unaligned_rows():
