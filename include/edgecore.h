@@ -493,8 +493,11 @@ int ec_attention_tree_dev(const float *q, int ldq, const uint16_t *kc, const uin
  * off); temp not above 0 takes the largest logit.  NaN counts as -inf, -inf is
  * not drawn, a row of nothing else gives -1.  prob [rows] (nullable): the
  * drawn token's share of the sum, 1 for the largest logit, 0 for -1.  Weights
- * and sums are 64-bit in an order-independent form: equal calls give equal
- * tokens.  Uses the library's workspace (as ec_attention_tree_dev); token and
+ * are rounded to whole steps of 2^-44 of the largest, their sums are exact in
+ * 64 bits: equal calls give equal tokens, a token more than 31 temps below the
+ * largest logit weighs nothing and is not drawn, and the prob of one that weighs
+ * w of the largest is off by 2^-45 / w of itself at most, besides its rounding
+ * to fp32.  Uses the library's workspace (as ec_attention_tree_dev); token and
  * prob overlap no other array. */
 int ec_sample_dev(const float *logits, int rows, int vocab, int ld, const float *temp, const int *top_k,
                   const float *top_p, const float *min_p, const double *u, int *token, float *prob);

@@ -218,6 +218,22 @@ def test_sample_many_rows():
         assert tok[r] == want[0] and abs(prob[r] - want[1]) <= 2 * U * want[1] + 1e-12
 
 
+def test_sample_unlikely_tokens():
+    """Drawn tokens of small weights: their probability to 2^-45 of the largest weight;
+    those that weigh less than half a step are never drawn."""
+    V, at = 5000, 4321
+    gaps = np.array([5.0, 10.0, 15.0, 20.0, 25.0, 28.0, 30.0, 30.4])
+    x = np.full((len(gaps), V), -1000.0, np.float32)
+    x[:, 17], x[:, at] = 3.0, 3.0 - gaps
+    got = ec.sample_dev(x, np.full(len(gaps), 1.0 - 2.0 ** -53))
+    w = np.exp((x[:, at].astype(np.float64) - 3.0))
+    assert (got[0] == at).all()
+    # half a step of the weight (and the exponential's own 2^-46 of it), one rounding to fp32
+    assert (np.abs(got[1] / (w / (1 + w)) - 1) <= 2.0 ** -45 / w + 2.0 ** -46 + 2 * U).all()
+    x[:, at] = 3.0 - 31.3
+    assert (ec.sample_dev(x, np.full(len(gaps), 1.0 - 2.0 ** -53))[0] == 17).all()
+
+
 def test_sample_as_the_driver():
     """With top_k alone and the driver's number the driver's token."""
     rng = np.random.default_rng(12)
