@@ -121,7 +121,7 @@ __global__ __launch_bounds__(256) void attn_tree_any_kernel(TreeAttnArgs a) {
 // under a power of two that brings it to 2^14: its low part's steps of 2^-24 are below
 // 2^-20 of the largest at worst), weights = hi + lo (off by 2^-23 of a weight or, below
 // 2^-1, by 2^-24 at most); keys and values are 16 bits as they are, so two products give
-// each sum.  The running maximum has weight 2^12, so that 2^-24 is 2^-36 of it: behind a
+// each sum.  The running maximum's parts are of 2^12, so that 2^-24 is 2^-36 of it: behind a
 // token that takes most of the weight stand thousands of small ones that matter
 // together.  It is raised only when a score passes it by a factor of 2^3 (the parts'
 // room), and the accumulated outputs are scaled only then: mostly in a part's first tile
@@ -142,8 +142,9 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 
 constexpr int kTp = 64;          // positions per tile
 constexpr float kRoom = 3.0f;    // how far scores may pass the running maximum (powers of two)
-constexpr float kLift = 12.0f;   // weights are 2^kLift times e^(x - m)
-static_assert(kLift + kRoom < 16.0f, "weights below 65504");
+constexpr int kLift = 12;        // the weights' parts are those of 2^kLift e^(x - m)
+constexpr float kLifted = 1 << kLift;
+static_assert(kLift + kRoom < 16.0f, "parts below 65504");
 
 // chunk c (16 bytes) of a tile's row r is at chunk c ^ swz(r): the 16-byte reads
 // of one chunk by 8 consecutive rows fall on distinct banks
@@ -254,8 +255,9 @@ __device__ __forceinline__ float row_sum(float v) {
   return __uint_as_float(x.x) + __uint_as_float(x.y);
 }
 
-// two values in two 16-bit parts each: hi their nearest 11 bits, lo the rest, both
-// stored as the nearest 16-bit value.  Nothing is cut: what is lost below the 16-bit
+// two values times 2^LIFT in two 16-bit parts each: hi their nearest 11 bits (the lift
+// comes with the rounding, in one addition to the value's bits), lo the rest, both stored
+// as the nearest 16-bit value.  Nothing is cut: what is lost below the 16-bit
 // steps, and of lo's products in the sums that the largest weights have filled, goes
 // either way, so that many small weights lose nothing together (lo from cut bits, which
 // is one instruction a value less, is never negative: 1.4e-5 instead of 1.9e-6 off over
@@ -266,13 +268,16 @@ __device__ __forceinline__ float row_sum(float v) {
 struct Parts {
   uint32_t hi, lo;
 };
+template <int LIFT = 0>
 __device__ __forceinline__ Parts split2(float x, float y) {
   typedef float v2f __attribute__((ext_vector_type(2)));
   typedef _Float16 v2h __attribute__((ext_vector_type(2)));
-  const float hx = __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xFFFFE000u),
-              hy = __uint_as_float((__float_as_uint(y) + 0x1000u) & 0xFFFFE000u);
+  constexpr uint32_t up = 0x1000u + ((uint32_t)LIFT << 23);
+  constexpr float lift = 1 << LIFT;
+  const float hx = __uint_as_float((__float_as_uint(x) + up) & 0xFFFFE000u),
+              hy = __uint_as_float((__float_as_uint(y) + up) & 0xFFFFE000u);
   return Parts{__builtin_bit_cast(uint32_t, __builtin_convertvector((v2f{hx, hy}), v2h)),
-               __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f{x - hx, y - hy}), v2h))};
+               __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f{__builtin_fmaf(x, lift, -hx), __builtin_fmaf(y, lift, -hy)}), v2h))};
 }
 __device__ __forceinline__ float half_of(v4u v, int e) { return h2f((uint16_t)(v[e >> 1] >> (16 * (e & 1)))); }
 
@@ -537,8 +542,8 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_tree_kernel(TreeAttnArgs a,
 #pragma unroll
         for (int r = 0; r < 4; r++) sc[pt][r] *= down;
     }
-    // exponents of the weights already (the sums began at kLift - mx): above kLift
-    // + kRoom the maximum moves
+    // exponents of the weights already (the sums began at -mx): above kRoom the maximum
+    // moves
     float top = -FLT_MAX;
 #pragma unroll
     for (int pt = 0; pt < 4; pt++)
@@ -546,13 +551,13 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_tree_kernel(TreeAttnArgs a,
       for (int r = 0; r < 4; r++) top = fmaxf(top, sc[pt][r]);
     if (__builtin_expect(__ballot(top > lim) != 0, 0)) {
       const float big = row_max(top);
-      const bool first = mx == -FLT_MAX, move = big > (first ? -FLT_MAX : kLift);
-      const float by = move ? big - kLift : 0.0f, back = first ? 0.0f : __builtin_amdgcn_exp2f(-by);
+      const bool first = mx == -FLT_MAX, move = big > (first ? -FLT_MAX : 0.0f);
+      const float by = move ? big : 0.0f, back = first ? 0.0f : __builtin_amdgcn_exp2f(-by);
       if (move) {
         mx = first ? big : mx + by;
-        lim = kLift + kRoom;
+        lim = kRoom;
       }
-      const float f = move || !first ? (kLift - mx) * up : 0.0f;
+      const float f = move || !first ? -mx * up : 0.0f;
       from = v4f{f, f, f, f};
       sum *= back;
 #pragma unroll
@@ -578,7 +583,7 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_tree_kernel(TreeAttnArgs a,
       }
 #pragma unroll
       for (int r = 0; r < 2; r++) {
-        const Parts f = split2(p[2 * r], p[2 * r + 1]);
+        const Parts f = split2<kLift>(p[2 * r], p[2 * r + 1]);
         ph[pt >> 1][2 * (pt & 1) + r] = f.hi;
         pl[pt >> 1][2 * (pt & 1) + r] = f.lo;
       }
@@ -630,7 +635,7 @@ __global__ __launch_bounds__(NW * 64, OCC) void attn_tree_kernel(TreeAttnArgs a,
   for (; tile < tile1; tile++) step(std::true_type{}, tile);
 
   if (!edges) tree_parent(parent, s.n, &ok);
-  const float l = ok ? row_sum(sum) : __builtin_nanf("");
+  const float l = ok ? row_sum(sum) * kLifted : __builtin_nanf("");  // as the outputs
   if (!live) return;
   if (!joins) {
     const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
