@@ -1144,6 +1144,39 @@ def test_release_between():
     assert np.array_equal(check_attention(c), first)
 
 
+def test_capture_without_a_workspace():
+    """A captured call whose workspace is not there yet is refused, the capture ends as
+    ever, and the same call runs after an eager one has made it."""
+    L = ec.lib()
+    if L.ec_release():
+        pytest.skip("models are loaded")
+    c = attn_case(52, 12, 2, 128, 2, 4, [900, 100])
+    rng = np.random.default_rng(53)
+    x, u = rng.normal(0, 2, (3, 5000)).astype(np.float32), rng.random(3)
+    nslots, Cr, _ = c["kc"].shape
+    E = 12 * 128
+    with ec._Call() as k:
+        a = [k.put("q", c["q"], np.float32), E, k.put("kc", c["kc"], np.uint16), k.put("vc", c["vc"], np.uint16), nslots, Cr, 12, 2,
+             128, *k.tree(c["slot"], c["past"], None, c["parent"]), 2, 4, Cr, 0, k.put("out", np.zeros_like(c["q"]), np.float32), E]
+        b = [k.put("x", x, np.float32), 3, 5000, 5000, None, None, None, None, k.put("u", u, np.float64),
+             k.put("token", np.zeros(3), np.int32), None]
+        for call, read in ((lambda: L.ec_attention_tree_dev(*a), lambda: k.get("out", np.float32, c["q"].shape)),
+                           (lambda: L.ec_sample_dev(*b), lambda: k.get("token", np.int32, 3))):
+            before = read()
+            with pytest.raises(AssertionError, match="inside a stream capture"):
+                _Graph(call)
+            assert np.array_equal(read(), before)
+            assert call() == 0 and L.ec_sync() == 0
+            want = read()
+            g = _Graph(call)
+            for _ in range(3):
+                g.replay()
+                assert L.ec_sync() == 0 and np.array_equal(read(), want)
+            g.close()
+        check_attention(c, got=k.get("out", np.float32, c["q"].shape))
+        assert [ref_sample(x[r], u[r])[0] for r in range(3)] == list(k.get("token", np.int32, 3))
+
+
 def test_profiled_calls():
     """The calls under the library's per-kernel timing."""
     import json
