@@ -25,9 +25,11 @@ __device__ __forceinline__ int window_lo(int window, int past, int depth) {
 // The form for any head size and alignment: one block per (node, head), tiles
 // of 256 positions, a position per thread for the scores and an element of the
 // head per thread for the sums, with the running maximum and sum.  Every query head
-// reads its keys and values anew, a thread a whole key: 8 nodes of 14 / 2 heads of 64
-// over 700 rows take 42 us (the matrix-core form and its join 10.6), 16 one-token
-// sequences of 12 / 12 heads over 1000 rows 91 (17).
+// reads its keys and values anew, a thread a whole key, and nothing is split over the
+// positions: calls of 8 nodes of 14 / 2 heads over 700 rows take 42 us at head size 64
+// (the matrix-core form and its join 10.6), 51 at 80, 72 at 112, 139 at 256; 16 one-token
+// sequences of 12 / 12 heads over 1000 rows 91 (17), 121, 177 and 338; 8 trees of 16 nodes,
+// 12 / 2 heads of 80, over 4000 rows 520 (22 at head size 96).
 constexpr int kTreeMaxHd = 512;
 __global__ __launch_bounds__(256) void attn_tree_any_kernel(TreeAttnArgs a) {
   __shared__ float q[kTreeMaxHd], p_s[256], red[4];
@@ -121,22 +123,27 @@ __global__ __launch_bounds__(256) void attn_tree_any_kernel(TreeAttnArgs a) {
 // under a power of two that brings it to 2^14: its low part's steps of 2^-24 are below
 // 2^-20 of the largest at worst), weights = hi + lo (off by 2^-23 of a weight or, below
 // 2^-1, by 2^-24 at most); keys and values are 16 bits as they are, so two products give
-// each sum.  The running maximum's parts are of 2^12, so that 2^-24 is 2^-36 of it: behind a
-// token that takes most of the weight stand thousands of small ones that matter
-// together.  It is raised only when a score passes it by a factor of 2^3 (the parts'
-// room), and the accumulated outputs are scaled only then: mostly in a part's first tile
-// (a lift of 2^4 and a room of 2^10 are no faster).
+// each sum.  The parts are of 2^12 times the weights, so that 2^-24 is 2^-36 of the
+// running maximum's: behind a token that takes most of the weight stand thousands of
+// small ones that matter together.  The maximum is raised only when a score passes it by a
+// factor of 2^3 (the parts' room), and the accumulated outputs are scaled only then: mostly
+// in a part's first tile (a room of 2^10 is no faster).  Over 1000 to 32600 positions of
+// which the first takes 1/2 to 0.99 of the weight, in one part or many, errors are up to
+// 2.1 times those of the same formula in plain fp32, over normal scores 0.2 to 0.9 times
+// them, of a few positions up to 1.3 times.
 //
-// What bounds it.  Two sequences of 64 nodes, 14 / 2 heads of 64, over 32600 rows: 38
-// us, 23 GFLOP of matrix products in two parts, 0.6 PFLOP/s.  The matrix cores are
-// busy 41% of it, the vector ALUs (16 exponentials, maxima, sums and the weights'
-// parts, 110 instructions a tile and wave) 47%; the two overlap in part only, and
-// every wave waits for its LDS reads in four places a tile.  Half of the products left
-// out (the low parts') would save 8 us, the exponentials 2, the loads none.  Slower or
-// no faster: two tiles of rows a wave, a third buffer, the next tile's keys read or
-// multiplied ahead, operands of all products read first (registers), priorities.
+// What bounds it.  Two sequences of 64 nodes, 14 / 2 heads of 64, over 32600 rows: 41
+// us, 23 GFLOP of matrix products in two parts, 0.56 PFLOP/s.  The matrix cores are
+// busy 37% of it, the vector ALUs (16 exponentials, maxima, sums and the weights'
+// parts, 120 instructions a tile and wave, and the matrix instructions' issue) 59%; the
+// two overlap in part only, and every wave waits for its LDS reads in four places a
+// tile.  Half of the products left out (the low parts') saved 8 us, the exponentials 2,
+// the loads none.  Slower or no faster: two tiles of rows a wave, a third buffer, the next
+// tile's keys read or multiplied ahead, operands of all products read first (registers),
+// priorities.  At head size 64 the 128 registers of 4 waves a SIMD spill 4 or 7, in front
+// of the loop over the tiles alone.
 // One-token sequences are bound by memory: 16 of 12 / 12 heads over 1000 rows, 43
-// MB, take 14 us, 3.1 TB/s (a plain sum reads 4.0).
+// MB, take 13.5 us, 3.2 TB/s (a plain sum reads 4.0).
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 
@@ -737,20 +744,23 @@ bool tiles_ok(const TreeAttnArgs &a) {
 }
 
 // Waves per block: 4 (64 rows) or 8 (128), by the rows that share a KV head.  Up to 64
-// rows, 8 waves would load faster but for more blocks' places: 16.8 instead of 14 us
+// rows, 8 waves would load faster but for more blocks' places: 15.7 instead of 13.5 us
 // for the one-token sequences above.  Over 64, 4 waves read the cache twice as often:
-// 48 instead of 38 us for the two long contexts, 18.4 instead of 17.5 for 8 trees of
+// 45 instead of 41 us for the two long contexts, 20.0 instead of 18.2 for 8 trees of
 // 16 nodes, 12 / 2 heads of 128, over 4000 rows.
 int tree_waves(const TreeAttnArgs &a) { return (long)a.t.N * (a.H / a.KVH) <= 64 ? 4 : 8; }
 
 // Row blocks and parts: blocks for the CUs' places, of at least a tile each.  Two a CU, at
-// head sizes above 64 with 8 waves one (LDS and registers leave room for no second:
-// two a CU, one after the other, take 22 instead of 17.5 us for the trees over 4000
-// rows), at those up to 64 with 4 waves three: 16 one-token sequences of 12 / 12 heads
-// over 1000 rows take 14.1 + 4.1 us (the join's) with two, 13.0 + 4.1 with three, 12.3 +
-// 4.7 with four, 32 of 14 / 2 heads over 2000 rows 13.1, 13.0 and 14.3 in all.  Three and
-// four a CU for 8 waves take 41 and 42 us instead of 38 for the long contexts.  With no
-// parts at all the trees take 101 us, 8 nodes over 700 rows 16 instead of 7 + 3.5.
+// head sizes above 64 with 8 waves one (180 registers leave room for no second: two a
+// CU, one after the other, take 24 + 7.0 us (the join's) instead of 18.2 + 5.6 for the
+// trees over 4000 rows), at those up to 64 with 4 waves three: 16 one-token sequences of
+// 12 / 12 heads over 1000 rows take 15.1 + 4.0 us with two, 13.5 + 4.2 with three, 13.7 +
+// 4.1 with four, 32 of 14 / 2 heads over 2000 rows took 13.1, 13.0 and 14.3 in all.  Three
+// and four a CU for 8 waves take 45 + 8.1 and 46 + 9.5 us instead of 41 + 6.4 for the long
+// contexts.  With no parts at all these take 520 us, the trees 106, 8 nodes over 700 rows
+// 16 instead of 7.4 + 3.6.  Where the sequences alone fill the places there are no parts,
+// whatever their lengths: 64 one-token sequences of 12 / 12 heads, one over 30000 rows
+// and 63 over 300, take 380 us, 16 of them (split) 32.
 TreeGrid tree_grid(const TreeAttnArgs &a) {
   TreeGrid g;
   const int waves = tree_waves(a), per = 16 * waves;

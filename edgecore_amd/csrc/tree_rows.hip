@@ -56,8 +56,9 @@ __device__ __forceinline__ RopeRow rope_row(const NormRopeArgs &a, int m) {
 }
 
 // The form for any head size and alignment: one block per token, a wave a head at
-// a time, its elements through the wave's row in LDS.  333 rows of 10 + 2 x 5 heads of
-// 80 take 9.7 us here, 5.9 in the form below.
+// a time, its elements through the wave's row in LDS.  Three prompts of up to 333 rows,
+// 10 + 2 x 5 heads of 80, take 9.7 us here, 6.3 in the form below.  Bound by latency:
+// three barriers for every four heads, stores of 2 bytes.
 constexpr int kRopeMaxHd = 512;
 __global__ __launch_bounds__(256) void qk_norm_rope_any_kernel(NormRopeArgs a) {
   __shared__ float row[4][kRopeMaxHd];
@@ -119,7 +120,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_any_kernel(NormRopeArgs a) {
 // lanes; a pair's other element is in the same lane (layout 1) or in lane +- rot / 8,
 // which holds its four (layout 0, rot a multiple of 8).  Every element is read and
 // written once: 2048 rows of 12 + 2 x 2 heads of 128, 27.5 MB, take 8.7 us (3.2 TB/s;
-// a copy of as much 5.4), 128 rows of 14 + 2 x 2 of 64 take 5.0, a launch and the
+// a copy of as much 5.4), 128 rows of 14 + 2 x 2 of 64 take 5.2, a launch and the
 // chain before the first store (a sequence's numbers, its tree, the angles), which
 // blocks of their own overlap best: with two rows a block the prompt's rows took 3%
 // longer, with four 24%, with four heads of a lane ahead 14%.  The form for any size

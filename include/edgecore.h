@@ -450,7 +450,8 @@ int ec_sample_candidates(const float *vals, const int *idx, int ncand, int vocab
 /* Rows of q | k | v (fp32, H + 2 KVH heads of hd <= 512, row stride ldx) into
  * q (fp32, row stride ldq; it may be qkv itself, with ldx) and the fp16 caches kc, vc
  * [nslots][C][KVH*hd] of one layer: per head of q and k
- *   y = x / sqrt(mean(x^2) + eps) * gamma    (a NULL gamma: y = x)
+ *   y = x / sqrt(mean(x^2) + eps) * gamma    (a NULL gamma: y = x; the squares
+ *                                             are added up in fp32)
  * then the first rot elements (even; 0: none) rotated by the angles position *
  * inv_freq[rot / 2] (device, fp64), cosine and sine times factor: pairs (i, i
  * + rot / 2) for layout 0, (2 i, 2 i + 1) for layout 1.  v is copied.  Without
@@ -476,8 +477,9 @@ int ec_rope_inv_freq(int rope_type, int dim, double theta, double factor, double
  * reach it, whatever they hold.  out may be q itself, but overlaps no other
  * array.  Of what a node sees, a score of +inf or NaN gives NaN, a score of
  * -inf (of an infinity in its key or query) weighs nothing or gives NaN, an
- * infinite value gives NaN or an infinity.  Uses the library's workspace: a captured call needs one of its size before the capture, as the
- * matrix-core GEMMs do. */
+ * infinite value gives NaN or an infinity.  Uses the library's workspace: a
+ * captured call needs one of its size before the capture, as the matrix-core
+ * GEMMs do. */
 int ec_attention_tree_dev(const float *q, int ldq, const uint16_t *kc, const uint16_t *vc, int nslots, int C, int H,
                           int KVH, int hd, const int *slot, const int *past, const int *nodes, const int *parent, int B,
                           int N, int max_past, int window, float *out, int ldo);
@@ -494,7 +496,7 @@ int ec_attention_tree_dev(const float *q, int ldq, const uint16_t *kc, const uin
  * not drawn, a row of nothing else gives -1.  prob [rows] (nullable): the
  * drawn token's share of the sum, 1 for the largest logit, 0 for -1.  Weights
  * are rounded to whole steps of 2^-44 of the largest, their sums are exact in
- * 64 bits: equal calls give equal tokens, a token more than 31 temps below the
+ * 64 bits: equal calls give equal tokens, a token more than 31.2 temps below the
  * largest logit weighs nothing and is not drawn, and the prob of one that weighs
  * w of the largest is off by 2^-45 / w of itself at most, besides its rounding
  * to fp32.  Uses the library's workspace (as ec_attention_tree_dev); token and
@@ -509,7 +511,8 @@ int ec_sample_dev(const float *logits, int rows, int vocab, int ld, const float 
  * token, new_past [B] past + npath, and in every layer of kc, vc
  * [layers][nslots][C][kv] the rows past + path[j] move to past + j.  No nodes,
  * or a sequence that takes no part: npath 0, next -1, new_past = past.  N <=
- * 64, kv <= 2^28, layers <= 2^20.  The outputs and caches overlap no other array of the call. */
+ * 64, kv <= 2^28, layers <= 2^20.  The outputs and caches overlap no other
+ * array of the call. */
 int ec_tree_accept_dev(uint16_t *kc, uint16_t *vc, int layers, int nslots, int C, int kv, const int *slot,
                        const int *past, const int *nodes, const int *parent, const int *token, const int *sampled,
                        int B, int N, int *path, int *npath, int *next, int *new_past);
