@@ -25,7 +25,7 @@ HIPFLAGS := --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -ffp-contract=off \
             -Xclang -target-feature -Xclang -packed-fp32-ops -Iinclude -I$(SRC) -Wall
 CFLAGS   := -O2 -std=c11 -Wall -Wextra -fPIC -Iinclude -ffp-contract=off
 
-HIPSRC := $(SRC)/kernels.hip $(SRC)/decode_step.hip $(SRC)/decode_step_gpt2.hip $(SRC)/decode_tail.hip $(SRC)/gemm_mfma.hip $(SRC)/gemm_f32.hip $(SRC)/attn_prefill.hip $(SRC)/topk.hip $(SRC)/sample_rows.hip $(SRC)/tree_rows.hip $(SRC)/attn_tree.hip $(SRC)/gemv_i8.hip $(SRC)/gemv_f16.hip $(SRC)/gemv_bf16.hip $(SRC)/gemv_regs.hip $(SRC)/runtime.hip
+HIPSRC := $(SRC)/kernels.hip $(SRC)/decode_step.hip $(SRC)/decode_step_gpt2.hip $(SRC)/decode_tail.hip $(SRC)/gemm_mfma.hip $(SRC)/gemm_f32.hip $(SRC)/attn_prefill.hip $(SRC)/topk.hip $(SRC)/sample_rows.hip $(SRC)/tree_rows.hip $(SRC)/attn_tree.hip $(SRC)/paged_rows.hip $(SRC)/attn_paged.hip $(SRC)/logits_edit.hip $(SRC)/gemv_i8.hip $(SRC)/gemv_f16.hip $(SRC)/gemv_bf16.hip $(SRC)/gemv_regs.hip $(SRC)/runtime.hip
 HIPOBJ := $(HIPSRC:$(SRC)/%.hip=$(OBJ)/%.o)
 
 all: $(LIB) $(RUNTIME) $(SYNTH) oracle
@@ -33,7 +33,7 @@ all: $(LIB) $(RUNTIME) $(SYNTH) oracle
 $(OBJ) $(PKG)/lib $(PKG)/bin:
 	mkdir -p $@
 
-$(OBJ)/%.o: $(SRC)/%.hip $(SRC)/ec_device.h $(SRC)/ec_kernels.h $(SRC)/attn_decode.h $(SRC)/gemv_impl.h $(SRC)/ec_expf.h $(SRC)/ec_quant.h $(SRC)/step_common.h $(SRC)/ec_tree.h include/edgecore.h | $(OBJ)
+$(OBJ)/%.o: $(SRC)/%.hip $(SRC)/ec_device.h $(SRC)/ec_kernels.h $(SRC)/attn_decode.h $(SRC)/gemv_impl.h $(SRC)/ec_expf.h $(SRC)/ec_quant.h $(SRC)/step_common.h $(SRC)/ec_tree.h $(SRC)/ec_pages.h $(SRC)/paged_cache.h include/edgecore.h | $(OBJ)
 	$(HIPCC) $(HIPFLAGS) -c $< -o $@
 
 $(OBJ)/ecm.o: $(SRC)/ecm.c include/edgecore.h | $(OBJ)

@@ -28,7 +28,8 @@ HEADER = REPO_DIR / "include" / "edgecore.h"
 __all__ = [
     "EdgeCoreError", "lib", "GPT2", "Model", "gemm_int8", "gemm_fp16_fp32",
     "gemm_bf16_fp32", "quantize_int8_symmetric", "synth", "sample_full", "sample_candidates", "topk_dev",
-    "qk_norm_rope_dev", "rope_inv_freq", "attention_tree_dev", "sample_dev", "tree_accept_dev", "PKG_DIR", "LIB_PATH",
+    "qk_norm_rope_dev", "rope_inv_freq", "attention_tree_dev", "sample_dev", "tree_accept_dev",
+    "PagedCache", "CACHE_TYPES", "Pages", "paged_append_dev", "attention_paged_dev", "paged_read_dev", "logits_edit_dev", "PKG_DIR", "LIB_PATH",
     "RUNTIME", "SYNTH", "HEADER",
 ]
 
@@ -72,6 +73,13 @@ class GPT2(C.Structure):
     ]
 
 
+class PagedCache(C.Structure):
+    """include/edgecore.h, EcPagedCache (device pointers)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("type", C.c_int), ("npages", C.c_int), ("page", C.c_int), ("KVH", C.c_int), ("hd", C.c_int),
+                ("table", C.c_void_p), ("ldt", C.c_int)]
+
+
 _LIB: Optional[C.CDLL] = None
 
 _P = C.c_void_p
@@ -105,6 +113,10 @@ _SIG = {
     "ec_rope_inv_freq": (_I, [_I, _I, C.c_double, C.c_double, C.c_double, _P]),
     "ec_attention_tree_dev": (_I, [_P, _I, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _I, _I, _I, _I, _P, _I]),
     "ec_tree_accept_dev": (_I, [_P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _I, _I, _P, _P, _P, _P]),
+    "ec_paged_append_dev": (_I, [_P, _P, _I, _P, _I, _I, _P, _P, C.c_double, _P, _I, _I, C.c_double, _P, _P, _I, _I]),
+    "ec_attention_paged_dev": (_I, [_P, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _P, _I]),
+    "ec_paged_read_dev": (_I, [_P, _P, _P, _I, _I, _P, _P, _I, _I, _P, _P]),
+    "ec_logits_edit_dev": (_I, [_P, _I, _P, _I, _I, _P, _I, _P, _P, _P, _P, _P, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P, _I]),
     "ec_rng_next": (C.c_uint, [C.POINTER(C.c_ulonglong)]),
     "ec_sample_full": (_I, [_P, _I, C.c_float, _I, C.POINTER(C.c_ulonglong)]),
     "ec_sample_candidates": (_I, [_P, _P, _I, _I, C.c_float, _I, C.POINTER(C.c_ulonglong)]),
@@ -637,6 +649,163 @@ def tree_accept_dev(kc: np.ndarray, vc: np.ndarray, past, token, sampled, slot=N
         _check(lib().ec_sync(), "ec_sync")
         return (c.get("path", np.int32, (B, N)), *(c.get(n, np.int32, B) for n in ("npath", "next", "new_past")),
                 c.get("kc", np.uint16, kc.shape), c.get("vc", np.uint16, vc.shape))
+
+
+# ---------------------------------------------------------------------------
+# serving from a paged cache, on host arrays copied to the device
+# ---------------------------------------------------------------------------
+
+CACHE_TYPES = ("fp16", "int8", "e4m3")
+
+
+class Pages:
+    """A layer's paged cache on the host, for the functions below: k / v
+    [npages][KVH][page][hd] (fp16 bits as uint16, or int8 / e4m3 codes as uint8), scales
+    [npages][KVH][page] (fp16 bits; None for fp16) and the tables [B][ldt]."""
+
+    def __init__(self, type: str, k: np.ndarray, v: np.ndarray, table, k_scale=None, v_scale=None):
+        want = np.uint16 if type == "fp16" else np.uint8
+        if type not in CACHE_TYPES or k.dtype != want or v.dtype != want or k.ndim != 4 or k.shape != v.shape:
+            raise ValueError(f"a cache of {type}: {k.dtype} {k.shape} and {v.dtype} {v.shape}")
+        if np.ndim(table) != 2:
+            raise ValueError(f"tables of shape {np.shape(table)}")
+        for n, s in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if (s is None) != (type == "fp16") or (s is not None and (s.dtype != np.uint16 or s.shape != k.shape[:3])):
+                raise ValueError(f"{n} of a cache of {type} {k.shape}")
+        self.type, self.k, self.v, self.k_scale, self.v_scale = type, k, v, k_scale, v_scale
+        self.table = np.asarray(table)
+
+    @classmethod
+    def empty(cls, type: str, npages: int, KVH: int, page: int, hd: int, table) -> "Pages":
+        shape, codes = (npages, KVH, page, hd), np.uint16 if type == "fp16" else np.uint8
+        s = [None, None] if type == "fp16" else [np.zeros(shape[:3], np.uint16) for _ in range(2)]
+        return cls(type, np.zeros(shape, codes), np.zeros(shape, codes), table, *s)
+
+    def put(self, c: "_Call") -> PagedCache:
+        npages, KVH, page, hd = self.k.shape
+        p = [c.put("pages." + n, getattr(self, n), getattr(self, n).dtype if getattr(self, n) is not None else None)
+             for n in ("k", "v", "k_scale", "v_scale")]
+        return PagedCache(*p, CACHE_TYPES.index(self.type), npages, page, KVH, hd, c.put("table", self.table, np.int32),
+                          self.table.shape[1])
+
+    def got(self, c: "_Call") -> "Pages":
+        """The cache after a call."""
+        a = {n: None if getattr(self, n) is None else c.get("pages." + n, getattr(self, n).dtype, getattr(self, n).shape)
+             for n in ("k", "v", "k_scale", "v_scale")}
+        return Pages(self.type, table=self.table, **a)
+
+
+def _paged_sized(pages: Pages, B: int, M: int, start, past) -> None:
+    _sized("past", past, B)
+    _sized("start", start, B + 1)
+    if pages.table.shape[0] != B or (start is None and M != B):
+        raise ValueError(f"tables of {pages.table.shape[0]} sequences and {M} rows for a call of {B}")
+
+
+def paged_append_dev(pages: Pages, qkv: np.ndarray, H: int, past, start=None, q_gamma=None, k_gamma=None, eps: float = 1e-6,
+                     inv_freq=None, layout: int = 0, factor: float = 1.0, q: Optional[np.ndarray] = None):
+    """ec_paged_append_dev on host arrays: qkv [M][(H+2*KVH)*hd] fp32; returns
+    (q [M][H*hd], pages) after the call (q: what the padding rows hold)."""
+    M, width = qkv.shape
+    _, KVH, _, hd = pages.k.shape
+    B = np.size(past)
+    for n, a, shape in (("qkv", qkv, (M, (H + 2 * KVH) * hd)), ("q", q, (M, H * hd)), ("q_gamma", q_gamma, (hd,)),
+                        ("k_gamma", k_gamma, (hd,))):
+        _sized(n, a, *shape)
+    _paged_sized(pages, B, M, start, past)
+    with _Call() as c:
+        cache = pages.put(c)
+        x = c.put("x", qkv, np.float32)
+        qp = c.put("q", np.zeros((M, H * hd), np.float32) if q is None else q, np.float32)
+        g = [c.put("qg", q_gamma, np.float32), c.put("kg", k_gamma, np.float32)]
+        f = c.put("f", inv_freq, np.float64)
+        _check(lib().ec_paged_append_dev(C.byref(cache), x, width, qp, H * hd, H, *g, eps, f,
+                                         0 if inv_freq is None else 2 * len(inv_freq), layout, factor,
+                                         c.put("start", start, np.int32), c.put("past", past, np.int32), B, M),
+               "ec_paged_append_dev")
+        _check(lib().ec_sync(), "ec_sync")
+        return c.get("q", np.float32, (M, H * hd)), pages.got(c)
+
+
+def attention_paged_dev(pages: Pages, q: np.ndarray, H: int, past, start=None, window: int = 0, sinks: int = 0,
+                        max_past: Optional[int] = None, out: Optional[np.ndarray] = None) -> np.ndarray:
+    """ec_attention_paged_dev on host arrays: q [M][H*hd] fp32; returns out
+    [M][H*hd] (out: what the padding rows hold; max_past: the tables' rows by default)."""
+    M, E = q.shape
+    _, KVH, page, hd = pages.k.shape
+    B = np.size(past)
+    if E != H * hd:
+        raise ValueError(f"q rows of {E} for {H} heads of {hd}")
+    _sized("out", out, M, E)
+    _paged_sized(pages, B, M, start, past)
+    with _Call() as c:
+        cache = pages.put(c)
+        o = c.put("out", np.zeros_like(q) if out is None else out, np.float32)
+        _check(lib().ec_attention_paged_dev(C.byref(cache), c.put("q", q, np.float32), E, H, c.put("start", start, np.int32),
+                                            c.put("past", past, np.int32), B, M,
+                                            min(pages.table.shape[1] * page, 1 << 30) if max_past is None else int(max_past),
+                                            int(window), int(sinks), o, E), "ec_attention_paged_dev")
+        _check(lib().ec_sync(), "ec_sync")
+        return c.get("out", np.float32, (M, E))
+
+
+def paged_read_dev(pages: Pages, kc: np.ndarray, vc: np.ndarray, first, count, slot=None, to=None,
+                   max_count: Optional[int] = None):
+    """ec_paged_read_dev on host arrays: kc / vc [nslots][C][KVH*hd] fp16 bits;
+    returns (kc, vc) after the call (max_count: the largest count by default)."""
+    nslots, Cr, kv = _caches(kc, vc, 3)
+    _, KVH, _, hd = pages.k.shape
+    B = np.size(first)
+    if kv != KVH * hd:
+        raise ValueError(f"cache rows of {kv} for {KVH} heads of {hd}")
+    for n, a in (("count", count), ("slot", slot), ("to", to)):
+        _sized(n, a, B)
+    _paged_sized(pages, B, B, None, first)
+    with _Call() as c:
+        cache = pages.put(c)
+        p = [c.put("kc", kc, np.uint16), c.put("vc", vc, np.uint16)]
+        _check(lib().ec_paged_read_dev(C.byref(cache), c.put("first", first, np.int32), c.put("count", count, np.int32), B,
+                                       max(1, int(np.max(count))) if max_count is None else int(max_count), *p, nslots, Cr,
+                                       c.put("slot", slot, np.int32), c.put("to", to, np.int32)), "ec_paged_read_dev")
+        _check(lib().ec_sync(), "ec_sync")
+        return c.get("kc", np.uint16, kc.shape), c.get("vc", np.uint16, vc.shape)
+
+
+def logits_edit_dev(logits: np.ndarray, text=None, len=None, prompt=None, token=None, nodes=None, parent=None, N: int = 1,
+                    repetition=None, frequency=None, presence=None, bias_token=None, bias=None, nbias=None, mask=None,
+                    vocab: Optional[int] = None, out: Optional[np.ndarray] = None) -> np.ndarray:
+    """ec_logits_edit_dev on host rows [B*N][ld] (vocab: the columns that count):
+    text [B][ldt], bias_token / bias [B][max_bias], mask [B*N][ldm] (uint32);
+    returns the edited rows (out: what is not written holds, the logits by default)."""
+    rows, ld = logits.shape
+    V = ld if vocab is None else int(vocab)
+    if rows % N:
+        raise ValueError(f"{rows} rows for sequences of {N}")
+    B = rows // N
+    for n, a, shape in (("len", len, (B,)), ("prompt", prompt, (B,)), ("token", token, (B, N)), ("nodes", nodes, (B,)),
+                        ("parent", parent, (B, N)), ("repetition", repetition, (B,)), ("frequency", frequency, (B,)),
+                        ("presence", presence, (B,)), ("nbias", nbias, (B,)), ("out", out, (rows, ld))):
+        _sized(n, a, *shape)
+    for n, a, r in (("text", text, B), ("bias_token", bias_token, B), ("bias", bias, B), ("mask", mask, rows)):
+        if a is not None and (np.ndim(a) != 2 or np.shape(a)[0] != r):
+            raise ValueError(f"{n} has shape {np.shape(a)}, not {r} rows")
+    if (text is None) != (len is None) or (bias is None) != (bias_token is None) or np.shape(bias) != np.shape(bias_token):
+        raise ValueError("texts without their lengths, or biases without their tokens")
+    with _Call() as c:
+        i32, f32 = np.int32, np.float32
+        x = c.put("x", logits, f32)
+        o = c.put("out", logits if out is None else out, f32)
+        p = {n: c.put(n, a, t) for n, a, t in (
+            ("text", text, i32), ("len", len, i32), ("prompt", prompt, i32), ("token", token, i32), ("nodes", nodes, i32),
+            ("parent", parent, i32), ("repetition", repetition, f32), ("frequency", frequency, f32),
+            ("presence", presence, f32), ("bias_token", bias_token, i32), ("bias", bias, f32), ("nbias", nbias, i32),
+            ("mask", mask, np.uint32))}
+        width = lambda a: 0 if a is None else np.shape(a)[1]  # noqa: E731
+        _check(lib().ec_logits_edit_dev(x, ld, o, ld, V, p["text"], width(text), p["len"], p["prompt"], p["token"], p["nodes"],
+                                        p["parent"], B, N, p["repetition"], p["frequency"], p["presence"], p["bias_token"],
+                                        p["bias"], p["nbias"], width(bias), p["mask"], width(mask)), "ec_logits_edit_dev")
+        _check(lib().ec_sync(), "ec_sync")
+        return c.get("out", f32, (rows, ld))
 
 
 # ---------------------------------------------------------------------------

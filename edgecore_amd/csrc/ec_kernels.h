@@ -8,6 +8,7 @@
 
 #include <type_traits>
 
+#include "ec_pages.h"
 #include "ec_tree.h"
 
 namespace ec {
@@ -531,6 +532,71 @@ struct AcceptArgs {
   int *path, *npath, *next, *new_past;
 };
 hipError_t tree_accept(const AcceptArgs &a, hipStream_t st);
+
+// operators over a paged cache (paged_rows.hip, attn_paged.hip): ec_pages.h's batch,
+// the element types of paged_cache.h
+enum CacheType { CACHE_F16 = 0, CACHE_I8 = 1, CACHE_E4M3 = 2 };
+struct PagedCacheArgs {
+  EcPageBatch t;
+  void *k, *v;         // [npages][KVH][page][hd]
+  uint16_t *ks, *vs;   // [npages][KVH][page] fp16 (null for CACHE_F16)
+  int type, hd;
+};
+struct PagedAppendArgs {
+  PagedCacheArgs c;
+  const float *x;  // [M][ldx]: q | k | v
+  int ldx;
+  float *q;
+  int ldq, H;
+  const float *q_gamma, *k_gamma;
+  double eps;
+  const double *inv_freq;
+  int rot, layout;
+  double factor;
+};
+int paged_append_max_hd();
+hipError_t paged_append(const PagedAppendArgs &a, hipStream_t st);
+
+struct PagedReadArgs {
+  PagedCacheArgs c;
+  const int *first, *count;
+  EcTreeBatch t;  // the slots' numbers alone: B, N (the largest count), nslots, C
+  const int *slot, *to;
+  uint16_t *kc, *vc;
+};
+hipError_t paged_read(const PagedReadArgs &a, hipStream_t st);
+
+struct PagedAttnArgs {
+  PagedCacheArgs c;
+  const float *q;
+  int ldq, H, max_past, window, sinks;
+  float scale;
+  float *out;
+  int ldo;
+  void *ws;
+};
+int attention_paged_max_hd();
+hipError_t attention_paged(const PagedAttnArgs &a, hipStream_t st);
+
+// logits before they are sampled (logits_edit.hip)
+struct EditArgs {
+  const float *logits;
+  int ld;
+  float *out;
+  int ldo, V;
+  const int *text;  // [B][ldt]
+  int ldt;
+  const int *len, *prompt, *token, *nodes, *parent;
+  int B, N;
+  const float *repetition, *frequency, *presence;
+  const int *bias_token;
+  const float *bias;
+  const int *nbias;
+  int max_bias;
+  const uint32_t *mask;
+  int ldm;
+};
+hipError_t logits_edit(const EditArgs &a, hipStream_t st);
 
 // elementwise device math (ec_device_math)
 enum { MATH_EXPF = 0, MATH_SILU = 1, MATH_GELU = 2, MATH_F32_TO_F16 = 3, MATH_F16_TO_F32 = 4, MATH_QUANT1 = 5, MATH_COPY = 6 };

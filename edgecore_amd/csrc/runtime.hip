@@ -2540,6 +2540,163 @@ extern "C" int ec_tree_accept_dev(uint16_t *kc, uint16_t *vc, int layers, int ns
   return 0;
 }
 
+// ---------------------------------------------------------------------------
+// serving from a paged cache: rows into it and back, attention, logits
+// ---------------------------------------------------------------------------
+
+// The call's batch and cache for the kernels; what the arrays hold is checked there
+// (ec_pages.h).
+static int paged_check(const char *fn, const EcPagedCache *c, PagedCacheArgs *a, int max_hd, int B, int M, const int *start,
+                       const int *past) {
+  if (!c) return set_err(-1, "%s: null pointer", fn);
+  if (c->type < EC_CACHE_F16 || c->type > EC_CACHE_E4M3) return set_err(-1, "%s: cache type %d", fn, c->type);
+  if (c->npages < 1 || c->page < 1 || c->KVH < 1 || c->hd < 1 || c->hd > max_hd || c->ldt < 1 || c->KVH > 65535 ||
+      (double)c->npages * c->page * c->KVH >= 0x1p31)
+    return set_err(-1, "%s: npages=%d pages of page=%d rows, KVH=%d (below 2^31 together), hd=%d (up to %d), ldt=%d", fn,
+                   c->npages, c->page, c->KVH, c->hd, max_hd, c->ldt);
+  if (!c->k || !c->v || !c->table || (c->type != EC_CACHE_F16 && (!c->k_scale || !c->v_scale)))
+    return set_err(-1, "%s: null pointer", fn);
+  if (B < 1 || B > 65535 || M < 1 || M > kMaxRows || (!start && M != B))
+    return set_err(-1, "%s: B=%d sequences (up to 65535), M=%d rows (up to %ld; B without starts)", fn, B, M, kMaxRows);
+  if (!past) return set_err(-1, "%s: null pointer", fn);
+  const long rows = (long)c->ldt * c->page;
+  *a = PagedCacheArgs{EcPageBatch{B, M, start, past, c->table, c->ldt, c->npages, c->page, c->KVH,
+                                  (int)(rows < EC_PAGES_ROWS ? rows : EC_PAGES_ROWS), 0, 0},
+                      c->k, c->v, c->type == EC_CACHE_F16 ? nullptr : c->k_scale,
+                      c->type == EC_CACHE_F16 ? nullptr : c->v_scale, c->type, c->hd};
+  ec_pages_divide(&a->t);
+  return 0;
+}
+
+struct PagedSpans {
+  Span k, v, ks, vs, table;
+};
+static PagedSpans paged_spans(const PagedCacheArgs &a) {
+  const size_t rows = (size_t)a.t.npages * a.t.page * a.t.KVH, n = rows * a.hd * (a.type == CACHE_F16 ? 2 : 1);
+  return PagedSpans{{a.k, n}, {a.v, n}, {a.ks, 2 * rows}, {a.vs, 2 * rows}, {a.t.table, (size_t)a.t.B * a.t.ldt * 4}};
+}
+// bytes of a cached row of all KV heads, keys and values
+static double paged_row_bytes(const PagedCacheArgs &a) {
+  return 2.0 * a.t.KVH * (a.type == CACHE_F16 ? 2.0 * a.hd : a.hd + 2.0);
+}
+
+extern "C" int ec_paged_append_dev(const EcPagedCache *cache, const float *qkv, int ldx, float *q, int ldq, int H,
+                                   const float *q_gamma, const float *k_gamma, double eps, const double *inv_freq, int rot,
+                                   int layout, double factor, const int *start, const int *past, int B, int M) {
+  const char *fn = "ec_paged_append_dev";
+  PagedCacheArgs c;
+  int r;
+  if ((r = paged_check(fn, cache, &c, paged_append_max_hd(), B, M, start, past))) return r;
+  const int KVH = c.t.KVH, hd = c.hd;
+  if ((r = heads_check(fn, H, KVH, hd, paged_append_max_hd()))) return r;
+  if ((long)ldx < (long)(H + 2 * (long)KVH) * hd || (long)ldq < (long)H * hd)
+    return set_err(-1, "%s: row strides ldx=%d ldq=%d", fn, ldx, ldq);
+  if (rot < 0 || rot > hd || rot % 2 || layout < 0 || layout > 1 || !(eps >= 0.0))
+    return set_err(-1, "%s: rot=%d (even, up to hd) layout=%d (0 half, 1 interleaved) eps=%g", fn, rot, layout, eps);
+  if (!qkv || !q || (rot > 0 && !inv_freq)) return set_err(-1, "%s: null pointer", fn);
+  const Span x = rows_span(qkv, M, ldx, (H + 2 * KVH) * hd, 4), qs = rows_span(q, M, ldq, H * hd, 4);
+  if (!(q == qkv && ldq == ldx) && qs.overlaps(x)) return set_err(-1, "%s: q overlaps qkv and is not its first columns", fn);
+  {
+    const PagedSpans p = paged_spans(c);
+    const size_t b4 = (size_t)B * 4, h4 = (size_t)hd * 4;
+    const Span in[] = {{q_gamma, h4}, {k_gamma, h4}, {inv_freq, (size_t)rot * 4}, {start, b4 + 4}, {past, b4}, p.table};
+    const Span out[] = {qs, p.k, p.v, p.ks, p.vs};
+    if (spans_clash(in, out) || x.overlaps(p.k) || x.overlaps(p.v) || x.overlaps(p.ks) || x.overlaps(p.vs))
+      return set_err(-1, "%s: q or the cache overlaps another array", fn);
+  }
+  EC_INIT();
+  const DeviceScope dev;
+  const PagedAppendArgs a{c, qkv, ldx, q, ldq, H, q_gamma, k_gamma, eps, inv_freq, rot, layout, factor};
+  EC_LAUNCH("paged_append", (double)M * (4.0 * hd * (2 * H + 2 * KVH) + paged_row_bytes(c)), paged_append(a, g_stream));
+  return 0;
+}
+
+extern "C" int ec_attention_paged_dev(const EcPagedCache *cache, const float *q, int ldq, int H, const int *start,
+                                      const int *past, int B, int M, int max_past, int window, int sinks, float *out,
+                                      int ldo) {
+  const char *fn = "ec_attention_paged_dev";
+  PagedCacheArgs c;
+  int r;
+  if ((r = paged_check(fn, cache, &c, attention_paged_max_hd(), B, M, start, past))) return r;
+  const int hd = c.hd;
+  if ((r = heads_check(fn, H, c.t.KVH, hd, attention_paged_max_hd()))) return r;
+  if ((long)ldq < (long)H * hd || (long)ldo < (long)H * hd || window < 0 || sinks < 0 || max_past < 0 || max_past > c.t.rows)
+    return set_err(-1, "%s: ldq=%d ldo=%d window=%d sinks=%d max_past=%d (a table of %d rows)", fn, ldq, ldo, window, sinks,
+                   max_past, c.t.rows);
+  if (!q || !out) return set_err(-1, "%s: null pointer", fn);
+  const Span qs = rows_span(q, M, ldq, H * hd, 4), os = rows_span(out, M, ldo, H * hd, 4);
+  if (!(out == q && ldo == ldq) && os.overlaps(qs)) return set_err(-1, "%s: out overlaps q and is not q", fn);
+  {
+    const PagedSpans p = paged_spans(c);
+    const Span in[] = {p.k, p.v, p.ks, p.vs, p.table, {start, (size_t)B * 4 + 4}, {past, (size_t)B * 4}};
+    const Span o[] = {os};
+    if (spans_clash(in, o)) return set_err(-1, "%s: out overlaps another array", fn);
+  }
+  EC_INIT();
+  const DeviceScope dev;
+  PagedAttnArgs a{c, q, ldq, H, max_past, window, sinks, (float)(1.0 / sqrt((double)hd)), out, ldo, nullptr};
+  EC_LAUNCH("attention_paged", (double)B * max_past * paged_row_bytes(c), attention_paged(a, g_stream));
+  return 0;
+}
+
+extern "C" int ec_paged_read_dev(const EcPagedCache *cache, const int *first, const int *count, int B, int max_count,
+                                 uint16_t *kc, uint16_t *vc, int nslots, int C, const int *slot, const int *to) {
+  const char *fn = "ec_paged_read_dev";
+  PagedCacheArgs c;
+  int r;
+  if ((r = paged_check(fn, cache, &c, paged_append_max_hd(), B, B, nullptr, first))) return r;
+  if (max_count < 1 || max_count > kMaxCacheRows || nslots < 1 || C < 1 || C > kMaxCacheRows)
+    return set_err(-1, "%s: max_count=%d, a cache of %d slots of %d rows (each up to %d)", fn, max_count, nslots, C, kMaxCacheRows);
+  if (!count || !kc || !vc) return set_err(-1, "%s: null pointer", fn);
+  const EcTreeBatch t{B, max_count, slot, to, count, nullptr, nslots, C, C};
+  {
+    const PagedSpans p = paged_spans(c);
+    const size_t b4 = (size_t)B * 4, kv = (size_t)c.t.KVH * c.hd;
+    const Span in[] = {p.k, p.v, p.ks, p.vs, p.table, {first, b4}, {count, b4}, {slot, b4}, {to, b4}};
+    const Span out[] = {cache_span(kc, 1, t, kv), cache_span(vc, 1, t, kv)};
+    if (spans_clash(in, out)) return set_err(-1, "%s: kc or vc overlaps another array", fn);
+  }
+  EC_INIT();
+  const DeviceScope dev;
+  const PagedReadArgs a{c, first, count, t, slot, to, kc, vc};
+  EC_LAUNCH("paged_read", (double)B * max_count * (paged_row_bytes(c) + 4.0 * c.t.KVH * c.hd), paged_read(a, g_stream));
+  return 0;
+}
+
+extern "C" int ec_logits_edit_dev(const float *logits, int ld, float *out, int ldo, int vocab, const int *text, int ldt,
+                                  const int *len, const int *prompt, const int *token, const int *nodes, const int *parent,
+                                  int B, int N, const float *repetition, const float *frequency, const float *presence,
+                                  const int *bias_token, const float *bias, const int *nbias, int max_bias,
+                                  const uint32_t *mask, int ldm) {
+  const char *fn = "ec_logits_edit_dev";
+  if (B < 1 || N < 1 || B > 65535 || N > 65535 || (long)B * N > kMaxRows || (token && N > EC_TREE_MAX))
+    return set_err(-1, "%s: B=%d sequences of N=%d rows (up to 65535 each, %ld together; %d nodes of a tree)", fn, B, N,
+                   kMaxRows, EC_TREE_MAX);
+  if (vocab < 1 || vocab > 1 << 18 || ld < vocab || ldo < vocab || (mask && ldm < (vocab + 31) / 32))
+    return set_err(-1, "%s: vocab=%d (up to %d) ld=%d ldo=%d ldm=%d", fn, vocab, 1 << 18, ld, ldo, ldm);
+  if (ldt < 0 || ldt > kMaxCacheRows || max_bias < 0 || max_bias > kMaxCacheRows)
+    return set_err(-1, "%s: ldt=%d max_bias=%d (up to %d)", fn, ldt, max_bias, kMaxCacheRows);
+  if (!logits || !out || (ldt > 0 && (!text || !len)) || (max_bias > 0 && (!bias_token || !bias)))
+    return set_err(-1, "%s: null pointer", fn);
+  const long rows = (long)B * N;
+  const Span x = rows_span(logits, rows, ld, vocab, 4), o = rows_span(out, rows, ldo, vocab, 4);
+  if (!(out == logits && ld == ldo) && o.overlaps(x)) return set_err(-1, "%s: out overlaps logits and is not logits", fn);
+  {
+    const size_t b4 = (size_t)B * 4, n4 = b4 * N;
+    const Span in[] = {{text, b4 * ldt}, {len, b4}, {prompt, b4}, {token, n4}, {nodes, b4}, {parent, n4}, {repetition, b4},
+                       {frequency, b4}, {presence, b4}, {bias_token, b4 * max_bias}, {bias, b4 * max_bias}, {nbias, b4},
+                       mask ? rows_span(mask, rows, ldm, (vocab + 31) / 32, 4) : Span{nullptr, 0}};
+    const Span outs[] = {o};
+    if (spans_clash(in, outs)) return set_err(-1, "%s: out overlaps another array", fn);
+  }
+  EC_INIT();
+  const DeviceScope dev;
+  const EditArgs a{logits, ld, out, ldo, vocab, text, ldt, ldt > 0 ? len : nullptr, prompt, token, nodes, parent, B, N, repetition,
+                   frequency, presence, bias_token, bias, max_bias > 0 ? nbias : nullptr, max_bias, mask, ldm};
+  EC_LAUNCH("logits_edit", (double)rows * vocab * (mask ? 8.125 : 8.0), logits_edit(a, g_stream));
+  return 0;
+}
+
 extern "C" void gpt2_forward(GPT2 *g, const int *tokens, const int *positions, const int *seqs, int M,
                              float *logits) {
   if (forward_impl(g, tokens, positions, seqs, M, 0, logits, nullptr)) {

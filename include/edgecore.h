@@ -517,6 +517,98 @@ int ec_tree_accept_dev(uint16_t *kc, uint16_t *vc, int layers, int nslots, int C
                        const int *past, const int *nodes, const int *parent, const int *token, const int *sampled,
                        int B, int N, int *path, int *npath, int *next, int *new_past);
 
+/* ---- serving from a paged cache ----
+ *
+ * No reference counterpart.  A cache in pages that a sequence's text takes as it
+ * grows, in 16 or 8 bits: new rows go in (ec_paged_append_dev), attend
+ * (ec_attention_paged_dev: a token, a chunk or a whole prompt of each sequence),
+ * and come back as rows of the fp16 slot cache (ec_paged_read_dev), for the
+ * operators for drafted tokens.  Calls, streams, errors and captures are as theirs.
+ *
+ * One layer's cache: keys and values [npages][KVH][page][hd], of
+ *   EC_CACHE_F16   fp16
+ *   EC_CACHE_I8    int8, -127 to 127
+ *   EC_CACHE_E4M3  8-bit floating point (1, 4 and 3 bits, largest 448)
+ * the 8-bit ones with scales k_scale, v_scale [npages][KVH][page] in fp16: a row of codes
+ * c and scale s stands for the fp16 values c s, which is what the attention takes and
+ * the read gives.  npages * KVH * page < 2^31, hd <= 512; pages of any size.
+ *   table [B][ldt]  row p of sequence b's text is row p % page of page table[b][p / page];
+ *                   a text has up to min(ldt * page, 2^30) rows
+ * Pages may be shared (a prefix of several texts); entries that a call needs no row of
+ * are not looked at.
+ *
+ * The batch: B <= 65535 sequences and M <= 2^22 rows, those of one sequence behind
+ * those of the one before it.
+ *   start [B + 1]  ascending, start[B] <= M: sequence b's new rows are start[b] ..
+ *                  start[b + 1] - 1 of the call, row i of them at position past + i.
+ *                  NULL: a row each, M = B.  Rows of no sequence are padding: what
+ *                  they would write stays as it was
+ *   past [B]       rows of the text that are in the cache already
+ *
+ * What these arrays hold is checked on the device: a sequence whose past is negative or
+ * whose text the table has no room for takes no part, and neither does a row on a page
+ * outside the cache: its rows of q / out are NaN, and nothing of it is written.  (Where the starts
+ * do not ascend, it is not said which rows of q / out are written, and by which
+ * sequence.)  No two rows of a call may go to one place of a page: what it then holds is
+ * not said. */
+enum { EC_CACHE_F16 = 0, EC_CACHE_I8 = 1, EC_CACHE_E4M3 = 2 };
+typedef struct {
+    void *k, *v;                 /* device, as all of these */
+    uint16_t *k_scale, *v_scale; /* NULL for EC_CACHE_F16 */
+    int type, npages, page, KVH, hd;
+    const int *table;
+    int ldt;
+} EcPagedCache;
+
+/* Rows of q | k | v into q and the pages, normed and rotated as by
+ * ec_qk_norm_rope_dev (which has gamma, eps, inv_freq, rot, layout and factor).  k's and v's codes and scales are those
+ * that the formulas give in 64 bits: s = max |y| / 127 (448) of the row, the next
+ * fp16 number from there up, c = y / s to the nearest code.  A row with a NaN or an infinity, or whose
+ * scale would pass 65504, stands for NaN; values above 65000 may come back infinite. */
+int ec_paged_append_dev(const EcPagedCache *cache, const float *qkv, int ldx, float *q, int ldq, int H,
+                        const float *q_gamma, const float *k_gamma, double eps, const double *inv_freq, int rot,
+                        int layout, double factor, const int *start, const int *past, int B, int M);
+
+/* Causal attention of the new rows, which are in the cache, scores times 1 /
+ * sqrt(hd), fp32: the token at position t sees the positions p <= t, with window > 0
+ * those of them with p > t - window or p < sinks (first tokens that stay visible).
+ * q [M][H*hd] (row stride ldq), out likewise (ldo); q head h reads KV head h * KVH / H.
+ * max_past: the largest past of the call (it sizes the launch; a sequence with a
+ * larger one takes no part).  Rows that a token does not see do not reach it, whatever
+ * they hold; infinities, and out in place of q, as for ec_attention_tree_dev.  A page
+ * outside the cache among those that a sequence's tokens see makes NaN of some or all of
+ * its rows.  Uses the library's workspace (as ec_attention_tree_dev). */
+int ec_attention_paged_dev(const EcPagedCache *cache, const float *q, int ldq, int H, const int *start, const int *past,
+                           int B, int M, int max_past, int window, int sinks, float *out, int ldo);
+
+/* Rows first[b] .. first[b] + count[b] - 1 of sequence b's text into rows to[b] on of
+ * slot slot[b] of the fp16 caches kc, vc [nslots][C][KVH*hd] (slot NULL: b; to NULL: 0).
+ * count <= max_count (which sizes the launch).  A sequence whose numbers name no rows of
+ * its table or its slot takes no part, nor does one whose rows of a slot overlap those of
+ * an earlier one of the call; a row on a page outside the cache comes back as NaN. */
+int ec_paged_read_dev(const EcPagedCache *cache, const int *first, const int *count, int B, int max_count, uint16_t *kc,
+                      uint16_t *vc, int nslots, int C, const int *slot, const int *to);
+
+/* Logits before ec_sample_dev, [B * N][vocab <= 2^18] fp32 (row strides ld and ldo; out may
+ * be logits itself): row b * N + i, node i of sequence b as in the operators for drafted
+ * tokens, gets
+ *   x / r where x > 0, else x r           for every token that its text has
+ *   - frequency * c - presence            for those that it has c > 0 times behind the prompt
+ *   + bias                                for those with one
+ *   -inf                                  where bit t % 32 of mask[row][t / 32] is 0
+ * text [B][ldt]: the sequence's tokens, len [B] of them, the first prompt [B] of them the
+ * prompt (NULL: none).  token [B * N] (NULL: none; with it N <= 64): the nodes' own tokens, so that those
+ * of a node and its ancestors (parent; NULL: the nodes before it) belong to its text, behind the prompt.
+ * nodes [B] (NULL: N): the rows behind them stay as they were.  repetition r, frequency,
+ * presence [B]: NULL: 1, 0, 0.  bias_token, bias [B][max_bias], nbias [B] (NULL: max_bias)
+ * of them; of entries for one token the last counts.  mask [B * N][ldm] (NULL: none).  Tokens
+ * outside the vocabulary are passed over.  A sequence whose len, nbias, nodes or parents are
+ * none gets NaN (with nodes outside [0, N]: all N rows).  No output but out; it overlaps no other array. */
+int ec_logits_edit_dev(const float *logits, int ld, float *out, int ldo, int vocab, const int *text, int ldt, const int *len,
+                       const int *prompt, const int *token, const int *nodes, const int *parent, int B, int N,
+                       const float *repetition, const float *frequency, const float *presence, const int *bias_token,
+                       const float *bias, const int *nbias, int max_bias, const uint32_t *mask, int ldm);
+
 /* sizeof(GPT2) as compiled into the library (lets foreign-function hosts
  * check their mirror of the struct). */
 size_t ec_gpt2_sizeof(void);
