@@ -33,7 +33,7 @@ all: $(LIB) $(RUNTIME) $(SYNTH) oracle
 $(OBJ) $(PKG)/lib $(PKG)/bin:
 	mkdir -p $@
 
-$(OBJ)/%.o: $(SRC)/%.hip $(SRC)/ec_device.h $(SRC)/ec_kernels.h $(SRC)/attn_decode.h $(SRC)/gemv_impl.h $(SRC)/ec_expf.h $(SRC)/ec_quant.h $(SRC)/step_common.h $(SRC)/ec_tree.h $(SRC)/ec_pages.h $(SRC)/paged_cache.h include/edgecore.h | $(OBJ)
+$(OBJ)/%.o: $(SRC)/%.hip $(SRC)/ec_device.h $(SRC)/ec_kernels.h $(SRC)/attn_decode.h $(SRC)/gemv_impl.h $(SRC)/ec_expf.h $(SRC)/ec_quant.h $(SRC)/step_common.h $(SRC)/ec_tree.h $(SRC)/ec_pages.h $(SRC)/paged_cache.h $(SRC)/attn_parts.h include/edgecore.h | $(OBJ)
 	$(HIPCC) $(HIPFLAGS) -c $< -o $@
 
 $(OBJ)/ecm.o: $(SRC)/ecm.c include/edgecore.h | $(OBJ)

@@ -7,7 +7,10 @@
 //
 // in fp32.  What a token does not see does not reach it, finite or not.
 #include <cfloat>
+#include <climits>
+#include <type_traits>
 
+#include "attn_parts.h"
 #include "ec_device.h"
 #include "ec_kernels.h"
 #include "paged_cache.h"
@@ -77,13 +80,1015 @@ __global__ __launch_bounds__(256) void attn_paged_any_kernel(PagedAttnArgs a) {
   }
 }
 
+// ---------------------------------------------------------------------------
+// The matrix-core forms (head sizes that are multiples of 16 up to 128, in LDS and
+// registers filled up with zeros to one of 32).  A unit of work is a tile of RT rows of one
+// KV head of one sequence (row r: token r / G, query head r % G of the G = H / KVH that
+// share it) and a part of the 64-position tiles that they see.
+// ---------------------------------------------------------------------------
+constexpr int kTp = 64;          // positions per tile
+constexpr float kRoom = 3.0f;    // how far scores may pass the running maximum (powers of two)
+constexpr int kLift = 12;        // the weights' parts are those of 2^kLift e^(x - m)
+constexpr float kLifted = 1 << kLift;
+static_assert(kLift + kRoom < 16.0f, "parts below 65504");
+constexpr long kGridRow = 1L << 20;
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+
+// target: units per KV head that the texts are split for (0: they are not); least: tiles of a
+// part, at least
+struct PagedGrid {
+  long units;
+  int target, least;
+};
+
+// The tiles that rows of tokens ta .. tb see: those of the first tokens that are not among
+// the window's, then the window's.
+struct Tiles {
+  int lo, sinks;     // positions from lo on and below sinks are seen
+  int front, first, n;  // tiles of the first tokens, the window's first one, all
+  __device__ __forceinline__ int at(int i) const { return (i < front ? i : i - front + first) * kTp; }
+};
+__device__ __forceinline__ Tiles tiles_of(const PagedAttnArgs &a, const EcPageSeq &s, int ta, int tb) {
+  Tiles t;
+  t.lo = a.window && s.past + ta >= a.window ? s.past + ta - a.window + 1 : 0;
+  t.sinks = min(a.sinks, t.lo);
+  t.first = t.lo / kTp;
+  t.front = min((t.sinks + kTp - 1) / kTp, t.first);
+  t.n = t.front + (s.past + tb) / kTp - t.first + 1;
+  return t;
+}
+
+// A sequence's row tiles, and no fewer tiles of positions than any of them has
+template <int RT>
+__device__ __forceinline__ int row_tiles(const PagedAttnArgs &a, const EcPageSeq &s) {
+  return ec_page_seq_mine(&a.c.t, s) ? (s.n * (a.H / a.c.t.KVH) + RT - 1) / RT : 0;
+}
+template <int RT>
+__device__ __forceinline__ int most_tiles(const PagedAttnArgs &a, const EcPageSeq &s) {
+  if (!ec_page_seq_ok(&a.c.t, s, a.max_past)) return 1;
+  const int all = (s.past + s.n - 1) / kTp + 1, G = a.H / a.c.t.KVH;
+  if (!a.window) return all;
+  // the tokens of a row tile, the tiles of the positions that they see
+  const int tokens = min((RT + G - 2) / G + 1, s.n);
+  const long seen = ((long)a.window + tokens) / kTp + 2 + ((long)min(a.sinks, s.past + s.n) + kTp - 1) / kTp;
+  return (int)min((long)all, seen);
+}
+
+// What a block does: part j of n of row tile rt of sequence c and KV head kvh.  at: the
+// unit of part 0 (the parts are KVH units from each other).
+struct Unit {
+  int c, rt, kvh, j, n;
+  uint32_t at;
+  EcPageSeq s;
+};
+__device__ __forceinline__ EcPageSeq lane_seq(EcPageSeq s, int l) {
+  return EcPageSeq{readlane(s.start, l), readlane(s.n, l), readlane(s.past, l)};
+}
+// By a wave, a sequence per lane.  The parts: as many of a row tile as its sequence's tiles are
+// times an even share of all tiles of the call, so that the units are alike, and a text
+// that is longer than the others is not what the call waits for.  Within a sequence the last
+// row tiles, which see most, come first, and the units of one part of the positions stand 8
+// apart where there are as many parts: on one XCD, whose L2 they share.
+template <int RT>
+__device__ __forceinline__ Unit find_unit(const PagedAttnArgs &a, const PagedGrid &gr, long x) {
+  const int lane = threadIdx.x & 63, B = a.c.t.B, KVH = a.c.t.KVH;
+  Unit u{-1, 0, 0, 0, 1, 0, {0, 0, 0}};
+  if (!gr.target) {
+    // sequence b's row tiles are among places start[b] G / RT + b and on, up to the next one's
+    const long places = gr.units / KVH, place = places - 1 - x / KVH;
+    const auto base = [&](int b) {
+      return (a.c.t.start ? (long)a.c.t.start[b] * (a.H / KVH) / RT : (long)b * (a.H / KVH) / RT) + b;
+    };
+    int lo = 0, hi = B;
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 63) / 64, b = lo + lane * step;
+      const uint64_t in = __ballot(b < hi && base(min(b, B - 1)) <= place);
+      const int k = in ? 63 - __clzll((long long)in) : 0;
+      lo += k * step;
+      hi = min(hi, lo + step);
+    }
+    u.s = ec_page_seq(&a.c.t, lo);
+    const long rt = place - base(lo);
+    if (rt < 0 || rt >= row_tiles<RT>(a, u.s)) return u;
+    u.c = lo;
+    u.rt = (int)rt;
+    u.kvh = (int)(x % KVH);
+    return u;
+  }
+  EcPageSeq s0{0, 0, 0};
+  int rt0 = 0, tiles0 = 0;
+  const auto seq = [&](int c, EcPageSeq &s, int &rt, int &tiles) {
+    s = ec_page_seq(&a.c.t, min(c, B - 1));
+    rt = c < B ? row_tiles<RT>(a, s) : 0;
+    tiles = rt ? most_tiles<RT>(a, s) : 0;
+  };
+  seq(lane, s0, rt0, tiles0);
+  unsigned long long all = 0;
+  for (int c0 = 0; c0 < B; c0 += 64) {
+    EcPageSeq s;
+    int rt = rt0, tiles = tiles0;
+    if (c0) seq(c0 + lane, s, rt, tiles);
+    all += readlane(wave_scan((unsigned long long)rt * tiles), 63);
+  }
+  const unsigned long long even = (all + gr.target - 1) / gr.target;
+  const int share = (int)min(max(even, (unsigned long long)gr.least), (unsigned long long)INT_MAX);
+  unsigned long long before = 0;
+  for (int c0 = 0; c0 < B; c0 += 64) {
+    EcPageSeq s = s0;
+    int rt = rt0, tiles = tiles0;
+    if (c0) seq(c0 + lane, s, rt, tiles);
+    const int n = (int)(((long)tiles + share - 1) / share);
+    const unsigned long long mine = (unsigned long long)rt * n * KVH, upto = before + wave_scan(mine);
+    const uint64_t hit = __ballot(mine && upto > (unsigned long long)x);
+    if (hit) {
+      const int l = __ffsll((unsigned long long)hit) - 1;
+      u.s = lane_seq(s, l);
+      u.c = c0 + l;
+      u.n = readlane(n, l);
+      const uint32_t i = (uint32_t)((unsigned long long)x - (readlane(upto, l) - readlane(mine, l))), groups = u.n * KVH;
+      u.rt = readlane(rt, l) - 1 - (int)(i / groups);
+      u.j = (int)(i % groups) / KVH;
+      u.kvh = (int)(i % groups) % KVH;
+      u.at = (uint32_t)x - u.j * KVH;
+      return u;
+    }
+    before = readlane(upto, 63);
+  }
+  return u;
+}
+
+// The parts' results: which rows of the call there are, per row and query head the place of
+// its part 0 and the number of parts, then per unit and row maxima and sums, outputs.
+struct PartRows {
+  int *rows;
+  uint2 *where;
+  float2 *ml;
+  float *o;
+};
+__device__ __forceinline__ PartRows part_rows(const PagedAttnArgs &a, const PagedGrid &gr, int rt) {
+  PartRows p;
+  p.rows = (int *)a.ws;
+  p.where = (uint2 *)(p.rows + 4);
+  p.ml = (float2 *)(p.where + (((size_t)a.c.t.M * a.H + 1) & ~(size_t)1));
+  p.o = (float *)(p.ml + (size_t)gr.units * rt);
+  return p;
+}
+size_t part_bytes(const PagedAttnArgs &a, const PagedGrid &gr, int rt, int hdp) {
+  return 16 + 8 * (((size_t)a.c.t.M * a.H + 1) & ~(size_t)1) + (size_t)gr.units * rt * (8 + 4 * (size_t)hdp);
+}
+
+// q in units of log2, so that a product is an exponent, in two 16-bit parts.  A row is
+// brought into the parts' range by a power of two (up; down: its inverse) where its largest
+// is outside [2^-4, 2^15) (below, the low parts' steps of 2^-24 would count).
+template <int N>
+__device__ __forceinline__ void split_row(float (&v)[N][8], float big, v4u (&hi)[N], v4u (&lo)[N], float *up, float *down, bool *plain) {
+  int e = 0;
+  if (!(big >= 0.0625f && big < 32768.0f) && big > 0.0f)
+    e = min(max(14 - ((int)(__float_as_uint(big) >> 23) - 127), -126), 100);
+  *up = __uint_as_float((uint32_t)(e + 127) << 23);
+  *down = __uint_as_float((uint32_t)(127 - e) << 23);
+  *plain = __ballot(e != 0) == 0;
+#pragma unroll
+  for (int k = 0; k < N; k++)
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const float x = v[k][2 * j] * *up, y = v[k][2 * j + 1] * *up;
+      const Parts f = split2(x, y);
+      hi[k][j] = f.hi;
+      lo[k][j] = (uint32_t)f2h(x - h2f((uint16_t)f.hi)) | (uint32_t)f2h(y - h2f((uint16_t)(f.hi >> 16))) << 16;
+    }
+}
+__device__ __forceinline__ void read8(float (&v)[8], const float *q, bool in, float f, float &big) {
+  float4 x = {0.0f, 0.0f, 0.0f, 0.0f}, y = x;
+  if (in) {
+    x = *reinterpret_cast<const float4 *>(q);
+    y = *reinterpret_cast<const float4 *>(q + 4);
+  }
+  v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    v[j] *= f;
+    big = fmaxf(big, fabsf(v[j]));
+  }
+}
+
+// which of the positions p0 .. p0 + 63 the token at position t sees
+__device__ __forceinline__ uint64_t tile_mask(const PagedAttnArgs &a, int p0, int t) {
+  uint64_t m = low_bits(t - p0 + 1);
+  if (a.window && t >= a.window) m &= ~low_bits(t - a.window + 1 - p0) | low_bits(min(a.sinks, t) - p0);
+  return m;
+}
+
+// eight elements of 16 or 8 bits as they come from the cache
+template <int TYPE>
+using Raw8 = std::conditional_t<TYPE == CACHE_F16, v4u, v2u>;
+template <int TYPE>
+__device__ __forceinline__ v4u to_f16(Raw8<TYPE> r, uint16_t scale) {
+  if constexpr (TYPE == CACHE_F16) return r;
+  else {
+    const v2h s = (v2h)__builtin_bit_cast(_Float16, scale);
+    return v4u{__builtin_bit_cast(uint32_t, cache_pair<TYPE, false>(r.x, s)), __builtin_bit_cast(uint32_t, cache_pair<TYPE, true>(r.x, s)),
+               __builtin_bit_cast(uint32_t, cache_pair<TYPE, false>(r.y, s)), __builtin_bit_cast(uint32_t, cache_pair<TYPE, true>(r.y, s))};
+  }
+}
+// values that are not finite become 0; whether there was one
+__device__ __forceinline__ bool only_finite(v4u &v) {
+  uint32_t hit = 0;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    // an exponent of all ones carries out of its field
+    const uint32_t e = v[j] & 0x7C007C00u;
+    const uint32_t bad = ((e & 0x7C00u) + 0x0400u) & 0x8000u, bad2 = ((e >> 16) + 0x0400u) & 0x8000u;
+    v[j] &= ~((bad ? 0xFFFFu : 0u) | (bad2 ? 0xFFFF0000u : 0u));
+    hit |= bad | bad2;
+  }
+  return hit != 0;
+}
+
+// the maximum and the sum over lanes l and l + 32
+__device__ __forceinline__ float pair_max(float v) {
+  const v2u x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(x.x), __uint_as_float(x.y));
+}
+__device__ __forceinline__ float pair_sum(float v) {
+  const v2u x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(x.x) + __uint_as_float(x.y);
+}
+
+__device__ __forceinline__ v16f mma32(v4u a, v4u b, v16f c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+}
+
+// Operands of ND groups of 32 elements, from rows 32 u .. 32 u + 31 of the tile: two of 16
+// positions each.  Lane l of 16 names 8 bytes of row l / 4 and gets element l of the four
+// rows.  The builtin would wait for all that is on its way.
+template <int HD, int ND>
+__device__ __forceinline__ void read_v32(const uint32_t *at, int u, v4u (&v)[2 * ND]) {
+  static_assert(ND == 1 || ND == 2, "groups of elements");
+  v2u x[4 * ND];
+  if constexpr (ND == 1) {
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %4 offset:%5\n\t"
+        "ds_read_b64_tr_b16 %1, %4 offset:%6\n\t"
+        "ds_read_b64_tr_b16 %2, %4 offset:%7\n\t"
+        "ds_read_b64_tr_b16 %3, %4 offset:%8\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3])
+        : "v"(at[0]), "i"(64 * HD * u), "i"(64 * HD * u + 16 * HD), "i"(64 * HD * u + 32 * HD), "i"(64 * HD * u + 48 * HD)
+        : "memory");
+  } else {
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %8 offset:%10\n\t"
+        "ds_read_b64_tr_b16 %1, %8 offset:%11\n\t"
+        "ds_read_b64_tr_b16 %2, %8 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %3, %8 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %4, %9 offset:%10\n\t"
+        "ds_read_b64_tr_b16 %5, %9 offset:%11\n\t"
+        "ds_read_b64_tr_b16 %6, %9 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %7, %9 offset:%13\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(x[4]), "=&v"(x[5]), "=&v"(x[6]), "=&v"(x[7])
+        : "v"(at[0]), "v"(at[1]), "i"(64 * HD * u), "i"(64 * HD * u + 16 * HD), "i"(64 * HD * u + 32 * HD),
+          "i"(64 * HD * u + 48 * HD)
+        : "memory");
+  }
+#pragma unroll
+  for (int e = 0; e < 2 * ND; e++) v[e] = v4u{x[2 * e].x, x[2 * e].y, x[2 * e + 1].x, x[2 * e + 1].y};
+}
+
+// Rows of a unit that takes no part
+template <int RT>
+__device__ __forceinline__ void mark_rows(const PagedAttnArgs &a, const PagedGrid &gr, const Unit &u) {
+  const int G = a.H / a.c.t.KVH, hd = a.c.hd, r0 = u.rt * RT, n = min(u.s.n * G - r0, RT);
+  for (int e = threadIdx.x; e < n * hd; e += blockDim.x) {
+    const int r = r0 + e / hd;
+    a.out[(size_t)(u.s.start + r / G) * a.ldo + (size_t)(u.kvh * G + r % G) * hd + e % hd] = __builtin_nanf("");
+  }
+  if (gr.target)
+    for (int e = threadIdx.x; e < n; e += blockDim.x)
+      part_rows(a, gr, RT).where[(size_t)(u.s.start + (r0 + e) / G) * a.H + u.kvh * G + (r0 + e) % G] = make_uint2(0, 1);
+}
+__device__ __forceinline__ void mark_call(const PagedAttnArgs &a, const PagedGrid &gr, long x) {
+  if (gr.target && x == 0 && threadIdx.x == 0) {
+    int *rows = (int *)a.ws;
+    rows[0] = a.c.t.start ? a.c.t.start[0] : 0;
+    rows[1] = a.c.t.start ? a.c.t.start[a.c.t.B] : a.c.t.M;
+  }
+}
+
+// Chunks of tokens: 128 rows of one KV head a block, 32 a wave; the waves share tiles of
+// keys and values that the block brings to LDS in fp16, the next tile on its way into
+// registers while the waves work on one.
+//
+// Products run transposed, K Q^T and V^T P^T, so that a lane keeps one row (lane & 31):
+// the scores' accumulators hold 16 of each 32 positions, its maximum and sum need one
+// exchange, with the lane 32 further on, and the weights are the second product's operand
+// as they stand: half h of the lanes takes 4 h .. 4 h + 3 of every run of 8 positions.  The
+// values, rows of the cache, are read for it by the transposing LDS load.
+//
+// fp32 by two 16-bit parts of q and of the weights, as in the attention of drafted tokens.
+template <int HDP, int TYPE>
+__global__ __launch_bounds__(256, 2) void attn_chunk_kernel(PagedAttnArgs a, PagedGrid gr) {
+  constexpr int RT = 128, CPR = HDP / 8, KS = HDP / 16, DT = HDP / 32, LPT = kTp * CPR / 256;
+  extern __shared__ __attribute__((aligned(16))) _Float16 lds[];  // [2 buffers][K, V][kTp][HDP]
+  const long x = (long)blockIdx.y * gridDim.x + blockIdx.x;
+  mark_call(a, gr, x);
+  if (x >= gr.units) return;
+  const Unit un = find_unit<RT>(a, gr, x);
+  if (un.c < 0) return;
+  const EcPageSeq s = un.s;
+  if (!ec_page_seq_ok(&a.c.t, s, a.max_past)) {
+    mark_rows<RT>(a, gr, un);
+    return;
+  }
+  const int t = threadIdx.x, lane = t & 63, ln = lane & 31, h = lane >> 5, hd = a.c.hd;
+  const int w = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int G = a.H / a.c.t.KVH, rows = s.n * G, r0 = un.rt * RT;
+  const int ta = r0 / G, tb = (min(rows, r0 + RT) - 1) / G;
+  const Tiles tl = tiles_of(a, s, ta, tb);
+  const int tile0 = (int)((long)tl.n * un.j / un.n), tile1 = (int)((long)tl.n * (un.j + 1) / un.n);
+
+  // ---- the tiles' way into LDS ----
+  // a thread's chunks of 8 elements; rows that no token of the block sees are another's that is
+  bool bad = false;
+  int pos[LPT], id[LPT];
+  Raw8<TYPE> kr[LPT], vr[LPT];
+  uint16_t ksc[LPT], vsc[LPT];
+  const auto find = [&](int tile) {
+#pragma unroll
+    for (int u = 0; u < LPT; u++) {
+      const int p = tl.at(tile) + (u * 256 + t) / CPR;
+      pos[u] = p >= tl.lo || p < tl.sinks ? min(p, s.past + tb) : tl.lo;
+      id[u] = page_id(a.c.t, un.c, pos[u]);
+    }
+  };
+  const auto load = [&] {
+#pragma unroll
+    for (int u = 0; u < LPT; u++) {
+      const uint32_t row = page_row(a.c.t, id[u], pos[u], un.kvh, &bad);
+      const int cc = (u * 256 + t) % CPR;
+      kr[u] = vr[u] = Raw8<TYPE>{};
+      if (8 * cc < hd) {
+        constexpr int B = TYPE == CACHE_F16 ? 2 : 1;
+        const size_t at = ((size_t)row * hd + 8 * cc) * B;
+        kr[u] = *(const Raw8<TYPE> *)((const char *)a.c.k + at);
+        vr[u] = *(const Raw8<TYPE> *)((const char *)a.c.v + at);
+      }
+      if constexpr (TYPE != CACHE_F16) {
+        ksc[u] = a.c.ks[row];
+        vsc[u] = a.c.vs[row];
+      }
+    }
+  };
+  if (tile0 < tile1) {
+    find(tile0);
+    load();
+    if (tile0 + 1 < tile1) find(tile0 + 1);
+  }
+
+  // ---- this lane's row of q ----
+  const int row = r0 + 32 * w + ln, rq = min(row, rows - 1), token = rq / G, head = un.kvh * G + (rq - token * G);
+  const int qpos = s.past + token;
+  v4u qh[KS], ql[KS];
+  float up, down;
+  bool plain;  // no row of the wave scaled
+  {
+    const float *q = a.q + (size_t)(s.start + token) * a.ldq + (size_t)head * hd + 8 * h;
+    float v[KS][8], big = 0.0f;
+#pragma unroll
+    for (int k = 0; k < KS; k++) read8(v[k], q + 16 * k, 16 * k + 8 * h < hd, a.scale * 1.44269504f, big);
+    split_row(v, pair_max(big), qh, ql, &up, &down, &plain);
+  }
+  const bool work = r0 + 32 * w < rows;
+  const int wa = (r0 + 32 * w) / G, wb = (min(rows, r0 + 32 * w + 32) - 1) / G;  // the wave's tokens
+
+  // the values' LDS addresses in a tile's first 8 rows (rows 8, 16 .. further on have the
+  // same swizzle)
+  typedef __attribute__((address_space(3))) void lvoid;
+  const uint32_t vbase = (uint32_t)(uintptr_t)(lvoid *)lds + 2 * kTp * HDP;
+  uint32_t vcol[DT];
+#pragma unroll
+  for (int d = 0; d < DT; d++) {
+    const int l = lane & 15, r = 4 * h + (l >> 2);
+    vcol[d] = (uint32_t)(r * HDP + ((4 * d + 2 * ((lane >> 4) & 1) + ((l & 3) >> 1)) ^ swz<HDP>(r)) * 8 + 4 * (l & 1)) * 2;
+  }
+
+  v16f o[DT];
+  float from = 0.0f, mx = -FLT_MAX, lim = -FLT_MAX, sum = 0.0f;  // from: what the row's products start at
+#pragma unroll
+  for (int d = 0; d < DT; d++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
+
+  constexpr int kBuf = 2 * kTp * HDP;  // elements of a buffer: K, then V
+  int buf = 0;
+  // One tile.  EDGE: one that some rows see in part: what they do not see has weight 0,
+  // and its values must be finite for that to be nothing.
+  auto step = [&](auto edge, int tile) {
+    constexpr bool EDGE = decltype(edge)::value;
+    const int p0 = tl.at(tile);
+    _Float16 *K = lds + buf, *V = K + kTp * HDP;
+    bool inf = false;
+#pragma unroll
+    for (int u = 0; u < LPT; u++) {
+      const int r = (u * 256 + t) / CPR, cc = (u * 256 + t) % CPR, at = r * HDP + (cc ^ swz<HDP>(r)) * 8;
+      *reinterpret_cast<v4u *>(K + at) = to_f16<TYPE>(kr[u], ksc[u]);
+      v4u v = to_f16<TYPE>(vr[u], vsc[u]);
+      if constexpr (EDGE) inf |= only_finite(v);
+      *reinterpret_cast<v4u *>(V + at) = v;
+    }
+    if (tile + 1 < tile1) {
+      load();
+      if (tile + 2 < tile1) find(tile + 2);
+    }
+    // the tile is there, and every wave is done with the one before it
+    if constexpr (EDGE) {
+      inf = __syncthreads_or(inf);
+    } else {
+      // the loads of the next tile go on
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    }
+    uint32_t vat[DT];
+#pragma unroll
+    for (int d = 0; d < DT; d++) vat[d] = vbase + 2 * (uint32_t)buf + vcol[d];
+    buf = kBuf - buf;
+    if (!work) return;
+    if constexpr (EDGE)
+      if (p0 > s.past + wb || (a.window && p0 + kTp - 1 <= s.past + wa - a.window && p0 >= a.sinks)) return;
+
+    // ---- scores: sc[pt][i] of position 32 pt + 8 (i / 4) + 4 h + i % 4 ----
+    v16f sc[2];
+#pragma unroll
+    for (int pt = 0; pt < 2; pt++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) sc[pt][i] = from;
+#pragma unroll
+    for (int k = 0; k < KS; k++) {
+      v4u kf[2];
+#pragma unroll
+      for (int pt = 0; pt < 2; pt++) {
+        const int r = 32 * pt + ln;
+        kf[pt] = *reinterpret_cast<const v4u *>(K + r * HDP + ((2 * k + h) ^ swz<HDP>(r)) * 8);
+      }
+      sc[0] = mma32(kf[0], qh[k], sc[0]);
+      sc[1] = mma32(kf[1], qh[k], sc[1]);
+      sc[0] = mma32(kf[0], ql[k], sc[0]);
+      sc[1] = mma32(kf[1], ql[k], sc[1]);
+    }
+
+    // ---- weights ----
+    if constexpr (EDGE) {
+      const uint64_t on = tile_mask(a, p0, qpos) >> (4 * h);
+#pragma unroll
+      for (int pt = 0; pt < 2; pt++)
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+          if (!((on >> (32 * pt + 8 * (i >> 2) + (i & 3))) & 1)) sc[pt][i] = -__builtin_inff();
+    }
+    if (__builtin_expect(!plain, 0)) {
+#pragma unroll
+      for (int pt = 0; pt < 2; pt++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) sc[pt][i] *= down;
+    }
+    // exponents of the weights already (the sums began at -mx): above kRoom the maximum
+    // moves
+    float top = -FLT_MAX;
+#pragma unroll
+    for (int pt = 0; pt < 2; pt++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) top = fmaxf(top, sc[pt][i]);
+    if (__builtin_expect(__ballot(top > lim) != 0, 0)) {
+      const float big = pair_max(top);
+      const bool first = mx == -FLT_MAX, move = big > (first ? -FLT_MAX : 0.0f);
+      const float by = move ? big : 0.0f, back = first ? 0.0f : __builtin_amdgcn_exp2f(-by);
+      if (move) {
+        mx = first ? big : mx + by;
+        lim = kRoom;
+      }
+      from = move || !first ? -mx * up : 0.0f;
+      sum *= back;
+#pragma unroll
+      for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[d][i] *= back;
+#pragma unroll
+      for (int pt = 0; pt < 2; pt++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) sc[pt][i] -= by;
+    }
+    // the tile's weights are added up before they meet the sum so far: one by one, those
+    // below half a step of it would be lost
+    v4u ph[2][2], pl[2][2];
+    float here[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int pt = 0; pt < 2; pt++)
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        const float p = __builtin_amdgcn_exp2f(sc[pt][i]), q = __builtin_amdgcn_exp2f(sc[pt][i + 1]);
+        here[0] += p;
+        here[1] += q;
+        const Parts f = split2<kLift>(p, q);
+        ph[pt][i >> 3][(i & 7) >> 1] = f.hi;
+        pl[pt][i >> 3][(i & 7) >> 1] = f.lo;
+      }
+    sum += here[0] + here[1];
+
+    // ---- outputs: o[d][i] of element 32 d + 8 (i / 4) + 4 h + i % 4 ----
+#pragma unroll
+    for (int pt = 0; pt < 2; pt++) {
+      constexpr int ND = DT % 2 ? 1 : 2;
+#pragma unroll
+      for (int d = 0; d < DT; d += ND) {
+        v4u vf[2 * ND];
+        if (pt == 0) read_v32<HDP, ND>(vat + d, 0, vf);
+        else read_v32<HDP, ND>(vat + d, 1, vf);
+#pragma unroll
+        for (int c = 0; c < 2; c++)
+#pragma unroll
+          for (int e = 0; e < ND; e++) o[d + e] = mma32(vf[2 * e + c], ph[pt][c], o[d + e]);
+#pragma unroll
+        for (int c = 0; c < 2; c++)
+#pragma unroll
+          for (int e = 0; e < ND; e++) o[d + e] = mma32(vf[2 * e + c], pl[pt][c], o[d + e]);
+      }
+    }
+
+    // values that are not finite, for the rows that see them
+    if (EDGE && __builtin_expect(inf, 0)) {
+      const uint64_t on = tile_mask(a, p0, qpos);
+      for (int pp = 0; pp < kTp && p0 + pp <= s.past + wb; pp++) {
+        if (!__ballot((on >> pp) & 1)) continue;
+        bool none = false;
+        const uint32_t r = page_row(a.c.t, page_id(a.c.t, un.c, p0 + pp), p0 + pp, un.kvh, &none);
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            const int e = 32 * d + 8 * (i >> 2) + 4 * h + (i & 3);
+            if (((on >> pp) & 1) && e < hd && (cache_value(a.c.v, a.c.vs, TYPE, r, hd, e) & 0x7C00u) == 0x7C00u)
+              o[d][i] = __builtin_nanf("");
+          }
+      }
+    }
+  };
+  // a tile that every token sees whole is no edge
+  for (int tile = tile0; tile < tile1; tile++) {
+    const int p0 = tl.at(tile);
+    const bool whole = p0 + kTp - 1 <= s.past + ta &&
+                       (!a.window || p0 > s.past + tb - a.window || p0 + kTp <= a.sinks);
+    if (whole) step(std::false_type{}, tile);
+    else step(std::true_type{}, tile);
+  }
+
+  const bool none = __syncthreads_or(bad);
+  const float l = none ? __builtin_nanf("") : pair_sum(sum) * kLifted;  // as the outputs
+  if (row >= rows) return;
+  if (gr.target) {
+    const PartRows pr = part_rows(a, gr, RT);
+    if (un.j == 0 && h == 0)
+      pr.where[(size_t)(s.start + token) * a.H + head] = make_uint2(un.at * RT + 32 * w + ln, un.n);
+    if (un.n > 1) {
+      const size_t at = (size_t)x * RT + 32 * w + ln;
+      if (h == 0) pr.ml[at] = make_float2(mx, l);
+      if (tile0 == tile1) return;
+      float *po = pr.o + at * HDP + 4 * h;
+#pragma unroll
+      for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          *reinterpret_cast<float4 *>(po + 32 * d + 8 * i) = make_float4(o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]);
+      return;
+    }
+  }
+  const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+  float *out = a.out + (size_t)(s.start + token) * a.ldo + (size_t)head * hd + 4 * h;
+#pragma unroll
+  for (int d = 0; d < DT; d++)
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (32 * d + 8 * i + 4 * h < hd)
+        *reinterpret_cast<float4 *>(out + 32 * d + 8 * i) =
+            make_float4(o[d][4 * i] * inv, o[d][4 * i + 1] * inv, o[d][4 * i + 2] * inv, o[d][4 * i + 3] * inv);
+}
+
+// Single tokens: 16 rows of one KV head a block.  Each of its four waves takes every
+// fourth of the part's steps of TP positions, without a barrier: keys come from the cache
+// as the matrix instruction's operand, values through the wave's own tile in LDS, which
+// transposes them; the next step's are on their way while a wave works on one.  The waves'
+// results are joined in LDS.
+template <int HDP, int TYPE>
+__global__ __launch_bounds__(256, 2) void attn_step_kernel(PagedAttnArgs a, PagedGrid gr) {
+  constexpr int RT = 16, TP = HDP <= 64 ? 64 : 32, PT = TP / 16, CPR = HDP / 8, KS = HDP / 32, DT = HDP / 16, ND = DT % 4 ? 2 : 4;
+  constexpr int EB = TYPE == CACHE_F16 ? 2 : 1, VC = TYPE == CACHE_F16 ? 1 : 2;  // chunks of 8 elements in 16 bytes
+  constexpr int LV = TP * CPR / VC / 64, PER = kTp / TP;
+  constexpr bool WIDE = TYPE != CACHE_F16 && KS % 2 == 0;  // two chunks of keys in 16 bytes
+  constexpr int LDO = HDP + 4, kLds = 4 * (TP * HDP * 2 > RT * LDO * 4 ? TP * HDP * 2 : RT * LDO * 4);
+  __shared__ __attribute__((aligned(16))) char lds[kLds];
+  __shared__ float2 ml[4][RT];
+  const long x = (long)blockIdx.y * gridDim.x + blockIdx.x;
+  mark_call(a, gr, x);
+  if (x >= gr.units) return;
+  const Unit un = find_unit<RT>(a, gr, x);
+  if (un.c < 0) return;
+  const EcPageSeq s = un.s;
+  if (!ec_page_seq_ok(&a.c.t, s, a.max_past)) {
+    mark_rows<RT>(a, gr, un);
+    return;
+  }
+  const int t = threadIdx.x, lane = t & 63, lr = lane & 15, lg = lane >> 4, hd = a.c.hd;
+  const int w = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int G = a.H / a.c.t.KVH, rows = s.n * G, r0 = un.rt * RT;
+  const int ta = r0 / G, tb = (min(rows, r0 + RT) - 1) / G;
+  const Tiles tl = tiles_of(a, s, ta, tb);
+  const int tile0 = (int)((long)tl.n * un.j / un.n), tile1 = (int)((long)tl.n * (un.j + 1) / un.n);
+  const int steps = (tile1 - tile0) * PER;
+  const auto pos_of = [&](int i) { return tl.at(tile0 + i / PER) + i % PER * TP; };
+
+  // ---- a step's keys and values ----
+  bool bad = false;
+  int pos, id = 0;
+  uint32_t crow = 0;  // lane l's position's row in the cache
+  v4u kr[PT][WIDE ? KS / 2 : KS], vr[LV];
+  uint16_t ksc[PT], vsc[LV];
+  const auto find = [&](int i) {
+    const int p = pos_of(i) + (lane & (TP - 1));
+    pos = p >= tl.lo || p < tl.sinks ? min(p, s.past + tb) : tl.lo;
+    id = page_id(a.c.t, un.c, pos);
+  };
+  const auto load = [&] {
+    crow = page_row(a.c.t, id, pos, un.kvh, &bad);
+#pragma unroll
+    for (int pt = 0; pt < PT; pt++) {
+      const uint32_t row = (uint32_t)__shfl((int)crow, 16 * pt + lr, 64);
+      const char *k = (const char *)a.c.k + (size_t)row * hd * EB;
+      if constexpr (TYPE != CACHE_F16) ksc[pt] = a.c.ks[row];
+#pragma unroll
+      for (int c = 0; c < (WIDE ? KS / 2 : KS); c++) {
+        kr[pt][c] = v4u{0, 0, 0, 0};
+        if constexpr (TYPE == CACHE_F16) {
+          if (32 * c + 8 * lg < hd) kr[pt][c] = *(const v4u *)(k + 2 * (32 * c + 8 * lg));
+        } else if constexpr (WIDE) {
+          if (lg * (HDP / 4) + 16 * c < hd) kr[pt][c] = *(const v4u *)(k + lg * (HDP / 4) + 16 * c);
+        } else {
+          if (lg * (HDP / 4) + 8 * c < hd) {
+            const v2u y = *(const v2u *)(k + lg * (HDP / 4) + 8 * c);
+            kr[pt][c].x = y.x;
+            kr[pt][c].y = y.y;
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < LV; u++) {
+      const int ch = u * 64 + lane, r = ch / (CPR / VC), cc = ch % (CPR / VC) * VC;
+      const uint32_t row = (uint32_t)__shfl((int)crow, r, 64);
+      vr[u] = v4u{0, 0, 0, 0};
+      if (8 * cc < hd) vr[u] = *(const v4u *)((const char *)a.c.v + ((size_t)row * hd + 8 * cc) * EB);
+      if constexpr (TYPE != CACHE_F16) vsc[u] = a.c.vs[row];
+    }
+  };
+  if (w < steps) {
+    find(w);
+    load();
+    if (w + 4 < steps) find(w + 4);
+  }
+
+  // ---- this lane's row of q; its elements in the order that the keys' have ----
+  const int row = r0 + lr, rq = min(row, rows - 1), token = rq / G, head = un.kvh * G + (rq - token * G);
+  const int qpos = s.past + token;
+  v4u qh[KS], ql[KS];
+  float up, down;
+  bool plain;
+  {
+    const float *q = a.q + (size_t)(s.start + token) * a.ldq + (size_t)head * hd;
+    float v[KS][8], big = 0.0f;
+#pragma unroll
+    for (int k = 0; k < KS; k++) {
+      const int e = TYPE == CACHE_F16 ? 32 * k + 8 * lg : lg * (HDP / 4) + 8 * k;
+      read8(v[k], q + e, e < hd, a.scale * 1.44269504f, big);
+    }
+    split_row(v, row_max(big), qh, ql, &up, &down, &plain);
+  }
+
+  // the values' LDS addresses in the tile's first 32 rows
+  typedef __attribute__((address_space(3))) void lvoid;
+  _Float16 *V = reinterpret_cast<_Float16 *>(lds) + w * TP * HDP;
+  const uint32_t vbase = (uint32_t)(uintptr_t)(lvoid *)V;
+  uint32_t vcol[DT];
+#pragma unroll
+  for (int d = 0; d < DT; d++) {
+    const int r = 4 * lg + (lr >> 2);
+    vcol[d] = (uint32_t)(r * HDP + ((2 * d + ((lr & 3) >> 1)) ^ swz<HDP>(r)) * 8 + 4 * (lr & 1)) * 2;
+  }
+
+  v4f o[DT], from = {0.0f, 0.0f, 0.0f, 0.0f};  // from: what the row's products start at
+  float mx = -FLT_MAX, lim = -FLT_MAX, sum = 0.0f;
+#pragma unroll
+  for (int d = 0; d < DT; d++) o[d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+
+  for (int i = w; i < steps; i += 4) {
+    const int p0 = pos_of(i);
+    const bool edge = !(p0 + TP - 1 <= s.past + ta && (!a.window || p0 > s.past + tb - a.window || p0 + TP <= a.sinks));
+    const uint32_t srow = crow;
+    // ---- scores: sc[pt][r] of position 16 pt + 4 lg + r ----
+    v4f sc[PT];
+#pragma unroll
+    for (int pt = 0; pt < PT; pt++) {
+      sc[pt] = from;
+#pragma unroll
+      for (int k = 0; k < KS; k++) {
+        v4u kf;
+        if constexpr (TYPE == CACHE_F16) kf = kr[pt][k];
+        else if constexpr (WIDE) kf = to_f16<TYPE>(k & 1 ? v2u{kr[pt][k / 2].z, kr[pt][k / 2].w} : v2u{kr[pt][k / 2].x, kr[pt][k / 2].y}, ksc[pt]);
+        else kf = to_f16<TYPE>(v2u{kr[pt][k].x, kr[pt][k].y}, ksc[pt]);
+        sc[pt] = mma(kf, qh[k], sc[pt]);
+        sc[pt] = mma(kf, ql[k], sc[pt]);
+      }
+    }
+    // ---- values into LDS ----
+    bool inf = false;
+#pragma unroll
+    for (int u = 0; u < LV; u++) {
+      const int ch = u * 64 + lane, r = ch / (CPR / VC), cc = ch % (CPR / VC) * VC;
+#pragma unroll
+      for (int c = 0; c < VC; c++) {
+        v4u v;
+        if constexpr (TYPE == CACHE_F16) v = vr[u];
+        else v = to_f16<TYPE>(c ? v2u{vr[u].z, vr[u].w} : v2u{vr[u].x, vr[u].y}, vsc[u]);
+        if (edge) inf |= only_finite(v);
+        *reinterpret_cast<v4u *>(V + r * HDP + ((cc + c) ^ swz<HDP>(r)) * 8) = v;
+      }
+    }
+    if (i + 4 < steps) {
+      load();
+      if (i + 8 < steps) find(i + 8);
+    }
+
+    // ---- weights ----
+    if (edge) {
+      const uint64_t on = tile_mask(a, p0, qpos) >> (4 * lg);
+#pragma unroll
+      for (int pt = 0; pt < PT; pt++)
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+          if (!((on >> (16 * pt + r)) & 1)) sc[pt][r] = -__builtin_inff();
+    }
+    if (__builtin_expect(!plain, 0)) {
+#pragma unroll
+      for (int pt = 0; pt < PT; pt++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) sc[pt][r] *= down;
+    }
+    float top = -FLT_MAX;
+#pragma unroll
+    for (int pt = 0; pt < PT; pt++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) top = fmaxf(top, sc[pt][r]);
+    if (__builtin_expect(__ballot(top > lim) != 0, 0)) {
+      const float big = row_max(top);
+      const bool first = mx == -FLT_MAX, move = big > (first ? -FLT_MAX : 0.0f);
+      const float by = move ? big : 0.0f, back = first ? 0.0f : __builtin_amdgcn_exp2f(-by);
+      if (move) {
+        mx = first ? big : mx + by;
+        lim = kRoom;
+      }
+      const float f = move || !first ? -mx * up : 0.0f;
+      from = v4f{f, f, f, f};
+      sum *= back;
+#pragma unroll
+      for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) o[d][r] *= back;
+#pragma unroll
+      for (int pt = 0; pt < PT; pt++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) sc[pt][r] -= by;
+    }
+    v4u ph[PT / 2], pl[PT / 2];
+    float here = 0.0f;
+#pragma unroll
+    for (int pt = 0; pt < PT; pt++) {
+      float p[4];
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        p[r] = __builtin_amdgcn_exp2f(sc[pt][r]);
+        here += p[r];
+      }
+#pragma unroll
+      for (int r = 0; r < 2; r++) {
+        const Parts f = split2<kLift>(p[2 * r], p[2 * r + 1]);
+        ph[pt >> 1][2 * (pt & 1) + r] = f.hi;
+        pl[pt >> 1][2 * (pt & 1) + r] = f.lo;
+      }
+    }
+    sum += here;
+
+    // ---- outputs: o[d][r] of element 16 d + 4 lg + r ----
+#pragma unroll
+    for (int u = 0; u < TP / 32; u++)
+#pragma unroll
+      for (int d = 0; d < DT; d += ND) {
+        v4u vf[ND];
+        if (u == 0) read_v<HDP, ND>(vcol + d, vbase, 0, vf);
+        else read_v<HDP, ND>(vcol + d, vbase, 1, vf);
+#pragma unroll
+        for (int e = 0; e < ND; e++) {
+          o[d + e] = mma(vf[e], ph[u], o[d + e]);
+          o[d + e] = mma(vf[e], pl[u], o[d + e]);
+        }
+      }
+
+    // values that are not finite, for the rows that see them
+    if (__builtin_expect(__ballot(inf) != 0, 0)) {
+      const uint64_t on = tile_mask(a, p0, qpos);
+      for (int pp = 0; pp < TP; pp++) {
+        const uint32_t r = (uint32_t)__shfl((int)srow, pp, 64);
+        if ((on >> pp) & 1) {
+#pragma unroll
+          for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+              const int e = 16 * d + 4 * lg + k;
+              if (e < hd && (cache_value(a.c.v, a.c.vs, TYPE, r, hd, e) & 0x7C00u) == 0x7C00u) o[d][k] = __builtin_nanf("");
+            }
+        }
+      }
+    }
+  }
+
+  // ---- the waves' results together ----
+  float l = row_sum(sum) * kLifted;  // as the outputs
+  if (__ballot(bad)) l = __builtin_nanf("");
+  __syncthreads();  // every wave is done with its tile
+  float *wo = reinterpret_cast<float *>(lds) + (w * RT + lr) * LDO + 4 * lg;
+#pragma unroll
+  for (int d = 0; d < DT; d++) *reinterpret_cast<v4f *>(wo + 16 * d) = o[d];
+  if (lg == 0) ml[w][lr] = make_float2(mx, l);
+  __syncthreads();
+  const int jr = t >> 4, jrow = r0 + jr;
+  if (jrow >= rows) return;
+  const int jt = jrow / G, jh = un.kvh * G + (jrow - jt * G);
+  float m = -FLT_MAX, f[4], jl = 0.0f;
+#pragma unroll
+  for (int k = 0; k < 4; k++) m = fmaxf(m, ml[k][jr].x);
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    f[k] = __builtin_amdgcn_exp2f(ml[k][jr].x - m);
+    jl = __builtin_fmaf(ml[k][jr].y, f[k], jl);
+  }
+  float scale = 1.0f;
+  float *to;
+  if (gr.target) {
+    const PartRows pr = part_rows(a, gr, RT);
+    if (un.j == 0 && (t & 15) == 0) pr.where[(size_t)(s.start + jt) * a.H + jh] = make_uint2(un.at * RT + jr, un.n);
+    to = pr.o + ((size_t)x * RT + jr) * HDP;
+    if (un.n > 1 && (t & 15) == 0) pr.ml[(size_t)x * RT + jr] = make_float2(m, jl);
+  }
+  if (!gr.target || un.n == 1) {
+    to = a.out + (size_t)(s.start + jt) * a.ldo + (size_t)jh * hd;
+    scale = jl > 0.0f || jl != jl ? 1.0f / jl : 0.0f;
+  }
+  for (int e = 4 * (t & 15); e < hd; e += 64) {
+    v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const v4f y = *reinterpret_cast<const v4f *>(reinterpret_cast<const float *>(lds) + (k * RT + jr) * LDO + e);
+#pragma unroll
+      for (int c = 0; c < 4; c++) v[c] = __builtin_fmaf(y[c], f[k], v[c]);
+    }
+    *reinterpret_cast<v4f *>(to + e) = v * scale;
+  }
+}
+
+// Joins the parts' outputs: per row the largest of their maxima, the sums and outputs
+// brought to it.  HDP / 4 lanes a row (a power of two of them: 24 of 32 at 96).
+template <int HDP>
+__global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedAttnArgs a, PagedGrid gr, int rt) {
+  constexpr int LPR = HDP == 96 ? 32 : HDP / 4, RPB = 256 / LPR, kRead = 8;
+  const int li = threadIdx.x % LPR;
+  const long r = (long)blockIdx.x * RPB + threadIdx.x / LPR;
+  if (r >= (long)a.c.t.M * a.H) return;
+  const PartRows pr = part_rows(a, gr, rt);
+  const int token = (int)(r / a.H);
+  if (token < pr.rows[0] || token >= pr.rows[1]) return;
+  const uint2 where = pr.where[r];
+  const size_t each = (size_t)a.c.t.KVH * rt;
+  const int n = (int)where.y;
+  // (where the starts do not ascend, a row's numbers may be an earlier call's)
+  if (n < 2 || where.x + (size_t)(n - 1) * each >= (size_t)gr.units * rt || 4 * li >= a.c.hd) return;
+  float m = -FLT_MAX, l = 0.0f;
+  float4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int i0 = 0; i0 < n; i0 += kRead) {
+    float2 u[kRead];
+    float4 v[kRead];
+#pragma unroll
+    for (int i = 0; i < kRead; i++) {
+      const size_t at = where.x + (size_t)min(i0 + i, n - 1) * each;
+      u[i] = pr.ml[at];
+      v[i] = *reinterpret_cast<const float4 *>(pr.o + at * HDP + 4 * li);
+    }
+    float big = m;
+#pragma unroll
+    for (int i = 0; i < kRead; i++)
+      if (i0 + i < n) big = fmaxf(big, u[i].x);
+    const float back = __builtin_amdgcn_exp2f(m - big);
+    m = big;
+    l *= back;
+    o = make_float4(o.x * back, o.y * back, o.z * back, o.w * back);
+#pragma unroll
+    for (int i = 0; i < kRead; i++)
+      if (i0 + i < n && u[i].y != 0.0f) {  // (outputs of a part without tiles are not there)
+        const float f = __builtin_amdgcn_exp2f(u[i].x - m);
+        l = __builtin_fmaf(u[i].y, f, l);
+        o.x = __builtin_fmaf(v[i].x, f, o.x);
+        o.y = __builtin_fmaf(v[i].y, f, o.y);
+        o.z = __builtin_fmaf(v[i].z, f, o.z);
+        o.w = __builtin_fmaf(v[i].w, f, o.w);
+      }
+  }
+  const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+  *reinterpret_cast<float4 *>(a.out + (size_t)token * a.ldo + (size_t)(r - (long)token * a.H) * a.c.hd + 4 * li) =
+      make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+}
+
+// heads and rows that the matrix-core forms' tiles and 16-byte accesses can take, and
+// whose rows (of query heads) count in an int
+bool tiles_ok(const PagedAttnArgs &a) {
+  if ((long)a.c.t.M * a.H > 1L << 30) return false;
+  const uintptr_t p = (uintptr_t)a.q | (uintptr_t)a.c.k | (uintptr_t)a.c.v | (uintptr_t)a.out;
+  return a.c.hd % 16 == 0 && a.c.hd <= 128 && !(p & 15) && a.ldq % 4 == 0 && a.ldo % 4 == 0;
+}
+int padded(int hd) { return (hd + 31) / 32 * 32; }
+
+// Rows of a tile: 16 where a sequence has on average no more
+int tile_rows(const PagedAttnArgs &a) { return (long)a.c.t.M * (a.H / a.c.t.KVH) <= 16L * a.c.t.B ? 16 : 128; }
+
+PagedGrid paged_grid(const PagedAttnArgs &a) {
+  const int rt = tile_rows(a), KVH = a.c.t.KVH;
+  const long tiles = (long)a.c.t.M * (a.H / KVH) / rt + a.c.t.B, places = 512 / KVH;
+  PagedGrid g;
+  g.least = rt == 16 ? 4 : 2;
+  long left = places - tiles;
+  if (left < places / 2) left = places / 2;
+  if (left < 1) left = 1;
+  long span = (long)a.max_past + a.c.t.M;
+  if (a.window && (long)a.window + a.c.t.M + a.sinks < span) span = (long)a.window + a.c.t.M + a.sinks;
+  g.target = tiles * KVH <= 2048 && span > (long)g.least * kTp ? (int)left : 0;
+  g.units = (tiles + g.target) * KVH;
+  return g;
+}
+
+template <int HDP, int TYPE>
+hipError_t launch_paged(const PagedAttnArgs &a, hipStream_t st) {
+  const PagedGrid g = paged_grid(a);
+  const long row = g.units < kGridRow ? g.units : kGridRow;
+  const dim3 grid((unsigned)row, (unsigned)((g.units + row - 1) / row));
+  if (tile_rows(a) == 16) klaunch((attn_step_kernel<HDP, TYPE>), grid, dim3(256), 0, st, a, g);
+  else klaunch((attn_chunk_kernel<HDP, TYPE>), grid, dim3(256), 2 * 2 * kTp * HDP * 2, st, a, g);
+  return hipGetLastError();
+}
+template <int HDP>
+hipError_t launch_paged(const PagedAttnArgs &a, hipStream_t st) {
+  if (a.c.type == CACHE_F16) return launch_paged<HDP, CACHE_F16>(a, st);
+  if (a.c.type == CACHE_I8) return launch_paged<HDP, CACHE_I8>(a, st);
+  return launch_paged<HDP, CACHE_E4M3>(a, st);
+}
+template <int HDP>
+hipError_t launch_join(const PagedAttnArgs &a, hipStream_t st) {
+  constexpr int rpb = 256 / (HDP == 96 ? 32 : HDP / 4);
+  klaunch((attn_paged_join_kernel<HDP>), dim3((unsigned)(((long)a.c.t.M * a.H + rpb - 1) / rpb)), dim3(256), 0, st, a, paged_grid(a),
+          tile_rows(a));
+  return hipGetLastError();
+}
+
 }  // namespace
 
 int attention_paged_max_hd() { return kPagedMaxHd; }
 
+bool attention_paged_joins(const PagedAttnArgs &a) { return tiles_ok(a) && paged_grid(a).target > 0; }
+
+size_t attention_paged_workspace(const PagedAttnArgs &a) {
+  return attention_paged_joins(a) ? part_bytes(a, paged_grid(a), tile_rows(a), padded(a.c.hd)) : 0;
+}
+
 hipError_t attention_paged(const PagedAttnArgs &a, hipStream_t st) {
+  if (tiles_ok(a)) {
+    if (a.c.hd <= 32) return launch_paged<32>(a, st);
+    if (a.c.hd <= 64) return launch_paged<64>(a, st);
+    if (a.c.hd <= 96) return launch_paged<96>(a, st);
+    return launch_paged<128>(a, st);
+  }
   klaunch(attn_paged_any_kernel, dim3(a.c.t.M, a.H), dim3(256), 0, st, a);
   return hipGetLastError();
+}
+
+hipError_t attention_paged_join(const PagedAttnArgs &a, hipStream_t st) {
+  if (a.c.hd <= 32) return launch_join<32>(a, st);
+  if (a.c.hd <= 64) return launch_join<64>(a, st);
+  if (a.c.hd <= 96) return launch_join<96>(a, st);
+  return launch_join<128>(a, st);
 }
 
 }  // namespace ec

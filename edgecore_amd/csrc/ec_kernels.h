@@ -576,7 +576,10 @@ struct PagedAttnArgs {
   void *ws;
 };
 int attention_paged_max_hd();
+size_t attention_paged_workspace(const PagedAttnArgs &a);  // bytes of ws
 hipError_t attention_paged(const PagedAttnArgs &a, hipStream_t st);
+bool attention_paged_joins(const PagedAttnArgs &a);  // whether a join follows
+hipError_t attention_paged_join(const PagedAttnArgs &a, hipStream_t st);
 
 // logits before they are sampled (logits_edit.hip)
 struct EditArgs {

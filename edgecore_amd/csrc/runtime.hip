@@ -453,7 +453,7 @@ struct W16Buf {
   void *retired[64] = {};
   int nretired = 0;
 };
-static W16Buf g_w16_parts, g_w16_rs, g_tree_ws, g_sample_ws;
+static W16Buf g_w16_parts, g_w16_rs, g_tree_ws, g_sample_ws, g_paged_ws;
 
 static int w16_grow(W16Buf &b, size_t bytes, const char *fn = "gemm") {
   if (bytes <= b.n) return 0;
@@ -2635,7 +2635,11 @@ extern "C" int ec_attention_paged_dev(const EcPagedCache *cache, const float *q,
   EC_INIT();
   const DeviceScope dev;
   PagedAttnArgs a{c, q, ldq, H, max_past, window, sinks, (float)(1.0 / sqrt((double)hd)), out, ldo, nullptr};
+  const size_t need = attention_paged_workspace(a);
+  if (need && (r = w16_grow(g_paged_ws, need, fn))) return r;
+  a.ws = g_paged_ws.p;
   EC_LAUNCH("attention_paged", (double)B * max_past * paged_row_bytes(c), attention_paged(a, g_stream));
+  if (attention_paged_joins(a)) EC_LAUNCH("attention_paged_join", (double)need, attention_paged_join(a, g_stream));
   return 0;
 }
 
@@ -2742,7 +2746,7 @@ extern "C" int ec_release(void) {
     if (g_kept_host.p) EC_HIP(hipHostFree(g_kept_host.p));
     g_kept_dev = g_kept_host = Staging{};
   }
-  for (W16Buf *b : {&g_w16_parts, &g_w16_rs, &g_tree_ws, &g_sample_ws}) {
+  for (W16Buf *b : {&g_w16_parts, &g_w16_rs, &g_tree_ws, &g_sample_ws, &g_paged_ws}) {
     if (b->p) EC_HIP(hipFree(b->p));
     for (int i = 0; i < b->nretired; i++) EC_HIP(hipFree(b->retired[i]));
     *b = W16Buf{};
