@@ -93,7 +93,6 @@ constexpr float kLifted = 1 << kLift;
 static_assert(kLift + kRoom < 16.0f, "parts below 65504");
 constexpr long kGridRow = 1L << 20;
 typedef float v16f __attribute__((ext_vector_type(16)));
-typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 
 // target: units per KV head that the texts are split for (0: they are not); least: tiles of a
 // part, at least
@@ -280,18 +279,6 @@ __device__ __forceinline__ uint64_t tile_mask(const PagedAttnArgs &a, int p0, in
   return m;
 }
 
-// eight elements of 16 or 8 bits as they come from the cache
-template <int TYPE>
-using Raw8 = std::conditional_t<TYPE == CACHE_F16, v4u, v2u>;
-template <int TYPE>
-__device__ __forceinline__ v4u to_f16(Raw8<TYPE> r, uint16_t scale) {
-  if constexpr (TYPE == CACHE_F16) return r;
-  else {
-    const v2h s = (v2h)__builtin_bit_cast(_Float16, scale);
-    return v4u{__builtin_bit_cast(uint32_t, cache_pair<TYPE, false>(r.x, s)), __builtin_bit_cast(uint32_t, cache_pair<TYPE, true>(r.x, s)),
-               __builtin_bit_cast(uint32_t, cache_pair<TYPE, false>(r.y, s)), __builtin_bit_cast(uint32_t, cache_pair<TYPE, true>(r.y, s))};
-  }
-}
 // values that are not finite become 0; whether there was one
 __device__ __forceinline__ bool only_finite(v4u &v) {
   uint32_t hit = 0;

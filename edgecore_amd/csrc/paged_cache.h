@@ -4,6 +4,8 @@
 // rows read back are those that the attention sees.
 #pragma once
 
+#include <type_traits>
+
 #include "ec_device.h"
 #include "ec_kernels.h"
 
@@ -49,6 +51,7 @@ __device__ __forceinline__ void cache_store(void *p, int type, size_t at, double
   else ((uint8_t *)p)[at] = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(cache_code_e4m3(y, s), 0.0f, 0, false);
 }
 
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 // two codes of a word (its low or high half) as fp16, times the scale
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 template <int TYPE, bool HI>
@@ -62,6 +65,18 @@ __device__ __forceinline__ v2h cache_pair(uint32_t w, v2h scale) {
   }
 }
 
+// eight elements of 16 or 8 bits as they come from the cache
+template <int TYPE>
+using Raw8 = std::conditional_t<TYPE == CACHE_F16, v4u, v2u>;
+template <int TYPE>
+__device__ __forceinline__ v4u to_f16(Raw8<TYPE> r, uint16_t scale) {
+  if constexpr (TYPE == CACHE_F16) return r;
+  else {
+    const v2h s = (v2h)__builtin_bit_cast(_Float16, scale);
+    return v4u{__builtin_bit_cast(uint32_t, cache_pair<TYPE, false>(r.x, s)), __builtin_bit_cast(uint32_t, cache_pair<TYPE, true>(r.x, s)),
+               __builtin_bit_cast(uint32_t, cache_pair<TYPE, false>(r.y, s)), __builtin_bit_cast(uint32_t, cache_pair<TYPE, true>(r.y, s))};
+  }
+}
 // element e of row `row`, in fp16 bits
 __device__ __forceinline__ uint16_t cache_value(const void *p, const uint16_t *scale, int type, size_t row, int hd, int e) {
   const size_t at = row * hd + e;

@@ -13,6 +13,9 @@
 //
 // k is computed in 64 bits: a code is a step of 1/127 of a row's largest, so that a
 // key near the border of two would show 32-bit roundings in all that is read.
+#include <algorithm>
+#include <type_traits>
+
 #include "ec_device.h"
 #include "ec_kernels.h"
 #include "paged_cache.h"
@@ -52,6 +55,7 @@ __device__ __forceinline__ double2 rope_cs64(int pos, double f, double factor) {
 // The form for any head size and alignment: one block per token, a wave a head at
 // a time, its elements through the wave's row in LDS.
 constexpr int kAppendMaxHd = 512;
+constexpr long kGridRow = 1L << 20;
 __global__ __launch_bounds__(256) void paged_append_any_kernel(PagedAppendArgs a) {
   __shared__ double row[4][kAppendMaxHd];
   __shared__ double2 cs[kAppendMaxHd / 2];
@@ -126,6 +130,152 @@ __global__ __launch_bounds__(256) void paged_append_any_kernel(PagedAppendArgs a
   }
 }
 
+// The form for head sizes that are multiples of 4 up to 256 and rows of whole
+// 16-byte chunks: a block per row, LPH lanes a head, four elements a lane.  A wave takes 64
+// / LPH heads at a time, of q (in 32 bits) or of k and v (in 64), those of k and v first:
+// they take longest.  A pair's other element is in the same lane (layout 1) or in lane +-
+// rot / 8, which holds its four (layout 0, rot a multiple of 8).
+template <int LPH, int TYPE>
+__global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
+  constexpr int GPW = 64 / LPH;  // heads of a wave
+  __shared__ double cosines[128], sines[128];
+  const int t = threadIdx.x, lane = t & 63, li = lane % LPH, e = 4 * li, hd = a.c.hd, KVH = a.c.t.KVH, H = a.H;
+  const int kvw = (2 * KVH + GPW - 1) / GPW, all = kvw + (H + GPW - 1) / GPW, waves = blockDim.x >> 6;
+  const size_t m = blockIdx.x;
+  const int half = a.rot >> 1;
+  const bool in = e < hd;
+  const float *x = a.x + m * a.ldx + e;
+  // the head of slot i's lanes: k and v, then q
+  const auto head_of = [&](int i) {
+    const int g = lane / LPH, h = i < kvw ? H + i * GPW + g : (i - kvw) * GPW + g;
+    return i < kvw ? (h < H + 2 * KVH ? h : -1) : h < H && i < all ? h : -1;
+  };
+  const auto read = [&](int h) {
+    float4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (in && h >= 0) v = *reinterpret_cast<const float4 *>(x + (size_t)h * hd);
+    return v;
+  };
+  int i = t >> 6, h = head_of(i);
+  float4 next = read(h);
+  double f = 0.0;
+  if (t < half) f = a.inv_freq[t];
+  const PagedRow rr = paged_row(a.c.t, blockIdx.x);
+  if (!rr.mine) return;
+  for (int j = t; j < half; j += blockDim.x) {
+    const double2 c = rope_cs64(rr.pos, j == t ? f : a.inv_freq[j], a.factor);
+    cosines[j] = c.x;
+    sines[j] = c.y;
+  }
+  __syncthreads();
+  const int far = half >> 2;  // lanes from an element to its pair's other one (layout 0)
+  const bool first = li < far;
+  const int src = (lane + (first ? far : -far)) & 63;
+  // four elements turned; in q's width or in 64 bits
+  const auto turn = [&](auto *v) {
+    using T = std::remove_pointer_t<decltype(v)>;
+    if (a.layout) {
+      if (e < a.rot)
+#pragma unroll
+        for (int k = 0; k < 4; k += 2)
+          if (e + k < a.rot) {
+            const T c = (T)cosines[2 * li + k / 2], s = (T)sines[2 * li + k / 2], p = v[k], q = v[k + 1];
+            v[k] = p * c - q * s;
+            v[k + 1] = p * s + q * c;
+          }
+    } else if (a.rot) {
+      T o[4];
+#pragma unroll
+      for (int k = 0; k < 4; k++) o[k] = __shfl(v[k], src, 64);
+      if (e < a.rot)
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const int j = 4 * (first ? li : li - far) + k;
+          const T c = (T)cosines[j], s = (T)sines[j];
+          v[k] = first ? v[k] * c - o[k] * s : v[k] * c + o[k] * s;
+        }
+    }
+  };
+  for (; i < all; i += waves) {
+    const float4 xv = next;
+    const int mine = h;
+    h = head_of(i + waves);
+    next = read(h);
+    if (i < kvw) {
+      const bool isv = mine >= H + KVH;
+      double y[4] = {xv.x, xv.y, xv.z, xv.w};
+      if (a.k_gamma) {
+        double sum = y[0] * y[0] + y[1] * y[1] + y[2] * y[2] + y[3] * y[3];
+#pragma unroll
+        for (int o = LPH / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+        if (in && !isv) {
+          const double s = 1.0 / sqrt(sum / hd + a.eps);
+          const float4 g = *reinterpret_cast<const float4 *>(a.k_gamma + e);
+          y[0] = y[0] * s * g.x;
+          y[1] = y[1] * s * g.y;
+          y[2] = y[2] * s * g.z;
+          y[3] = y[3] * s * g.w;
+        }
+      }
+      double z[4] = {y[0], y[1], y[2], y[3]};
+      turn(z);
+      if (!isv)
+#pragma unroll
+        for (int k = 0; k < 4; k++) y[k] = z[k];
+      const int kvh = isv ? mine - H - KVH : mine - H;
+      const size_t at = rr.row + (size_t)kvh * a.c.t.page;
+      void *to = isv ? a.c.v : a.c.k;
+      if constexpr (TYPE == CACHE_F16) {
+        if (in && mine >= 0 && rr.ok)
+          *reinterpret_cast<uint2 *>((uint16_t *)to + at * hd + e) =
+              make_uint2((uint32_t)cache_f16(y[0]) | (uint32_t)cache_f16(y[1]) << 16, (uint32_t)cache_f16(y[2]) | (uint32_t)cache_f16(y[3]) << 16);
+      } else {
+        // the row's largest by its bits: a NaN's are above every number's
+        uint64_t top = 0;
+#pragma unroll
+        for (int k = 0; k < 4; k++) top = max(top, __builtin_bit_cast(uint64_t, y[k]) & ~(1ull << 63));
+#pragma unroll
+        for (int o = LPH / 2; o > 0; o >>= 1) top = max(top, (uint64_t)__shfl_xor((unsigned long long)top, o, 64));
+        const double largest = __builtin_bit_cast(double, top);
+        const uint16_t sc = largest != largest ? 0x7E00 : cache_scale(largest, TYPE);
+        const double s = h2f(sc);
+        uint32_t w = 0;
+        if constexpr (TYPE == CACHE_I8) {
+#pragma unroll
+          for (int k = 0; k < 4; k++) w |= (uint32_t)(cache_code_i8(y[k], s) & 255) << (8 * k);
+        } else {
+          w = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(cache_code_e4m3(y[0], s), cache_code_e4m3(y[1], s), 0, false);
+          w = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(cache_code_e4m3(y[2], s), cache_code_e4m3(y[3], s), (int)w, true);
+        }
+        if (in && mine >= 0 && rr.ok) {
+          *reinterpret_cast<uint32_t *>((uint8_t *)to + at * hd + e) = w;
+          if (li == 0) (isv ? a.c.vs : a.c.ks)[at] = sc;
+        }
+      }
+    } else {
+      float y[4] = {xv.x, xv.y, xv.z, xv.w};
+      if (a.q_gamma) {
+        float sum = y[0] * y[0] + y[1] * y[1] + y[2] * y[2] + y[3] * y[3];
+#pragma unroll
+        for (int o = LPH / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+        if (in) {
+          const float s = 1.0f / sqrtf(sum / (float)hd + (float)a.eps);
+          const float4 g = *reinterpret_cast<const float4 *>(a.q_gamma + e);
+          y[0] = y[0] * s * g.x;
+          y[1] = y[1] * s * g.y;
+          y[2] = y[2] * s * g.z;
+          y[3] = y[3] * s * g.w;
+        }
+      }
+      turn(y);
+      if (in && mine >= 0) {
+        const float nan = __builtin_nanf("");
+        *reinterpret_cast<float4 *>(a.q + m * a.ldq + (size_t)mine * hd + e) =
+            rr.ok ? make_float4(y[0], y[1], y[2], y[3]) : make_float4(nan, nan, nan, nan);
+      }
+    }
+  }
+}
+
 // whether sequence b's rows of its slot share one with those of an earlier sequence
 __device__ __forceinline__ bool read_clashes(const PagedReadArgs &a, int b, EcTreeSeq s) {
   if (!a.slot) return false;
@@ -137,14 +287,15 @@ __device__ __forceinline__ bool read_clashes(const PagedReadArgs &a, int b, EcTr
   return __ballot(hit) != 0;
 }
 
-// One block per 16 rows of a sequence, an element a thread.
-constexpr int kReadRows = 16;
-__global__ __launch_bounds__(256) void paged_read_any_kernel(PagedReadArgs a) {
+// The form for any head size and alignment: one block per `per` rows of a sequence, an
+// element a thread.
+__global__ __launch_bounds__(256) void paged_read_any_kernel(PagedReadArgs a, int per) {
   const int b = blockIdx.y, t = threadIdx.x, hd = a.c.hd, KVH = a.c.t.KVH;
   const EcTreeSeq s{a.slot ? a.slot[b] : b, a.to ? a.to[b] : 0, a.count[b]};
   const int first = a.first[b];
   if (!ec_tree_seq_ok(&a.t, s) || first < 0 || s.n > a.c.t.rows || first > a.c.t.rows - s.n || read_clashes(a, b, s)) return;
-  for (int i = blockIdx.x * kReadRows; i < min(s.n, (int)(blockIdx.x + 1) * kReadRows); i++) {
+  const int i0 = blockIdx.x * per;
+  for (int i = i0; i < min(s.n, i0 + per); i++) {
     const int p = first + i;
     bool bad = false;
     const size_t row = page_row(a.c.t, page_id(a.c.t, b, p), p, 0, &bad);
@@ -158,17 +309,89 @@ __global__ __launch_bounds__(256) void paged_read_any_kernel(PagedReadArgs a) {
   }
 }
 
+// The form for head sizes that are multiples of 8: eight elements a thread at a time,
+// those of a KV head's rows one behind the other, as they stand in a page.
+template <int TYPE>
+__global__ __launch_bounds__(256) void paged_read_kernel(PagedReadArgs a, int per) {
+  const int b = blockIdx.y, t = threadIdx.x, hd = a.c.hd, KVH = a.c.t.KVH;
+  const EcTreeSeq s{a.slot ? a.slot[b] : b, a.to ? a.to[b] : 0, a.count[b]};
+  const int first = a.first[b], i0 = blockIdx.x * per;
+  if (!ec_tree_seq_ok(&a.t, s) || i0 >= s.n || first < 0 || s.n > a.c.t.rows || first > a.c.t.rows - s.n || read_clashes(a, b, s)) return;
+  const int n = min(per, s.n - i0), cpr = hd / 8, items = KVH * n * cpr;
+  const size_t base = ((size_t)s.slot * a.t.C + (s.past + i0)) * ((size_t)KVH * hd);
+  constexpr int UN = 2;
+  for (int j0 = t; j0 < items; j0 += 256 * UN) {
+    Raw8<TYPE> k[UN], v[UN];
+    uint16_t ks[UN], vs[UN];
+    size_t to[UN];
+    bool bad[UN];
+#pragma unroll
+    for (int u = 0; u < UN; u++) {
+      const int j = min(j0 + 256 * u, items - 1), r = j / cpr, cc = j - r * cpr, h = r / n, p = first + i0 + (r - h * n);
+      bad[u] = false;
+      const size_t row = page_row(a.c.t, page_id(a.c.t, b, p), p, h, &bad[u]);
+      constexpr int B = TYPE == CACHE_F16 ? 2 : 1;
+      k[u] = *(const Raw8<TYPE> *)((const char *)a.c.k + (row * hd + 8 * cc) * B);
+      v[u] = *(const Raw8<TYPE> *)((const char *)a.c.v + (row * hd + 8 * cc) * B);
+      if constexpr (TYPE != CACHE_F16) {
+        ks[u] = a.c.ks[row];
+        vs[u] = a.c.vs[row];
+      }
+      to[u] = base + (size_t)(r - h * n) * (KVH * hd) + h * hd + 8 * cc;
+    }
+#pragma unroll
+    for (int u = 0; u < UN; u++) {
+      if (j0 + 256 * u >= items) break;
+      const v4u none = {0x7E007E00u, 0x7E007E00u, 0x7E007E00u, 0x7E007E00u};
+      *reinterpret_cast<v4u *>(a.kc + to[u]) = bad[u] ? none : to_f16<TYPE>(k[u], ks[u]);
+      *reinterpret_cast<v4u *>(a.vc + to[u]) = bad[u] ? none : to_f16<TYPE>(v[u], vs[u]);
+    }
+  }
+}
+
 }  // namespace
 
 int paged_append_max_hd() { return kAppendMaxHd; }
 
+// rows that the vector form's 16-byte (caches: of four elements) accesses can take
+static bool append_vector_ok(const PagedAppendArgs &a) {
+  const uintptr_t p = (uintptr_t)a.x | (uintptr_t)a.q | (uintptr_t)a.q_gamma | (uintptr_t)a.k_gamma;
+  return a.c.hd % 4 == 0 && a.c.hd <= 256 && a.ldx % 4 == 0 && a.ldq % 4 == 0 && !(p & 15) &&
+         !(((uintptr_t)a.c.k | (uintptr_t)a.c.v) & (a.c.type == CACHE_F16 ? 7 : 3)) && (a.layout || a.rot % 8 == 0);
+}
+
+template <int LPH>
+static void launch_append(const PagedAppendArgs &a, hipStream_t st) {
+  constexpr int gpw = 64 / LPH;
+  const int slots = (a.H + gpw - 1) / gpw + (2 * a.c.t.KVH + gpw - 1) / gpw;
+  const dim3 grid(a.c.t.M), block(slots < 4 ? 64 * slots : 256);
+  if (a.c.type == CACHE_F16) klaunch((paged_append_kernel<LPH, CACHE_F16>), grid, block, 0, st, a);
+  else if (a.c.type == CACHE_I8) klaunch((paged_append_kernel<LPH, CACHE_I8>), grid, block, 0, st, a);
+  else klaunch((paged_append_kernel<LPH, CACHE_E4M3>), grid, block, 0, st, a);
+}
+
 hipError_t paged_append(const PagedAppendArgs &a, hipStream_t st) {
-  klaunch(paged_append_any_kernel, dim3(a.c.t.M), dim3(256), 0, st, a);
+  if (!append_vector_ok(a)) klaunch(paged_append_any_kernel, dim3(a.c.t.M), dim3(256), 0, st, a);
+  else if (a.c.hd <= 32) launch_append<8>(a, st);
+  else if (a.c.hd <= 64) launch_append<16>(a, st);
+  else if (a.c.hd <= 128) launch_append<32>(a, st);
+  else launch_append<64>(a, st);
   return hipGetLastError();
 }
 
 hipError_t paged_read(const PagedReadArgs &a, hipStream_t st) {
-  klaunch(paged_read_any_kernel, dim3((a.t.N + kReadRows - 1) / kReadRows, a.t.B), dim3(256), 0, st, a);
+  const int al = a.c.type == CACHE_F16 ? 15 : 7;
+  const bool vec = a.c.hd % 8 == 0 && !(((uintptr_t)a.c.k | (uintptr_t)a.c.v) & al) && !(((uintptr_t)a.kc | (uintptr_t)a.vc) & 15);
+  // blocks of up to 64 rows, of fewer where that would leave CUs without one; of more where
+  // they would be more than a grid's dimension has room for
+  const long most = std::min({(long)a.t.N, (long)a.c.t.rows, (long)a.t.C});
+  long per = most * a.t.B / 2048;
+  per = std::max(per < 8 ? 8 : per > 64 ? 64 : per, (most + kGridRow - 1) / kGridRow);
+  const dim3 grid((unsigned)((most + per - 1) / per), a.t.B);
+  if (!vec) klaunch(paged_read_any_kernel, grid, dim3(256), 0, st, a, (int)per);
+  else if (a.c.type == CACHE_F16) klaunch(paged_read_kernel<CACHE_F16>, grid, dim3(256), 0, st, a, (int)per);
+  else if (a.c.type == CACHE_I8) klaunch(paged_read_kernel<CACHE_I8>, grid, dim3(256), 0, st, a, (int)per);
+  else klaunch(paged_read_kernel<CACHE_E4M3>, grid, dim3(256), 0, st, a, (int)per);
   return hipGetLastError();
 }
 
