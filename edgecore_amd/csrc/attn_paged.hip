@@ -7,7 +7,6 @@
 //
 // in fp32.  What a token does not see does not reach it, finite or not.
 #include <cfloat>
-#include <climits>
 #include <type_traits>
 
 #include "attn_parts.h"
@@ -28,7 +27,7 @@ __global__ __launch_bounds__(256) void attn_paged_any_kernel(PagedAttnArgs a) {
   __shared__ float part[256];
   __shared__ uint32_t row_s[256];
   const int t = threadIdx.x, hd = a.c.hd;
-  const int h = blockIdx.y, m = blockIdx.x, kvh = h / (a.H / a.c.t.KVH);
+  const int h = blockIdx.y, m = blockIdx.x, kvh = h / a.G;
   const int b = page_seq_of(a.c.t, m);
   if (b < 0) return;
   const EcPageSeq s = ec_page_seq(&a.c.t, b);
@@ -88,9 +87,8 @@ __global__ __launch_bounds__(256) void attn_paged_any_kernel(PagedAttnArgs a) {
 // ---------------------------------------------------------------------------
 constexpr int kTp = 64;          // positions per tile
 constexpr float kRoom = 3.0f;    // how far scores may pass the running maximum (powers of two)
-constexpr int kLift = 12;        // the weights' parts are those of 2^kLift e^(x - m)
-constexpr float kLifted = 1 << kLift;
-static_assert(kLift + kRoom < 16.0f, "parts below 65504");
+constexpr float kLift = 12.0f;   // the weights are 2^kLift e^(x - m)
+static_assert(kLift + kRoom < 16.0f, "weights below 65504");
 constexpr long kGridRow = 1L << 20;
 typedef float v16f __attribute__((ext_vector_type(16)));
 
@@ -121,15 +119,15 @@ __device__ __forceinline__ Tiles tiles_of(const PagedAttnArgs &a, const EcPageSe
 // A sequence's row tiles, and no fewer tiles of positions than any of them has
 template <int RT>
 __device__ __forceinline__ int row_tiles(const PagedAttnArgs &a, const EcPageSeq &s) {
-  return ec_page_seq_mine(&a.c.t, s) ? (s.n * (a.H / a.c.t.KVH) + RT - 1) / RT : 0;
+  return ec_page_seq_mine(&a.c.t, s) ? (s.n * a.G + RT - 1) / RT : 0;
 }
 template <int RT>
 __device__ __forceinline__ int most_tiles(const PagedAttnArgs &a, const EcPageSeq &s) {
   if (!ec_page_seq_ok(&a.c.t, s, a.max_past)) return 1;
-  const int all = (s.past + s.n - 1) / kTp + 1, G = a.H / a.c.t.KVH;
+  const int all = (s.past + s.n - 1) / kTp + 1;
   if (!a.window) return all;
   // the tokens of a row tile, the tiles of the positions that they see
-  const int tokens = min((RT + G - 2) / G + 1, s.n);
+  const int tokens = min((RT + a.G - 2) / a.G + 1, s.n);
   const long seen = ((long)a.window + tokens) / kTp + 2 + ((long)min(a.sinks, s.past + s.n) + kTp - 1) / kTp;
   return (int)min((long)all, seen);
 }
@@ -157,7 +155,7 @@ __device__ __forceinline__ Unit find_unit(const PagedAttnArgs &a, const PagedGri
     // sequence b's row tiles are among places start[b] G / RT + b and on, up to the next one's
     const long places = gr.units / KVH, place = places - 1 - x / KVH;
     const auto base = [&](int b) {
-      return (a.c.t.start ? (long)a.c.t.start[b] * (a.H / KVH) / RT : (long)b * (a.H / KVH) / RT) + b;
+      return (long)(a.c.t.start ? a.c.t.start[b] : b) * a.G / RT + b;
     };
     int lo = 0, hi = B;
     while (hi - lo > 1) {
@@ -190,14 +188,13 @@ __device__ __forceinline__ Unit find_unit(const PagedAttnArgs &a, const PagedGri
     if (c0) seq(c0 + lane, s, rt, tiles);
     all += readlane(wave_scan((unsigned long long)rt * tiles), 63);
   }
-  const unsigned long long even = (all + gr.target - 1) / gr.target;
-  const int share = (int)min(max(even, (unsigned long long)gr.least), (unsigned long long)INT_MAX);
+  const uint32_t share = (uint32_t)fmin(fmax(ceil((double)all / gr.target), (double)gr.least), 0x1p30);
   unsigned long long before = 0;
   for (int c0 = 0; c0 < B; c0 += 64) {
     EcPageSeq s = s0;
     int rt = rt0, tiles = tiles0;
     if (c0) seq(c0 + lane, s, rt, tiles);
-    const int n = (int)(((long)tiles + share - 1) / share);
+    const int n = (int)(((uint32_t)tiles + share - 1) / share);
     const unsigned long long mine = (unsigned long long)rt * n * KVH, upto = before + wave_scan(mine);
     const uint64_t hit = __ballot(mine && upto > (unsigned long long)x);
     if (hit) {
@@ -207,14 +204,20 @@ __device__ __forceinline__ Unit find_unit(const PagedAttnArgs &a, const PagedGri
       u.n = readlane(n, l);
       const uint32_t i = (uint32_t)((unsigned long long)x - (readlane(upto, l) - readlane(mine, l))), groups = u.n * KVH;
       u.rt = readlane(rt, l) - 1 - (int)(i / groups);
-      u.j = (int)(i % groups) / KVH;
-      u.kvh = (int)(i % groups) % KVH;
+      const uint32_t g = i % groups;
+      u.j = (int)(g / KVH);
+      u.kvh = (int)(g - u.j * KVH);
       u.at = (uint32_t)x - u.j * KVH;
       return u;
     }
     before = readlane(upto, 63);
   }
   return u;
+}
+
+// where part i of n parts of the tiles starts (products below 2^48: the quotient's floor is exact)
+__device__ __forceinline__ int part_at(int tiles, int i, int n) {
+  return n == 1 ? (i ? tiles : 0) : (int)((double)tiles * i / n);
 }
 
 // The parts' results: which rows of the call there are, per row and query head the place of
@@ -270,6 +273,20 @@ __device__ __forceinline__ void read8(float (&v)[8], const float *q, bool in, fl
     v[j] *= f;
     big = fmaxf(big, fabsf(v[j]));
   }
+}
+
+// two weights in two 16-bit parts each, the nearest and the nearest of the rest
+__device__ __forceinline__ Parts split_near(float x, float y, float minus) {
+  typedef float v2f __attribute__((ext_vector_type(2)));
+  const v2h hi = __builtin_convertvector((v2f{x, y}), v2h);
+  const v2f lo = {__builtin_fmaf((float)hi.x, minus, x), __builtin_fmaf((float)hi.y, minus, y)};
+  return Parts{__builtin_bit_cast(uint32_t, hi), __builtin_bit_cast(uint32_t, __builtin_convertvector(lo, v2h))};
+}
+// -1, unknown to the compiler: it would make two instructions of a mixed-precision difference
+__device__ __forceinline__ float minus_one() {
+  float m = -1.0f;
+  asm volatile("" : "+s"(m));
+  return m;
 }
 
 // which of the positions p0 .. p0 + 63 the token at position t sees
@@ -347,7 +364,7 @@ __device__ __forceinline__ void read_v32(const uint32_t *at, int u, v4u (&v)[2 *
 // Rows of a unit that takes no part
 template <int RT>
 __device__ __forceinline__ void mark_rows(const PagedAttnArgs &a, const PagedGrid &gr, const Unit &u) {
-  const int G = a.H / a.c.t.KVH, hd = a.c.hd, r0 = u.rt * RT, n = min(u.s.n * G - r0, RT);
+  const int G = a.G, hd = a.c.hd, r0 = u.rt * RT, n = min(u.s.n * G - r0, RT);
   for (int e = threadIdx.x; e < n * hd; e += blockDim.x) {
     const int r = r0 + e / hd;
     a.out[(size_t)(u.s.start + r / G) * a.ldo + (size_t)(u.kvh * G + r % G) * hd + e % hd] = __builtin_nanf("");
@@ -377,8 +394,10 @@ __device__ __forceinline__ void mark_call(const PagedAttnArgs &a, const PagedGri
 // fp32 by two 16-bit parts of q and of the weights, as in the attention of drafted tokens.
 template <int HDP, int TYPE>
 __global__ __launch_bounds__(256, 2) void attn_chunk_kernel(PagedAttnArgs a, PagedGrid gr) {
-  constexpr int RT = 128, CPR = HDP / 8, KS = HDP / 16, DT = HDP / 32, LPT = kTp * CPR / 256;
-  extern __shared__ __attribute__((aligned(16))) _Float16 lds[];  // [2 buffers][K, V][kTp][HDP]
+  constexpr int RT = 128, TP = HDP <= 64 ? 64 : 32, PT = TP / 32, PER = kTp / TP, CPR = HDP / 8, KS = HDP / 16, DT = HDP / 32,
+                LPT = (TP * CPR + 255) / 256;
+  extern __shared__ __attribute__((aligned(16))) _Float16 lds[];  // [2 buffers][K, V][TP][HDP]
+  __shared__ __attribute__((aligned(16))) int infinite[2][4];  // of a buffer: which wave brought values that are not finite
   const long x = (long)blockIdx.y * gridDim.x + blockIdx.x;
   mark_call(a, gr, x);
   if (x >= gr.units) return;
@@ -391,10 +410,12 @@ __global__ __launch_bounds__(256, 2) void attn_chunk_kernel(PagedAttnArgs a, Pag
   }
   const int t = threadIdx.x, lane = t & 63, ln = lane & 31, h = lane >> 5, hd = a.c.hd;
   const int w = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int G = a.H / a.c.t.KVH, rows = s.n * G, r0 = un.rt * RT;
+  const int G = a.G, rows = s.n * G, r0 = un.rt * RT;
   const int ta = r0 / G, tb = (min(rows, r0 + RT) - 1) / G;
   const Tiles tl = tiles_of(a, s, ta, tb);
-  const int tile0 = (int)((long)tl.n * un.j / un.n), tile1 = (int)((long)tl.n * (un.j + 1) / un.n);
+  const int tile0 = part_at(tl.n, un.j, un.n), tile1 = part_at(tl.n, un.j + 1, un.n);
+  const int steps = (tile1 - tile0) * PER;
+  const auto pos_of = [&](int i) { return tl.at(tile0 + i / PER) + i % PER * TP; };
 
   // ---- the tiles' way into LDS ----
   // a thread's chunks of 8 elements; rows that no token of the block sees are another's that is
@@ -402,10 +423,10 @@ __global__ __launch_bounds__(256, 2) void attn_chunk_kernel(PagedAttnArgs a, Pag
   int pos[LPT], id[LPT];
   Raw8<TYPE> kr[LPT], vr[LPT];
   uint16_t ksc[LPT], vsc[LPT];
-  const auto find = [&](int tile) {
+  const auto find = [&](int i) {
 #pragma unroll
     for (int u = 0; u < LPT; u++) {
-      const int p = tl.at(tile) + (u * 256 + t) / CPR;
+      const int p = pos_of(i) + min((u * 256 + t) / CPR, TP - 1);
       pos[u] = p >= tl.lo || p < tl.sinks ? min(p, s.past + tb) : tl.lo;
       id[u] = page_id(a.c.t, un.c, pos[u]);
     }
@@ -428,10 +449,10 @@ __global__ __launch_bounds__(256, 2) void attn_chunk_kernel(PagedAttnArgs a, Pag
       }
     }
   };
-  if (tile0 < tile1) {
-    find(tile0);
+  if (steps) {
+    find(0);
     load();
-    if (tile0 + 1 < tile1) find(tile0 + 1);
+    if (steps > 1) find(1);
   }
 
   // ---- this lane's row of q ----
@@ -447,13 +468,11 @@ __global__ __launch_bounds__(256, 2) void attn_chunk_kernel(PagedAttnArgs a, Pag
     for (int k = 0; k < KS; k++) read8(v[k], q + 16 * k, 16 * k + 8 * h < hd, a.scale * 1.44269504f, big);
     split_row(v, pair_max(big), qh, ql, &up, &down, &plain);
   }
-  const bool work = r0 + 32 * w < rows;
-  const int wa = (r0 + 32 * w) / G, wb = (min(rows, r0 + 32 * w + 32) - 1) / G;  // the wave's tokens
 
   // the values' LDS addresses in a tile's first 8 rows (rows 8, 16 .. further on have the
   // same swizzle)
   typedef __attribute__((address_space(3))) void lvoid;
-  const uint32_t vbase = (uint32_t)(uintptr_t)(lvoid *)lds + 2 * kTp * HDP;
+  const uint32_t vbase = (uint32_t)(uintptr_t)(lvoid *)lds + 2 * TP * HDP;
   uint32_t vcol[DT];
 #pragma unroll
   for (int d = 0; d < DT; d++) {
@@ -461,122 +480,125 @@ __global__ __launch_bounds__(256, 2) void attn_chunk_kernel(PagedAttnArgs a, Pag
     vcol[d] = (uint32_t)(r * HDP + ((4 * d + 2 * ((lane >> 4) & 1) + ((l & 3) >> 1)) ^ swz<HDP>(r)) * 8 + 4 * (l & 1)) * 2;
   }
 
+  uint64_t nans = 0;  // elements of o that an infinity or NaN reaches
   v16f o[DT];
+  const float minus = minus_one();
   float from = 0.0f, mx = -FLT_MAX, lim = -FLT_MAX, sum = 0.0f;  // from: what the row's products start at
 #pragma unroll
   for (int d = 0; d < DT; d++)
 #pragma unroll
     for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
 
-  constexpr int kBuf = 2 * kTp * HDP;  // elements of a buffer: K, then V
-  int buf = 0;
-  // One tile.  EDGE: one that some rows see in part: what they do not see has weight 0,
-  // and its values must be finite for that to be nothing.
-  auto step = [&](auto edge, int tile) {
+  constexpr int kBuf = 2 * TP * HDP;  // elements of a buffer: K, then V
+  // Step i's tile from registers into LDS, the next one on its way.  EDGE: a tile that some
+  // rows see in part: what they do not see has weight 0, and its values must be finite for that
+  // to be nothing.  Whether one was not.
+  const auto stage = [&](auto edge, int i) {
     constexpr bool EDGE = decltype(edge)::value;
-    const int p0 = tl.at(tile);
-    _Float16 *K = lds + buf, *V = K + kTp * HDP;
+    _Float16 *K = lds + (i & 1) * kBuf, *V = K + TP * HDP;
     bool inf = false;
 #pragma unroll
     for (int u = 0; u < LPT; u++) {
       const int r = (u * 256 + t) / CPR, cc = (u * 256 + t) % CPR, at = r * HDP + (cc ^ swz<HDP>(r)) * 8;
+      if (TP * CPR % 256 && r >= TP) break;
       *reinterpret_cast<v4u *>(K + at) = to_f16<TYPE>(kr[u], ksc[u]);
       v4u v = to_f16<TYPE>(vr[u], vsc[u]);
       if constexpr (EDGE) inf |= only_finite(v);
       *reinterpret_cast<v4u *>(V + at) = v;
     }
-    if (tile + 1 < tile1) {
+    if (i + 1 < steps) {
       load();
-      if (tile + 2 < tile1) find(tile + 2);
+      if (i + 2 < steps) find(i + 2);
     }
-    // the tile is there, and every wave is done with the one before it
     if constexpr (EDGE) {
-      inf = __syncthreads_or(inf);
-    } else {
-      // the loads of the next tile go on
-      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      const int any = __ballot(inf) != 0;
+      if (lane == 0) infinite[i & 1][w] = any;
     }
+    // the tile is there, and every wave is done with the one before it; the loads of the next
+    // one go on
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  };
+  const auto compute = [&](auto edge, int i) {
+    constexpr bool EDGE = decltype(edge)::value;
+    const int p0 = pos_of(i);
+    const _Float16 *K = lds + (i & 1) * kBuf;
     uint32_t vat[DT];
 #pragma unroll
-    for (int d = 0; d < DT; d++) vat[d] = vbase + 2 * (uint32_t)buf + vcol[d];
-    buf = kBuf - buf;
-    if (!work) return;
-    if constexpr (EDGE)
-      if (p0 > s.past + wb || (a.window && p0 + kTp - 1 <= s.past + wa - a.window && p0 >= a.sinks)) return;
+    for (int d = 0; d < DT; d++) vat[d] = vbase + 2 * (uint32_t)((i & 1) * kBuf) + vcol[d];
 
     // ---- scores: sc[pt][i] of position 32 pt + 8 (i / 4) + 4 h + i % 4 ----
-    v16f sc[2];
+    v16f sc[PT];
 #pragma unroll
-    for (int pt = 0; pt < 2; pt++)
+    for (int pt = 0; pt < PT; pt++)
 #pragma unroll
       for (int i = 0; i < 16; i++) sc[pt][i] = from;
 #pragma unroll
     for (int k = 0; k < KS; k++) {
-      v4u kf[2];
+      v4u kf[PT];
 #pragma unroll
-      for (int pt = 0; pt < 2; pt++) {
+      for (int pt = 0; pt < PT; pt++) {
         const int r = 32 * pt + ln;
         kf[pt] = *reinterpret_cast<const v4u *>(K + r * HDP + ((2 * k + h) ^ swz<HDP>(r)) * 8);
       }
-      sc[0] = mma32(kf[0], qh[k], sc[0]);
-      sc[1] = mma32(kf[1], qh[k], sc[1]);
-      sc[0] = mma32(kf[0], ql[k], sc[0]);
-      sc[1] = mma32(kf[1], ql[k], sc[1]);
+#pragma unroll
+      for (int pt = 0; pt < PT; pt++) sc[pt] = mma32(kf[pt], qh[k], sc[pt]);
+#pragma unroll
+      for (int pt = 0; pt < PT; pt++) sc[pt] = mma32(kf[pt], ql[k], sc[pt]);
     }
 
     // ---- weights ----
     if constexpr (EDGE) {
       const uint64_t on = tile_mask(a, p0, qpos) >> (4 * h);
 #pragma unroll
-      for (int pt = 0; pt < 2; pt++)
+      for (int pt = 0; pt < PT; pt++)
 #pragma unroll
         for (int i = 0; i < 16; i++)
           if (!((on >> (32 * pt + 8 * (i >> 2) + (i & 3))) & 1)) sc[pt][i] = -__builtin_inff();
     }
     if (__builtin_expect(!plain, 0)) {
 #pragma unroll
-      for (int pt = 0; pt < 2; pt++)
+      for (int pt = 0; pt < PT; pt++)
 #pragma unroll
         for (int i = 0; i < 16; i++) sc[pt][i] *= down;
     }
-    // exponents of the weights already (the sums began at -mx): above kRoom the maximum
-    // moves
+    // exponents of the weights already (the sums began at kLift - mx): kRoom above kLift the
+    // maximum moves
     float top = -FLT_MAX;
 #pragma unroll
-    for (int pt = 0; pt < 2; pt++)
+    for (int pt = 0; pt < PT; pt++)
 #pragma unroll
       for (int i = 0; i < 16; i++) top = fmaxf(top, sc[pt][i]);
     if (__builtin_expect(__ballot(top > lim) != 0, 0)) {
       const float big = pair_max(top);
-      const bool first = mx == -FLT_MAX, move = big > (first ? -FLT_MAX : 0.0f);
-      const float by = move ? big : 0.0f, back = first ? 0.0f : __builtin_amdgcn_exp2f(-by);
+      const bool first = mx == -FLT_MAX, move = big > (first ? -FLT_MAX : kLift);
+      const float by = move ? big - kLift : 0.0f, back = first ? 0.0f : __builtin_amdgcn_exp2f(-by);
       if (move) {
         mx = first ? big : mx + by;
-        lim = kRoom;
+        lim = kLift + kRoom;
       }
-      from = move || !first ? -mx * up : 0.0f;
+      from = move || !first ? (kLift - mx) * up : 0.0f;
       sum *= back;
 #pragma unroll
       for (int d = 0; d < DT; d++)
 #pragma unroll
         for (int i = 0; i < 16; i++) o[d][i] *= back;
 #pragma unroll
-      for (int pt = 0; pt < 2; pt++)
+      for (int pt = 0; pt < PT; pt++)
 #pragma unroll
         for (int i = 0; i < 16; i++) sc[pt][i] -= by;
     }
     // the tile's weights are added up before they meet the sum so far: one by one, those
     // below half a step of it would be lost
-    v4u ph[2][2], pl[2][2];
+    v4u ph[PT][2], pl[PT][2];
     float here[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int pt = 0; pt < 2; pt++)
+    for (int pt = 0; pt < PT; pt++)
 #pragma unroll
       for (int i = 0; i < 16; i += 2) {
         const float p = __builtin_amdgcn_exp2f(sc[pt][i]), q = __builtin_amdgcn_exp2f(sc[pt][i + 1]);
         here[0] += p;
         here[1] += q;
-        const Parts f = split2<kLift>(p, q);
+        const Parts f = split_near(p, q, minus);
         ph[pt][i >> 3][(i & 7) >> 1] = f.hi;
         pl[pt][i >> 3][(i & 7) >> 1] = f.lo;
       }
@@ -584,7 +606,7 @@ __global__ __launch_bounds__(256, 2) void attn_chunk_kernel(PagedAttnArgs a, Pag
 
     // ---- outputs: o[d][i] of element 32 d + 8 (i / 4) + 4 h + i % 4 ----
 #pragma unroll
-    for (int pt = 0; pt < 2; pt++) {
+    for (int pt = 0; pt < PT; pt++) {
       constexpr int ND = DT % 2 ? 1 : 2;
 #pragma unroll
       for (int d = 0; d < DT; d += ND) {
@@ -603,34 +625,55 @@ __global__ __launch_bounds__(256, 2) void attn_chunk_kernel(PagedAttnArgs a, Pag
     }
 
     // values that are not finite, for the rows that see them
-    if (EDGE && __builtin_expect(inf, 0)) {
+    v4i any = {0, 0, 0, 0};
+    if constexpr (EDGE) any = *reinterpret_cast<const v4i *>(infinite[i & 1]);
+    if (EDGE && __builtin_expect((any.x | any.y | any.z | any.w) != 0, 0)) {
       const uint64_t on = tile_mask(a, p0, qpos);
-      for (int pp = 0; pp < kTp && p0 + pp <= s.past + wb; pp++) {
-        if (!__ballot((on >> pp) & 1)) continue;
+      for (int pp = 0; pp < TP && p0 + pp <= s.past + tb; pp++) {
+        if (!((on >> pp) & 1)) continue;
         bool none = false;
         const uint32_t r = page_row(a.c.t, page_id(a.c.t, un.c, p0 + pp), p0 + pp, un.kvh, &none);
-#pragma unroll
-        for (int d = 0; d < DT; d++)
-#pragma unroll
-          for (int i = 0; i < 16; i++) {
-            const int e = 32 * d + 8 * (i >> 2) + 4 * h + (i & 3);
-            if (((on >> pp) & 1) && e < hd && (cache_value(a.c.v, a.c.vs, TYPE, r, hd, e) & 0x7C00u) == 0x7C00u)
-              o[d][i] = __builtin_nanf("");
-          }
+        for (int e = 0; e < 16 * DT; e++) {
+          const int at = 32 * (e >> 4) + 8 * ((e & 15) >> 2) + 4 * h + (e & 3);
+          if (at < hd && (cache_value(a.c.v, a.c.vs, TYPE, r, hd, at) & 0x7C00u) == 0x7C00u) nans |= 1ull << e;
+        }
       }
     }
   };
-  // a tile that every token sees whole is no edge
-  for (int tile = tile0; tile < tile1; tile++) {
-    const int p0 = tl.at(tile);
-    const bool whole = p0 + kTp - 1 <= s.past + ta &&
-                       (!a.window || p0 > s.past + tb - a.window || p0 + kTp <= a.sinks);
-    if (whole) step(std::false_type{}, tile);
-    else step(std::true_type{}, tile);
+  // the steps whose tiles every token sees whole, and those in front of and behind them (the
+  // first tokens' always: they are few)
+  const int low = max(a.window ? s.past + tb - a.window + 1 : 0, 0) - tl.first * kTp, step0 = (tl.front - tile0) * PER;
+  const int whole0 = min(max(step0 + (max(low, 0) + TP - 1) / TP, 0), steps);
+  const int whole1 = min(max(step0 + (s.past + ta + 1 - tl.first * kTp) / TP, whole0), steps);
+  if (r0 + 32 * w < rows) {
+    int i = 0;
+    for (; i < whole0; i++) {
+      stage(std::true_type{}, i);
+      compute(std::true_type{}, i);
+    }
+    for (; i < whole1; i++) {
+      stage(std::false_type{}, i);
+      compute(std::false_type{}, i);
+    }
+    for (; i < steps; i++) {
+      stage(std::true_type{}, i);
+      compute(std::true_type{}, i);
+    }
+  } else {  // no row of the wave's own: it brings its share of the tiles
+    for (int i = 0; i < steps; i++)
+      if (i < whole0 || i >= whole1) stage(std::true_type{}, i);
+      else stage(std::false_type{}, i);
+  }
+  if (__builtin_expect(nans != 0, 0)) {
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+      for (int i = 0; i < 16; i++)
+        if ((nans >> (16 * d + i)) & 1) o[d][i] = __builtin_nanf("");
   }
 
   const bool none = __syncthreads_or(bad);
-  const float l = none ? __builtin_nanf("") : pair_sum(sum) * kLifted;  // as the outputs
+  const float l = none ? __builtin_nanf("") : pair_sum(sum);
   if (row >= rows) return;
   if (gr.target) {
     const PartRows pr = part_rows(a, gr, RT);
@@ -686,10 +729,10 @@ __global__ __launch_bounds__(256, 2) void attn_step_kernel(PagedAttnArgs a, Page
   }
   const int t = threadIdx.x, lane = t & 63, lr = lane & 15, lg = lane >> 4, hd = a.c.hd;
   const int w = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int G = a.H / a.c.t.KVH, rows = s.n * G, r0 = un.rt * RT;
+  const int G = a.G, rows = s.n * G, r0 = un.rt * RT;
   const int ta = r0 / G, tb = (min(rows, r0 + RT) - 1) / G;
   const Tiles tl = tiles_of(a, s, ta, tb);
-  const int tile0 = (int)((long)tl.n * un.j / un.n), tile1 = (int)((long)tl.n * (un.j + 1) / un.n);
+  const int tile0 = part_at(tl.n, un.j, un.n), tile1 = part_at(tl.n, un.j + 1, un.n);
   const int steps = (tile1 - tile0) * PER;
   const auto pos_of = [&](int i) { return tl.at(tile0 + i / PER) + i % PER * TP; };
 
@@ -771,6 +814,7 @@ __global__ __launch_bounds__(256, 2) void attn_step_kernel(PagedAttnArgs a, Page
   }
 
   v4f o[DT], from = {0.0f, 0.0f, 0.0f, 0.0f};  // from: what the row's products start at
+  const float minus = minus_one();
   float mx = -FLT_MAX, lim = -FLT_MAX, sum = 0.0f;
 #pragma unroll
   for (int d = 0; d < DT; d++) o[d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
@@ -835,13 +879,13 @@ __global__ __launch_bounds__(256, 2) void attn_step_kernel(PagedAttnArgs a, Page
       for (int r = 0; r < 4; r++) top = fmaxf(top, sc[pt][r]);
     if (__builtin_expect(__ballot(top > lim) != 0, 0)) {
       const float big = row_max(top);
-      const bool first = mx == -FLT_MAX, move = big > (first ? -FLT_MAX : 0.0f);
-      const float by = move ? big : 0.0f, back = first ? 0.0f : __builtin_amdgcn_exp2f(-by);
+      const bool first = mx == -FLT_MAX, move = big > (first ? -FLT_MAX : kLift);
+      const float by = move ? big - kLift : 0.0f, back = first ? 0.0f : __builtin_amdgcn_exp2f(-by);
       if (move) {
         mx = first ? big : mx + by;
-        lim = kRoom;
+        lim = kLift + kRoom;
       }
-      const float f = move || !first ? -mx * up : 0.0f;
+      const float f = move || !first ? (kLift - mx) * up : 0.0f;
       from = v4f{f, f, f, f};
       sum *= back;
 #pragma unroll
@@ -865,7 +909,7 @@ __global__ __launch_bounds__(256, 2) void attn_step_kernel(PagedAttnArgs a, Page
       }
 #pragma unroll
       for (int r = 0; r < 2; r++) {
-        const Parts f = split2<kLift>(p[2 * r], p[2 * r + 1]);
+        const Parts f = split_near(p[2 * r], p[2 * r + 1], minus);
         ph[pt >> 1][2 * (pt & 1) + r] = f.hi;
         pl[pt >> 1][2 * (pt & 1) + r] = f.lo;
       }
@@ -906,7 +950,7 @@ __global__ __launch_bounds__(256, 2) void attn_step_kernel(PagedAttnArgs a, Page
   }
 
   // ---- the waves' results together ----
-  float l = row_sum(sum) * kLifted;  // as the outputs
+  float l = row_sum(sum);
   if (__ballot(bad)) l = __builtin_nanf("");
   __syncthreads();  // every wave is done with its tile
   float *wo = reinterpret_cast<float *>(lds) + (w * RT + lr) * LDO + 4 * lg;
@@ -1010,11 +1054,11 @@ bool tiles_ok(const PagedAttnArgs &a) {
 int padded(int hd) { return (hd + 31) / 32 * 32; }
 
 // Rows of a tile: 16 where a sequence has on average no more
-int tile_rows(const PagedAttnArgs &a) { return (long)a.c.t.M * (a.H / a.c.t.KVH) <= 16L * a.c.t.B ? 16 : 128; }
+int tile_rows(const PagedAttnArgs &a) { return (long)a.c.t.M * a.G <= 16L * a.c.t.B ? 16 : 128; }
 
 PagedGrid paged_grid(const PagedAttnArgs &a) {
   const int rt = tile_rows(a), KVH = a.c.t.KVH;
-  const long tiles = (long)a.c.t.M * (a.H / KVH) / rt + a.c.t.B, places = 512 / KVH;
+  const long tiles = (long)a.c.t.M * a.G / rt + a.c.t.B, places = 512 / KVH;
   PagedGrid g;
   g.least = rt == 16 ? 4 : 2;
   long left = places - tiles;
@@ -1033,7 +1077,7 @@ hipError_t launch_paged(const PagedAttnArgs &a, hipStream_t st) {
   const long row = g.units < kGridRow ? g.units : kGridRow;
   const dim3 grid((unsigned)row, (unsigned)((g.units + row - 1) / row));
   if (tile_rows(a) == 16) klaunch((attn_step_kernel<HDP, TYPE>), grid, dim3(256), 0, st, a, g);
-  else klaunch((attn_chunk_kernel<HDP, TYPE>), grid, dim3(256), 2 * 2 * kTp * HDP * 2, st, a, g);
+  else klaunch((attn_chunk_kernel<HDP, TYPE>), grid, dim3(256), 2 * 2 * (HDP <= 64 ? 64 : 32) * HDP * 2, st, a, g);
   return hipGetLastError();
 }
 template <int HDP>

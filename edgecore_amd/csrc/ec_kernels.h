@@ -569,7 +569,7 @@ hipError_t paged_read(const PagedReadArgs &a, hipStream_t st);
 struct PagedAttnArgs {
   PagedCacheArgs c;
   const float *q;
-  int ldq, H, max_past, window, sinks;
+  int ldq, H, G, max_past, window, sinks;  // G = H / KVH
   float scale;
   float *out;
   int ldo;

@@ -2634,7 +2634,7 @@ extern "C" int ec_attention_paged_dev(const EcPagedCache *cache, const float *q,
   }
   EC_INIT();
   const DeviceScope dev;
-  PagedAttnArgs a{c, q, ldq, H, max_past, window, sinks, (float)(1.0 / sqrt((double)hd)), out, ldo, nullptr};
+  PagedAttnArgs a{c, q, ldq, H, H / c.t.KVH, max_past, window, sinks, (float)(1.0 / sqrt((double)hd)), out, ldo, nullptr};
   const size_t need = attention_paged_workspace(a);
   if (need && (r = w16_grow(g_paged_ws, need, fn))) return r;
   a.ws = g_paged_ws.p;
