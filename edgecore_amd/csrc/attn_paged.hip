@@ -92,11 +92,11 @@ static_assert(kLift + kRoom < 16.0f, "weights below 65504");
 constexpr long kGridRow = 1L << 20;
 typedef float v16f __attribute__((ext_vector_type(16)));
 
-// target: units per KV head that the texts are split for (0: they are not); least: tiles of a
-// part, at least
+// places: units per KV head that run at once; target: parts per KV head that the texts are split
+// into where there is no room for all at once (0: they are not split); least: tiles of a part, at least
 struct PagedGrid {
   long units;
-  int target, least;
+  int places, target, least;
 };
 
 // The tiles that rows of tokens ta .. tb see: those of the first tokens that are not among
@@ -181,14 +181,33 @@ __device__ __forceinline__ Unit find_unit(const PagedAttnArgs &a, const PagedGri
     tiles = rt ? most_tiles<RT>(a, s) : 0;
   };
   seq(lane, s0, rt0, tiles0);
-  unsigned long long all = 0;
+  unsigned long long all = 0, least = 0;
   for (int c0 = 0; c0 < B; c0 += 64) {
     EcPageSeq s;
     int rt = rt0, tiles = tiles0;
     if (c0) seq(c0 + lane, s, rt, tiles);
     all += readlane(wave_scan((unsigned long long)rt * tiles), 63);
+    least += readlane(wave_scan((uint32_t)rt), 63);
   }
-  const uint32_t share = (uint32_t)fmin(fmax(ceil((double)all / gr.target), (double)gr.least), 0x1p30);
+  // the smallest share whose units all have a place at once; where none of a few has, one
+  // whose units are no more than target and the row tiles
+  uint32_t share = (uint32_t)fmin(fmax(ceil((double)all / gr.places), (double)gr.least), 0x1p30);
+  for (int k = 0;; k++) {
+    unsigned long long units = least;
+    for (int c0 = 0; c0 < B && least <= (unsigned long long)gr.places; c0 += 64) {
+      if (!c0) units = 0;
+      EcPageSeq s;
+      int rt = rt0, tiles = tiles0;
+      if (c0) seq(c0 + lane, s, rt, tiles);
+      units += readlane(wave_scan((unsigned long long)rt * (((uint32_t)tiles + share - 1) / share)), 63);
+    }
+    if (units <= (unsigned long long)gr.places) break;
+    if (k == 8 || least > (unsigned long long)gr.places) {
+      share = (uint32_t)fmin(fmax(ceil((double)all / gr.target), (double)gr.least), 0x1p30);
+      break;
+    }
+    share += max(1u, share >> 4);
+  }
   unsigned long long before = 0;
   for (int c0 = 0; c0 < B; c0 += 64) {
     EcPageSeq s = s0;
@@ -324,41 +343,15 @@ __device__ __forceinline__ v16f mma32(v4u a, v4u b, v16f c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
 
-// Operands of ND groups of 32 elements, from rows 32 u .. 32 u + 31 of the tile: two of 16
-// positions each.  Lane l of 16 names 8 bytes of row l / 4 and gets element l of the four
-// rows.  The builtin would wait for all that is on its way.
-template <int HD, int ND>
-__device__ __forceinline__ void read_v32(const uint32_t *at, int u, v4u (&v)[2 * ND]) {
-  static_assert(ND == 1 || ND == 2, "groups of elements");
-  v2u x[4 * ND];
-  if constexpr (ND == 1) {
-    asm volatile(
-        "ds_read_b64_tr_b16 %0, %4 offset:%5\n\t"
-        "ds_read_b64_tr_b16 %1, %4 offset:%6\n\t"
-        "ds_read_b64_tr_b16 %2, %4 offset:%7\n\t"
-        "ds_read_b64_tr_b16 %3, %4 offset:%8\n\t"
-        "s_waitcnt lgkmcnt(0)"
-        : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3])
-        : "v"(at[0]), "i"(64 * HD * u), "i"(64 * HD * u + 16 * HD), "i"(64 * HD * u + 32 * HD), "i"(64 * HD * u + 48 * HD)
-        : "memory");
-  } else {
-    asm volatile(
-        "ds_read_b64_tr_b16 %0, %8 offset:%10\n\t"
-        "ds_read_b64_tr_b16 %1, %8 offset:%11\n\t"
-        "ds_read_b64_tr_b16 %2, %8 offset:%12\n\t"
-        "ds_read_b64_tr_b16 %3, %8 offset:%13\n\t"
-        "ds_read_b64_tr_b16 %4, %9 offset:%10\n\t"
-        "ds_read_b64_tr_b16 %5, %9 offset:%11\n\t"
-        "ds_read_b64_tr_b16 %6, %9 offset:%12\n\t"
-        "ds_read_b64_tr_b16 %7, %9 offset:%13\n\t"
-        "s_waitcnt lgkmcnt(0)"
-        : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(x[4]), "=&v"(x[5]), "=&v"(x[6]), "=&v"(x[7])
-        : "v"(at[0]), "v"(at[1]), "i"(64 * HD * u), "i"(64 * HD * u + 16 * HD), "i"(64 * HD * u + 32 * HD),
-          "i"(64 * HD * u + 48 * HD)
-        : "memory");
-  }
-#pragma unroll
-  for (int e = 0; e < 2 * ND; e++) v[e] = v4u{x[2 * e].x, x[2 * e].y, x[2 * e + 1].x, x[2 * e + 1].y};
+// The operand of 32 elements' values at 16 positions, two reads of four rows of the tile:
+// lane l of 16 names 8 bytes of row l / 4 and gets element l of the four rows.
+template <int HD>
+__device__ __forceinline__ v4u read_v32(uint32_t at, int row) {
+  typedef short v4s __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) v4s lv4s;
+  const v2u x = __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lv4s *)(uintptr_t)(at + 2 * HD * row)));
+  const v2u y = __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lv4s *)(uintptr_t)(at + 2 * HD * (row + 8))));
+  return v4u{x.x, x.y, y.x, y.y};
 }
 
 // Rows of a unit that takes no part
@@ -394,8 +387,8 @@ __device__ __forceinline__ void mark_call(const PagedAttnArgs &a, const PagedGri
 // fp32 by two 16-bit parts of q and of the weights, as in the attention of drafted tokens.
 template <int HDP, int TYPE>
 __global__ __launch_bounds__(256, 2) void attn_chunk_kernel(PagedAttnArgs a, PagedGrid gr) {
-  constexpr int RT = 128, TP = HDP <= 64 ? 64 : 32, PT = TP / 32, PER = kTp / TP, CPR = HDP / 8, KS = HDP / 16, DT = HDP / 32,
-                LPT = (TP * CPR + 255) / 256;
+  constexpr int RT = 128, NT = 256, TP = HDP <= 64 ? 64 : 32, PT = TP / 32, PER = kTp / TP, CPR = HDP / 8, KS = HDP / 16, DT = HDP / 32,
+                LPT = (TP * CPR + NT - 1) / NT;
   extern __shared__ __attribute__((aligned(16))) _Float16 lds[];  // [2 buffers][K, V][TP][HDP]
   __shared__ __attribute__((aligned(16))) int infinite[2][4];  // of a buffer: which wave brought values that are not finite
   const long x = (long)blockIdx.y * gridDim.x + blockIdx.x;
@@ -426,7 +419,7 @@ __global__ __launch_bounds__(256, 2) void attn_chunk_kernel(PagedAttnArgs a, Pag
   const auto find = [&](int i) {
 #pragma unroll
     for (int u = 0; u < LPT; u++) {
-      const int p = pos_of(i) + min((u * 256 + t) / CPR, TP - 1);
+      const int p = pos_of(i) + min((u * NT + t) / CPR, TP - 1);
       pos[u] = p >= tl.lo || p < tl.sinks ? min(p, s.past + tb) : tl.lo;
       id[u] = page_id(a.c.t, un.c, pos[u]);
     }
@@ -435,7 +428,7 @@ __global__ __launch_bounds__(256, 2) void attn_chunk_kernel(PagedAttnArgs a, Pag
 #pragma unroll
     for (int u = 0; u < LPT; u++) {
       const uint32_t row = page_row(a.c.t, id[u], pos[u], un.kvh, &bad);
-      const int cc = (u * 256 + t) % CPR;
+      const int cc = (u * NT + t) % CPR;
       kr[u] = vr[u] = Raw8<TYPE>{};
       if (8 * cc < hd) {
         constexpr int B = TYPE == CACHE_F16 ? 2 : 1;
@@ -483,7 +476,10 @@ __global__ __launch_bounds__(256, 2) void attn_chunk_kernel(PagedAttnArgs a, Pag
   uint64_t nans = 0;  // elements of o that an infinity or NaN reaches
   v16f o[DT];
   const float minus = minus_one();
-  float from = 0.0f, mx = -FLT_MAX, lim = -FLT_MAX, sum = 0.0f;  // from: what the row's products start at
+  v16f from;  // what the row's products start at, as the matrix instruction takes it
+#pragma unroll
+  for (int i = 0; i < 16; i++) from[i] = 0.0f;
+  float mx = -FLT_MAX, lim = -FLT_MAX, sum = 0.0f;
 #pragma unroll
   for (int d = 0; d < DT; d++)
 #pragma unroll
@@ -499,8 +495,8 @@ __global__ __launch_bounds__(256, 2) void attn_chunk_kernel(PagedAttnArgs a, Pag
     bool inf = false;
 #pragma unroll
     for (int u = 0; u < LPT; u++) {
-      const int r = (u * 256 + t) / CPR, cc = (u * 256 + t) % CPR, at = r * HDP + (cc ^ swz<HDP>(r)) * 8;
-      if (TP * CPR % 256 && r >= TP) break;
+      const int r = (u * NT + t) / CPR, cc = (u * NT + t) % CPR, at = r * HDP + (cc ^ swz<HDP>(r)) * 8;
+      if (TP * CPR % NT && r >= TP) break;
       *reinterpret_cast<v4u *>(K + at) = to_f16<TYPE>(kr[u], ksc[u]);
       v4u v = to_f16<TYPE>(vr[u], vsc[u]);
       if constexpr (EDGE) inf |= only_finite(v);
@@ -529,9 +525,7 @@ __global__ __launch_bounds__(256, 2) void attn_chunk_kernel(PagedAttnArgs a, Pag
     // ---- scores: sc[pt][i] of position 32 pt + 8 (i / 4) + 4 h + i % 4 ----
     v16f sc[PT];
 #pragma unroll
-    for (int pt = 0; pt < PT; pt++)
-#pragma unroll
-      for (int i = 0; i < 16; i++) sc[pt][i] = from;
+    for (int pt = 0; pt < PT; pt++) sc[pt] = from;
 #pragma unroll
     for (int k = 0; k < KS; k++) {
       v4u kf[PT];
@@ -576,7 +570,9 @@ __global__ __launch_bounds__(256, 2) void attn_chunk_kernel(PagedAttnArgs a, Pag
         mx = first ? big : mx + by;
         lim = kLift + kRoom;
       }
-      from = move || !first ? (kLift - mx) * up : 0.0f;
+      const float f = move || !first ? (kLift - mx) * up : 0.0f;
+#pragma unroll
+      for (int i = 0; i < 16; i++) from[i] = f;
       sum *= back;
 #pragma unroll
       for (int d = 0; d < DT; d++)
@@ -607,20 +603,17 @@ __global__ __launch_bounds__(256, 2) void attn_chunk_kernel(PagedAttnArgs a, Pag
     // ---- outputs: o[d][i] of element 32 d + 8 (i / 4) + 4 h + i % 4 ----
 #pragma unroll
     for (int pt = 0; pt < PT; pt++) {
-      constexpr int ND = DT % 2 ? 1 : 2;
+      v4u vf[2][DT];
 #pragma unroll
-      for (int d = 0; d < DT; d += ND) {
-        v4u vf[2 * ND];
-        if (pt == 0) read_v32<HDP, ND>(vat + d, 0, vf);
-        else read_v32<HDP, ND>(vat + d, 1, vf);
+      for (int c = 0; c < 2; c++)
 #pragma unroll
-        for (int c = 0; c < 2; c++)
+        for (int d = 0; d < DT; d++) vf[c][d] = read_v32<HDP>(vat[d], 32 * pt + 16 * c);
 #pragma unroll
-          for (int e = 0; e < ND; e++) o[d + e] = mma32(vf[2 * e + c], ph[pt][c], o[d + e]);
+      for (int c = 0; c < 2; c++) {
 #pragma unroll
-        for (int c = 0; c < 2; c++)
+        for (int d = 0; d < DT; d++) o[d] = mma32(vf[c][d], ph[pt][c], o[d]);
 #pragma unroll
-          for (int e = 0; e < ND; e++) o[d + e] = mma32(vf[2 * e + c], pl[pt][c], o[d + e]);
+        for (int d = 0; d < DT; d++) o[d] = mma32(vf[c][d], pl[pt][c], o[d]);
       }
     }
 
@@ -1067,7 +1060,8 @@ PagedGrid paged_grid(const PagedAttnArgs &a) {
   long span = (long)a.max_past + a.c.t.M;
   if (a.window && (long)a.window + a.c.t.M + a.sinks < span) span = (long)a.window + a.c.t.M + a.sinks;
   g.target = tiles * KVH <= 2048 && span > (long)g.least * kTp ? (int)left : 0;
-  g.units = (tiles + g.target) * KVH;
+  g.places = (int)(places < 1 ? 1 : places);
+  g.units = (g.target && tiles + g.target < g.places ? g.places : tiles + g.target) * KVH;
   return g;
 }
 
