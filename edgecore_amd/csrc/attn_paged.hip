@@ -696,20 +696,20 @@ __global__ __launch_bounds__(256, 2) void attn_chunk_kernel(PagedAttnArgs a, Pag
             make_float4(o[d][4 * i] * inv, o[d][4 * i + 1] * inv, o[d][4 * i + 2] * inv, o[d][4 * i + 3] * inv);
 }
 
-// Single tokens: 16 rows of one KV head a block.  Each of its four waves takes every
-// fourth of the part's steps of TP positions, without a barrier: keys come from the cache
+// Single tokens: 16 rows of one KV head a block.  Each of its NW waves takes every
+// NW-th of the part's steps of TP positions, without a barrier: keys come from the cache
 // as the matrix instruction's operand, values through the wave's own tile in LDS, which
 // transposes them; the next step's are on their way while a wave works on one.  The waves'
 // results are joined in LDS.
-template <int HDP, int TYPE>
-__global__ __launch_bounds__(256, 2) void attn_step_kernel(PagedAttnArgs a, PagedGrid gr) {
-  constexpr int RT = 16, TP = HDP <= 64 ? 64 : 32, PT = TP / 16, CPR = HDP / 8, KS = HDP / 32, DT = HDP / 16, ND = DT % 4 ? 2 : 4;
+template <int HDP, int TYPE, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void attn_step_kernel(PagedAttnArgs a, PagedGrid gr) {
+  constexpr int RT = 16, NT = 64 * NW, TP = HDP <= 64 ? 64 : 32, PT = TP / 16, CPR = HDP / 8, KS = HDP / 32, DT = HDP / 16, ND = DT % 4 ? 2 : 4;
   constexpr int EB = TYPE == CACHE_F16 ? 2 : 1, VC = TYPE == CACHE_F16 ? 1 : 2;  // chunks of 8 elements in 16 bytes
   constexpr int LV = TP * CPR / VC / 64, PER = kTp / TP;
   constexpr bool WIDE = TYPE != CACHE_F16 && KS % 2 == 0;  // two chunks of keys in 16 bytes
-  constexpr int LDO = HDP + 4, kLds = 4 * (TP * HDP * 2 > RT * LDO * 4 ? TP * HDP * 2 : RT * LDO * 4);
+  constexpr int LDO = HDP + 4, kLds = NW * (TP * HDP * 2 > RT * LDO * 4 ? TP * HDP * 2 : RT * LDO * 4);
   __shared__ __attribute__((aligned(16))) char lds[kLds];
-  __shared__ float2 ml[4][RT];
+  __shared__ float2 ml[NW][RT];
   const long x = (long)blockIdx.y * gridDim.x + blockIdx.x;
   mark_call(a, gr, x);
   if (x >= gr.units) return;
@@ -731,7 +731,7 @@ __global__ __launch_bounds__(256, 2) void attn_step_kernel(PagedAttnArgs a, Page
 
   // ---- a step's keys and values ----
   bool bad = false;
-  int pos, id = 0;
+  int pos = 0, id = 0;
   uint32_t crow = 0;  // lane l's position's row in the cache
   v4u kr[PT][WIDE ? KS / 2 : KS], vr[LV];
   uint16_t ksc[PT], vsc[LV];
@@ -775,7 +775,7 @@ __global__ __launch_bounds__(256, 2) void attn_step_kernel(PagedAttnArgs a, Page
   if (w < steps) {
     find(w);
     load();
-    if (w + 4 < steps) find(w + 4);
+    if (w + NW < steps) find(w + NW);
   }
 
   // ---- this lane's row of q; its elements in the order that the keys' have ----
@@ -812,7 +812,7 @@ __global__ __launch_bounds__(256, 2) void attn_step_kernel(PagedAttnArgs a, Page
 #pragma unroll
   for (int d = 0; d < DT; d++) o[d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 
-  for (int i = w; i < steps; i += 4) {
+  for (int i = w; i < steps; i += NW) {
     const int p0 = pos_of(i);
     const bool edge = !(p0 + TP - 1 <= s.past + ta && (!a.window || p0 > s.past + tb - a.window || p0 + TP <= a.sinks));
     const uint32_t srow = crow;
@@ -845,9 +845,9 @@ __global__ __launch_bounds__(256, 2) void attn_step_kernel(PagedAttnArgs a, Page
         *reinterpret_cast<v4u *>(V + r * HDP + ((cc + c) ^ swz<HDP>(r)) * 8) = v;
       }
     }
-    if (i + 4 < steps) {
+    if (i + NW < steps) {
       load();
-      if (i + 8 < steps) find(i + 8);
+      if (i + 2 * NW < steps) find(i + 2 * NW);
     }
 
     // ---- weights ----
@@ -951,14 +951,15 @@ __global__ __launch_bounds__(256, 2) void attn_step_kernel(PagedAttnArgs a, Page
   for (int d = 0; d < DT; d++) *reinterpret_cast<v4f *>(wo + 16 * d) = o[d];
   if (lg == 0) ml[w][lr] = make_float2(mx, l);
   __syncthreads();
-  const int jr = t >> 4, jrow = r0 + jr;
+  constexpr int LPR = NT / RT;
+  const int jr = t / LPR, jc = t % LPR, jrow = r0 + jr;
   if (jrow >= rows) return;
   const int jt = jrow / G, jh = un.kvh * G + (jrow - jt * G);
-  float m = -FLT_MAX, f[4], jl = 0.0f;
+  float m = -FLT_MAX, f[NW], jl = 0.0f;
 #pragma unroll
-  for (int k = 0; k < 4; k++) m = fmaxf(m, ml[k][jr].x);
+  for (int k = 0; k < NW; k++) m = fmaxf(m, ml[k][jr].x);
 #pragma unroll
-  for (int k = 0; k < 4; k++) {
+  for (int k = 0; k < NW; k++) {
     f[k] = __builtin_amdgcn_exp2f(ml[k][jr].x - m);
     jl = __builtin_fmaf(ml[k][jr].y, f[k], jl);
   }
@@ -966,18 +967,18 @@ __global__ __launch_bounds__(256, 2) void attn_step_kernel(PagedAttnArgs a, Page
   float *to;
   if (gr.target) {
     const PartRows pr = part_rows(a, gr, RT);
-    if (un.j == 0 && (t & 15) == 0) pr.where[(size_t)(s.start + jt) * a.H + jh] = make_uint2(un.at * RT + jr, un.n);
+    if (un.j == 0 && jc == 0) pr.where[(size_t)(s.start + jt) * a.H + jh] = make_uint2(un.at * RT + jr, un.n);
     to = pr.o + ((size_t)x * RT + jr) * HDP;
-    if (un.n > 1 && (t & 15) == 0) pr.ml[(size_t)x * RT + jr] = make_float2(m, jl);
+    if (un.n > 1 && jc == 0) pr.ml[(size_t)x * RT + jr] = make_float2(m, jl);
   }
   if (!gr.target || un.n == 1) {
     to = a.out + (size_t)(s.start + jt) * a.ldo + (size_t)jh * hd;
     scale = jl > 0.0f || jl != jl ? 1.0f / jl : 0.0f;
   }
-  for (int e = 4 * (t & 15); e < hd; e += 64) {
+  for (int e = 4 * jc; e < hd; e += 4 * LPR) {
     v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int k = 0; k < 4; k++) {
+    for (int k = 0; k < NW; k++) {
       const v4f y = *reinterpret_cast<const v4f *>(reinterpret_cast<const float *>(lds) + (k * RT + jr) * LDO + e);
 #pragma unroll
       for (int c = 0; c < 4; c++) v[c] = __builtin_fmaf(y[c], f[k], v[c]);
@@ -1059,7 +1060,7 @@ PagedGrid paged_grid(const PagedAttnArgs &a) {
   if (left < 1) left = 1;
   long span = (long)a.max_past + a.c.t.M;
   if (a.window && (long)a.window + a.c.t.M + a.sinks < span) span = (long)a.window + a.c.t.M + a.sinks;
-  g.target = tiles * KVH <= 2048 && span > (long)g.least * kTp ? (int)left : 0;
+  g.target = tiles * KVH <= 2048 && span > (rt == 16 ? 1024 : g.least * kTp) ? (int)left : 0;
   g.places = (int)(places < 1 ? 1 : places);
   g.units = (g.target && tiles + g.target < g.places ? g.places : tiles + g.target) * KVH;
   return g;
@@ -1070,7 +1071,8 @@ hipError_t launch_paged(const PagedAttnArgs &a, hipStream_t st) {
   const PagedGrid g = paged_grid(a);
   const long row = g.units < kGridRow ? g.units : kGridRow;
   const dim3 grid((unsigned)row, (unsigned)((g.units + row - 1) / row));
-  if (tile_rows(a) == 16) klaunch((attn_step_kernel<HDP, TYPE>), grid, dim3(256), 0, st, a, g);
+  if (tile_rows(a) == 16 && g.target) klaunch((attn_step_kernel<HDP, TYPE, 4>), grid, dim3(256), 0, st, a, g);
+  else if (tile_rows(a) == 16) klaunch((attn_step_kernel<HDP, TYPE, 8>), grid, dim3(512), 0, st, a, g);
   else klaunch((attn_chunk_kernel<HDP, TYPE>), grid, dim3(256), 2 * 2 * (HDP <= 64 ? 64 : 32) * HDP * 2, st, a, g);
   return hipGetLastError();
 }

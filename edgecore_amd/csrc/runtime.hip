@@ -2366,6 +2366,7 @@ extern "C" int ec_attention_dev(const float *q, int ldq, const uint16_t *kc, con
 // opened; what device arrays hold is checked in the kernels (ec_tree.h).
 constexpr long kMaxRows = 1L << 22;       // rows of a call (grids and row offsets stay in 32 bits)
 constexpr int kMaxCacheRows = 1 << 30;    // of a slot
+constexpr int kMaxText = 1 << 29;         // tokens that are counted (two bits of a count are marks)
 constexpr int kMaxKv = 1 << 28;           // elements of a cache row (twice as many columns count in an int)
 constexpr int kMaxLayers = 1 << 20;       // blocks of a grid's dimension
 
@@ -2678,8 +2679,8 @@ extern "C" int ec_logits_edit_dev(const float *logits, int ld, float *out, int l
                    kMaxRows, EC_TREE_MAX);
   if (vocab < 1 || vocab > 1 << 18 || ld < vocab || ldo < vocab || (mask && ldm < (vocab + 31) / 32))
     return set_err(-1, "%s: vocab=%d (up to %d) ld=%d ldo=%d ldm=%d", fn, vocab, 1 << 18, ld, ldo, ldm);
-  if (ldt < 0 || ldt > kMaxCacheRows || max_bias < 0 || max_bias > kMaxCacheRows)
-    return set_err(-1, "%s: ldt=%d max_bias=%d (up to %d)", fn, ldt, max_bias, kMaxCacheRows);
+  if (ldt < 0 || ldt > kMaxText || max_bias < 0 || max_bias > kMaxText)
+    return set_err(-1, "%s: ldt=%d max_bias=%d (up to %d)", fn, ldt, max_bias, kMaxText);
   if (!logits || !out || (ldt > 0 && (!text || !len)) || (max_bias > 0 && (!bias_token || !bias)))
     return set_err(-1, "%s: null pointer", fn);
   const long rows = (long)B * N;

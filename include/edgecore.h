@@ -596,7 +596,7 @@ int ec_paged_read_dev(const EcPagedCache *cache, const int *first, const int *co
  *   - frequency * c - presence            for those that it has c > 0 times behind the prompt
  *   + bias                                for those with one
  *   -inf                                  where bit t % 32 of mask[row][t / 32] is 0
- * text [B][ldt]: the sequence's tokens, len [B] of them, the first prompt [B] of them the
+ * text [B][ldt <= 2^29]: the sequence's tokens, len [B] of them, the first prompt [B] of them the
  * prompt (NULL: none).  token [B * N] (NULL: none; with it N <= 64): the nodes' own tokens, so that those
  * of a node and its ancestors (parent; NULL: the nodes before it) belong to its text, behind the prompt.
  * nodes [B] (NULL: N): the rows behind them stay as they were.  repetition r, frequency,
