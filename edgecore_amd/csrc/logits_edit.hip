@@ -12,58 +12,61 @@ namespace ec {
 
 namespace {
 
-// One block per CHUNK tokens of the vocabulary and some of a sequence's rows.  The text is
+// One block per 1024 tokens of the vocabulary and 8 of a sequence's rows.  The text is
 // counted into a table of the chunk in LDS (whole numbers: the order does not show), from
 // which every thread takes its tokens' counts and biases into registers, for all rows; a token
 // that is also a node's is marked, and its count of a row's line is added where it comes up.
 // So the rows need no barrier, and each is read while the one before it is worked on.  VEC:
 // rows of whole 16-byte chunks, four tokens of a thread beside each other; otherwise they
-// stand 256 apart.
-constexpr int kEditRows = 8;
+// stand 256 apart.  STREAM: rows that are more than the L2s hold go past them.
+//
+// Bound by memory: 112 of 128 rows of 151936, 138 MB, with texts of 4000 tokens, biases and
+// masks, take 26 us (a launch's 4 aside), 5.3 TB/s (a copy of 1 GiB 5.1); through the L2s
+// 33, in blocks of 16 rows of 2048 tokens 43.  Every block reads its sequence's whole text: with
+// one row a sequence that is more than the row's part from 2000 tokens on (128 rows: 31 us for
+// texts of 500, 57 for 8000).  One row takes no longer than a launch.
+constexpr int kEditChunk = 1024, kEditRows = 8;
 constexpr uint32_t kSeen = 1u << 31, kNode = 1u << 30;  // of the prompt; the token of a node
+constexpr double kL2 = 32 << 20;                        // bytes of the 8 L2s together
 
-template <int CHUNK, bool VEC>
+template <bool VEC, bool STREAM>
 __global__ __launch_bounds__(256) void logits_edit_kernel(EditArgs a) {
-  constexpr int Q = CHUNK / 1024;  // fours of a thread
-  __shared__ uint32_t count[CHUNK], bias_at[CHUNK];  // bias_at: the entry's index and 1
+  __shared__ uint32_t count[kEditChunk], bias_at[kEditChunk];  // bias_at: the entry's index and 1
   __shared__ uint64_t line[EC_TREE_MAX];
   __shared__ int node[EC_TREE_MAX];
-  const int t = threadIdx.x, v0 = blockIdx.x * CHUNK, nv = min(CHUNK, a.V - v0);
+  const int t = threadIdx.x, v0 = blockIdx.x * kEditChunk, nv = min(kEditChunk, a.V - v0);
   const int b = blockIdx.y, i0 = blockIdx.z * kEditRows;
   const int nodes = a.nodes ? a.nodes[b] : a.N, rows = nodes >= 0 && nodes <= a.N ? nodes : a.N;
   if (i0 >= rows) return;
   const int len = a.len ? a.len[b] : 0, prompt = a.prompt ? a.prompt[b] : 0, nbias = a.nbias ? a.nbias[b] : a.max_bias;
   bool ok = nodes == rows && len >= 0 && len <= a.ldt && nbias >= 0 && nbias <= a.max_bias;
-  // the k-th token of the q-th four of this thread, in the chunk
-  const auto tok = [&](int q, int k) { return VEC ? 1024 * q + 4 * t + k : 1024 * q + 256 * k + t; };
+  // the k-th token of this thread, in the chunk
+  const auto tok = [&](int k) { return VEC ? 4 * t + k : 256 * k + t; };
   struct Row {
-    float x[Q][4];
-    uint32_t allow[Q][VEC ? 1 : 4];
+    float x[4];
+    uint32_t allow[VEC ? 1 : 4];
   };
   const auto read = [&](int i, Row &row) {
     const size_t r = (size_t)b * a.N + i;
+    if constexpr (VEC) {
+      if (tok(0) >= nv) return;
+      const float4 y = *reinterpret_cast<const float4 *>(a.logits + r * a.ld + v0 + tok(0));
+      row.x[0] = y.x, row.x[1] = y.y, row.x[2] = y.z, row.x[3] = y.w;
+      if (a.mask) row.allow[0] = a.mask[r * a.ldm + ((v0 + tok(0)) >> 5)];
+    } else {
 #pragma unroll
-    for (int q = 0; q < Q; q++) {
-      if constexpr (VEC) {
-        if (tok(q, 0) >= nv) break;
-        const float4 y = *reinterpret_cast<const float4 *>(a.logits + r * a.ld + v0 + tok(q, 0));
-        row.x[q][0] = y.x, row.x[q][1] = y.y, row.x[q][2] = y.z, row.x[q][3] = y.w;
-        if (a.mask) row.allow[q][0] = a.mask[r * a.ldm + ((v0 + tok(q, 0)) >> 5)];
-      } else {
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-          if (tok(q, k) < nv) {
-            row.x[q][k] = a.logits[r * a.ld + v0 + tok(q, k)];
-            if (a.mask) row.allow[q][k] = a.mask[r * a.ldm + ((v0 + tok(q, k)) >> 5)];
-          }
-      }
+      for (int k = 0; k < 4; k++)
+        if (tok(k) < nv) {
+          row.x[k] = a.logits[r * a.ld + v0 + tok(k)];
+          if (a.mask) row.allow[k] = a.mask[r * a.ldm + ((v0 + tok(k)) >> 5)];
+        }
     }
   };
   const float rep = a.repetition ? a.repetition[b] : 1.0f, freq = a.frequency ? a.frequency[b] : 0.0f,
               pres = a.presence ? a.presence[b] : 0.0f;
   Row next;
   read(i0, next);
-  for (int e = t; e < CHUNK; e += 256) {
+  for (int e = t; e < kEditChunk; e += 256) {
     count[e] = 0;
     if (a.max_bias) bias_at[e] = 0;
   }
@@ -80,11 +83,14 @@ __global__ __launch_bounds__(256) void logits_edit_kernel(EditArgs a) {
   if (a.token) ok = ok && line[0] != 0;
   if (ok) {
     const int *text = a.text + (size_t)b * a.ldt;
-    constexpr int UN = 8;
+    constexpr int UN = 8;  // mostly none of them is of the chunk: one test for all
     for (int j0 = t; j0 < len; j0 += 256 * UN) {
-      uint32_t e[UN];
+      uint32_t e[UN], least = ~0u;
 #pragma unroll
       for (int u = 0; u < UN; u++) e[u] = (uint32_t)text[min(j0 + 256 * u, len - 1)] - (uint32_t)v0;
+#pragma unroll
+      for (int u = 0; u < UN; u++) least = min(least, e[u]);
+      if (least >= (uint32_t)nv) continue;
 #pragma unroll
       for (int u = 0; u < UN; u++)
         if (e[u] < (uint32_t)nv && j0 + 256 * u < len) {
@@ -102,67 +108,66 @@ __global__ __launch_bounds__(256) void logits_edit_kernel(EditArgs a) {
     }
     __syncthreads();
   }
-  uint32_t c[Q][4];
-  float bias[Q][4];
+  uint32_t c[4];
+  float bias[4];
 #pragma unroll
-  for (int q = 0; q < Q; q++)
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-      c[q][k] = count[tok(q, k)];
-      const uint32_t at = ok && nbias ? bias_at[tok(q, k)] : 0;
-      bias[q][k] = at ? a.bias[(size_t)b * a.max_bias + (at - 1)] : 0.0f;
-    }
+  for (int k = 0; k < 4; k++) {
+    c[k] = count[tok(k)];
+    const uint32_t at = ok && nbias ? bias_at[tok(k)] : 0;
+    bias[k] = at ? a.bias[(size_t)b * a.max_bias + (at - 1)] : 0.0f;
+  }
   const int i1 = min(rows, i0 + kEditRows);
   for (int i = i0; i < i1; i++) {
-    const size_t r = (size_t)b * a.N + i;
     Row row = next;
     if (i + 1 < i1) read(i + 1, next);
 #pragma unroll
-    for (int q = 0; q < Q; q++) {
-#pragma unroll
-      for (int k = 0; k < 4; k++) {
-        uint32_t n = c[q][k] & ~(kSeen | kNode);
-        bool seen = (c[q][k] & ~kNode) != 0;
-        if (__builtin_expect((c[q][k] & kNode) != 0, 0)) {
-          uint32_t more = 0;
+    for (int k = 0; k < 4; k++) {
+      uint32_t n = c[k] & ~(kSeen | kNode);
+      bool seen = (c[k] & ~kNode) != 0;
+      if (__builtin_expect((c[k] & kNode) != 0, 0)) {
+        uint32_t more = 0;
 #pragma unroll 1
-          for (uint64_t up = line[i]; up; up &= up - 1) more += node[__ffsll((unsigned long long)up) - 1] == v0 + tok(q, k);
-          n += more;
-          seen |= more != 0;
-        }
-        float y = row.x[q][k];
-        if (seen) y = y > 0.0f ? y / rep : y * rep;
-        if (n) y = (y - freq * (float)n) - pres;
-        if (bias[q][k] != 0.0f) y += bias[q][k];
-        if (a.mask && !((row.allow[q][VEC ? 0 : k] >> ((v0 + tok(q, k)) & 31)) & 1)) y = -__builtin_inff();
-        row.x[q][k] = ok ? y : __builtin_nanf("");
+        for (uint64_t up = line[i]; up; up &= up - 1) more += node[__ffsll((unsigned long long)up) - 1] == v0 + tok(k);
+        n += more;
+        seen |= more != 0;
       }
-      if constexpr (VEC) {
-        if (tok(q, 0) < nv)
-          *reinterpret_cast<float4 *>(a.out + r * a.ldo + v0 + tok(q, 0)) = make_float4(row.x[q][0], row.x[q][1], row.x[q][2], row.x[q][3]);
-      } else {
+      float y = row.x[k];
+      if (seen) y = y > 0.0f ? y / rep : y * rep;
+      if (n) y = (y - freq * (float)n) - pres;
+      if (bias[k] != 0.0f) y += bias[k];
+      if (a.mask && !((row.allow[VEC ? 0 : k] >> ((v0 + tok(k)) & 31)) & 1)) y = -__builtin_inff();
+      row.x[k] = ok ? y : __builtin_nanf("");
+    }
+    float *out = a.out + ((size_t)b * a.N + i) * a.ldo + v0;
+    if constexpr (VEC) {
+      typedef float v4f __attribute__((ext_vector_type(4)));
+      const v4f y = {row.x[0], row.x[1], row.x[2], row.x[3]};
+      v4f *to = reinterpret_cast<v4f *>(out + tok(0));
+      if (tok(0) < nv) {
+        if constexpr (STREAM) __builtin_nontemporal_store(y, to);
+        else *to = y;
+      }
+    } else {
 #pragma unroll
-        for (int k = 0; k < 4; k++)
-          if (tok(q, k) < nv) a.out[r * a.ldo + v0 + tok(q, k)] = row.x[q][k];
-      }
+      for (int k = 0; k < 4; k++)
+        if (tok(k) < nv) {
+          if constexpr (STREAM) __builtin_nontemporal_store(row.x[k], out + tok(k));
+          else out[tok(k)] = row.x[k];
+        }
     }
   }
 }
 
 }  // namespace
 
-template <int CHUNK>
-static void launch_edit(const EditArgs &a, hipStream_t st) {
-  const dim3 grid((a.V + CHUNK - 1) / CHUNK, a.B, (a.N + kEditRows - 1) / kEditRows);
-  const bool vec = a.V % 4 == 0 && a.ld % 4 == 0 && a.ldo % 4 == 0 && !(((uintptr_t)a.logits | (uintptr_t)a.out) & 15);
-  if (vec) klaunch((logits_edit_kernel<CHUNK, true>), grid, dim3(256), 0, st, a);
-  else klaunch((logits_edit_kernel<CHUNK, false>), grid, dim3(256), 0, st, a);
-}
-
 hipError_t logits_edit(const EditArgs &a, hipStream_t st) {
-  const long blocks = (long)((a.V + 2047) / 2048) * a.B * ((a.N + kEditRows - 1) / kEditRows);
-  if (blocks >= 512) launch_edit<2048>(a, st);
-  else launch_edit<1024>(a, st);
+  const dim3 grid((a.V + kEditChunk - 1) / kEditChunk, a.B, (a.N + kEditRows - 1) / kEditRows);
+  const bool vec = a.V % 4 == 0 && a.ld % 4 == 0 && a.ldo % 4 == 0 && !(((uintptr_t)a.logits | (uintptr_t)a.out) & 15);
+  const bool stream = (double)a.B * a.N * a.V * 4 > kL2;
+  if (vec && stream) klaunch((logits_edit_kernel<true, true>), grid, dim3(256), 0, st, a);
+  else if (vec) klaunch((logits_edit_kernel<true, false>), grid, dim3(256), 0, st, a);
+  else if (stream) klaunch((logits_edit_kernel<false, true>), grid, dim3(256), 0, st, a);
+  else klaunch((logits_edit_kernel<false, false>), grid, dim3(256), 0, st, a);
   return hipGetLastError();
 }
 
