@@ -6,6 +6,7 @@
 //   o   = sum_p e^(x_p - m) v_p / sum_p e^(x_p - m),  m = max_p x_p
 //
 // in fp32.  What a token does not see does not reach it, finite or not.
+#include <algorithm>
 #include <cfloat>
 #include <type_traits>
 
@@ -374,6 +375,306 @@ __device__ __forceinline__ void mark_call(const PagedAttnArgs &a, const PagedGri
   }
 }
 
+// Single tokens: 16 rows of one KV head a block.  Each of its NW waves takes every
+// NW-th of the part's steps of TP positions, without a barrier: keys come from the cache
+// as the matrix instruction's operand, values through the wave's own tile in LDS, which
+// transposes them; the next step's are on their way while a wave works on one.  The waves'
+// results are joined in LDS.
+// The chunks' kernel takes it for sequences of that few rows among others.
+template <int HDP, int NW>
+constexpr int step_lds() {
+  const int tile = (HDP <= 64 ? 64 : 32) * HDP * 2, joined = 16 * (HDP + 4) * 4;
+  return NW * (tile > joined ? tile : joined);
+}
+// URT: rows of a unit's places in the workspace
+template <int HDP, int TYPE, int NW, int URT>
+__device__ __forceinline__ void step_unit(const PagedAttnArgs &a, const PagedGrid &gr, const Unit &un, long x, char *lds, float2 (&ml)[NW][16]) {
+  constexpr int RT = 16, NT = 64 * NW, TP = HDP <= 64 ? 64 : 32, PT = TP / 16, CPR = HDP / 8, KS = HDP / 32, DT = HDP / 16, ND = DT % 4 ? 2 : 4;
+  constexpr int EB = TYPE == CACHE_F16 ? 2 : 1, VC = TYPE == CACHE_F16 ? 1 : 2;  // chunks of 8 elements in 16 bytes
+  constexpr int LV = TP * CPR / VC / 64, PER = kTp / TP;
+  constexpr bool WIDE = TYPE != CACHE_F16 && KS % 2 == 0;  // two chunks of keys in 16 bytes
+  constexpr int LDO = HDP + 4;
+  const EcPageSeq s = un.s;
+  const int t = threadIdx.x, lane = t & 63, lr = lane & 15, lg = lane >> 4, hd = a.c.hd;
+  const int w = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int G = a.G, rows = s.n * G, r0 = un.rt * RT;
+  const int ta = r0 / G, tb = (min(rows, r0 + RT) - 1) / G;
+  const Tiles tl = tiles_of(a, s, ta, tb);
+  const int tile0 = part_at(tl.n, un.j, un.n), tile1 = part_at(tl.n, un.j + 1, un.n);
+  const int steps = (tile1 - tile0) * PER;
+  const auto pos_of = [&](int i) { return tl.at(tile0 + i / PER) + i % PER * TP; };
+
+  // ---- a step's keys and values ----
+  bool bad = false;
+  int pos = 0, id = 0;
+  uint32_t crow = 0;  // lane l's position's row in the cache
+  v4u kr[PT][WIDE ? KS / 2 : KS], vr[LV];
+  uint16_t ksc[PT], vsc[LV];
+  const auto find = [&](int i) {
+    const int p = pos_of(i) + (lane & (TP - 1));
+    pos = p >= tl.lo || p < tl.sinks ? min(p, s.past + tb) : tl.lo;
+    id = page_id(a.c.t, un.c, pos);
+  };
+  const auto load = [&] {
+    crow = page_row(a.c.t, id, pos, un.kvh, &bad);
+#pragma unroll
+    for (int pt = 0; pt < PT; pt++) {
+      const uint32_t row = (uint32_t)__shfl((int)crow, 16 * pt + lr, 64);
+      const char *k = (const char *)a.c.k + (size_t)row * hd * EB;
+      if constexpr (TYPE != CACHE_F16) ksc[pt] = a.c.ks[row];
+#pragma unroll
+      for (int c = 0; c < (WIDE ? KS / 2 : KS); c++) {
+        kr[pt][c] = v4u{0, 0, 0, 0};
+        if constexpr (TYPE == CACHE_F16) {
+          if (32 * c + 8 * lg < hd) kr[pt][c] = *(const v4u *)(k + 2 * (32 * c + 8 * lg));
+        } else if constexpr (WIDE) {
+          if (lg * (HDP / 4) + 16 * c < hd) kr[pt][c] = *(const v4u *)(k + lg * (HDP / 4) + 16 * c);
+        } else {
+          if (lg * (HDP / 4) + 8 * c < hd) {
+            const v2u y = *(const v2u *)(k + lg * (HDP / 4) + 8 * c);
+            kr[pt][c].x = y.x;
+            kr[pt][c].y = y.y;
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < LV; u++) {
+      const int ch = u * 64 + lane, r = ch / (CPR / VC), cc = ch % (CPR / VC) * VC;
+      const uint32_t row = (uint32_t)__shfl((int)crow, r, 64);
+      vr[u] = v4u{0, 0, 0, 0};
+      if (8 * cc < hd) vr[u] = *(const v4u *)((const char *)a.c.v + ((size_t)row * hd + 8 * cc) * EB);
+      if constexpr (TYPE != CACHE_F16) vsc[u] = a.c.vs[row];
+    }
+  };
+  if (w < steps) {
+    find(w);
+    load();
+    if (w + NW < steps) find(w + NW);
+  }
+
+  // ---- this lane's row of q; its elements in the order that the keys' have ----
+  const int row = r0 + lr, rq = min(row, rows - 1), token = rq / G, head = un.kvh * G + (rq - token * G);
+  const int qpos = s.past + token;
+  v4u qh[KS], ql[KS];
+  float up, down;
+  bool plain;
+  {
+    const float *q = a.q + (size_t)(s.start + token) * a.ldq + (size_t)head * hd;
+    float v[KS][8], big = 0.0f;
+#pragma unroll
+    for (int k = 0; k < KS; k++) {
+      const int e = TYPE == CACHE_F16 ? 32 * k + 8 * lg : lg * (HDP / 4) + 8 * k;
+      read8(v[k], q + e, e < hd, a.scale * 1.44269504f, big);
+    }
+    split_row(v, row_max(big), qh, ql, &up, &down, &plain);
+  }
+
+  // the values' LDS addresses in the tile's first 32 rows
+  typedef __attribute__((address_space(3))) void lvoid;
+  _Float16 *V = reinterpret_cast<_Float16 *>(lds) + w * TP * HDP;
+  const uint32_t vbase = (uint32_t)(uintptr_t)(lvoid *)V;
+  uint32_t vcol[DT];
+#pragma unroll
+  for (int d = 0; d < DT; d++) {
+    const int r = 4 * lg + (lr >> 2);
+    vcol[d] = (uint32_t)(r * HDP + ((2 * d + ((lr & 3) >> 1)) ^ swz<HDP>(r)) * 8 + 4 * (lr & 1)) * 2;
+  }
+
+  v4f o[DT], from = {0.0f, 0.0f, 0.0f, 0.0f};  // from: what the row's products start at
+  const float minus = minus_one();
+  float mx = -FLT_MAX, lim = -FLT_MAX, sum = 0.0f;
+#pragma unroll
+  for (int d = 0; d < DT; d++) o[d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+
+  for (int i = w; i < steps; i += NW) {
+    const int p0 = pos_of(i);
+    const bool edge = !(p0 + TP - 1 <= s.past + ta && (!a.window || p0 > s.past + tb - a.window || p0 + TP <= a.sinks));
+    const uint32_t srow = crow;
+    // ---- scores: sc[pt][r] of position 16 pt + 4 lg + r ----
+    v4f sc[PT];
+#pragma unroll
+    for (int pt = 0; pt < PT; pt++) {
+      sc[pt] = from;
+#pragma unroll
+      for (int k = 0; k < KS; k++) {
+        v4u kf;
+        if constexpr (TYPE == CACHE_F16) kf = kr[pt][k];
+        else if constexpr (WIDE) kf = to_f16<TYPE>(k & 1 ? v2u{kr[pt][k / 2].z, kr[pt][k / 2].w} : v2u{kr[pt][k / 2].x, kr[pt][k / 2].y}, ksc[pt]);
+        else kf = to_f16<TYPE>(v2u{kr[pt][k].x, kr[pt][k].y}, ksc[pt]);
+        sc[pt] = mma(kf, qh[k], sc[pt]);
+        sc[pt] = mma(kf, ql[k], sc[pt]);
+      }
+    }
+    // ---- values into LDS ----
+    bool inf = false;
+#pragma unroll
+    for (int u = 0; u < LV; u++) {
+      const int ch = u * 64 + lane, r = ch / (CPR / VC), cc = ch % (CPR / VC) * VC;
+#pragma unroll
+      for (int c = 0; c < VC; c++) {
+        v4u v;
+        if constexpr (TYPE == CACHE_F16) v = vr[u];
+        else v = to_f16<TYPE>(c ? v2u{vr[u].z, vr[u].w} : v2u{vr[u].x, vr[u].y}, vsc[u]);
+        if (edge) inf |= only_finite(v);
+        *reinterpret_cast<v4u *>(V + r * HDP + ((cc + c) ^ swz<HDP>(r)) * 8) = v;
+      }
+    }
+    if (i + NW < steps) {
+      load();
+      if (i + 2 * NW < steps) find(i + 2 * NW);
+    }
+
+    // ---- weights ----
+    if (edge) {
+      const uint64_t on = tile_mask(a, p0, qpos) >> (4 * lg);
+#pragma unroll
+      for (int pt = 0; pt < PT; pt++)
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+          if (!((on >> (16 * pt + r)) & 1)) sc[pt][r] = -__builtin_inff();
+    }
+    if (__builtin_expect(!plain, 0)) {
+#pragma unroll
+      for (int pt = 0; pt < PT; pt++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) sc[pt][r] *= down;
+    }
+    float top = -FLT_MAX;
+#pragma unroll
+    for (int pt = 0; pt < PT; pt++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) top = fmaxf(top, sc[pt][r]);
+    if (__builtin_expect(__ballot(top > lim) != 0, 0)) {
+      const float big = row_max(top);
+      const bool first = mx == -FLT_MAX, move = big > (first ? -FLT_MAX : kLift);
+      const float by = move ? big - kLift : 0.0f, back = first ? 0.0f : __builtin_amdgcn_exp2f(-by);
+      if (move) {
+        mx = first ? big : mx + by;
+        lim = kLift + kRoom;
+      }
+      const float f = move || !first ? (kLift - mx) * up : 0.0f;
+      from = v4f{f, f, f, f};
+      sum *= back;
+#pragma unroll
+      for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) o[d][r] *= back;
+#pragma unroll
+      for (int pt = 0; pt < PT; pt++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) sc[pt][r] -= by;
+    }
+    v4u ph[PT / 2], pl[PT / 2];
+    float here = 0.0f;
+#pragma unroll
+    for (int pt = 0; pt < PT; pt++) {
+      float p[4];
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        p[r] = __builtin_amdgcn_exp2f(sc[pt][r]);
+        here += p[r];
+      }
+#pragma unroll
+      for (int r = 0; r < 2; r++) {
+        const Parts f = split_near(p[2 * r], p[2 * r + 1], minus);
+        ph[pt >> 1][2 * (pt & 1) + r] = f.hi;
+        pl[pt >> 1][2 * (pt & 1) + r] = f.lo;
+      }
+    }
+    sum += here;
+
+    // ---- outputs: o[d][r] of element 16 d + 4 lg + r ----
+#pragma unroll
+    for (int u = 0; u < TP / 32; u++)
+#pragma unroll
+      for (int d = 0; d < DT; d += ND) {
+        v4u vf[ND];
+        if (u == 0) read_v<HDP, ND>(vcol + d, vbase, 0, vf);
+        else read_v<HDP, ND>(vcol + d, vbase, 1, vf);
+#pragma unroll
+        for (int e = 0; e < ND; e++) {
+          o[d + e] = mma(vf[e], ph[u], o[d + e]);
+          o[d + e] = mma(vf[e], pl[u], o[d + e]);
+        }
+      }
+
+    // values that are not finite, for the rows that see them
+    if (__builtin_expect(__ballot(inf) != 0, 0)) {
+      const uint64_t on = tile_mask(a, p0, qpos);
+      for (int pp = 0; pp < TP; pp++) {
+        const uint32_t r = (uint32_t)__shfl((int)srow, pp, 64);
+        if ((on >> pp) & 1) {
+#pragma unroll
+          for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+              const int e = 16 * d + 4 * lg + k;
+              if (e < hd && (cache_value(a.c.v, a.c.vs, TYPE, r, hd, e) & 0x7C00u) == 0x7C00u) o[d][k] = __builtin_nanf("");
+            }
+        }
+      }
+    }
+  }
+
+  // ---- the waves' results together ----
+  float l = row_sum(sum);
+  if (__ballot(bad)) l = __builtin_nanf("");
+  __syncthreads();  // every wave is done with its tile
+  float *wo = reinterpret_cast<float *>(lds) + (w * RT + lr) * LDO + 4 * lg;
+#pragma unroll
+  for (int d = 0; d < DT; d++) *reinterpret_cast<v4f *>(wo + 16 * d) = o[d];
+  if (lg == 0) ml[w][lr] = make_float2(mx, l);
+  __syncthreads();
+  constexpr int LPR = NT / RT;
+  const int jr = t / LPR, jc = t % LPR, jrow = r0 + jr;
+  if (jrow >= rows) return;
+  const int jt = jrow / G, jh = un.kvh * G + (jrow - jt * G);
+  float m = -FLT_MAX, f[NW], jl = 0.0f;
+#pragma unroll
+  for (int k = 0; k < NW; k++) m = fmaxf(m, ml[k][jr].x);
+#pragma unroll
+  for (int k = 0; k < NW; k++) {
+    f[k] = __builtin_amdgcn_exp2f(ml[k][jr].x - m);
+    jl = __builtin_fmaf(ml[k][jr].y, f[k], jl);
+  }
+  float scale = 1.0f;
+  float *to;
+  if (gr.target) {
+    const PartRows pr = part_rows(a, gr, URT);
+    if (un.j == 0 && jc == 0) pr.where[(size_t)(s.start + jt) * a.H + jh] = make_uint2(un.at * URT + jr, un.n);
+    to = pr.o + ((size_t)x * URT + jr) * HDP;
+    if (un.n > 1 && jc == 0) pr.ml[(size_t)x * URT + jr] = make_float2(m, jl);
+  }
+  if (!gr.target || un.n == 1) {
+    to = a.out + (size_t)(s.start + jt) * a.ldo + (size_t)jh * hd;
+    scale = jl > 0.0f || jl != jl ? 1.0f / jl : 0.0f;
+  }
+  for (int e = 4 * jc; e < hd; e += 4 * LPR) {
+    v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < NW; k++) {
+      const v4f y = *reinterpret_cast<const v4f *>(reinterpret_cast<const float *>(lds) + (k * RT + jr) * LDO + e);
+#pragma unroll
+      for (int c = 0; c < 4; c++) v[c] = __builtin_fmaf(y[c], f[k], v[c]);
+    }
+    *reinterpret_cast<v4f *>(to + e) = v * scale;
+  }
+}
+
+template <int HDP, int TYPE, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void attn_step_kernel(PagedAttnArgs a, PagedGrid gr) {
+  __shared__ __attribute__((aligned(16))) char lds[step_lds<HDP, NW>()];
+  __shared__ float2 ml[NW][16];
+  const long x = (long)blockIdx.y * gridDim.x + blockIdx.x;
+  mark_call(a, gr, x);
+  if (x >= gr.units) return;
+  const Unit un = find_unit<16>(a, gr, x);
+  if (un.c < 0) return;
+  if (!ec_page_seq_ok(&a.c.t, un.s, a.max_past)) mark_rows<16>(a, gr, un);
+  else step_unit<HDP, TYPE, NW, 16>(a, gr, un, x, lds, ml);
+}
+
 // Chunks of tokens: 128 rows of one KV head a block, 32 a wave; the waves share tiles of
 // keys and values that the block brings to LDS in fp16, the next tile on its way into
 // registers while the waves work on one.
@@ -399,6 +700,11 @@ __global__ __launch_bounds__(256, 2) void attn_chunk_kernel(PagedAttnArgs a, Pag
   const EcPageSeq s = un.s;
   if (!ec_page_seq_ok(&a.c.t, s, a.max_past)) {
     mark_rows<RT>(a, gr, un);
+    return;
+  }
+  if (s.n * a.G <= 16) {
+    __shared__ float2 ml[4][16];
+    step_unit<HDP, TYPE, 4, RT>(a, gr, un, x, (char *)lds, ml);
     return;
   }
   const int t = threadIdx.x, lane = t & 63, ln = lane & 31, h = lane >> 5, hd = a.c.hd;
@@ -696,297 +1002,6 @@ __global__ __launch_bounds__(256, 2) void attn_chunk_kernel(PagedAttnArgs a, Pag
             make_float4(o[d][4 * i] * inv, o[d][4 * i + 1] * inv, o[d][4 * i + 2] * inv, o[d][4 * i + 3] * inv);
 }
 
-// Single tokens: 16 rows of one KV head a block.  Each of its NW waves takes every
-// NW-th of the part's steps of TP positions, without a barrier: keys come from the cache
-// as the matrix instruction's operand, values through the wave's own tile in LDS, which
-// transposes them; the next step's are on their way while a wave works on one.  The waves'
-// results are joined in LDS.
-template <int HDP, int TYPE, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void attn_step_kernel(PagedAttnArgs a, PagedGrid gr) {
-  constexpr int RT = 16, NT = 64 * NW, TP = HDP <= 64 ? 64 : 32, PT = TP / 16, CPR = HDP / 8, KS = HDP / 32, DT = HDP / 16, ND = DT % 4 ? 2 : 4;
-  constexpr int EB = TYPE == CACHE_F16 ? 2 : 1, VC = TYPE == CACHE_F16 ? 1 : 2;  // chunks of 8 elements in 16 bytes
-  constexpr int LV = TP * CPR / VC / 64, PER = kTp / TP;
-  constexpr bool WIDE = TYPE != CACHE_F16 && KS % 2 == 0;  // two chunks of keys in 16 bytes
-  constexpr int LDO = HDP + 4, kLds = NW * (TP * HDP * 2 > RT * LDO * 4 ? TP * HDP * 2 : RT * LDO * 4);
-  __shared__ __attribute__((aligned(16))) char lds[kLds];
-  __shared__ float2 ml[NW][RT];
-  const long x = (long)blockIdx.y * gridDim.x + blockIdx.x;
-  mark_call(a, gr, x);
-  if (x >= gr.units) return;
-  const Unit un = find_unit<RT>(a, gr, x);
-  if (un.c < 0) return;
-  const EcPageSeq s = un.s;
-  if (!ec_page_seq_ok(&a.c.t, s, a.max_past)) {
-    mark_rows<RT>(a, gr, un);
-    return;
-  }
-  const int t = threadIdx.x, lane = t & 63, lr = lane & 15, lg = lane >> 4, hd = a.c.hd;
-  const int w = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int G = a.G, rows = s.n * G, r0 = un.rt * RT;
-  const int ta = r0 / G, tb = (min(rows, r0 + RT) - 1) / G;
-  const Tiles tl = tiles_of(a, s, ta, tb);
-  const int tile0 = part_at(tl.n, un.j, un.n), tile1 = part_at(tl.n, un.j + 1, un.n);
-  const int steps = (tile1 - tile0) * PER;
-  const auto pos_of = [&](int i) { return tl.at(tile0 + i / PER) + i % PER * TP; };
-
-  // ---- a step's keys and values ----
-  bool bad = false;
-  int pos = 0, id = 0;
-  uint32_t crow = 0;  // lane l's position's row in the cache
-  v4u kr[PT][WIDE ? KS / 2 : KS], vr[LV];
-  uint16_t ksc[PT], vsc[LV];
-  const auto find = [&](int i) {
-    const int p = pos_of(i) + (lane & (TP - 1));
-    pos = p >= tl.lo || p < tl.sinks ? min(p, s.past + tb) : tl.lo;
-    id = page_id(a.c.t, un.c, pos);
-  };
-  const auto load = [&] {
-    crow = page_row(a.c.t, id, pos, un.kvh, &bad);
-#pragma unroll
-    for (int pt = 0; pt < PT; pt++) {
-      const uint32_t row = (uint32_t)__shfl((int)crow, 16 * pt + lr, 64);
-      const char *k = (const char *)a.c.k + (size_t)row * hd * EB;
-      if constexpr (TYPE != CACHE_F16) ksc[pt] = a.c.ks[row];
-#pragma unroll
-      for (int c = 0; c < (WIDE ? KS / 2 : KS); c++) {
-        kr[pt][c] = v4u{0, 0, 0, 0};
-        if constexpr (TYPE == CACHE_F16) {
-          if (32 * c + 8 * lg < hd) kr[pt][c] = *(const v4u *)(k + 2 * (32 * c + 8 * lg));
-        } else if constexpr (WIDE) {
-          if (lg * (HDP / 4) + 16 * c < hd) kr[pt][c] = *(const v4u *)(k + lg * (HDP / 4) + 16 * c);
-        } else {
-          if (lg * (HDP / 4) + 8 * c < hd) {
-            const v2u y = *(const v2u *)(k + lg * (HDP / 4) + 8 * c);
-            kr[pt][c].x = y.x;
-            kr[pt][c].y = y.y;
-          }
-        }
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < LV; u++) {
-      const int ch = u * 64 + lane, r = ch / (CPR / VC), cc = ch % (CPR / VC) * VC;
-      const uint32_t row = (uint32_t)__shfl((int)crow, r, 64);
-      vr[u] = v4u{0, 0, 0, 0};
-      if (8 * cc < hd) vr[u] = *(const v4u *)((const char *)a.c.v + ((size_t)row * hd + 8 * cc) * EB);
-      if constexpr (TYPE != CACHE_F16) vsc[u] = a.c.vs[row];
-    }
-  };
-  if (w < steps) {
-    find(w);
-    load();
-    if (w + NW < steps) find(w + NW);
-  }
-
-  // ---- this lane's row of q; its elements in the order that the keys' have ----
-  const int row = r0 + lr, rq = min(row, rows - 1), token = rq / G, head = un.kvh * G + (rq - token * G);
-  const int qpos = s.past + token;
-  v4u qh[KS], ql[KS];
-  float up, down;
-  bool plain;
-  {
-    const float *q = a.q + (size_t)(s.start + token) * a.ldq + (size_t)head * hd;
-    float v[KS][8], big = 0.0f;
-#pragma unroll
-    for (int k = 0; k < KS; k++) {
-      const int e = TYPE == CACHE_F16 ? 32 * k + 8 * lg : lg * (HDP / 4) + 8 * k;
-      read8(v[k], q + e, e < hd, a.scale * 1.44269504f, big);
-    }
-    split_row(v, row_max(big), qh, ql, &up, &down, &plain);
-  }
-
-  // the values' LDS addresses in the tile's first 32 rows
-  typedef __attribute__((address_space(3))) void lvoid;
-  _Float16 *V = reinterpret_cast<_Float16 *>(lds) + w * TP * HDP;
-  const uint32_t vbase = (uint32_t)(uintptr_t)(lvoid *)V;
-  uint32_t vcol[DT];
-#pragma unroll
-  for (int d = 0; d < DT; d++) {
-    const int r = 4 * lg + (lr >> 2);
-    vcol[d] = (uint32_t)(r * HDP + ((2 * d + ((lr & 3) >> 1)) ^ swz<HDP>(r)) * 8 + 4 * (lr & 1)) * 2;
-  }
-
-  v4f o[DT], from = {0.0f, 0.0f, 0.0f, 0.0f};  // from: what the row's products start at
-  const float minus = minus_one();
-  float mx = -FLT_MAX, lim = -FLT_MAX, sum = 0.0f;
-#pragma unroll
-  for (int d = 0; d < DT; d++) o[d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-
-  for (int i = w; i < steps; i += NW) {
-    const int p0 = pos_of(i);
-    const bool edge = !(p0 + TP - 1 <= s.past + ta && (!a.window || p0 > s.past + tb - a.window || p0 + TP <= a.sinks));
-    const uint32_t srow = crow;
-    // ---- scores: sc[pt][r] of position 16 pt + 4 lg + r ----
-    v4f sc[PT];
-#pragma unroll
-    for (int pt = 0; pt < PT; pt++) {
-      sc[pt] = from;
-#pragma unroll
-      for (int k = 0; k < KS; k++) {
-        v4u kf;
-        if constexpr (TYPE == CACHE_F16) kf = kr[pt][k];
-        else if constexpr (WIDE) kf = to_f16<TYPE>(k & 1 ? v2u{kr[pt][k / 2].z, kr[pt][k / 2].w} : v2u{kr[pt][k / 2].x, kr[pt][k / 2].y}, ksc[pt]);
-        else kf = to_f16<TYPE>(v2u{kr[pt][k].x, kr[pt][k].y}, ksc[pt]);
-        sc[pt] = mma(kf, qh[k], sc[pt]);
-        sc[pt] = mma(kf, ql[k], sc[pt]);
-      }
-    }
-    // ---- values into LDS ----
-    bool inf = false;
-#pragma unroll
-    for (int u = 0; u < LV; u++) {
-      const int ch = u * 64 + lane, r = ch / (CPR / VC), cc = ch % (CPR / VC) * VC;
-#pragma unroll
-      for (int c = 0; c < VC; c++) {
-        v4u v;
-        if constexpr (TYPE == CACHE_F16) v = vr[u];
-        else v = to_f16<TYPE>(c ? v2u{vr[u].z, vr[u].w} : v2u{vr[u].x, vr[u].y}, vsc[u]);
-        if (edge) inf |= only_finite(v);
-        *reinterpret_cast<v4u *>(V + r * HDP + ((cc + c) ^ swz<HDP>(r)) * 8) = v;
-      }
-    }
-    if (i + NW < steps) {
-      load();
-      if (i + 2 * NW < steps) find(i + 2 * NW);
-    }
-
-    // ---- weights ----
-    if (edge) {
-      const uint64_t on = tile_mask(a, p0, qpos) >> (4 * lg);
-#pragma unroll
-      for (int pt = 0; pt < PT; pt++)
-#pragma unroll
-        for (int r = 0; r < 4; r++)
-          if (!((on >> (16 * pt + r)) & 1)) sc[pt][r] = -__builtin_inff();
-    }
-    if (__builtin_expect(!plain, 0)) {
-#pragma unroll
-      for (int pt = 0; pt < PT; pt++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) sc[pt][r] *= down;
-    }
-    float top = -FLT_MAX;
-#pragma unroll
-    for (int pt = 0; pt < PT; pt++)
-#pragma unroll
-      for (int r = 0; r < 4; r++) top = fmaxf(top, sc[pt][r]);
-    if (__builtin_expect(__ballot(top > lim) != 0, 0)) {
-      const float big = row_max(top);
-      const bool first = mx == -FLT_MAX, move = big > (first ? -FLT_MAX : kLift);
-      const float by = move ? big - kLift : 0.0f, back = first ? 0.0f : __builtin_amdgcn_exp2f(-by);
-      if (move) {
-        mx = first ? big : mx + by;
-        lim = kLift + kRoom;
-      }
-      const float f = move || !first ? (kLift - mx) * up : 0.0f;
-      from = v4f{f, f, f, f};
-      sum *= back;
-#pragma unroll
-      for (int d = 0; d < DT; d++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) o[d][r] *= back;
-#pragma unroll
-      for (int pt = 0; pt < PT; pt++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) sc[pt][r] -= by;
-    }
-    v4u ph[PT / 2], pl[PT / 2];
-    float here = 0.0f;
-#pragma unroll
-    for (int pt = 0; pt < PT; pt++) {
-      float p[4];
-#pragma unroll
-      for (int r = 0; r < 4; r++) {
-        p[r] = __builtin_amdgcn_exp2f(sc[pt][r]);
-        here += p[r];
-      }
-#pragma unroll
-      for (int r = 0; r < 2; r++) {
-        const Parts f = split_near(p[2 * r], p[2 * r + 1], minus);
-        ph[pt >> 1][2 * (pt & 1) + r] = f.hi;
-        pl[pt >> 1][2 * (pt & 1) + r] = f.lo;
-      }
-    }
-    sum += here;
-
-    // ---- outputs: o[d][r] of element 16 d + 4 lg + r ----
-#pragma unroll
-    for (int u = 0; u < TP / 32; u++)
-#pragma unroll
-      for (int d = 0; d < DT; d += ND) {
-        v4u vf[ND];
-        if (u == 0) read_v<HDP, ND>(vcol + d, vbase, 0, vf);
-        else read_v<HDP, ND>(vcol + d, vbase, 1, vf);
-#pragma unroll
-        for (int e = 0; e < ND; e++) {
-          o[d + e] = mma(vf[e], ph[u], o[d + e]);
-          o[d + e] = mma(vf[e], pl[u], o[d + e]);
-        }
-      }
-
-    // values that are not finite, for the rows that see them
-    if (__builtin_expect(__ballot(inf) != 0, 0)) {
-      const uint64_t on = tile_mask(a, p0, qpos);
-      for (int pp = 0; pp < TP; pp++) {
-        const uint32_t r = (uint32_t)__shfl((int)srow, pp, 64);
-        if ((on >> pp) & 1) {
-#pragma unroll
-          for (int d = 0; d < DT; d++)
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-              const int e = 16 * d + 4 * lg + k;
-              if (e < hd && (cache_value(a.c.v, a.c.vs, TYPE, r, hd, e) & 0x7C00u) == 0x7C00u) o[d][k] = __builtin_nanf("");
-            }
-        }
-      }
-    }
-  }
-
-  // ---- the waves' results together ----
-  float l = row_sum(sum);
-  if (__ballot(bad)) l = __builtin_nanf("");
-  __syncthreads();  // every wave is done with its tile
-  float *wo = reinterpret_cast<float *>(lds) + (w * RT + lr) * LDO + 4 * lg;
-#pragma unroll
-  for (int d = 0; d < DT; d++) *reinterpret_cast<v4f *>(wo + 16 * d) = o[d];
-  if (lg == 0) ml[w][lr] = make_float2(mx, l);
-  __syncthreads();
-  constexpr int LPR = NT / RT;
-  const int jr = t / LPR, jc = t % LPR, jrow = r0 + jr;
-  if (jrow >= rows) return;
-  const int jt = jrow / G, jh = un.kvh * G + (jrow - jt * G);
-  float m = -FLT_MAX, f[NW], jl = 0.0f;
-#pragma unroll
-  for (int k = 0; k < NW; k++) m = fmaxf(m, ml[k][jr].x);
-#pragma unroll
-  for (int k = 0; k < NW; k++) {
-    f[k] = __builtin_amdgcn_exp2f(ml[k][jr].x - m);
-    jl = __builtin_fmaf(ml[k][jr].y, f[k], jl);
-  }
-  float scale = 1.0f;
-  float *to;
-  if (gr.target) {
-    const PartRows pr = part_rows(a, gr, RT);
-    if (un.j == 0 && jc == 0) pr.where[(size_t)(s.start + jt) * a.H + jh] = make_uint2(un.at * RT + jr, un.n);
-    to = pr.o + ((size_t)x * RT + jr) * HDP;
-    if (un.n > 1 && jc == 0) pr.ml[(size_t)x * RT + jr] = make_float2(m, jl);
-  }
-  if (!gr.target || un.n == 1) {
-    to = a.out + (size_t)(s.start + jt) * a.ldo + (size_t)jh * hd;
-    scale = jl > 0.0f || jl != jl ? 1.0f / jl : 0.0f;
-  }
-  for (int e = 4 * jc; e < hd; e += 4 * LPR) {
-    v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int k = 0; k < NW; k++) {
-      const v4f y = *reinterpret_cast<const v4f *>(reinterpret_cast<const float *>(lds) + (k * RT + jr) * LDO + e);
-#pragma unroll
-      for (int c = 0; c < 4; c++) v[c] = __builtin_fmaf(y[c], f[k], v[c]);
-    }
-    *reinterpret_cast<v4f *>(to + e) = v * scale;
-  }
-}
-
 // Joins the parts' outputs: per row the largest of their maxima, the sums and outputs
 // brought to it.  HDP / 4 lanes a row (a power of two of them: 24 of 32 at 96).
 template <int HDP>
@@ -1073,7 +1088,7 @@ hipError_t launch_paged(const PagedAttnArgs &a, hipStream_t st) {
   const dim3 grid((unsigned)row, (unsigned)((g.units + row - 1) / row));
   if (tile_rows(a) == 16 && g.target) klaunch((attn_step_kernel<HDP, TYPE, 4>), grid, dim3(256), 0, st, a, g);
   else if (tile_rows(a) == 16) klaunch((attn_step_kernel<HDP, TYPE, 8>), grid, dim3(512), 0, st, a, g);
-  else klaunch((attn_chunk_kernel<HDP, TYPE>), grid, dim3(256), 2 * 2 * (HDP <= 64 ? 64 : 32) * HDP * 2, st, a, g);
+  else klaunch((attn_chunk_kernel<HDP, TYPE>), grid, dim3(256), std::max(2 * 2 * (HDP <= 64 ? 64 : 32) * HDP * 2, step_lds<HDP, 4>()), st, a, g);
   return hipGetLastError();
 }
 template <int HDP>
