@@ -1053,10 +1053,10 @@ __global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedAttnArgs a, P
       make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
-// heads and rows that the matrix-core forms' tiles and 16-byte accesses can take, and
-// whose rows (of query heads) count in an int
+// heads and rows that the matrix-core forms' tiles and 16-byte accesses can take, whose rows
+// (of query heads) count in an int, and no more blocks of sequences without rows than that
 bool tiles_ok(const PagedAttnArgs &a) {
-  if ((long)a.c.t.M * a.H > 1L << 30) return false;
+  if ((long)a.c.t.M * a.H > 1L << 30 || (long)a.c.t.B * a.c.t.KVH > 1L << 30) return false;
   const uintptr_t p = (uintptr_t)a.q | (uintptr_t)a.c.k | (uintptr_t)a.c.v | (uintptr_t)a.out;
   return a.c.hd % 16 == 0 && a.c.hd <= 128 && !(p & 15) && a.ldq % 4 == 0 && a.ldo % 4 == 0;
 }

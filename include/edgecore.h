@@ -539,7 +539,7 @@ int ec_tree_accept_dev(uint16_t *kc, uint16_t *vc, int layers, int nslots, int C
  *
  * The batch: B <= 65535 sequences and M <= 2^22 rows, those of one sequence behind
  * those of the one before it.
- *   start [B + 1]  ascending, start[B] <= M: sequence b's new rows are start[b] ..
+ *   start [B + 1]  ascending, 0 <= start[0], start[B] <= M: sequence b's new rows are start[b] ..
  *                  start[b + 1] - 1 of the call, row i of them at position past + i.
  *                  NULL: a row each, M = B.  Rows of no sequence are padding: what
  *                  they would write stays as it was
@@ -548,7 +548,7 @@ int ec_tree_accept_dev(uint16_t *kc, uint16_t *vc, int layers, int nslots, int C
  * What these arrays hold is checked on the device: a sequence whose past is negative or
  * whose text the table has no room for takes no part, and neither does a row on a page
  * outside the cache: its rows of q / out are NaN, and nothing of it is written.  (Where the starts
- * do not ascend, it is not said which rows of q / out are written, and by which
+ * do not ascend so, it is not said which rows of q / out are written, and by which
  * sequence.)  No two rows of a call may go to one place of a page: what it then holds is
  * not said. */
 enum { EC_CACHE_F16 = 0, EC_CACHE_I8 = 1, EC_CACHE_E4M3 = 2 };
