@@ -344,6 +344,16 @@ __device__ __forceinline__ v16f mma32(v4u a, v4u b, v16f c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
 
+// The wait between the last of the scores' products and what reads them, 12 states for these
+// instructions (8 passes): in a block behind a branch the compiler can leave it out (it did for
+// the maximum, behind the test of `plain`: heads of 65 to 128 came out without the last products' low
+// parts, now and then)
+__device__ __forceinline__ void settle(v16f (&v)[1]) { asm volatile("s_nop 11" : "+v"(v[0])); }
+__device__ __forceinline__ void settle(v16f (&v)[2]) { asm volatile("s_nop 11" : "+v"(v[0]), "+v"(v[1])); }
+// and for those of 4 passes, 8 states
+__device__ __forceinline__ void settle(v4f (&v)[2]) { asm volatile("s_nop 7" : "+v"(v[0]), "+v"(v[1])); }
+__device__ __forceinline__ void settle(v4f (&v)[4]) { asm volatile("s_nop 7" : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3])); }
+
 // The operand of 32 elements' values at 16 positions, two reads of four rows of the tile:
 // lane l of 16 names 8 bytes of row l / 4 and gets element l of the four rows.
 template <int HD>
@@ -526,6 +536,7 @@ __device__ __forceinline__ void step_unit(const PagedAttnArgs &a, const PagedGri
     }
 
     // ---- weights ----
+    settle(sc);
     if (edge) {
       const uint64_t on = tile_mask(a, p0, qpos) >> (4 * lg);
 #pragma unroll
@@ -845,6 +856,7 @@ __global__ __launch_bounds__(256, 2) void attn_chunk_kernel(PagedAttnArgs a, Pag
 #pragma unroll
       for (int pt = 0; pt < PT; pt++) sc[pt] = mma32(kf[pt], ql[k], sc[pt]);
     }
+    settle(sc);
 
     // ---- weights ----
     if constexpr (EDGE) {

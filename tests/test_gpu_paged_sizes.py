@@ -203,6 +203,16 @@ def test_capture_without_a_workspace():
         check(c, got=np.concatenate((want, np.full((1, E), 7.25, np.float32))))
 
 
+@pytest.mark.parametrize("type", ec.CACHE_TYPES)
+@pytest.mark.parametrize("H,KVH,hd", [(12, 2, 128), (16, 4, 96), (14, 2, 64), (8, 1, 32)])
+def test_chunks_same_bits(type, H, KVH, hd):
+    """Every result is there when it is read: equal calls give equal bits."""
+    c = attn_case(17, type, H, KVH, hd, 16, [3000], [500])
+    want = check(c, rows=[(0, 0), (0, 300), (0, 499)])
+    for _ in range(8):
+        assert np.array_equal(call(c), want)
+
+
 def test_same_call_same_bits():
     """Nothing depends on an order of arrival."""
     for args in (("e4m3", 14, 2, 64, 64, [7500, 100], [200, 1]), ("int8", 12, 2, 128, 16, [4000, 30, 900], [1, 1, 1])):
