@@ -62,6 +62,13 @@ __device__ __forceinline__ v4f mma(float a, float b, v4f c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
+// The wait between the last products and what reads them, 10 states for this instruction (8
+// passes): behind a branch the compiler can leave some of it out (it did in the SwiGLU forms)
+__device__ __forceinline__ void settle(v4f (&c)[1][2]) { asm volatile("s_nop 9" : "+v"(c[0][0]), "+v"(c[0][1])); }
+__device__ __forceinline__ void settle(v4f (&c)[2][2]) {
+  asm volatile("s_nop 9" : "+v"(c[0][0]), "+v"(c[0][1]), "+v"(c[1][0]), "+v"(c[1][1]));
+}
+
 // the value of output [m][n] from its sum v (SwiGLU: gate v and up u)
 template <int EPI>
 __device__ __forceinline__ void finish(const GemvArgs &a, int m, int n, float v, float u, const uint64_t *etab) {
@@ -150,6 +157,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void gemm_f32_rows_kernel(GemvArgs 
             for (int i = 0; i < TI; i++)
 #pragma unroll
               for (int h = 0; h < 2; h++) c[i][h] = mma(fa[u][i][h][e], fw[4 * h + e], c[i][h]);
+          settle(c);
 #pragma unroll
           for (int i = 0; i < TI; i++) acc[i][j] = acc[i][j] + (c[i][0] + c[i][1]);
         }
