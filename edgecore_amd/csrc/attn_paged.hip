@@ -6,6 +6,13 @@
 //   o   = sum_p e^(x_p - m) v_p / sum_p e^(x_p - m),  m = max_p x_p
 //
 // in fp32.  What a token does not see does not reach it, finite or not.
+//
+// One pass over the keys and values with the running maximum and sum; tiles of them meet 16
+// rows (single tokens: bound by the cache's bytes) or 128 (chunks: by the matrix cores and the
+// vector ALUs, which a wave uses in turn and two waves of a SIMD in part beside each other).
+// Texts are split into parts where their row tiles do not fill the chip, and the parts joined
+// by a second launch.  Times below are kernels' in us by the library's timing, of which a launch
+// is 4; cases are sequences x tokens, query / KV heads x head size, rows of the texts.
 #include <algorithm>
 #include <cfloat>
 #include <type_traits>
@@ -21,7 +28,9 @@ namespace {
 
 // The form for any head size and alignment: one block per (token, head), tiles
 // of 256 positions, a position per thread for the scores and an element of the
-// head per thread for the sums, with the running maximum and sum.
+// head per thread for the sums, with the running maximum and sum.  Every query head reads
+// its keys again, by elements: right, not fast (64 x 1, 12 / 2 x 126, 4000: 1360; at 128 the matrix cores'
+// forms take 31).
 constexpr int kPagedMaxHd = 512;
 __global__ __launch_bounds__(256) void attn_paged_any_kernel(PagedAttnArgs a) {
   __shared__ float q[kPagedMaxHd], p_s[256], red[4];
@@ -93,8 +102,9 @@ static_assert(kLift + kRoom < 16.0f, "weights below 65504");
 constexpr long kGridRow = 1L << 20;
 typedef float v16f __attribute__((ext_vector_type(16)));
 
-// places: units per KV head that run at once; target: parts per KV head that the texts are split
-// into where there is no room for all at once (0: they are not split); least: tiles of a part, at least
+// places: units per KV head that run at once (512: two blocks a CU); target: parts per KV head that
+// the texts are split into where there is no room for all at once (0: they are not split); least:
+// tiles of a part, at least
 struct PagedGrid {
   long units;
   int places, target, least;
@@ -144,8 +154,10 @@ __device__ __forceinline__ EcPageSeq lane_seq(EcPageSeq s, int l) {
   return EcPageSeq{readlane(s.start, l), readlane(s.n, l), readlane(s.past, l)};
 }
 // By a wave, a sequence per lane.  The parts: as many of a row tile as its sequence's tiles are
-// times an even share of all tiles of the call, so that the units are alike, and a text
-// that is longer than the others is not what the call waits for.  Within a sequence the last
+// times a share of all tiles of the call, so that the units are alike, and a text that is longer
+// than the others is not what the call waits for.  The share is the smallest with which all units
+// run at once: with as many units as places on average, some of them start when others end (512
+// tokens, 14 / 2 x 64, 7500: 50 against 45).  The search takes 0.4 to 1 us.  Within a sequence the last
 // row tiles, which see most, come first, and the units of one part of the positions stand 8
 // apart where there are as many parts: on one XCD, whose L2 they share.
 template <int RT>
@@ -390,7 +402,12 @@ __device__ __forceinline__ void mark_call(const PagedAttnArgs &a, const PagedGri
 // as the matrix instruction's operand, values through the wave's own tile in LDS, which
 // transposes them; the next step's are on their way while a wave works on one.  The waves'
 // results are joined in LDS.
-// The chunks' kernel takes it for sequences of that few rows among others.
+// The chunks' kernel takes it for sequences of that few rows among others (24 sequences, one
+// of 333 tokens, 14 / 2 x 64, 1500: 22.2 a call; with tiles of 128 for all 24.6).
+//
+// 64 x 1, 12 / 2 x 128 of int8, 4000: 31.6, 118 MB at 4.3 TB/s (a copy of 1 GiB 5.1, a plain sum of 128 MiB
+// 4.6); two steps on their way instead of one 33.  One sequence, 14 / 2 x 64 of fp16, 700: 9.8,
+// the chain of the starts, the table, two steps' keys and the waves' join.
 template <int HDP, int NW>
 constexpr int step_lds() {
   const int tile = (HDP <= 64 ? 64 : 32) * HDP * 2, joined = 16 * (HDP + 4) * 4;
@@ -696,7 +713,15 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_step_kernel(PagedAttnArgs a, 
 // as they stand: half h of the lanes takes 4 h .. 4 h + 3 of every run of 8 positions.  The
 // values, rows of the cache, are read for it by the transposing LDS load.
 //
-// fp32 by two 16-bit parts of q and of the weights, as in the attention of drafted tokens.
+// fp32 by two 16-bit parts of q and of the weights (the keys and values are fp16 as they
+// are): the parts' second products are a quarter of the time.
+//
+// 1 x 512, 14 / 2 x 64 of e4m3, 7500: 46, 0.67 PFLOP/s of products in two parts (a library's fp16
+// product reaches 1.15); 4 x 2048, 12 / 2 x 128 of fp16 from their start: 121, 0.73.  Matrix cores 34 to 44% and
+// vector ALUs 45 to 53% busy: a tile takes a wave 2.3 us beside another wave, 1.5 alone.  Measured and not
+// taken: tiles of 32 positions at 64 elements (chunk 51), with three waves a SIMD (57: spills),
+// blocks of 256 rows (chunk 45, prompt 135), wave priorities, loads behind the barrier, keys a
+// step ahead (all the same), a join by the last block of a row tile (chunk 52, 24 mixed sequences 32).
 template <int HDP, int TYPE>
 __global__ __launch_bounds__(256, 2) void attn_chunk_kernel(PagedAttnArgs a, PagedGrid gr) {
   constexpr int RT = 128, NT = 256, TP = HDP <= 64 ? 64 : 32, PT = TP / 32, PER = kTp / TP, CPR = HDP / 8, KS = HDP / 16, DT = HDP / 32,
@@ -1074,20 +1099,28 @@ bool tiles_ok(const PagedAttnArgs &a) {
 }
 int padded(int hd) { return (hd + 31) / 32 * 32; }
 
-// Rows of a tile: 16 where a sequence has on average no more
+// Rows of a tile: 16 where a sequence has on average no more (8 x 1 and x 2, 12 / 2 x 128, 4000: 10.6 + 4.7
+// and 11.1 + 4.7 with the join, in tiles of 128 10.8 + 6.8 and 12.0 + 6.8; 8 x 48, 12 / 12 x 64: 37 and 32.  Between
+// them either may be faster, by up to 5 us, and the average says little of the longest chunk.)
 int tile_rows(const PagedAttnArgs &a) { return (long)a.c.t.M * a.G <= 16L * a.c.t.B ? 16 : 128; }
 
 PagedGrid paged_grid(const PagedAttnArgs &a) {
   const int rt = tile_rows(a), KVH = a.c.t.KVH;
   const long tiles = (long)a.c.t.M * a.G / rt + a.c.t.B, places = 512 / KVH;
   PagedGrid g;
+  // (chunks: 1 x 8, 12 / 2 x 128, 4000: 11.7 + 6.9 with parts of two tiles, 15.6 + 4.6 of four)
   g.least = rt == 16 ? 4 : 2;
   long left = places - tiles;
   if (left < places / 2) left = places / 2;
   if (left < 1) left = 1;
-  long span = (long)a.max_past + a.c.t.M;
-  if (a.window && (long)a.window + a.c.t.M + a.sinks < span) span = (long)a.window + a.c.t.M + a.sinks;
-  g.target = tiles * KVH <= 2048 && span > (rt == 16 ? 1024 : g.least * kTp) ? (int)left : 0;
+  // Not split: texts that one block is through with before a join is, single tokens' up to 1024
+  // positions (1 x 1, 14 / 2 x 64: 10.3 against 7.8 + 4.1 at 900, 14.8 against 7.9 + 3.9 at 2000), of wider heads 640
+  // (12 / 2 x 128: 11.1 against 9.4 + 3.9 at 500, 15.3 against 9.9 + 4.0 at 900); and calls whose row tiles fill
+  // the chip several times without (600 x 1, 12 / 2 x 128, 1000: 75, split 101; 60 x 100, 12 / 12 x 64, 1000: 79, split 72).
+  const long new_rows = rt == 16 ? a.c.t.M / a.c.t.B + 1 : a.c.t.M;
+  long span = a.max_past + new_rows;
+  if (a.window && a.window + new_rows + a.sinks < span) span = a.window + new_rows + a.sinks;
+  g.target = tiles * KVH <= (rt == 128 ? 2048 : 1024) && span > (rt == 128 ? g.least * kTp : a.c.hd <= 64 ? 1024 : 640) ? (int)left : 0;
   g.places = (int)(places < 1 ? 1 : places);
   g.units = (g.target && tiles + g.target < g.places ? g.places : tiles + g.target) * KVH;
   return g;
@@ -1098,7 +1131,9 @@ hipError_t launch_paged(const PagedAttnArgs &a, hipStream_t st) {
   const PagedGrid g = paged_grid(a);
   const long row = g.units < kGridRow ? g.units : kGridRow;
   const dim3 grid((unsigned)row, (unsigned)((g.units + row - 1) / row));
-  if (tile_rows(a) == 16 && g.target) klaunch((attn_step_kernel<HDP, TYPE, 4>), grid, dim3(256), 0, st, a, g);
+  // eight waves a block where every block has a CU to itself (64 x 1, 12 / 2 x 128, 300: 10.3, with four
+  // 11.2), four where they share one (100 x 1, 12 / 12 x 64, 300: 27, with eight 39) or are joined
+  if (tile_rows(a) == 16 && (g.target || g.units > 256)) klaunch((attn_step_kernel<HDP, TYPE, 4>), grid, dim3(256), 0, st, a, g);
   else if (tile_rows(a) == 16) klaunch((attn_step_kernel<HDP, TYPE, 8>), grid, dim3(512), 0, st, a, g);
   else klaunch((attn_chunk_kernel<HDP, TYPE>), grid, dim3(256), std::max(2 * 2 * (HDP <= 64 ? 64 : 32) * HDP * 2, step_lds<HDP, 4>()), st, a, g);
   return hipGetLastError();

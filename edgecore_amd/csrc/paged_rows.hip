@@ -134,7 +134,10 @@ __global__ __launch_bounds__(256) void paged_append_any_kernel(PagedAppendArgs a
 // The form for head sizes that are multiples of 4 up to 256 and rows of whole
 // 16-byte chunks: a block per row, LPH lanes a head, four elements a lane.  A wave takes 64
 // / LPH heads at a time, of q (in 32 bits) or of k and v (in 64), those of k and v first:
-// they take longest.  A pair's other element is in the same lane (layout 1) or in lane +-
+// they take longest.  Bound by the chain of start, length and page in front of the stores and
+// by the 64-bit roundings: 2 x 1500 rows of 14 + 2 2 heads of 64 in 12.0 us (fp16 10.7; a launch's 4
+// with them), 12 + 2 2 of 128 in 15.5; the form for any size takes 32 at heads of 62 and 39 at
+// 126.  64 rows take 5.  A pair's other element is in the same lane (layout 1) or in lane +-
 // rot / 8, which holds its four (layout 0, rot a multiple of 8).
 template <int LPH, int TYPE>
 __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
