@@ -156,8 +156,9 @@ __device__ __forceinline__ EcPageSeq lane_seq(EcPageSeq s, int l) {
 // By a wave, a sequence per lane.  The parts: as many of a row tile as its sequence's tiles are
 // times a share of all tiles of the call, so that the units are alike, and a text that is longer
 // than the others is not what the call waits for.  The share is the smallest with which all units
-// run at once: with as many units as places on average, some of them start when others end (512
-// tokens, 14 / 2 x 64, 7500: 50 against 45).  The search takes 0.4 to 1 us.  Within a sequence the last
+// run at once: with as many units as places on average, some of them start when others end (a call
+// of 6 x 256, 12 / 12 x 64, window 1000: 39.4 against 33.9; 64 x 1, 12 / 2 x 128, 4000: 38.2 against 34.5).
+// The search takes 0.4 to 1 us.  Within a sequence the last
 // row tiles, which see most, come first, and the units of one part of the positions stand 8
 // apart where there are as many parts: on one XCD, whose L2 they share.
 template <int RT>
@@ -403,7 +404,7 @@ __device__ __forceinline__ void mark_call(const PagedAttnArgs &a, const PagedGri
 // transposes them; the next step's are on their way while a wave works on one.  The waves'
 // results are joined in LDS.
 // The chunks' kernel takes it for sequences of that few rows among others (24 sequences, one
-// of 333 tokens, 14 / 2 x 64, 1500: 22.2 a call; with tiles of 128 for all 24.6).
+// of 333 tokens, 14 / 2 x 64, 1500: 22.2 a call; with tiles of 128 for all 24.8).
 //
 // 64 x 1, 12 / 2 x 128 of int8, 4000: 31.6, 118 MB at 4.3 TB/s (a copy of 1 GiB 5.1, a plain sum of 128 MiB
 // 4.6); two steps on their way instead of one 33.  One sequence, 14 / 2 x 64 of fp16, 700: 9.8,
@@ -716,8 +717,8 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_step_kernel(PagedAttnArgs a, 
 // fp32 by two 16-bit parts of q and of the weights (the keys and values are fp16 as they
 // are): the parts' second products are a quarter of the time.
 //
-// 1 x 512, 14 / 2 x 64 of e4m3, 7500: 46, 0.67 PFLOP/s of products in two parts (a library's fp16
-// product reaches 1.15); 4 x 2048, 12 / 2 x 128 of fp16 from their start: 121, 0.73.  Matrix cores 34 to 44% and
+// 1 x 512, 14 / 2 x 64 of e4m3, 7500: 45 to 47 by card, 0.67 PFLOP/s of products in two parts (a library's fp16
+// product reaches 1.15); 4 x 2048, 12 / 2 x 128 of fp16 from their start: 120 to 124, 0.72.  Matrix cores 34 to 44% and
 // vector ALUs 45 to 53% busy: a tile takes a wave 2.3 us beside another wave, 1.5 alone.  Measured and not
 // taken: tiles of 32 positions at 64 elements (chunk 51), with three waves a SIMD (57: spills),
 // blocks of 256 rows (chunk 45, prompt 135), wave priorities, loads behind the barrier, keys a
