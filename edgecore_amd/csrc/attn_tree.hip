@@ -28,9 +28,9 @@ __device__ __forceinline__ int window_lo(int window, int past, int depth) {
 // head per thread for the sums, with the running maximum and sum.  Every query head
 // reads its keys and values anew, a thread a whole key, and nothing is split over the
 // positions: calls of 8 nodes of 14 / 2 heads over 700 rows take 42 us at head size 64
-// (the matrix-core form and its join 10.6), 51 at 80, 72 at 112, 139 at 256; 16 one-token
-// sequences of 12 / 12 heads over 1000 rows 91 (17), 121, 177 and 338; 8 trees of 16 nodes,
-// 12 / 2 heads of 80, over 4000 rows 520 (22 at head size 96).
+// (the matrix-core form and its join 10.6), 53 at 80, 75 at 112, 143 at 256; 16 one-token
+// sequences of 12 / 12 heads over 1000 rows 91 (17), 124, 182 and 353; 8 trees of 16 nodes,
+// 12 / 2 heads of 80, over 4000 rows 530 (22 at head size 96).
 constexpr int kTreeMaxHd = 512;
 __global__ __launch_bounds__(256) void attn_tree_any_kernel(TreeAttnArgs a) {
   __shared__ float q[kTreeMaxHd], p_s[256], red[4];
@@ -86,10 +86,17 @@ __global__ __launch_bounds__(256) void attn_tree_any_kernel(TreeAttnArgs a) {
     mx = mt;
     const int n = min(256, end - p0);
     for (int r = 0, d = d0; r < kTreeMaxHd / 256; r++, d += 256) {
-      acc[r] *= back;
+      // in sums of 16 positions, these in the tile's: one by one, weights below half a step of
+      // what there is would be lost (32000 positions beside one that has 0.99: 5e-5 of the outputs)
+      float tile = 0.0f;
       if (g < groups && d < a.hd)
-        for (int j = g; j < n; j += groups)
-          if (p_s[j] >= 0.0f) acc[r] = __builtin_fmaf(p_s[j], h2f(a.vc[base + (size_t)(p0 + j) * kv + d]), acc[r]);
+        for (int j0 = g; j0 < n; j0 += 16 * groups) {
+          float some = 0.0f;
+          for (int j = j0; j < min(n, j0 + 16 * groups); j += groups)
+            if (p_s[j] >= 0.0f) some = __builtin_fmaf(p_s[j], h2f(a.vc[base + (size_t)(p0 + j) * kv + d]), some);
+          tile += some;
+        }
+      acc[r] = __builtin_fmaf(acc[r], back, tile);
     }
     __syncthreads();
   }
