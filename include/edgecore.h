@@ -602,8 +602,8 @@ int ec_paged_read_dev(const EcPagedCache *cache, const int *first, const int *co
  * nodes [B] (NULL: N): the rows behind them stay as they were.  repetition r, frequency,
  * presence [B]: NULL: 1, 0, 0.  bias_token, bias [B][max_bias], nbias [B] (NULL: max_bias)
  * of them; of entries for one token the last counts.  mask [B * N][ldm] (NULL: none).  Tokens
- * outside the vocabulary are passed over.  A sequence whose len, nbias, nodes or parents are
- * none gets NaN (with nodes outside [0, N]: all N rows).  No output but out; it overlaps no other array. */
+ * outside the vocabulary are passed over.  A sequence whose len, nbias, nodes or (with token)
+ * parents are none gets NaN (with nodes outside [0, N]: all N rows).  No output but out; it overlaps no other array. */
 int ec_logits_edit_dev(const float *logits, int ld, float *out, int ldo, int vocab, const int *text, int ldt, const int *len,
                        const int *prompt, const int *token, const int *nodes, const int *parent, int B, int N,
                        const float *repetition, const float *frequency, const float *presence, const int *bias_token,
