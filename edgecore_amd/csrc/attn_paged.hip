@@ -11,8 +11,8 @@
 // rows (single tokens: bound by the cache's bytes) or 128 (chunks: by the matrix cores and the
 // vector ALUs, which a wave uses in turn and two waves of a SIMD in part beside each other).
 // Texts are split into parts where their row tiles do not fill the chip, and the parts joined
-// by a second launch.  Times below are kernels' in us by the library's timing, of which a launch
-// is 4; cases are sequences x tokens, query / KV heads x head size, rows of the texts.
+// by a second launch.  Times below are kernels' in us by the library's timing, by which the
+// shortest kernels take 4; cases are sequences x tokens, query / KV heads x head size, rows of the texts.
 #include <algorithm>
 #include <cfloat>
 #include <type_traits>
@@ -413,9 +413,10 @@ __device__ __forceinline__ void mark_call(const PagedAttnArgs &a, const PagedGri
 // The chunks' kernel takes it for sequences of that few rows among others (24 sequences, one
 // of 333 tokens, 14 / 2 x 64, 1500: 22.2 a call; with tiles of 128 for all 24.8).
 //
-// 64 x 1, 12 / 2 x 128 of int8, 4000: 31.6, 118 MB at 4.3 TB/s (a copy of 1 GiB 5.1, a plain sum of 128 MiB
-// 4.6); two steps on their way instead of one 33.  One sequence, 14 / 2 x 64 of fp16, 700: 9.8,
-// the chain of the starts, the table, two steps' keys and the waves' join.
+// 64 x 1, 12 / 2 x 128 of int8, 4000: 32 where three caches take turns, 29.5 over and over on one, 118
+// MB at 3.7 and 4.0 TB/s (a plain sum over and over on as many bytes 26.4); two steps on their way
+// instead of one 33.  One sequence, 14 / 2 x 64 of fp16, 700: 10.3, the chain of the starts, the
+// table, two steps' keys and the waves' join.
 template <int HDP, int NW>
 constexpr int step_lds() {
   const int tile = (HDP <= 64 ? 64 : 32) * HDP * 2, joined = 16 * (HDP + 4) * 4;
@@ -722,10 +723,16 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_step_kernel(PagedAttnArgs a, 
 // values, rows of the cache, are read for it by the transposing LDS load.
 //
 // fp32 by two 16-bit parts of q and of the weights (the keys and values are fp16 as they
-// are): the parts' second products are a quarter of the time.
+// are): the parts' second products are a quarter of the time.  The scores' sums start at kLift -
+// m (`from`, here and in the single tokens' form), so that they are exponents as they come; a
+// step's rounding is then that of a number of up to kLift and the maximum's size instead of the
+// sum's own.  Modelled on the CPU (2000 positions, queries and keys of unit variance) the
+// outputs are 4.7e-7 off with it and 2.3e-7 without for heads of 64, 6.5e-7 and 2.7e-7 for
+// 128; sums from 0 would take an addition a score, and their tests' bounds hold both.
 //
-// 1 x 512, 14 / 2 x 64 of e4m3, 7500: 45 to 47 by card, 0.67 PFLOP/s of products in two parts (a library's fp16
-// product reaches 1.15); 4 x 2048, 12 / 2 x 128 of fp16 from their start: 120 to 124, 0.72.  Matrix cores 34 to 44% and
+// 1 x 512, 14 / 2 x 64 of e4m3, 7500: 44 to 47 by card, 0.60 to 0.65 PFLOP/s of products in two parts (a
+// library's fp16 product reaches 1.15); up to 4 x 2048, 12 / 2 x 128 of fp16 from their start: 120 to 125 for
+// 42 GFLOP, 132 for 47, 0.67 to 0.71; 10 to 20 more in the first tens of calls.  Matrix cores 34 to 44% and
 // vector ALUs 45 to 53% busy: a tile takes a wave 2.3 us beside another wave, 1.5 alone.  Measured and not
 // taken: tiles of 32 positions at 64 elements (chunk 51), with three waves a SIMD (57: spills),
 // blocks of 256 rows (chunk 45, prompt 135), wave priorities, loads behind the barrier, keys a
@@ -1108,8 +1115,11 @@ bool tiles_ok(const PagedAttnArgs &a) {
 int padded(int hd) { return (hd + 31) / 32 * 32; }
 
 // Rows of a tile: 16 where a sequence has on average no more (8 x 1 and x 2, 12 / 2 x 128, 4000: 10.6 + 4.7
-// and 11.1 + 4.7 with the join, in tiles of 128 10.8 + 6.8 and 12.0 + 6.8; 8 x 48, 12 / 12 x 64: 37 and 32.  Between
-// them either may be faster, by up to 5 us, and the average says little of the longest chunk.)
+// and 11.1 + 4.7 with the join, in tiles of 128 10.8 + 6.8 and 12.0 + 6.8; 8 x 48, 12 / 12 x 64: 36 and 33).
+// The average says little of the longest chunk: where one stands among single tokens either may be
+// faster (12 / 12 x 64 over 4000, a call in tiles of 16 and of 128: 512 tokens among 64 sequences 112 and 109, among 40
+// 84 and 101, among 35 78 and 62; 300 among 24 over 2000 30 and 58; 64 among 64 87 and 95; 12 / 2 x 128: 150 among 64 51
+// and 57).  How long the chunks are is in device memory, which the host does not read.
 int tile_rows(const PagedAttnArgs &a) { return (long)a.c.t.M * a.G <= 16L * a.c.t.B ? 16 : 128; }
 
 PagedGrid paged_grid(const PagedAttnArgs &a) {

@@ -27,9 +27,9 @@ __device__ __forceinline__ int window_lo(int window, int past, int depth) {
 // of 256 positions, a position per thread for the scores and an element of the
 // head per thread for the sums, with the running maximum and sum.  Every query head
 // reads its keys and values anew, a thread a whole key, and nothing is split over the
-// positions: calls of 8 nodes of 14 / 2 heads over 700 rows take 42 us at head size 64
+// positions: calls of 8 nodes of 14 / 2 heads over 700 rows take 41 us at head size 64
 // (the matrix-core form and its join 10.6), 53 at 80, 75 at 112, 143 at 256; 16 one-token
-// sequences of 12 / 12 heads over 1000 rows 91 (17), 124, 182 and 353; 8 trees of 16 nodes,
+// sequences of 12 / 12 heads over 1000 rows 96 (17), 124, 182 and 353; 8 trees of 16 nodes,
 // 12 / 2 heads of 80, over 4000 rows 530 (22 at head size 96).
 constexpr int kTreeMaxHd = 512;
 __global__ __launch_bounds__(256) void attn_tree_any_kernel(TreeAttnArgs a) {

@@ -21,10 +21,12 @@ namespace {
 // stand 256 apart.  STREAM: rows that are more than the L2s hold go past them.
 //
 // Bound by memory: 112 of 128 rows of 151936, 138 MB, with texts of 4000 tokens, biases and
-// masks, take 26 us (a launch's 4 aside), 5.3 TB/s (a copy of 1 GiB 5.1); through the L2s
-// 33, in blocks of 16 rows of 2048 tokens 43.  Every block reads its sequence's whole text: with
-// one row a sequence that is more than the row's part from 2000 tokens on (128 rows: 31 us for
-// texts of 500, 57 for 8000).  One row takes no longer than a launch.
+// masks, take 30 us where three inputs take turns, 4.6 TB/s (a copy of 1 GiB 5.1), and 39 where
+// eight do; through the L2s 37 and 40.  As many rows of 50257 take 20, at 2.2 TB/s: they begin at
+// any address, and a thread's tokens are read one by one.  Every block reads its sequence's
+// whole text: with one row a sequence that is more than the row's part from 2000 tokens on (128
+// rows: 33 us for texts of 500, 56 for 8000; of 50257 tokens 17 and 26).  One row takes as long
+// as the shortest kernels.
 constexpr int kEditChunk = 1024, kEditRows = 8;
 constexpr uint32_t kSeen = 1u << 31, kNode = 1u << 30;  // of the prompt; the token of a node
 constexpr double kL2 = 32 << 20;                        // bytes of the 8 L2s together

@@ -135,9 +135,9 @@ __global__ __launch_bounds__(256) void paged_append_any_kernel(PagedAppendArgs a
 // 16-byte chunks: a block per row, LPH lanes a head, four elements a lane.  A wave takes 64
 // / LPH heads at a time, of q (in 32 bits) or of k and v (in 64), those of k and v first:
 // they take longest.  Bound by the chain of start, length and page in front of the stores and
-// by the 64-bit roundings: 2 x 1500 rows of 14 + 2 2 heads of 64 in 12.0 us (fp16 10.7; a launch's 4
-// with them), 12 + 2 2 of 128 in 15.5; the form for any size takes 32 at heads of 62 and 39 at
-// 126.  64 rows take 5.  A pair's other element is in the same lane (layout 1) or in lane +-
+// by the 64-bit roundings: 2 x 1500 rows of 14 + 2 2 heads of 64 in 12.9 us (fp16 10.9), 12 + 2 2
+// of 128 in 15.4; the form for any size takes 30 at heads of 62 and 37 at 126.  64 rows take 5, as
+// the shortest kernels do.  A pair's other element is in the same lane (layout 1) or in lane +-
 // rot / 8, which holds its four (layout 0, rot a multiple of 8).
 template <int LPH, int TYPE>
 __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
@@ -316,8 +316,9 @@ __global__ __launch_bounds__(256) void paged_read_any_kernel(PagedReadArgs a, in
 // The form for head sizes that are multiples of 8: eight elements a thread at a time,
 // those of a KV head's rows one behind the other, as they stand in a page.  STREAM: rows that
 // are more than the L2s hold go past them.  Bound by memory: 112000 rows of 2 heads of 128
-// from e4m3, 173 MB, take 23 us (a launch's 4 aside), 7.5 TB/s with what the last-level cache
-// holds of them (a copy of 1 GiB 5.1); through the L2s 37.
+// from e4m3, 173 MB, take 27 us where three caches take turns, 6.3 TB/s with what the last-level
+// cache holds of them (a copy of 172 MiB over and over 5.3), and 35 where eight do; through the L2s
+// 37 and 38.
 template <int TYPE, bool STREAM>
 __global__ __launch_bounds__(256) void paged_read_kernel(PagedReadArgs a, int per) {
   const int b = blockIdx.y, t = threadIdx.x, hd = a.c.hd, KVH = a.c.t.KVH;
