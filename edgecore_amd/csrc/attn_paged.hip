@@ -1133,7 +1133,10 @@ PagedGrid paged_grid(const PagedAttnArgs &a) {
   if (left < 1) left = 1;
   // Not split: texts that one block is through with before a join is, single tokens' up to 1024
   // positions (1 x 1, 14 / 2 x 64: 10.3 against 7.8 + 4.1 at 900, 14.8 against 7.9 + 3.9 at 2000), of wider heads 640
-  // (12 / 2 x 128: 11.1 against 9.4 + 3.9 at 500, 15.3 against 9.9 + 4.0 at 900); and calls whose row tiles fill
+  // (12 / 2 x 128: 11.1 against 9.4 + 3.9 at 500, 15.3 against 9.9 + 4.0 at 900).  Whole calls of fp16 back to
+  // back, unsplit against split, whose join's launch is then partly hidden: 8 / 1 x 32 8.1 against 8.6 at 1024, 9.6
+  // against 8.7 at 1500; 14 / 2 x 64 9.9 against 10.4 at 640, 12.8 against 10.4 at 1024; 16 / 4 x 96 10.5 against 12.6 at
+  // 500, 13.1 against 12.5 at 640; 12 / 2 x 128 13.4 against 14.8 at 500, 17.7 against 14.8 at 640.  And calls whose row tiles fill
   // the chip several times without (600 x 1, 12 / 2 x 128, 1000: 75, split 101; 60 x 100, 12 / 12 x 64, 1000: 79, split 72).
   const long new_rows = rt == 16 ? a.c.t.M / a.c.t.B + 1 : a.c.t.M;
   long span = a.max_past + new_rows;
